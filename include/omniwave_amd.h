@@ -544,6 +544,52 @@ int ow_bwd_block(const void* grad, const void* x, const void* const* small, cons
                  const OwPlan* plan, int32_t batch, int32_t rd, int32_t dtype, int32_t flags, float eps, void* dx,
                  float* grads, void* cast, int32_t cast_dtype, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * The norms around a block with its gate, residual scale and residual (the reference has the norm before
+ * the block, its LayerScale, drop-path and residual as eager steps, omniweave/models/block.py:83-108, and
+ * no norm after it):
+ *
+ *   p    = delta / sqrt(mean_c delta^2 + eps) * post_weight    (post_weight NULL: p = delta)
+ *   out  = x + scale[image] * gate * p                         (delta NULL: out = x, not written)
+ *   next = out / sqrt(mean_c out^2 + eps) * next_weight        (next_weight NULL: not written)
+ *
+ * x, delta: `rows` rows of `channels` values of `dtype`, value stride 1, row strides in values (any
+ * alignment); an image is rows_per_image consecutive rows, and rows are whole images.  gate: [C], or
+ * [images][C] with gate_per_image; scale: [images] fp32; each weight has a dtype of its own.  Sums and
+ * intermediates are fp32 and each output is rounded once: next is formed from the unrounded out.  At most
+ * 8,192 channels and 2^31 - 1 rows.  out and next are contiguous.
+ *
+ * The backward takes dout and dnext (each NULL where it has none, with row strides) and writes those of
+ * dx, ddelta (contiguous, `dtype`), dpost_weight, dgate and dnext_weight (in their weights' dtypes) that
+ * are not NULL.  Weight gradients are summed in a fixed order over ow_block_norms_bwd_workspace bytes of
+ * workspace (not needed, and NULL, where no weight gradient is asked for).  rows, channels >= 1 there.
+ */
+typedef struct OwBlockNorms {
+  int64_t rows;
+  int64_t rows_per_image;
+  int64_t x_stride;
+  int64_t delta_stride;
+  const void* x;
+  const void* delta;
+  const void* post_weight;
+  const void* gate;
+  const float* scale;
+  const void* next_weight;
+  int32_t channels;
+  int32_t dtype;
+  int32_t post_dtype;
+  int32_t gate_dtype;
+  int32_t next_dtype;
+  int32_t gate_per_image;
+  float eps;
+} OwBlockNorms;
+
+int ow_block_norms_fwd(const OwBlockNorms* norms, void* out, void* next, void* stream);
+size_t ow_block_norms_bwd_workspace(const OwBlockNorms* norms);
+int ow_block_norms_bwd(const OwBlockNorms* norms, const void* dout, int64_t dout_stride, const void* dnext,
+                       int64_t dnext_stride, void* dx, void* ddelta, void* dpost_weight, void* dgate,
+                       void* dnext_weight, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -31,6 +31,28 @@ class OwPlan(ctypes.Structure):
     ]
 
 
+class OwBlockNorms(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("rows_per_image", ctypes.c_int64),
+        ("x_stride", ctypes.c_int64),
+        ("delta_stride", ctypes.c_int64),
+        ("x", ctypes.c_void_p),
+        ("delta", ctypes.c_void_p),
+        ("post_weight", ctypes.c_void_p),
+        ("gate", ctypes.c_void_p),
+        ("scale", ctypes.c_void_p),
+        ("next_weight", ctypes.c_void_p),
+        ("channels", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("post_dtype", ctypes.c_int32),
+        ("gate_dtype", ctypes.c_int32),
+        ("next_dtype", ctypes.c_int32),
+        ("gate_per_image", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+    ]
+
+
 _SIGNATURES = {
     "ow_version": (ctypes.c_int, []),
     "ow_last_error": (ctypes.c_char_p, []),
@@ -231,6 +253,13 @@ _SIGNATURES = {
         ctypes.c_int,
         [ctypes.c_void_p] * 5 + [ctypes.c_int32] + [ctypes.c_void_p] * 4 + [ctypes.c_size_t] + [ctypes.c_void_p] * 5
         + [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p],
+    ),
+    "ow_block_norms_fwd": (ctypes.c_int, [ctypes.POINTER(OwBlockNorms)] + [ctypes.c_void_p] * 3),
+    "ow_block_norms_bwd_workspace": (ctypes.c_size_t, [ctypes.POINTER(OwBlockNorms)]),
+    "ow_block_norms_bwd": (
+        ctypes.c_int,
+        [ctypes.POINTER(OwBlockNorms), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64]
+        + [ctypes.c_void_p] * 6 + [ctypes.c_size_t, ctypes.c_void_p],
     ),
     "ow_bwd_params": (
         ctypes.c_int,
