@@ -590,6 +590,63 @@ int ow_block_norms_bwd(const OwBlockNorms* norms, const void* dout, int64_t dout
                        int64_t dnext_stride, void* dx, void* ddelta, void* dpost_weight, void* dgate,
                        void* dnext_weight, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * One AdamW step over a list of tensors of one parameter dtype (the reference trains with
+ * torch.optim.AdamW, a gradient-norm clip and finite checks, omniweave/training/engine.py:204-258):
+ *
+ *   g <- grad * min(1, max_norm / (norm + 1e-6))        (partials given; norm = sqrt of their sum)
+ *   m <- b1 m + (1 - b1) g;   v <- b2 v + (1 - b2) g^2
+ *   p <- p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ *
+ * in fp32; t is one more than the tensor's step counters.  With partials whose norm is not finite
+ * nothing is written but norm_out.
+ *
+ *   param, grad    numel values of the dtype, contiguous (any alignment)
+ *   step           int32, one per OW_ADAMW_CHUNK values, all equal: the steps done
+ *   state_bits 32  exp_avg = m, exp_avg_sq = v: fp32
+ *   state_bits 8   exp_avg = m, exp_avg_sq = sqrt(v): e4m3fn codes, one fp32 scale per OW_ADAMW_BLOCK
+ *                  values (largest magnitude / 448) in exp_avg_scale, exp_avg_sq_scale; value = code * scale.
+ *                  A root above zero is held as 2^-9 scales at least; a scale below 2^-126 as 0.
+ *   master         with use_master: fp32 parameters, which are updated, and param is their rounding
+ *   group          index into groups; lr_device: NULL, or the learning rate as one fp32 on the device
+ *
+ * ow_grad_norm writes sums of squares of the gradients (fp64, fixed order); ow_grad_norm_partials says
+ * how many.  Several lists (dtypes) make one norm when their partials lie one after another.  norm_out: the
+ * norm (fp32), or NULL.  Tensors must not overlap.  No memory is allocated and nothing waits for the device.
+ */
+#define OW_ADAMW_CHUNK 4096
+#define OW_ADAMW_BLOCK 256
+#define OW_GRAD_NORM_PARTIALS 1024 /* per launch of up to 274 tensors */
+
+typedef struct OwAdamwTensor {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale;
+  float* exp_avg_sq_scale;
+  float* master;
+  int32_t* step;
+  int64_t numel;
+  int64_t group;
+} OwAdamwTensor;
+
+typedef struct OwAdamwGroup {
+  double lr;
+  double beta1;
+  double beta2;
+  double eps;
+  double weight_decay;
+  const float* lr_device;
+} OwAdamwGroup;
+
+int64_t ow_grad_norm_partials(const OwAdamwTensor* tensors, int32_t count);
+int ow_grad_norm(const OwAdamwTensor* tensors, int32_t count, int32_t dtype, double* partials, int64_t n_partials,
+                 void* stream);
+int ow_adamw_step(const OwAdamwTensor* tensors, int32_t count, const OwAdamwGroup* groups, int32_t n_groups,
+                  int32_t dtype, int32_t state_bits, int32_t use_master, const double* partials, int64_t n_partials,
+                  double max_norm, float* norm_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

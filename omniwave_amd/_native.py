@@ -53,6 +53,19 @@ class OwBlockNorms(ctypes.Structure):
     ]
 
 
+class OwAdamwTensor(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale",
+                                                     "exp_avg_sq_scale", "master", "step")]
+    _fields_ += [("numel", ctypes.c_int64), ("group", ctypes.c_int64)]
+
+
+class OwAdamwGroup(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_double) for name in ("lr", "beta1", "beta2", "eps", "weight_decay")]
+    _fields_ += [("lr_device", ctypes.c_void_p)]
+
+
+OW_ADAMW_CHUNK, OW_ADAMW_BLOCK = 4096, 256
+
 _SIGNATURES = {
     "ow_version": (ctypes.c_int, []),
     "ow_last_error": (ctypes.c_char_p, []),
@@ -260,6 +273,16 @@ _SIGNATURES = {
         ctypes.c_int,
         [ctypes.POINTER(OwBlockNorms), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64]
         + [ctypes.c_void_p] * 6 + [ctypes.c_size_t, ctypes.c_void_p],
+    ),
+    "ow_grad_norm_partials": (ctypes.c_int64, [ctypes.c_void_p, ctypes.c_int32]),
+    "ow_grad_norm": (
+        ctypes.c_int,
+        [ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p],
+    ),
+    "ow_adamw_step": (
+        ctypes.c_int,
+        [ctypes.c_void_p, ctypes.c_int32, ctypes.POINTER(OwAdamwGroup)] + [ctypes.c_int32] * 4
+        + [ctypes.c_void_p, ctypes.c_int64, ctypes.c_double, ctypes.c_void_p, ctypes.c_void_p],
     ),
     "ow_bwd_params": (
         ctypes.c_int,

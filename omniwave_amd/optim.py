@@ -1,0 +1,339 @@
+"""AdamW over all parameters of a model at once, as HIP kernels (``adamw.hip``).
+
+``AdamW`` is a ``torch.optim.Optimizer`` (the reference trains with ``torch.optim.AdamW``, a clip of the
+gradients' norm and a check that it is finite, omniweave/training/engine.py:204-258): one launch updates as
+many tensors as fit in a kernel's arguments, the clip needs one more, and nothing waits for the device, so
+a step can be captured into a HIP graph.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from itertools import chain
+from operator import is_
+
+import numpy as np
+import torch
+from torch import Tensor
+
+from omniwave_amd import _native
+from omniwave_amd.hip import _DTYPE_CODE, SUPPORTED_DTYPES, _stream_ptr
+from omniwave_amd.norms import gpu_reason
+
+CHUNK, BLOCK = _native.OW_ADAMW_CHUNK, _native.OW_ADAMW_BLOCK
+FP8 = torch.float8_e4m3fn
+FP8_MOST = 448.0
+MIN_8BIT_VALUES = 4096  # smaller tensors keep 32-bit states: their bytes do not matter, their errors do
+_FIELDS = len(_native.OwAdamwTensor._fields_)  # of 8 bytes each
+_GRAD = 1  # field
+
+
+def _blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def _encode(values: Tensor, least: bool) -> tuple[Tensor, Tensor]:
+    """fp32 values as e4m3fn and a scale per block (``least``: what is above zero stays above zero)."""
+    flat = values.detach().float().reshape(-1)
+    n = flat.numel()
+    rows = torch.nn.functional.pad(flat, (0, -n % BLOCK)).reshape(-1, BLOCK)
+    scale = rows.abs().amax(1) / FP8_MOST
+    scale = torch.where(scale < torch.finfo(torch.float32).tiny, 0.0, scale)
+    inv = torch.where(scale > 0, 1.0 / scale, 0.0)
+    codes = (rows * inv[:, None]).clamp(-FP8_MOST, FP8_MOST).to(FP8)
+    if least:
+        codes = torch.where((rows > 0) & (codes.float() == 0), 2.0 ** -9, codes.float()).to(FP8)
+    return codes.reshape(-1)[:n].reshape(values.shape), scale
+
+
+def _decode(codes: Tensor, scale: Tensor) -> Tensor:
+    flat = codes.float().reshape(-1)
+    return (flat * scale.repeat_interleave(BLOCK)[:flat.numel()]).reshape(codes.shape)
+
+
+class _Kind:
+    """Tensors of one dtype and state layout: one list for the native calls."""
+
+    __slots__ = ("dtype", "bits", "master", "params", "columns", "table", "partials")
+
+    def __init__(self, dtype, bits, master) -> None:
+        self.dtype, self.bits, self.master = dtype, bits, master
+        self.params: list[Tensor] = []
+
+
+class AdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW`` on the framework's kernels.
+
+    ``state_bits``: 32, or 8 for states of tensors of at least 4,096 values in e4m3fn with an fp32 scale
+    for every 256 values (the second moment as its root).  ``master_weights``: keep fp32 copies of bf16 /
+    fp16 parameters and update those, so that updates smaller than a parameter's rounding step are not
+    lost.  ``max_grad_norm``: scale the gradients of each step so that their norm over all parameters is
+    at most this, and skip the step (parameters, states and counters) where the norm is not finite;
+    ``grad_norm`` is then the last step's norm, on the device.
+
+    Parameters: contiguous, of fp32, bf16 or fp16, on one gfx950 GPU; gradients of the same dtype, dense.
+    ``lr`` may be a 0-dim fp32 tensor on the GPU, which a captured step reads anew; other
+    hyperparameters of a captured step are those of its capture.  States are made by the first step, which
+    therefore is not captured.
+
+    ``state[p]``: ``step`` (int32, the steps done, one for every 4,096 values), ``exp_avg`` and
+    ``exp_avg_sq`` (fp32), or ``exp_avg`` and ``exp_avg_sq_root`` (e4m3fn) with ``exp_avg_scale`` and
+    ``exp_avg_sq_root_scale``, and ``master``.  ``load_state_dict`` also takes the states of
+    ``torch.optim.AdamW`` and those of another ``state_bits``.
+    """
+
+    grad_norm: Tensor | None = None
+    _plan: tuple[list[list[Tensor]], list[_Kind]] | None = None
+
+    def __init__(self, params, lr: float | Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, *, state_bits: int = 32, master_weights: bool = False,
+                 max_grad_norm: float | None = None) -> None:
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits!r}")
+        if max_grad_norm is not None and not (max_grad_norm > 0 and math.isfinite(max_grad_norm)):
+            raise ValueError(f"max_grad_norm must be positive and finite, got {max_grad_norm!r}")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+        self.state_bits, self.master_weights, self.max_grad_norm = state_bits, bool(master_weights), max_grad_norm
+
+    def add_param_group(self, param_group: dict) -> None:
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        try:
+            _hyper(group)
+            if len(set(group["params"])) != len(group["params"]):
+                raise ValueError("a parameter is in its group twice")
+            for p in group["params"]:
+                if p.dtype not in SUPPORTED_DTYPES:
+                    raise ValueError(f"unsupported parameter dtype {p.dtype}; expected float32, bfloat16 or float16")
+                if p.layout != torch.strided or not p.is_contiguous():
+                    raise ValueError(f"a parameter of shape {tuple(p.shape)} is not contiguous")
+        except ValueError:
+            self.param_groups.pop()
+            raise
+        self._plan = None
+
+    def __getstate__(self) -> dict:
+        kept = {k: getattr(self, k) for k in ("state_bits", "master_weights", "max_grad_norm")}
+        return {**super().__getstate__(), **kept}
+
+    # -- states ---------------------------------------------------------------------------
+
+    def _layout(self, p: Tensor) -> dict[str, tuple[torch.dtype, tuple]]:
+        """Names, dtypes and shapes of ``p``'s states."""
+        n = p.numel()
+        entry: dict[str, tuple[torch.dtype, tuple]] = {"step": (torch.int32, (-(-n // CHUNK),))}
+        if self.state_bits == 8 and n >= MIN_8BIT_VALUES:
+            scales = (torch.float32, (_blocks(n),))
+            entry.update(exp_avg=(FP8, p.shape), exp_avg_sq_root=(FP8, p.shape), exp_avg_scale=scales,
+                         exp_avg_sq_root_scale=scales)
+        else:
+            entry.update(exp_avg=(torch.float32, p.shape), exp_avg_sq=(torch.float32, p.shape))
+        if self.master_weights and p.dtype != torch.float32:
+            entry["master"] = (torch.float32, p.shape)
+        return entry
+
+    def _first_state(self, p: Tensor) -> None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW makes its states in the first step of a parameter, which cannot be captured: "
+                               "run one step before the capture")
+        entry = self.state[p]
+        for name, (dtype, shape) in self._layout(p).items():
+            if name == "master":
+                entry[name] = p.detach().float()
+            else:
+                entry[name] = torch.zeros(shape, dtype=torch.uint8 if dtype == FP8 else dtype, device=p.device)
+                if dtype == FP8:
+                    entry[name] = entry[name].view(FP8)
+
+    def _check_state(self, p: Tensor) -> None:
+        entry = self.state[p]
+        for name, (dtype, shape) in self._layout(p).items():
+            t = entry.get(name)
+            if not isinstance(t, Tensor) or t.dtype != dtype or t.shape != shape or t.device != p.device \
+                    or not t.is_contiguous():
+                got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, Tensor) else repr(t)
+                raise ValueError(f"state {name!r} of a parameter of shape {tuple(p.shape)} must be {dtype} {tuple(shape)}, "
+                                 f"contiguous on {p.device}; got {got}")
+
+    def load_state_dict(self, state_dict: dict) -> None:
+        """``torch.optim.Optimizer.load_state_dict``; states keep their own dtypes, and those of
+        ``torch.optim.AdamW`` or another ``state_bits`` are converted."""
+        super().load_state_dict(state_dict)
+        saved = state_dict["state"]
+        ids = chain.from_iterable(g["params"] for g in state_dict["param_groups"])
+        params = chain.from_iterable(g["params"] for g in self.param_groups)
+        for i, p in zip(ids, params):
+            if i in saved:
+                self.state[p] = self._adopt(p, saved[i])
+        self._plan = None
+
+    @torch.no_grad()
+    def _adopt(self, p: Tensor, saved: dict) -> dict:
+        layout = self._layout(p)
+        second = "exp_avg_sq_root" if "exp_avg_sq_root" in saved else "exp_avg_sq"
+        scales = ("exp_avg_scale", "exp_avg_sq_root_scale") if second == "exp_avg_sq_root" else ()
+        missing = [k for k in ("step", "exp_avg", second, *scales) if k not in saved]
+        if missing:
+            raise ValueError(f"the saved state of a parameter of shape {tuple(p.shape)} has no {missing}")
+        step = saved["step"]
+        if isinstance(step, Tensor):
+            step = step.reshape(-1)[0].item() if step.numel() else 0
+        entry = {"step": torch.full(layout["step"][1], int(step), dtype=torch.int32, device=p.device)}
+        own = {k: v.to(p.device) for k, v in saved.items() if isinstance(v, Tensor) and k != "step"}
+        same = all(k in own and own[k].dtype == d for k, (d, _) in layout.items() if k not in ("step", "master"))
+        if same:
+            entry.update({k: own[k].clone(memory_format=torch.contiguous_format) for k in layout if k not in ("step", "master")})
+        else:
+            if "exp_avg_sq_root" in own:
+                m = _decode(own["exp_avg"], own["exp_avg_scale"])
+                root = _decode(own["exp_avg_sq_root"], own["exp_avg_sq_root_scale"])
+                v = root.square()
+            else:
+                m, v = own["exp_avg"].float(), own["exp_avg_sq"].float()
+                root = v.sqrt()
+            if "exp_avg_sq_root" in layout:
+                entry["exp_avg"], entry["exp_avg_scale"] = _encode(m, False)
+                entry["exp_avg_sq_root"], entry["exp_avg_sq_root_scale"] = _encode(root, True)
+            else:
+                entry["exp_avg"], entry["exp_avg_sq"] = m.contiguous(), v.contiguous()
+        if "master" in layout:
+            entry["master"] = own["master"].float().clone() if "master" in own else p.detach().float()
+        return entry
+
+    # -- the step -------------------------------------------------------------------------
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        active = [[p for p in group["params"] if p.grad is not None and p.numel()] for group in self.param_groups]
+        if not any(active):
+            return loss
+        plan = self._plan
+        if plan is None or not _same(plan[0], active) or not self._current(plan[1]):
+            plan = self._plan = self._make_plan(active)
+        device = plan[1][0].params[0].device
+        hyper = (_native.OwAdamwGroup * len(self.param_groups))(*[_hyper(g, device) for g in self.param_groups])
+        if device.index != torch.cuda.current_device():
+            with torch.cuda.device(device):
+                self._launch(plan[1], hyper, device)
+        else:
+            self._launch(plan[1], hyper, device)
+        return loss
+
+    def _launch(self, kinds: list[_Kind], hyper, device: torch.device) -> None:
+        lib, stream = _native.lib(), _stream_ptr(device)
+        keep = [_gradients(kind) for kind in kinds]  # copies of strided gradients live until the launches are queued
+        partials, total, norm_ptr = None, 0, None
+        if self.max_grad_norm is not None:
+            total = sum(kind.partials for kind in kinds)
+            partials = torch.empty(total, dtype=torch.float64, device=device)
+            self.grad_norm = torch.empty((), dtype=torch.float32, device=device)
+            norm_ptr = self.grad_norm.data_ptr()
+            at = 0
+            for kind in kinds:
+                _native.check(lib.ow_grad_norm(kind.table.ctypes.data, len(kind.params), _DTYPE_CODE[kind.dtype],
+                                               partials.data_ptr() + 8 * at, kind.partials, stream), "ow_grad_norm")
+                at += kind.partials
+        for kind in kinds:
+            _native.check(
+                lib.ow_adamw_step(kind.table.ctypes.data, len(kind.params), hyper, len(hyper), _DTYPE_CODE[kind.dtype],
+                                  kind.bits, int(kind.master), None if partials is None else partials.data_ptr(), total,
+                                  self.max_grad_norm or 0.0, norm_ptr, stream), "ow_adamw_step")
+            norm_ptr = None
+        del keep
+
+    def _make_plan(self, active: list[list[Tensor]]) -> tuple[list[list[Tensor]], list[_Kind]]:
+        groups = {p: i for i, params in enumerate(active) for p in params}
+        first = next(iter(groups))
+        device, reason = first.device, gpu_reason(first)
+        if reason is not None:
+            raise RuntimeError(f"hip AdamW not supported: {reason}")
+        kinds: dict[tuple, _Kind] = {}
+        for p in groups:
+            if p.device != device:
+                raise ValueError(f"parameters on {device} and {p.device}: an optimizer's parameters are on one GPU")
+            if not p.is_contiguous():
+                raise ValueError(f"a parameter of shape {tuple(p.shape)} is not contiguous")
+            if not self.state[p]:
+                self._first_state(p)
+            self._check_state(p)
+            entry = self.state[p]
+            key = (p.dtype, 8 if "exp_avg_sq_root" in self._layout(p) else 32, self.master_weights and p.dtype != torch.float32)
+            kinds.setdefault(key, _Kind(*key)).params.append(p)
+        for kind in kinds.values():
+            kind.columns = _columns(kind, self.state)
+            kind.table = np.zeros((len(kind.params), _FIELDS), dtype=np.int64)
+            kind.table[:, 0], kind.table[:, 2:8] = kind.columns[0], np.array(kind.columns[1:], dtype=np.int64).T
+            kind.table[:, 8] = [p.numel() for p in kind.params]
+            kind.table[:, 9] = [groups[p] for p in kind.params]
+            kind.partials = _native.lib().ow_grad_norm_partials(kind.table.ctypes.data, len(kind.params))
+        return active, list(kinds.values())
+
+    def _current(self, kinds: list[_Kind]) -> bool:
+        """Whether every parameter and state still lies where the plan has it (anything else is
+        checked and planned anew)."""
+        return all(_columns(kind, self.state) == kind.columns for kind in kinds)
+
+
+def _same(a: list[list[Tensor]], b: list[list[Tensor]]) -> bool:
+    return len(a) == len(b) and all(len(x) == len(y) and all(map(is_, x, y)) for x, y in zip(a, b))
+
+
+def _columns(kind: _Kind, state) -> list[list[int]]:
+    """Addresses of the parameters and their states, by field (the gradients' apart)."""
+    entries = [state[p] for p in kind.params]
+    none = [0] * len(entries)
+    try:
+        cols = [[p.data_ptr() for p in kind.params], [e["exp_avg"].data_ptr() for e in entries]]
+        if kind.bits == 8:
+            cols += [[e["exp_avg_sq_root"].data_ptr() for e in entries], [e["exp_avg_scale"].data_ptr() for e in entries],
+                     [e["exp_avg_sq_root_scale"].data_ptr() for e in entries]]
+        else:
+            cols += [[e["exp_avg_sq"].data_ptr() for e in entries], none, none]
+        cols += [[e["master"].data_ptr() for e in entries] if kind.master else none, [e["step"].data_ptr() for e in entries]]
+    except KeyError:
+        return []
+    return cols
+
+
+def _gradients(kind: _Kind) -> list[Tensor]:
+    """Writes the gradients' addresses into the kind's table; returns the tensors that hold them."""
+    grads = [p.grad for p in kind.params]
+    for i, (p, g) in enumerate(zip(kind.params, grads)):
+        if g.layout != torch.strided:
+            raise RuntimeError("AdamW takes dense gradients")
+        if not g.is_contiguous():
+            grads[i] = g = g.contiguous()
+        if g.numel() != p.numel() or g.dtype != kind.dtype or g.device != p.device:
+            raise ValueError(f"the gradient of a {p.dtype} parameter of shape {tuple(p.shape)} is {g.dtype} {tuple(g.shape)} "
+                             f"on {g.device}")
+    kind.table[:, _GRAD] = [g.data_ptr() for g in grads]
+    return grads
+
+
+def _hyper(group: dict, device: torch.device | None = None) -> tuple:
+    """A group's hyperparameters as OwAdamwGroup's fields."""
+    lr, (beta1, beta2), eps, decay = group["lr"], group["betas"], group["eps"], group["weight_decay"]
+    lr_device = None
+    if isinstance(lr, Tensor):
+        if lr.numel() != 1 or not lr.is_floating_point():
+            raise ValueError("lr must be a number or a floating point tensor of one value")
+        if lr.is_cuda:
+            if lr.dtype != torch.float32 or (device is not None and lr.device != device):
+                raise ValueError(f"lr on a GPU must be float32 on the parameters' device, got {lr.dtype} on {lr.device}")
+            lr_device, lr = lr.data_ptr(), 0.0
+        else:
+            lr = float(lr)
+    if not (lr >= 0.0 and math.isfinite(lr)):
+        raise ValueError(f"lr must be finite and not negative, got {lr}")
+    if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0):
+        raise ValueError(f"betas must be in [0, 1), got {(beta1, beta2)}")
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError(f"eps must be finite and not negative, got {eps}")
+    if not (decay >= 0.0 and math.isfinite(decay)):
+        raise ValueError(f"weight_decay must be finite and not negative, got {decay}")
+    return lr, beta1, beta2, eps, decay, lr_device
