@@ -647,6 +647,46 @@ int ow_adamw_step(const OwAdamwTensor* tensors, int32_t count, const OwAdamwGrou
                   int32_t dtype, int32_t state_bits, int32_t use_master, const double* partials, int64_t n_partials,
                   double max_norm, float* norm_out, void* stream);
 
+/*
+ * Softmax cross-entropy of rows of logits (the loss that the reference's training takes from torch, with
+ * the two weighted labels of mixed images, omniweave/training/engine.py:134-300):
+ *
+ *   loss_r = -sum_k q_k log softmax(x)_k,  q = (1 - smoothing) (l [a] + (1 - l) [b]) + smoothing / classes
+ *
+ * for rows whose target is not ignore_index, 0 for the others; their sum, or their mean over the counted
+ * rows (NaN where there are none).  target_b NULL: one label (l = 1); else l is mix[row], or mix_value where
+ * mix is NULL.  Labels outside [0, classes) make the row's loss and gradient NaN.  row_stride: values between
+ * rows (any alignment; value stride 1).
+ *
+ * Forward: stats [rows][2] (what the backward needs), losses [rows], and with a reduction loss [1],
+ * the result, and weight [1], a row's weight in it (both NULL without).  Backward: the forward's stats and
+ * weight, upstream [1] or, without a reduction, [rows]; grad [rows][classes] of the logits' dtype.
+ */
+#define OW_REDUCE_NONE 0
+#define OW_REDUCE_SUM 1
+#define OW_REDUCE_MEAN 2
+
+typedef struct OwCrossEntropy {
+  int64_t rows;
+  int64_t classes;
+  int64_t row_stride;
+  int64_t ignore_index;
+  const void* logits;
+  const int64_t* target;
+  const int64_t* target_b;
+  const float* mix;
+  float mix_value;
+  float smoothing;
+  int32_t dtype;
+  int32_t reduction;
+} OwCrossEntropy;
+
+size_t ow_cross_entropy_workspace(const OwCrossEntropy* ce);
+int ow_cross_entropy_fwd(const OwCrossEntropy* ce, float* stats, float* losses, float* loss, float* weight, void* workspace,
+                         size_t workspace_bytes, void* stream);
+int ow_cross_entropy_bwd(const OwCrossEntropy* ce, const float* stats, const float* weight, const float* upstream,
+                         void* grad, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,6 +9,7 @@ __version__ = "0.1.0"
 from omniwave_amd.bigemm import bigemm, register_backend
 from omniwave_amd.block import enable_fp8
 from omniwave_amd.hip import bigemm_block_hip, bigemm_delta_hip, hip_is_supported
+from omniwave_amd.loss import cross_entropy_hip
 from omniwave_amd.norms import block_norms_hip, rms_norm_hip
 from omniwave_amd.optim import AdamW
 from omniwave_amd.registry import create_model, create_model_from_config
@@ -25,6 +26,7 @@ __all__ = [
     "build_stage_schedule",
     "create_model",
     "create_model_from_config",
+    "cross_entropy_hip",
     "enable_fp8",
     "hip_is_supported",
     "register_backend",

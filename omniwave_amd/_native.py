@@ -64,6 +64,14 @@ class OwAdamwGroup(ctypes.Structure):
     _fields_ += [("lr_device", ctypes.c_void_p)]
 
 
+class OwCrossEntropy(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int64) for name in ("rows", "classes", "row_stride", "ignore_index")]
+    _fields_ += [(name, ctypes.c_void_p) for name in ("logits", "target", "target_b", "mix")]
+    _fields_ += [("mix_value", ctypes.c_float), ("smoothing", ctypes.c_float), ("dtype", ctypes.c_int32),
+                 ("reduction", ctypes.c_int32)]
+
+
+OW_REDUCE = {"none": 0, "sum": 1, "mean": 2}
 OW_ADAMW_CHUNK, OW_ADAMW_BLOCK = 4096, 256
 
 _SIGNATURES = {
@@ -284,6 +292,11 @@ _SIGNATURES = {
         [ctypes.c_void_p, ctypes.c_int32, ctypes.POINTER(OwAdamwGroup)] + [ctypes.c_int32] * 4
         + [ctypes.c_void_p, ctypes.c_int64, ctypes.c_double, ctypes.c_void_p, ctypes.c_void_p],
     ),
+    "ow_cross_entropy_workspace": (ctypes.c_size_t, [ctypes.POINTER(OwCrossEntropy)]),
+    "ow_cross_entropy_fwd": (
+        ctypes.c_int, [ctypes.POINTER(OwCrossEntropy)] + [ctypes.c_void_p] * 5 + [ctypes.c_size_t, ctypes.c_void_p],
+    ),
+    "ow_cross_entropy_bwd": (ctypes.c_int, [ctypes.POINTER(OwCrossEntropy)] + [ctypes.c_void_p] * 5),
     "ow_bwd_params": (
         ctypes.c_int,
         [ctypes.c_void_p] * 3 + [ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]

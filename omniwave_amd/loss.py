@@ -1,0 +1,184 @@
+"""Softmax cross-entropy of logits with its gradient, as HIP kernels (``cross_entropy.hip``)."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from omniwave_amd import _native
+from omniwave_amd.hip import _DTYPE_CODE, SUPPORTED_DTYPES, _plain
+from omniwave_amd.norms import _on, _rows, gpu_reason
+
+_NAME = {v: k for k, v in _native.OW_REDUCE.items()}
+
+
+def _check(logits, target, target_b, mix, label_smoothing, ignore_index, reduction) -> None:
+    """Raise for what the kernels do not take, before anything touches the GPU."""
+    if reduction not in _native.OW_REDUCE:
+        raise ValueError(f"reduction must be 'none', 'sum' or 'mean', got {reduction!r}")
+    if not isinstance(ignore_index, int):
+        raise ValueError(f"ignore_index must be an integer, got {ignore_index!r}")
+    if logits.dtype not in SUPPORTED_DTYPES:
+        raise ValueError(f"unsupported dtype {logits.dtype}; expected float16, bfloat16 or float32")
+    if logits.dim() < 1 or not 1 <= logits.shape[-1] < 1 << 30:
+        raise ValueError(f"logits must be [..., classes] with 1 to 2^30 - 1 classes, got {tuple(logits.shape)}")
+    if math.prod(logits.shape[:-1]) >= 1 << 31:
+        raise ValueError(f"{math.prod(logits.shape[:-1])} rows; fewer than 2^31 are supported")
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError(f"label_smoothing must be in [0, 1], got {label_smoothing}")
+    for name, t in (("target", target), ("target_b", target_b)):
+        if t is not None and (t.dtype != torch.int64 or t.shape != logits.shape[:-1] or t.device != logits.device):
+            raise ValueError(f"{name} must be int64 {tuple(logits.shape[:-1])} on {logits.device}, got {t.dtype} "
+                             f"{tuple(t.shape)} on {t.device}")
+    if (target_b is None) != (mix is None):
+        raise ValueError("target_b and mix, the weight of target, come together")
+    if isinstance(mix, Tensor):
+        if mix.shape != target.shape or not mix.is_floating_point() or mix.device != logits.device:
+            raise ValueError(f"mix must be a number or floating point {tuple(target.shape)} on {logits.device}, got "
+                             f"{mix.dtype} {tuple(mix.shape)} on {mix.device}")
+        if mix.requires_grad:
+            raise ValueError("mix carries no gradient; detach it")
+    elif mix is not None and not 0.0 <= mix <= 1.0:
+        raise ValueError(f"mix must be in [0, 1], got {mix}")
+
+
+def _descriptor(logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction):
+    """The C descriptor and the tensors it points into."""
+    logits, stride = _rows(logits)
+    keep = [logits, *[None if t is None else t.contiguous() for t in (target, target_b)],
+            None if mix is None else mix.to(torch.float32).contiguous()]
+    return _native.OwCrossEntropy(target.numel(), logits.shape[-1], stride, ignore_index,
+                                  *[None if t is None else t.data_ptr() for t in keep], mix_value, label_smoothing,
+                                  _DTYPE_CODE[logits.dtype], reduction), keep
+
+
+def _run_forward(logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction):
+    """(the loss, or the losses of the rows; a row's weight in the loss, or None; statistics of the rows)."""
+    rows, device = target.numel(), logits.device
+    desc, _keep = _descriptor(logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction)
+    lib = _native.lib()
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):  # the size goes by the device's compute units
+            ws_bytes = lib.ow_cross_entropy_workspace(ctypes.byref(desc))
+    else:
+        ws_bytes = lib.ow_cross_entropy_workspace(ctypes.byref(desc))
+    f32 = dict(dtype=torch.float32, device=device)
+    losses, stats = torch.empty(rows, **f32), torch.empty((rows, 2), **f32)
+    workspace = torch.empty(ws_bytes // 4, **f32) if ws_bytes else None
+    loss = weight = None
+    if _NAME[reduction] != "none":
+        loss, weight = torch.empty((), **f32), torch.empty((), **f32)
+    _on(device, lib.ow_cross_entropy_fwd, ctypes.byref(desc), stats.data_ptr(), losses.data_ptr(),
+        None if loss is None else loss.data_ptr(), None if weight is None else weight.data_ptr(),
+        None if workspace is None else workspace.data_ptr(), ws_bytes)
+    return losses.reshape(target.shape) if loss is None else loss, weight, stats
+
+
+def _run_backward(up, weight, stats, logits, target, target_b, mix, mix_value, label_smoothing, ignore_index,
+                  reduction) -> Tensor:
+    """The logits' gradient; ``up``: the upstream gradient of the loss (a value) or the losses."""
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    if not grad.numel():
+        return grad
+    desc, _keep = _descriptor(logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction)
+    up = up.to(torch.float32).contiguous()
+    _on(logits.device, _native.lib().ow_cross_entropy_bwd, ctypes.byref(desc), stats.data_ptr(),
+        None if weight is None else weight.data_ptr(), up.data_ptr(), grad.data_ptr())
+    return grad
+
+
+class _PlainLoss(torch.autograd.Function):
+    """``cross_entropy_fwd`` with its gradient, without the dispatcher's cost."""
+
+    @staticmethod
+    def forward(ctx, logits, target, target_b, mix, *options):
+        loss, weight, stats = _run_forward(logits, target, target_b, mix, *options)
+        ctx.save_for_backward(logits, target, target_b, mix, weight, stats)
+        ctx.options = options
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, up):
+        logits, target, target_b, mix, weight, stats = ctx.saved_tensors
+        return (_run_backward(up, weight, stats, logits, target, target_b, mix, *ctx.options), *[None] * 7)
+
+
+@torch.library.custom_op("omniwave_amd::cross_entropy_fwd", mutates_args=())
+def cross_entropy_fwd(logits: Tensor, target: Tensor, target_b: Tensor | None, mix: Tensor | None, mix_value: float,
+                      label_smoothing: float, ignore_index: int, reduction: int) -> tuple[Tensor, Tensor, Tensor]:
+    """(the loss, or the losses of the rows; a row's weight in the loss, empty without a reduction; the rows'
+    statistics) of ``cross_entropy_hip``."""
+    loss, weight, stats = _run_forward(logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction)
+    return loss, stats.new_empty(0) if weight is None else weight, stats
+
+
+@cross_entropy_fwd.register_fake
+def _cross_entropy_fwd_fake(logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction):
+    none = _NAME[reduction] == "none"
+    f32 = dict(dtype=torch.float32)
+    return (logits.new_empty(target.shape if none else (), **f32), logits.new_empty(0 if none else (), **f32),
+            logits.new_empty((target.numel(), 2), **f32))
+
+
+@torch.library.custom_op("omniwave_amd::cross_entropy_bwd", mutates_args=())
+def cross_entropy_bwd(up: Tensor, weight: Tensor, stats: Tensor, logits: Tensor, target: Tensor, target_b: Tensor | None,
+                      mix: Tensor | None, mix_value: float, label_smoothing: float, ignore_index: int,
+                      reduction: int) -> Tensor:
+    """The logits' gradient."""
+    return _run_backward(up, weight if weight.numel() else None, stats, logits, target, target_b, mix, mix_value,
+                         label_smoothing, ignore_index, reduction)
+
+
+@cross_entropy_bwd.register_fake
+def _cross_entropy_bwd_fake(up, weight, stats, logits, target, target_b, mix, mix_value, label_smoothing, ignore_index,
+                            reduction):
+    return logits.new_empty(logits.shape)
+
+
+def _setup_context(ctx, inputs, output):
+    logits, target, target_b, mix, *options = inputs
+    _, weight, stats = output
+    ctx.mark_non_differentiable(weight, stats)
+    ctx.save_for_backward(logits, target, target_b, mix, weight, stats)
+    ctx.options = options
+
+
+def _backward(ctx, up, _weight, _stats):
+    logits, target, target_b, mix, weight, stats = ctx.saved_tensors
+    return (cross_entropy_bwd(up, weight, stats, logits, target, target_b, mix, *ctx.options), *[None] * 7)
+
+
+cross_entropy_fwd.register_autograd(_backward, setup_context=_setup_context)
+
+
+def cross_entropy_hip(logits: Tensor, target: Tensor, *, target_b: Tensor | None = None,
+                      mix: Tensor | float | None = None, label_smoothing: float = 0.0, ignore_index: int = -100,
+                      reduction: str = "mean") -> Tensor:
+    """Cross-entropy of ``softmax(logits)`` (``[..., classes]``, float16, bfloat16 or float32, rows at any
+    one distance) and int64 labels ``target`` (``[...]``), as ``torch.nn.functional.cross_entropy`` has it
+    for class labels, in float32 whatever the logits' dtype.
+
+    ``target_b`` with ``mix``: a second label of weight ``1 - mix`` beside the first one's ``mix`` (mixed
+    images; a number or one for each row).  ``label_smoothing``: the weight of the uniform distribution.
+    Rows whose ``target`` is ``ignore_index`` count neither in the loss nor in the mean, and have no
+    gradient; a mean of no rows is NaN.  A label outside ``[0, classes)`` makes its row NaN.
+    ``reduction``: ``"mean"``, ``"sum"`` or ``"none"``.  Differentiable once in the logits.
+    """
+    _check(logits, target, target_b, mix, label_smoothing, ignore_index, reduction)
+    reason = gpu_reason(logits)
+    if reason is not None:
+        raise RuntimeError(f"hip cross-entropy not supported: {reason}")
+    mix_value = 1.0
+    if mix is not None and not isinstance(mix, Tensor):
+        mix, mix_value = None, float(mix)
+    args = (logits, target, target_b, mix, mix_value, float(label_smoothing), ignore_index, _native.OW_REDUCE[reduction])
+    if not _plain(logits, target, target_b, mix):
+        return cross_entropy_fwd(*args)[0]
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _PlainLoss.apply(*args)
+    return _run_forward(*args)[0]
