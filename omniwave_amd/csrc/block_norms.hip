@@ -52,6 +52,11 @@ struct NormsArgs {
 };
 constexpr int kWantPost = 1, kWantNext = 2, kWantGate = 4;
 
+// Waves per SIMD that the kernels' registers leave room for (vectors of `vec` values): grids are as many
+// workgroups as run at once.
+constexpr int fwd_waves(int vec, bool ragged) { return vec == 8 && ragged ? 5 : 6; }
+constexpr int bwd_waves(int vec) { return vec == 8 ? 3 : 4; }
+
 template <int T>
 constexpr int kThreads = T > 256 ? T : 256;
 
@@ -75,21 +80,18 @@ struct Place {
       }
     }
   }
-  // 1 where a value counts in sums over the row, else 0.
-  __device__ __forceinline__ float counts(int k, int j) const {
-    return col[k] >= 0 && j >= dup[k] && j < n ? 1.f : 0.f;
-  }
-  __device__ __forceinline__ void load(const typename R::Elem* row, int k, bool valid, float (&v)[V]) const {
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = 0.f;
-    if (!valid || col[k] < 0) return;
+  // Whether a value counts in sums over the row.
+  __device__ __forceinline__ bool counts(int k, int j) const { return col[k] >= 0 && j >= dup[k] && j < n; }
+  __device__ __forceinline__ typename R::Raw load(const typename R::Elem* row, int k, bool valid) const {
+    if (!valid || col[k] < 0) return R::zero();
     if (RAGGED && n < V) {
+      typename R::Raw w = R::zero();
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        if (j < n) v[j] = R::to_f32(row[j]);
-    } else {
-      R::load(row + col[k], v);
+        if (j < n) R::set(w, j, row[j]);
+      return w;
     }
+    return R::raw(row + col[k]);
   }
   __device__ __forceinline__ void store(typename R::Elem* row, int k, bool valid, const float (&v)[V]) const {
     if (!valid || col[k] < 0) return;
@@ -105,13 +107,24 @@ struct Place {
   __device__ __forceinline__ void weight(const void* p, int32_t dtype, int64_t base, int k, float absent,
                                          float (&v)[V]) const {
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      v[j] = p != nullptr && col[k] >= 0 && j < n ? load_any(p, dtype, base + col[k] + j) : absent;
+    for (int j = 0; j < V; ++j) v[j] = absent;
+    if (p == nullptr || col[k] < 0) return;
+    if (RAGGED && n < V) {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (j < n) v[j] = load_any(p, dtype, base + j);
+    } else {
+      load_any_vec<V>(p, dtype, base + col[k], v);
+    }
   }
 };
 
+// a b where the value counts in its row's sums, else 0 (a mask of ones and zeros; whole vectors need none).
+template <bool RAGGED>
+__device__ __forceinline__ float counted(float a, float mask) { return RAGGED ? a * mask : a; }
+
 template <class Ty, int T, int K, bool RAGGED>
-__global__ void __launch_bounds__(kThreads<T>) block_norms_fwd_kernel(NormsArgs a) {
+__global__ void __launch_bounds__(kThreads<T>, fwd_waves(Row<Ty>::kVec, RAGGED)) block_norms_fwd_kernel(NormsArgs a) {
   typedef Row<Ty> R;
   typedef typename R::Elem Elem;
   constexpr int V = R::kVec, ROWS = kThreads<T> / T;
@@ -129,16 +142,34 @@ __global__ void __launch_bounds__(kThreads<T>) block_norms_fwd_kernel(NormsArgs 
     at.weight(per_image ? nullptr : a.n.gate, a.n.gate_dtype, 0, k, 1.f, gate[k]);
     at.weight(a.n.next_weight, a.n.next_dtype, 0, k, 1.f, nextw[k]);
   }
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * ROWS; base < a.n.rows;
-       base += static_cast<int64_t>(gridDim.x) * ROWS) {
+  float mask[K][V];
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int j = 0; j < V; ++j) mask[k][j] = at.counts(k, j) ? 1.f : 0.f;
+
+  // A row is read while the one before it is computed.
+  typename R::Raw xn[K], dn[K];
+  auto read = [&](int64_t row) {
+    const bool valid = row < a.n.rows;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      xn[k] = at.load(static_cast<const Elem*>(a.n.x) + row * a.n.x_stride, k, valid);
+      dn[k] = at.load(static_cast<const Elem*>(a.n.delta) + row * a.n.delta_stride, k, valid && has_delta);
+    }
+  };
+  const int64_t step = static_cast<int64_t>(gridDim.x) * ROWS;
+  read(static_cast<int64_t>(blockIdx.x) * ROWS + slot);
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * ROWS; base < a.n.rows; base += step) {
     const int64_t row = base + slot;
     const bool valid = row < a.n.rows;
     float x[K][V], d[K][V];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      at.load(static_cast<const Elem*>(a.n.x) + row * a.n.x_stride, k, valid, x[k]);
-      if (has_delta) at.load(static_cast<const Elem*>(a.n.delta) + row * a.n.delta_stride, k, valid, d[k]);
+      R::widen(xn[k], x[k]);
+      R::widen(dn[k], d[k]);
     }
+    read(row + step);
     if (has_delta) {
       float f = 1.f;
       if (a.n.scale != nullptr || per_image) {
@@ -154,7 +185,7 @@ __global__ void __launch_bounds__(kThreads<T>) block_norms_fwd_kernel(NormsArgs 
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-          for (int j = 0; j < V; ++j) ss[0] += RAGGED ? d[k][j] * d[k][j] * at.counts(k, j) : d[k][j] * d[k][j];
+          for (int j = 0; j < V; ++j) ss[0] += d[k][j] * counted<RAGGED>(d[k][j], mask[k][j]);
         row_sums<T>(ss, red, turn);
         const float r1 = rsqrtf(ss[0] * a.inv_c + a.n.eps);
 #pragma unroll
@@ -174,7 +205,7 @@ __global__ void __launch_bounds__(kThreads<T>) block_norms_fwd_kernel(NormsArgs 
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int j = 0; j < V; ++j) ss[0] += RAGGED ? x[k][j] * x[k][j] * at.counts(k, j) : x[k][j] * x[k][j];
+        for (int j = 0; j < V; ++j) ss[0] += x[k][j] * counted<RAGGED>(x[k][j], mask[k][j]);
       row_sums<T>(ss, red, turn);
       const float r2 = rsqrtf(ss[0] * a.inv_c + a.n.eps);
 #pragma unroll
@@ -190,7 +221,7 @@ __global__ void __launch_bounds__(kThreads<T>) block_norms_fwd_kernel(NormsArgs 
 // One workgroup takes a contiguous share of a segment's rows, so its sums over rows are partial sums
 // of that segment: norms_sum_kernel adds them in a fixed order.
 template <class Ty, int T, int K, bool RAGGED>
-__global__ void __launch_bounds__(kThreads<T>) block_norms_bwd_kernel(NormsArgs a) {
+__global__ void __launch_bounds__(kThreads<T>, bwd_waves(Row<Ty>::kVec)) block_norms_bwd_kernel(NormsArgs a) {
   typedef Row<Ty> R;
   typedef typename R::Elem Elem;
   constexpr int V = R::kVec, ROWS = kThreads<T> / T, COLS = T * K * V;
@@ -208,13 +239,16 @@ __global__ void __launch_bounds__(kThreads<T>) block_norms_bwd_kernel(NormsArgs 
   const int64_t seg_last = parted ? seg_first + 1 : (static_cast<int64_t>(blockIdx.x) + 1) * a.segments / a.n_part;
 
   float post[K][V], gate[K][V], nextw[K][V];
-  float s_post[K][V], s_next[K][V], s_gate[K][V];
+  float s_post[K][V], s_next[K][V], s_gate[K][V], mask[K][V];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     at.weight(a.n.post_weight, a.n.post_dtype, 0, k, 1.f, post[k]);
     at.weight(a.n.next_weight, a.n.next_dtype, 0, k, 1.f, nextw[k]);
 #pragma unroll
-    for (int j = 0; j < V; ++j) s_post[k][j] = s_next[k][j] = 0.f;
+    for (int j = 0; j < V; ++j) {
+      s_post[k][j] = s_next[k][j] = 0.f;
+      mask[k][j] = at.counts(k, j) ? 1.f : 0.f;
+    }
   }
   // put(column, sum over the workgroup's rows) of a thread's sums.
   auto each_sum = [&](const float (&s)[K][V], auto&& put) {
@@ -235,7 +269,7 @@ __global__ void __launch_bounds__(kThreads<T>) block_norms_bwd_kernel(NormsArgs 
           if constexpr (ROWS > 1) {
             for (int r = 1; r < ROWS; ++r) sum += sums[r * COLS + (k * V + j) * T + t];
           }
-          if (at.counts(k, j) != 0.f) put(at.col[k] + j, sum);
+          if (at.counts(k, j)) put(at.col[k] + j, sum);
         }
     }
   };
@@ -252,17 +286,30 @@ __global__ void __launch_bounds__(kThreads<T>) block_norms_bwd_kernel(NormsArgs 
 #pragma unroll
     for (int j = 0; j < V; ++j) s_gate[k][j] = 0.f;
   }
+  typename R::Raw xn[K], dn[K], gn[K], hn[K];
+  auto read = [&](int64_t row) {  // while the row before it is computed
+    const bool valid = row < end;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      xn[k] = at.load(static_cast<const Elem*>(a.n.x) + row * a.n.x_stride, k, valid && has_next);
+      dn[k] = at.load(static_cast<const Elem*>(a.n.delta) + row * a.n.delta_stride, k, valid && has_delta);
+      gn[k] = at.load(static_cast<const Elem*>(a.dout) + row * a.dout_stride, k, valid && a.dout != nullptr);
+      hn[k] = at.load(static_cast<const Elem*>(a.dnext) + row * a.dnext_stride, k, valid && has_next);
+    }
+  };
+  read(first + slot);
   for (int64_t base = first; base < end; base += ROWS) {
     const int64_t row = base + slot;
     const bool valid = row < end;
     float x[K][V], d[K][V], g[K][V], h[K][V];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      at.load(static_cast<const Elem*>(a.n.x) + row * a.n.x_stride, k, valid && has_next, x[k]);
-      at.load(static_cast<const Elem*>(a.n.delta) + row * a.n.delta_stride, k, valid && has_delta, d[k]);
-      at.load(static_cast<const Elem*>(a.dout) + row * a.dout_stride, k, valid && a.dout != nullptr, g[k]);
-      at.load(static_cast<const Elem*>(a.dnext) + row * a.dnext_stride, k, valid && has_next, h[k]);
+      R::widen(xn[k], x[k]);
+      R::widen(dn[k], d[k]);
+      R::widen(gn[k], g[k]);
+      R::widen(hn[k], h[k]);
     }
+    read(row + ROWS);
     float f = 1.f, r1 = 1.f;
     if (has_delta) {
       if (a.n.scale != nullptr)
@@ -272,7 +319,7 @@ __global__ void __launch_bounds__(kThreads<T>) block_norms_bwd_kernel(NormsArgs 
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-          for (int j = 0; j < V; ++j) ss[0] += RAGGED ? d[k][j] * d[k][j] * at.counts(k, j) : d[k][j] * d[k][j];
+          for (int j = 0; j < V; ++j) ss[0] += d[k][j] * counted<RAGGED>(d[k][j], mask[k][j]);
         row_sums<T>(ss, red, turn);
         r1 = rsqrtf(ss[0] * a.inv_c + a.n.eps);
       }
@@ -284,7 +331,7 @@ __global__ void __launch_bounds__(kThreads<T>) block_norms_bwd_kernel(NormsArgs 
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           if (has_delta) x[k][j] += f * gate[k][j] * (d[k][j] * (r1 * post[k][j]));  // out
-          const float w = RAGGED ? x[k][j] * at.counts(k, j) : x[k][j];
+          const float w = counted<RAGGED>(x[k][j], mask[k][j]);
           ss[0] += w * x[k][j];
           ss[1] += w * (h[k][j] * nextw[k][j]);
         }
@@ -314,7 +361,7 @@ __global__ void __launch_bounds__(kThreads<T>) block_norms_bwd_kernel(NormsArgs 
           const float q = e * gate[k][j];
           s_post[k][j] += q * u;
           g[k][j] = q * post[k][j];
-          ss[0] += RAGGED ? d[k][j] * g[k][j] * at.counts(k, j) : d[k][j] * g[k][j];
+          ss[0] += g[k][j] * counted<RAGGED>(d[k][j], mask[k][j]);
         }
       if (has_post) {
         row_sums<T>(ss, red, turn);
@@ -400,11 +447,12 @@ struct Parts {
 };
 
 // How the backward's rows are shared out: segments (images where the gate is per image, else one), each
-// to seg_parts workgroups, about four per compute unit in all and none without a row group; more
-// segments than that go several to a workgroup.
+// to seg_parts workgroups, as many in all as run at once and none without a row group; more segments
+// than that go several to a workgroup.
 Parts backward_parts(const OwBlockNorms& n) {
-  const int at_once = rows_at_once(n.channels, n.dtype == OW_DTYPE_F32 ? 4 : 8);
-  const int64_t most = 4 * static_cast<int64_t>(device_cus());
+  const int vec = n.dtype == OW_DTYPE_F32 ? 4 : 8, threads = threads_of(n.channels, vec);
+  const int at_once = rows_at_once(n.channels, vec);
+  const int64_t most = static_cast<int64_t>(device_cus()) * bwd_waves(vec) * 256 / (threads > 256 ? threads : 256);
   Parts p;
   p.segments = n.gate != nullptr && n.gate_per_image ? n.rows / n.rows_per_image : 1;
   p.seg_rows = n.rows / p.segments;
@@ -421,7 +469,8 @@ void launch(const NormsArgs& a, bool backward, hipStream_t s) {
     hipLaunchKernelGGL((block_norms_bwd_kernel<Ty, T, K, RAGGED>), dim3(a.n_part), dim3(kThreads<T>), 0, s, a);
     return;
   }
-  const int64_t groups = (a.n.rows + ROWS - 1) / ROWS, most = static_cast<int64_t>(device_cus()) * 32 * 64 / kThreads<T>;
+  const int64_t groups = (a.n.rows + ROWS - 1) / ROWS;
+  const int64_t most = static_cast<int64_t>(device_cus()) * fwd_waves(Row<Ty>::kVec, RAGGED) * 256 / kThreads<T>;
   hipLaunchKernelGGL((block_norms_fwd_kernel<Ty, T, K, RAGGED>), dim3(static_cast<unsigned>(groups < most ? groups : most)),
                      dim3(kThreads<T>), 0, s, a);
 }

@@ -12,14 +12,18 @@ typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 template <class Ty>
 struct Row {  // BF16, F16
   typedef uint16_t Elem;
+  typedef u32x4 Raw;  // a vector as memory holds it
   static constexpr int kVec = 8;
   static __device__ __forceinline__ float to_f32(Elem e) { return Ty::to_f32(e); }
   static __device__ __forceinline__ Elem from_f32(float f) { return Ty::from_f32(f); }
-  static __device__ __forceinline__ void load(const Elem* p, float (&v)[kVec]) {
-    const u32x4 w = *reinterpret_cast<const u32x4_any*>(p);
+  static __device__ __forceinline__ Raw raw(const Elem* p) { return *reinterpret_cast<const u32x4_any*>(p); }
+  static __device__ __forceinline__ Raw zero() { return u32x4{0u, 0u, 0u, 0u}; }
+  static __device__ __forceinline__ void set(Raw& w, int j, Elem e) { w[j >> 1] |= static_cast<uint32_t>(e) << (16 * (j & 1)); }
+  static __device__ __forceinline__ void widen(const Raw& w, float (&v)[kVec]) {
 #pragma unroll
     for (int j = 0; j < kVec; ++j) v[j] = Ty::to_f32(j & 1 ? hi16(w[j >> 1]) : lo16(w[j >> 1]));
   }
+  static __device__ __forceinline__ void load(const Elem* p, float (&v)[kVec]) { widen(raw(p), v); }
   static __device__ __forceinline__ void store(Elem* p, const float (&v)[kVec]) {
     u32x4 w;
 #pragma unroll
@@ -32,14 +36,18 @@ struct F32;
 template <>
 struct Row<F32> {
   typedef float Elem;
+  typedef f32x4 Raw;
   static constexpr int kVec = 4;
   static __device__ __forceinline__ float to_f32(Elem e) { return e; }
   static __device__ __forceinline__ Elem from_f32(float f) { return f; }
-  static __device__ __forceinline__ void load(const Elem* p, float (&v)[kVec]) {
-    const f32x4 w = *reinterpret_cast<const f32x4_any*>(p);
+  static __device__ __forceinline__ Raw raw(const Elem* p) { return *reinterpret_cast<const f32x4_any*>(p); }
+  static __device__ __forceinline__ Raw zero() { return f32x4{0.f, 0.f, 0.f, 0.f}; }
+  static __device__ __forceinline__ void set(Raw& w, int j, Elem e) { w[j] = e; }
+  static __device__ __forceinline__ void widen(const Raw& w, float (&v)[kVec]) {
 #pragma unroll
     for (int j = 0; j < kVec; ++j) v[j] = w[j];
   }
+  static __device__ __forceinline__ void load(const Elem* p, float (&v)[kVec]) { widen(raw(p), v); }
   static __device__ __forceinline__ void store(Elem* p, const float (&v)[kVec]) {
     *reinterpret_cast<f32x4_any*>(p) = f32x4{v[0], v[1], v[2], v[3]};
   }
@@ -54,6 +62,35 @@ __device__ __forceinline__ float load_any(const void* p, int32_t dtype, int64_t 
 __device__ __forceinline__ void store_any(void* p, int32_t dtype, int64_t i, float v) {
   if (dtype == OW_DTYPE_F32) static_cast<float*>(p)[i] = v;
   else static_cast<uint16_t*>(p)[i] = dtype == OW_DTYPE_BF16 ? BF16::from_f32(v) : F16::from_f32(v);
+}
+
+// Values i .. i + N - 1 of a tensor of a type known at run time (N = 4 or 8), at any address: the
+// type is looked at once, so that the loads are in flight together.
+template <int N>
+__device__ __forceinline__ void load_any_vec(const void* p, int32_t dtype, int64_t i, float (&v)[N]) {
+  if (dtype == OW_DTYPE_F32) {
+#pragma unroll
+    for (int h = 0; h < N / 4; ++h) {
+      const f32x4 w = *reinterpret_cast<const f32x4_any*>(static_cast<const float*>(p) + i + 4 * h);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[4 * h + j] = w[j];
+    }
+    return;
+  }
+  typedef u32x2 __attribute__((aligned(2))) u32x2_any;
+  uint32_t w[N / 2];
+#pragma unroll
+  for (int h = 0; h < N / 4; ++h) {
+    const u32x2 u = *reinterpret_cast<const u32x2_any*>(static_cast<const uint16_t*>(p) + i + 4 * h);
+    w[2 * h] = u.x, w[2 * h + 1] = u.y;
+  }
+  if (dtype == OW_DTYPE_BF16) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = BF16::to_f32(j & 1 ? hi16(w[j >> 1]) : lo16(w[j >> 1]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = F16::to_f32(j & 1 ? hi16(w[j >> 1]) : lo16(w[j >> 1]));
+  }
 }
 
 struct AddOp {
