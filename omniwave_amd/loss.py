@@ -11,9 +11,7 @@ from torch.autograd.function import once_differentiable
 
 from omniwave_amd import _native
 from omniwave_amd.hip import _DTYPE_CODE, SUPPORTED_DTYPES, _plain
-from omniwave_amd.norms import _on, _rows, gpu_reason
-
-_NAME = {v: k for k, v in _native.OW_REDUCE.items()}
+from omniwave_amd.norms import _lies, _on, _rows, gpu_reason
 
 
 def _check(logits, target, target_b, mix, label_smoothing, ignore_index, reduction) -> None:
@@ -57,37 +55,46 @@ def _descriptor(logits, target, target_b, mix, mix_value, label_smoothing, ignor
 
 
 def _run_forward(logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction):
-    """(the loss, or the losses of the rows; a row's weight in the loss, or None; statistics of the rows)."""
-    rows, device = target.numel(), logits.device
-    desc, _keep = _descriptor(logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction)
-    lib = _native.lib()
+    """(the loss, or the losses of the rows; what the backward needs beside the inputs; the descriptor and
+    whether it points at the inputs themselves).  The second: the statistics of the rows, a row's weight in
+    the loss and, with a reduction, the losses."""
+    device, reduced = logits.device, reduction != 0
+    desc, keep = _descriptor(logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction)
+    rows, lib = desc.rows, _native.lib()
+    ref = ctypes.byref(desc)
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):  # the size goes by the device's compute units
-            ws_bytes = lib.ow_cross_entropy_workspace(ctypes.byref(desc))
+            ws_bytes = lib.ow_cross_entropy_workspace(ref)
     else:
-        ws_bytes = lib.ow_cross_entropy_workspace(ctypes.byref(desc))
-    f32 = dict(dtype=torch.float32, device=device)
-    losses, stats = torch.empty(rows, **f32), torch.empty((rows, 2), **f32)
-    workspace = torch.empty(ws_bytes // 4, **f32) if ws_bytes else None
-    loss = weight = None
-    if _NAME[reduction] != "none":
-        loss, weight = torch.empty((), **f32), torch.empty((), **f32)
-    _on(device, lib.ow_cross_entropy_fwd, ctypes.byref(desc), stats.data_ptr(), losses.data_ptr(),
-        None if loss is None else loss.data_ptr(), None if weight is None else weight.data_ptr(),
-        None if workspace is None else workspace.data_ptr(), ws_bytes)
-    return losses.reshape(target.shape) if loss is None else loss, weight, stats
+        ws_bytes = lib.ow_cross_entropy_workspace(ref)
+    aux = torch.empty(2 * rows + 1 + (rows if reduced else 0), dtype=torch.float32, device=device)
+    loss = torch.empty(() if reduced else target.shape, dtype=torch.float32, device=device)
+    workspace = torch.empty(ws_bytes // 4, dtype=torch.float32, device=device) if ws_bytes else None
+    at, out = aux.data_ptr(), loss.data_ptr()
+    weight = at + 8 * rows
+    _on(device, lib.ow_cross_entropy_fwd, ref, at, weight + 4 if reduced else out, out if reduced else None,
+        weight if reduced else None, None if workspace is None else workspace.data_ptr(), ws_bytes)
+    inputs = keep[0] is logits and keep[1] is target and keep[2] is target_b and keep[3] is mix
+    return loss, aux, desc if inputs else None
 
 
-def _run_backward(up, weight, stats, logits, target, target_b, mix, mix_value, label_smoothing, ignore_index,
-                  reduction) -> Tensor:
-    """The logits' gradient; ``up``: the upstream gradient of the loss (a value) or the losses."""
+def _run_backward(up, aux, desc, logits, target, target_b, mix, *options) -> Tensor:
+    """The logits' gradient; ``up``: the upstream gradient of the loss (a value) or the losses; ``desc``:
+    the forward's descriptor, or None."""
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     if not grad.numel():
         return grad
-    desc, _keep = _descriptor(logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction)
-    up = up.to(torch.float32).contiguous()
-    _on(logits.device, _native.lib().ow_cross_entropy_bwd, ctypes.byref(desc), stats.data_ptr(),
-        None if weight is None else weight.data_ptr(), up.data_ptr(), grad.data_ptr())
+    # The forward's descriptor serves where the inputs came back as they were (hooks on saved tensors may
+    # hand out copies).
+    if desc is None or logits.data_ptr() != desc.logits or target.data_ptr() != desc.target \
+            or (target_b is not None and target_b.data_ptr() != desc.target_b) \
+            or (mix is not None and mix.data_ptr() != desc.mix) or not _lies(logits, desc.row_stride):
+        desc, _keep = _descriptor(logits, target, target_b, mix, *options)
+    if up.dtype != torch.float32 or not up.is_contiguous():
+        up = up.to(torch.float32).contiguous()
+    at = aux.data_ptr()
+    _on(logits.device, _native.lib().ow_cross_entropy_bwd, ctypes.byref(desc), at,
+        at + 8 * desc.rows if desc.reduction else None, up.data_ptr(), grad.data_ptr())
     return grad
 
 
@@ -96,61 +103,64 @@ class _PlainLoss(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, target, target_b, mix, *options):
-        loss, weight, stats = _run_forward(logits, target, target_b, mix, *options)
-        ctx.save_for_backward(logits, target, target_b, mix, weight, stats)
+        loss, aux, ctx.desc = _run_forward(logits, target, target_b, mix, *options)
+        ctx.save_for_backward(logits, target, target_b, mix, aux)
         ctx.options = options
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, up):
-        logits, target, target_b, mix, weight, stats = ctx.saved_tensors
-        return (_run_backward(up, weight, stats, logits, target, target_b, mix, *ctx.options), *[None] * 7)
+        if torch.is_grad_enabled():
+            return _PlainLoss._once(ctx, up)
+        logits, target, target_b, mix, aux = ctx.saved_tensors
+        return _run_backward(up, aux, ctx.desc, logits, target, target_b, mix, *ctx.options), *_NO_GRADS
+
+    @staticmethod
+    @once_differentiable
+    def _once(ctx, up):
+        return _PlainLoss.backward(ctx, up)
+
+
+_NO_GRADS = (None,) * 7  # of the other arguments
 
 
 @torch.library.custom_op("omniwave_amd::cross_entropy_fwd", mutates_args=())
 def cross_entropy_fwd(logits: Tensor, target: Tensor, target_b: Tensor | None, mix: Tensor | None, mix_value: float,
-                      label_smoothing: float, ignore_index: int, reduction: int) -> tuple[Tensor, Tensor, Tensor]:
-    """(the loss, or the losses of the rows; a row's weight in the loss, empty without a reduction; the rows'
-    statistics) of ``cross_entropy_hip``."""
-    loss, weight, stats = _run_forward(logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction)
-    return loss, stats.new_empty(0) if weight is None else weight, stats
+                      label_smoothing: float, ignore_index: int, reduction: int) -> tuple[Tensor, Tensor]:
+    """(the loss, or the losses of the rows; what the backward needs) of ``cross_entropy_hip``."""
+    return _run_forward(logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction)[:2]
 
 
 @cross_entropy_fwd.register_fake
 def _cross_entropy_fwd_fake(logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction):
-    none = _NAME[reduction] == "none"
-    f32 = dict(dtype=torch.float32)
-    return (logits.new_empty(target.shape if none else (), **f32), logits.new_empty(0 if none else (), **f32),
-            logits.new_empty((target.numel(), 2), **f32))
+    rows = target.numel()
+    return (logits.new_empty(() if reduction else target.shape, dtype=torch.float32),
+            logits.new_empty(2 * rows + 1 + (rows if reduction else 0), dtype=torch.float32))
 
 
 @torch.library.custom_op("omniwave_amd::cross_entropy_bwd", mutates_args=())
-def cross_entropy_bwd(up: Tensor, weight: Tensor, stats: Tensor, logits: Tensor, target: Tensor, target_b: Tensor | None,
+def cross_entropy_bwd(up: Tensor, aux: Tensor, logits: Tensor, target: Tensor, target_b: Tensor | None,
                       mix: Tensor | None, mix_value: float, label_smoothing: float, ignore_index: int,
                       reduction: int) -> Tensor:
     """The logits' gradient."""
-    return _run_backward(up, weight if weight.numel() else None, stats, logits, target, target_b, mix, mix_value,
-                         label_smoothing, ignore_index, reduction)
+    return _run_backward(up, aux, None, logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction)
 
 
 @cross_entropy_bwd.register_fake
-def _cross_entropy_bwd_fake(up, weight, stats, logits, target, target_b, mix, mix_value, label_smoothing, ignore_index,
-                            reduction):
+def _cross_entropy_bwd_fake(up, aux, logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction):
     return logits.new_empty(logits.shape)
 
 
 def _setup_context(ctx, inputs, output):
     logits, target, target_b, mix, *options = inputs
-    _, weight, stats = output
-    ctx.mark_non_differentiable(weight, stats)
-    ctx.save_for_backward(logits, target, target_b, mix, weight, stats)
+    ctx.mark_non_differentiable(output[1])
+    ctx.save_for_backward(logits, target, target_b, mix, output[1])
     ctx.options = options
 
 
-def _backward(ctx, up, _weight, _stats):
-    logits, target, target_b, mix, weight, stats = ctx.saved_tensors
-    return (cross_entropy_bwd(up, weight, stats, logits, target, target_b, mix, *ctx.options), *[None] * 7)
+def _backward(ctx, up, _aux):
+    logits, target, target_b, mix, aux = ctx.saved_tensors
+    return cross_entropy_bwd(up, aux, logits, target, target_b, mix, *ctx.options), *_NO_GRADS
 
 
 cross_entropy_fwd.register_autograd(_backward, setup_context=_setup_context)

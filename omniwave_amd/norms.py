@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from operator import is_
 
 import torch
 from torch import Tensor
@@ -92,6 +93,14 @@ def _rows(t: Tensor) -> tuple[Tensor, int]:
     return t.contiguous(), c
 
 
+def _lies(t: Tensor, stride: int) -> bool:
+    """Whether ``_rows(t)`` is ``t`` itself with this distance."""
+    if t.is_contiguous():
+        return stride == t.shape[-1]
+    r, got = _rows(t)
+    return r is t and got == stride
+
+
 def _descriptor(x, delta, post_weight, gate, scale, next_weight, eps):
     """The C descriptor and the tensors it points into."""
     keep = [x, delta, post_weight, gate, scale, next_weight]
@@ -125,44 +134,57 @@ def _empty(t: Tensor) -> Tensor:
     return torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
-def _run_forward(x, delta, post_weight, gate, scale, next_weight, eps) -> tuple[Tensor | None, Tensor | None]:
+def _run_forward(x, delta, post_weight, gate, scale, next_weight, eps):
+    """(out or None, next or None, the descriptor where it points at the inputs themselves, else None)."""
     out = _empty(x) if delta is not None else None
     nxt = _empty(x) if next_weight is not None else None
-    if x.numel():
-        desc, _keep = _descriptor(x, delta, post_weight, gate, scale, next_weight, eps)
-        _on(x.device, _native.lib().ow_block_norms_fwd, ctypes.byref(desc), None if out is None else out.data_ptr(),
-            None if nxt is None else nxt.data_ptr())
-    return out, nxt
+    if not x.numel():
+        return out, nxt, None
+    desc, keep = _descriptor(x, delta, post_weight, gate, scale, next_weight, eps)
+    _on(x.device, _native.lib().ow_block_norms_fwd, ctypes.byref(desc), None if out is None else out.data_ptr(),
+        None if nxt is None else nxt.data_ptr())
+    inputs = all(map(is_, keep, (x, delta, post_weight, gate, scale, next_weight)))
+    return out, nxt, desc if inputs else None
 
 
-def _run_backward(dout, dnext, x, delta, post_weight, gate, scale, next_weight, eps, want) -> list[Tensor | None]:
+def _run_backward(dout, dnext, desc, x, delta, post_weight, gate, scale, next_weight, eps, want) -> list[Tensor | None]:
     """Gradients of x, delta, post_weight, gate and next_weight where ``want`` asks for them and they
-    exist; ``dout`` / ``dnext`` None: that output has no upstream gradient."""
-    sources = (x, delta, post_weight, gate, next_weight)
-    grads = [_empty(t) if w and t is not None else None for t, w in zip(sources, want)]
+    exist; ``dout`` / ``dnext`` None: that output has no upstream gradient; ``desc``: the forward's
+    descriptor, or None."""
+    grads = [_empty(t) if w and t is not None else None for t, w in zip((x, delta, post_weight, gate, next_weight), want)]
     if x.numel() == 0 or (dout is None and dnext is None):
         return [None if g is None else g.zero_() for g in grads]
+    ptr = [None if g is None else g.data_ptr() for g in grads]
     if dnext is None and grads[4] is not None:
         grads[4].zero_()
-    desc, _keep = _descriptor(x, delta, post_weight, gate, scale, next_weight, eps)
-    upstream, strides = [], []
-    for g in (dout, dnext):
-        g, stride = (None, 0) if g is None else _rows(g)
-        upstream.append(g)
-        strides.append(stride)
-    lib = _native.lib()
-    ws_bytes = 0
-    workspace = None
-    if any(g is not None for g in grads[2:]):
-        with torch.cuda.device(x.device):  # the size goes by the device's compute units
-            ws_bytes = lib.ow_block_norms_bwd_workspace(ctypes.byref(desc))
-        workspace = torch.empty(ws_bytes // 4, dtype=torch.float32, device=x.device)
-    ptr = [None if g is None else g.data_ptr() for g in grads]
-    if dnext is None:
         ptr[4] = None
-    up = [None if g is None else g.data_ptr() for g in upstream]
-    _on(x.device, lib.ow_block_norms_bwd, ctypes.byref(desc), up[0], strides[0], up[1], strides[1], *ptr,
-        None if workspace is None else workspace.data_ptr(), ws_bytes)
+    # The forward's descriptor serves where the inputs came back as they were (hooks on saved tensors may
+    # hand out copies).
+    if desc is None or x.data_ptr() != desc.x or not _lies(x, desc.x_stride) \
+            or (delta is not None and (delta.data_ptr() != desc.delta or not _lies(delta, desc.delta_stride))) \
+            or (post_weight is not None and post_weight.data_ptr() != desc.post_weight) \
+            or (gate is not None and gate.data_ptr() != desc.gate) \
+            or (scale is not None and scale.data_ptr() != desc.scale) \
+            or (next_weight is not None and next_weight.data_ptr() != desc.next_weight):
+        desc, _keep = _descriptor(x, delta, post_weight, gate, scale, next_weight, eps)
+    out_ptr, out_stride, next_ptr, next_stride = None, 0, None, 0
+    if dout is not None:
+        dout, out_stride = _rows(dout)
+        out_ptr = dout.data_ptr()
+    if dnext is not None:
+        dnext, next_stride = _rows(dnext)
+        next_ptr = dnext.data_ptr()
+    lib, ref, device = _native.lib(), ctypes.byref(desc), x.device
+    workspace, ws_bytes, ws_ptr = None, 0, None
+    if ptr[2] or ptr[3] or ptr[4]:
+        if device.index != torch.cuda.current_device():
+            with torch.cuda.device(device):  # the size goes by the device's compute units
+                ws_bytes = lib.ow_block_norms_bwd_workspace(ref)
+        else:
+            ws_bytes = lib.ow_block_norms_bwd_workspace(ref)
+        workspace = torch.empty(ws_bytes // 4, dtype=torch.float32, device=device)
+        ws_ptr = workspace.data_ptr()
+    _on(device, lib.ow_block_norms_bwd, ref, out_ptr, out_stride, next_ptr, next_stride, *ptr, ws_ptr, ws_bytes)
     return grads
 
 
@@ -173,17 +195,22 @@ class _PlainNorms(torch.autograd.Function):
     def forward(ctx, x, delta, post_weight, gate, scale, next_weight, eps):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, delta, post_weight, gate, scale, next_weight)
+        out, nxt, ctx.desc = _run_forward(x, delta, post_weight, gate, scale, next_weight, eps)
         ctx.eps = eps
-        return _run_forward(x, delta, post_weight, gate, scale, next_weight, eps)
+        return out, nxt
+
+    @staticmethod
+    def backward(ctx, dout, dnext):
+        if torch.is_grad_enabled():
+            return _PlainNorms._once(ctx, dout, dnext)
+        need = ctx.needs_input_grad
+        grads = _run_backward(dout, dnext, ctx.desc, *ctx.saved_tensors, ctx.eps, (need[0], need[1], need[2], need[3], need[5]))
+        return grads[0], grads[1], grads[2], grads[3], None, grads[4], None
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, dout, dnext):
-        x, delta, post_weight, gate, scale, next_weight = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        grads = _run_backward(dout, dnext, x, delta, post_weight, gate, scale, next_weight, ctx.eps,
-                              (need[0], need[1], need[2], need[3], need[5]))
-        return grads[0], grads[1], grads[2], grads[3], None, grads[4], None
+    def _once(ctx, dout, dnext):
+        return _PlainNorms.backward(ctx, dout, dnext)
 
 
 @torch.library.custom_op("omniwave_amd::block_norms_fwd", mutates_args=())
@@ -191,7 +218,7 @@ def block_norms_fwd(x: Tensor, delta: Tensor | None, post_weight: Tensor | None,
                     scale: Tensor | None, next_weight: Tensor | None, eps: float) -> tuple[Tensor, Tensor]:
     """(out, next) of ``block_norms_hip``; empty where there is none (``out`` without ``delta``, ``next``
     without ``next_weight``)."""
-    out, nxt = _run_forward(x, delta, post_weight, gate, scale, next_weight, eps)
+    out, nxt, _ = _run_forward(x, delta, post_weight, gate, scale, next_weight, eps)
     return x.new_empty(0) if out is None else out, x.new_empty(0) if nxt is None else nxt
 
 
@@ -206,7 +233,7 @@ def block_norms_bwd(dout: Tensor | None, dnext: Tensor | None, x: Tensor, delta:
                     post_weight: Tensor | None, gate: Tensor | None, scale: Tensor | None, next_weight: Tensor | None,
                     eps: float, want: list[bool]) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
     """Gradients of x, delta, post_weight, gate and next_weight; empty where ``want`` is false."""
-    grads = _run_backward(dout, dnext, x, delta, post_weight, gate, scale, next_weight, eps, want)
+    grads = _run_backward(dout, dnext, None, x, delta, post_weight, gate, scale, next_weight, eps, want)
     return tuple(x.new_empty(0) if g is None else g for g in grads)
 
 
@@ -250,7 +277,7 @@ def _norms(x, delta, post_weight, gate, scale, next_weight, eps) -> tuple[Tensor
         return (None if delta is None else out), (None if next_weight is None else nxt)
     if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors]):
         return _PlainNorms.apply(*tensors, eps)
-    return _run_forward(*tensors, eps)
+    return _run_forward(*tensors, eps)[:2]
 
 
 def block_norms_hip(x: Tensor, delta: Tensor, *, post_weight: Tensor | None = None, gate: Tensor | None = None,
