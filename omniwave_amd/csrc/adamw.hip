@@ -11,7 +11,7 @@
 //
 // Steps are counted on the device, so that a captured step counts and a skipped one does not: one
 // counter per chunk, all of a tensor's equal, so that no workgroup waits for another's read before it
-// writes.  1 - b^t is formed in fp64 (b^t is near one for small t).
+// writes.
 //
 // 8-bit states: 256 consecutive values (one wave's vectors) share an fp32 scale, their largest magnitude
 // over 448; a value is held as the nearest e4m3fn number of its ratio to the scale.  The second moment is
@@ -19,7 +19,9 @@
 // that is not zero is never held as zero, since m / (0 + eps) would be a step of m / eps.  The update
 // itself uses the unrounded m and v.  Arithmetic is not contracted to fused multiply-adds: rounding
 // after each operation is what the states' definition says, and a value next to a border of two codes
-// then falls on the same side everywhere.
+// then falls on the same side everywhere.  Roots and the update's quotient are the hardware's, within a
+// unit in the last place each; 1 - b^t is formed as -expm1(t ln b), which keeps its relative precision
+// where b^t is near one.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -31,19 +33,18 @@ namespace {
 
 constexpr int kChunk = OW_ADAMW_CHUNK;  // values of a workgroup
 constexpr int kBlock = OW_ADAMW_BLOCK;  // values that share a scale: 64 lanes x 4
-constexpr int kThreadsA = 256;
-constexpr int kIters = kChunk / (4 * kThreadsA);
+constexpr int kThreads = 256;
+constexpr int kIters = kChunk / (4 * kThreads);
 constexpr int kGroups = 8;              // hyperparameter sets of a launch
 constexpr int kArgBytes = 4096 - 256;   // of the tensor and hyperparameter tables
 constexpr float kFp8Most = 448.f;
-constexpr uint32_t kFp8Least = 1;       // code of 2^-9
+constexpr float kFp8Least = 0x1p-9f;    // the least e4m3fn number above zero
 constexpr float kLeastScale = 1.17549435e-38f;  // smaller (subnormal) scales: a block of zeros
-static_assert(kBlock == 256 && kChunk % (4 * kThreadsA) == 0, "a wave's vectors are a block");
+static_assert(kBlock == 4 * 64, "a wave's vectors are a block");
 
 struct Hyper {
   const float* lr_device;  // NULL: lr
-  double log2_b1, log2_b2;
-  float lr, decay, b1, c1, b2, c2, eps, unused;
+  float ln_b1, ln_b2, lr, decay, b1, c1, b2, c2, eps, unused;
 };
 
 enum { kParam, kGrad, kM, kV, kStep, kMScale, kVScale, kPtrs8, kPtrs32 = kMScale };
@@ -62,16 +63,19 @@ struct Table {
   uint8_t group[N];
 };
 
-// Tensor of chunk c: the last one whose first chunk is not past c.
-template <class T>
+// Tensor of chunk c, the last one whose first chunk is not past c: every lane looks at one of them (a
+// bisection would wait for one argument after the other).
+template <int N, class T>
 __device__ __forceinline__ int tensor_of(const T& t, int count, uint32_t c) {
-  int lo = 0, hi = count;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (t.first[mid] <= c) lo = mid;
-    else hi = mid;
+  const int lane = threadIdx.x & 63;
+  int found = 0;
+#pragma unroll
+  for (int base = 0; base < N; base += 64) {
+    const int i = base + lane;
+    const bool before = i < count && t.first[i < N ? i : 0] <= c;
+    found += __popcll(__ballot(before));
   }
-  return lo;
+  return __builtin_amdgcn_readfirstlane(found) - 1;
 }
 
 typedef uint32_t __attribute__((aligned(1))) u32_any;
@@ -134,33 +138,44 @@ __device__ __forceinline__ void decode4(uint32_t w, float scale, float (&v)[4]) 
   v[2] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(w), 2) * scale;
   v[3] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(w), 3) * scale;
 }
-// Codes of four values and the scale of their block (all 64 lanes).
+// Codes of four values and the scale of their block (all 64 lanes); ROOT: values from zero up, of which
+// none above zero becomes zero.  A ratio exceeds 448 by its rounding at most, which the conversion
+// rounds back.  Magnitudes are compared as integers: a NaN is the largest, so that its block's scale and with it
+// the block are none.
+template <bool ROOT>
 __device__ __forceinline__ uint32_t encode4(const float (&v)[4], float& scale) {
 #pragma clang fp contract(off)
-  float most = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-  most = lanes_reduce<MaxOp, 64>(most);
-  scale = most / kFp8Most;
+  uint32_t most = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t u = ROOT ? __float_as_uint(v[j]) : __float_as_uint(v[j]) & 0x7fffffffu;
+    most = u > most ? u : most;
+  }
+  most = lanes_reduce<MaxUintOp, 64>(most);
+  scale = __uint_as_float(most) / kFp8Most;
   if (scale < kLeastScale) scale = 0.f;
   const float inv = scale != 0.f ? 1.f / scale : 0.f;
-  float y[4];  // a value that is no number stays none
+  float y[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     y[j] = v[j] * inv;
-    y[j] = y[j] > kFp8Most ? kFp8Most : y[j] < -kFp8Most ? -kFp8Most : y[j];
+    if (ROOT) y[j] = v[j] > 0.f && y[j] < kFp8Least ? kFp8Least : y[j];
   }
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
   return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true));
 }
 
-// Sum of the partial sums of squares, in a fixed order; every thread gets it.
-__device__ __forceinline__ double sum_partials(const double* partials, int n, double* lds) {
-  double sum = 0.0;
-  for (int i = threadIdx.x; i < n; i += kThreadsA) sum += partials[i];
+// Sum over a workgroup of WAVES waves; every thread gets it.
+template <int WAVES>
+__device__ __forceinline__ double workgroup_sum(double sum, double* lds) {
 #pragma unroll
   for (int m = 32; m > 0; m >>= 1) sum += __shfl_xor(sum, m);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = sum;
   __syncthreads();
-  return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+  sum = lds[0];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) sum += lds[w];
+  return sum;
 }
 
 template <int PTRS>
@@ -176,83 +191,98 @@ template <class Ty, int BITS, bool MASTER>
 constexpr int kPtrsOf = (BITS == 8 ? kPtrs8 : kPtrs32) + (MASTER ? 1 : 0);
 
 template <class Ty, int BITS, bool MASTER>
-__global__ void __launch_bounds__(kThreadsA) adamw_kernel(StepArgs<kPtrsOf<Ty, BITS, MASTER>> a) {
+__global__ void __launch_bounds__(kThreads, 4) adamw_kernel(StepArgs<kPtrsOf<Ty, BITS, MASTER>> a) {
 #pragma clang fp contract(off)
   constexpr int PTRS = kPtrsOf<Ty, BITS, MASTER>;
-  __shared__ double lds[4];
+  __shared__ double lds[kThreads / 64];
   const uint32_t chunk = blockIdx.x;
-  const int i = tensor_of(a.t, a.count, chunk);
+  const int i = tensor_of<Table<PTRS>::N>(a.t, a.count, chunk);
   const uint32_t local = chunk - a.t.first[i];
   const uint32_t next = i + 1 < a.count ? a.t.first[i + 1] : gridDim.x;
   const int n = chunk + 1 == next ? a.t.last[i] + 1 : kChunk;  // values of this chunk
-  const int64_t base = static_cast<int64_t>(local) * kChunk;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t base = static_cast<int64_t>(local) * kChunk, block0 = static_cast<int64_t>(local) * (kChunk / kBlock);
+
+  // Everything is read before anything is written: a vector's loads do not wait for the stores of the
+  // one before it, nor for the counter and the norm.
+  float p[kIters][4], g[kIters][4], m[kIters][4], v[kIters][4];
+  uint32_t mw[kIters], vw[kIters];
+  float ms[kIters], vs[kIters];
+#pragma unroll
+  for (int k = 0; k < kIters; ++k) {
+    const int block = wave + k * (kThreads / 64), at = block * kBlock + 4 * lane;
+    const int left = n - at;
+    const int64_t idx = base + at;
+    if constexpr (MASTER) load4<F32>(a.t.ptr[PTRS - 1][i], idx, left, p[k]);
+    else load4<Ty>(a.t.ptr[kParam][i], idx, left, p[k]);
+    load4<Ty>(a.t.ptr[kGrad][i], idx, left, g[k]);
+    if constexpr (BITS == 8) {
+      const bool held = block * kBlock < n;  // wave-uniform: the block has values
+      ms[k] = held ? static_cast<const float*>(a.t.ptr[kMScale][i])[block0 + block] : 0.f;
+      vs[k] = held ? static_cast<const float*>(a.t.ptr[kVScale][i])[block0 + block] : 0.f;
+      mw[k] = load_codes(a.t.ptr[kM][i], idx, left);
+      vw[k] = load_codes(a.t.ptr[kV][i], idx, left);
+    } else {
+      load4<F32>(a.t.ptr[kM][i], idx, left, m[k]);
+      load4<F32>(a.t.ptr[kV][i], idx, left, v[k]);
+    }
+  }
 
   float coef = 1.f;
   if (a.partials != nullptr) {
-    const float norm = static_cast<float>(sqrt(sum_partials(a.partials, a.n_partials, lds)));
+    double sum = 0.0;  // in a fixed order, every workgroup alike
+    for (int k = threadIdx.x; k < a.n_partials; k += kThreads) sum += a.partials[k];
+    const float norm = static_cast<float>(sqrt(workgroup_sum<kThreads / 64>(sum, lds)));
     if (chunk == 0 && threadIdx.x == 0 && a.norm_out != nullptr) *a.norm_out = norm;
-    if (!(norm < __builtin_inff())) return;  // every workgroup alike: the step is skipped
+    if (!(norm < __builtin_inff())) return;  // the step is skipped
     coef = fminf(static_cast<float>(a.max_norm) / (norm + 1e-6f), 1.f);
   }
   const Hyper& h = a.t.hyper[a.t.group[i]];
   int32_t* counter = static_cast<int32_t*>(a.t.ptr[kStep][i]) + local;
-  const double t = static_cast<double>(*counter + 1);
+  const int32_t steps = *counter + 1;
+  const float t = static_cast<float>(steps);
   const float lr = h.lr_device != nullptr ? *h.lr_device : h.lr;
-  const float step = static_cast<float>(static_cast<double>(lr) / (1.0 - exp2(t * h.log2_b1)));
-  const float unbias = static_cast<float>(1.0 / sqrt(1.0 - exp2(t * h.log2_b2)));
+  const float step = lr / -expm1f(t * h.ln_b1);
+  const float unbias = 1.f / sqrtf(-expm1f(t * h.ln_b2));
   const float keep = 1.f - lr * h.decay;
   __syncthreads();  // every thread has read the counter
-  if (threadIdx.x == 0) *counter = static_cast<int32_t>(t);
+  if (threadIdx.x == 0) *counter = steps;
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int k = 0; k < kIters; ++k) {
-    const int block = wave * kIters + k;  // of 256 values
-    const int at = block * kBlock + 4 * lane;
+    const int block = wave + k * (kThreads / 64), at = block * kBlock + 4 * lane;
     if (block * kBlock >= n) break;  // wave-uniform
     const int left = n - at;
     const int64_t idx = base + at;
-    float p[4], g[4], m[4], v[4];
-    if constexpr (MASTER) load4<F32>(a.t.ptr[PTRS - 1][i], idx, left, p);
-    else load4<Ty>(a.t.ptr[kParam][i], idx, left, p);
-    load4<Ty>(a.t.ptr[kGrad][i], idx, left, g);
-    const int64_t sb = static_cast<int64_t>(local) * (kChunk / kBlock) + block;
     if constexpr (BITS == 8) {
-      decode4(load_codes(a.t.ptr[kM][i], idx, left), static_cast<const float*>(a.t.ptr[kMScale][i])[sb], m);
-      decode4(load_codes(a.t.ptr[kV][i], idx, left), static_cast<const float*>(a.t.ptr[kVScale][i])[sb], v);
+      decode4(mw[k], ms[k], m[k]);
+      decode4(vw[k], vs[k], v[k]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = v[j] * v[j];
-    } else {
-      load4<F32>(a.t.ptr[kM][i], idx, left, m);
-      load4<F32>(a.t.ptr[kV][i], idx, left, v);
+      for (int j = 0; j < 4; ++j) v[k][j] = v[k][j] * v[k][j];
     }
     float root[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float gj = g[j] * coef;
-      m[j] = m[j] * h.b1 + gj * h.c1;
-      v[j] = v[j] * h.b2 + gj * gj * h.c2;
-      root[j] = sqrtf(v[j]);
-      p[j] = p[j] * keep - step * (m[j] / (root[j] * unbias + h.eps));
+      const float gj = g[k][j] * coef;
+      m[k][j] = m[k][j] * h.b1 + gj * h.c1;
+      v[k][j] = v[k][j] * h.b2 + gj * gj * h.c2;
+      root[j] = __builtin_amdgcn_sqrtf(v[k][j]);
+      p[k][j] = p[k][j] * keep - step * (m[k][j] * __builtin_amdgcn_rcpf(root[j] * unbias + h.eps));
     }
-    if constexpr (MASTER) store4<F32>(a.t.ptr[PTRS - 1][i], idx, left, p);
-    store4<Ty>(a.t.ptr[kParam][i], idx, left, p);
+    if constexpr (MASTER) store4<F32>(a.t.ptr[PTRS - 1][i], idx, left, p[k]);
+    store4<Ty>(a.t.ptr[kParam][i], idx, left, p[k]);
     if constexpr (BITS == 8) {
-      float ms, vs;
-      const uint32_t mw = encode4(m, ms);
-      uint32_t vw = encode4(root, vs);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (root[j] > 0.f && ((vw >> (8 * j)) & 0xff) == 0) vw |= kFp8Least << (8 * j);
-      store_codes(a.t.ptr[kM][i], idx, left, mw);
-      store_codes(a.t.ptr[kV][i], idx, left, vw);
+      mw[k] = encode4<false>(m[k], ms[k]);
+      vw[k] = encode4<true>(root, vs[k]);
+      store_codes(a.t.ptr[kM][i], idx, left, mw[k]);
+      store_codes(a.t.ptr[kV][i], idx, left, vw[k]);
       if (lane == 0) {
-        static_cast<float*>(a.t.ptr[kMScale][i])[sb] = ms;
-        static_cast<float*>(a.t.ptr[kVScale][i])[sb] = vs;
+        static_cast<float*>(a.t.ptr[kMScale][i])[block0 + block] = ms[k];
+        static_cast<float*>(a.t.ptr[kVScale][i])[block0 + block] = vs[k];
       }
     } else {
-      store4<F32>(a.t.ptr[kM][i], idx, left, m);
-      store4<F32>(a.t.ptr[kV][i], idx, left, v);
+      store4<F32>(a.t.ptr[kM][i], idx, left, m[k]);
+      store4<F32>(a.t.ptr[kV][i], idx, left, v[k]);
     }
   }
 }
@@ -269,17 +299,17 @@ struct NormArgs {
 };
 
 template <class Ty>
-__global__ void __launch_bounds__(kThreadsA) grad_norm_kernel(NormArgs a) {
-  __shared__ double lds[4];
+__global__ void __launch_bounds__(kThreads) grad_norm_kernel(NormArgs a) {
+  __shared__ double lds[kThreads / 64];
   double sum = 0.0;
   for (uint32_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
-    const int i = tensor_of(a, a.count, chunk);
+    const int i = tensor_of<NormArgs::N>(a, a.count, chunk);
     const uint32_t local = chunk - a.first[i];
     const uint32_t next = i + 1 < a.count ? a.first[i + 1] : a.chunks;
     const int n = chunk + 1 == next ? a.last[i] + 1 : kChunk;
 #pragma unroll
     for (int k = 0; k < kIters; ++k) {
-      const int at = (k * kThreadsA + threadIdx.x) * 4;
+      const int at = (k * kThreads + threadIdx.x) * 4;
       if (at < n) {
         float g[4];
         load4<Ty>(a.grad[i], static_cast<int64_t>(local) * kChunk + at, n - at, g);
@@ -288,11 +318,8 @@ __global__ void __launch_bounds__(kThreadsA) grad_norm_kernel(NormArgs a) {
       }
     }
   }
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) sum += __shfl_xor(sum, m);
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) a.partials[blockIdx.x] = (lds[0] + lds[1]) + (lds[2] + lds[3]);
+  sum = workgroup_sum<kThreads / 64>(sum, lds);
+  if (threadIdx.x == 0) a.partials[blockIdx.x] = sum;
 }
 
 int64_t chunks_of(int64_t numel) { return (numel + kChunk - 1) / kChunk; }
@@ -336,8 +363,8 @@ int launch_step(const OwAdamwTensor* t, int32_t count, const OwAdamwGroup* group
         const OwAdamwGroup& y = groups[x.group];
         Hyper& h = a.t.hyper[g];
         h.lr_device = y.lr_device;
-        h.log2_b1 = log2(y.beta1);
-        h.log2_b2 = log2(y.beta2);
+        h.ln_b1 = static_cast<float>(log(y.beta1));
+        h.ln_b2 = static_cast<float>(log(y.beta2));
         h.lr = static_cast<float>(y.lr);
         h.decay = static_cast<float>(y.weight_decay);
         h.b1 = static_cast<float>(y.beta1);
@@ -363,7 +390,7 @@ int launch_step(const OwAdamwTensor* t, int32_t count, const OwAdamwGroup* group
       chunks += chunks_of(x.numel);
       ++at;
     }
-    hipLaunchKernelGGL((adamw_kernel<Ty, BITS, MASTER>), dim3(static_cast<unsigned>(chunks)), dim3(kThreadsA), 0, s, a);
+    hipLaunchKernelGGL((adamw_kernel<Ty, BITS, MASTER>), dim3(static_cast<unsigned>(chunks)), dim3(kThreads), 0, s, a);
     if (int rc = hip_status(hipGetLastError(), "adamw_kernel launch")) return rc;
   }
   return OW_OK;
@@ -386,7 +413,7 @@ int launch_norm(const OwAdamwTensor* t, int32_t count, double* partials, hipStre
     a.chunks = static_cast<uint32_t>(chunks);
     a.partials = partials;
     partials += OW_GRAD_NORM_PARTIALS;
-    hipLaunchKernelGGL((grad_norm_kernel<Ty>), dim3(OW_GRAD_NORM_PARTIALS), dim3(kThreadsA), 0, s, a);
+    hipLaunchKernelGGL((grad_norm_kernel<Ty>), dim3(OW_GRAD_NORM_PARTIALS), dim3(kThreads), 0, s, a);
     if (int rc = hip_status(hipGetLastError(), "grad_norm_kernel launch")) return rc;
   }
   return OW_OK;

@@ -100,23 +100,32 @@ struct MaxOp {
   static __device__ __forceinline__ float apply(float a, float b) { return fmaxf(a, b); }
 };
 
+struct MaxUintOp {
+  static __device__ __forceinline__ uint32_t apply(uint32_t a, uint32_t b) { return a > b ? a : b; }
+};
+
 // Op over aligned groups of T lanes (8, 16, 32 or 64); every lane gets the result.  Mirrors within a row of
 // 16 lanes, then gfx950's row and half swaps: of two copies of v, permlane16_swap leaves the even
 // rows in one and the odd rows in the other (permlane32_swap: the halves).
-template <class Op, int T>
-__device__ __forceinline__ float lanes_reduce(float v) {
-  static_assert(T == 8 || T == 16 || T == 32 || T == 64, "lanes of a row");
-  v = Op::apply(v, dpp_f32<0xb1, 0xf>(v));                             // quad_perm 1,0,3,2
-  v = Op::apply(v, dpp_f32<0x4e, 0xf>(v));                             // quad_perm 2,3,0,1
-  v = Op::apply(v, dpp_f32<0x141, 0xf>(v));                            // row_half_mirror
-  if constexpr (T >= 16) v = Op::apply(v, dpp_f32<0x140, 0xf>(v));     // row_mirror
+template <class Op, int T, class V>
+__device__ __forceinline__ V lanes_reduce(V v) {
+  static_assert((T == 8 || T == 16 || T == 32 || T == 64) && sizeof(V) == 4, "lanes of a row");
+  auto bits = [](V x) { return __builtin_bit_cast(uint32_t, x); };
+  auto value = [](uint32_t x) { return __builtin_bit_cast(V, x); };
+  auto dpp = [&](V x, auto ctrl) {
+    return value(__builtin_amdgcn_update_dpp(0u, bits(x), decltype(ctrl)::value, 0xf, 0xf, false));
+  };
+  v = Op::apply(v, dpp(v, std::integral_constant<int, 0xb1>{}));   // quad_perm 1,0,3,2
+  v = Op::apply(v, dpp(v, std::integral_constant<int, 0x4e>{}));   // quad_perm 2,3,0,1
+  v = Op::apply(v, dpp(v, std::integral_constant<int, 0x141>{}));  // row_half_mirror
+  if constexpr (T >= 16) v = Op::apply(v, dpp(v, std::integral_constant<int, 0x140>{}));  // row_mirror
   if constexpr (T >= 32) {
-    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = Op::apply(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    const auto s = __builtin_amdgcn_permlane16_swap(bits(v), bits(v), false, false);
+    v = Op::apply(value(s[0]), value(s[1]));
   }
   if constexpr (T >= 64) {
-    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = Op::apply(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    const auto s = __builtin_amdgcn_permlane32_swap(bits(v), bits(v), false, false);
+    v = Op::apply(value(s[0]), value(s[1]));
   }
   return v;
 }

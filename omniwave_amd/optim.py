@@ -25,8 +25,7 @@ CHUNK, BLOCK = _native.OW_ADAMW_CHUNK, _native.OW_ADAMW_BLOCK
 FP8 = torch.float8_e4m3fn
 FP8_MOST = 448.0
 MIN_8BIT_VALUES = 4096  # smaller tensors keep 32-bit states: their bytes do not matter, their errors do
-_FIELDS = len(_native.OwAdamwTensor._fields_)  # of 8 bytes each
-_GRAD = 1  # field
+_GRAD = 1  # field of OwAdamwTensor, whose fields are 8 bytes each
 
 
 def _blocks(n: int) -> int:
@@ -52,16 +51,6 @@ def _decode(codes: Tensor, scale: Tensor) -> Tensor:
     return (flat * scale.repeat_interleave(BLOCK)[:flat.numel()]).reshape(codes.shape)
 
 
-class _Kind:
-    """Tensors of one dtype and state layout: one list for the native calls."""
-
-    __slots__ = ("dtype", "bits", "master", "params", "columns", "table", "partials")
-
-    def __init__(self, dtype, bits, master) -> None:
-        self.dtype, self.bits, self.master = dtype, bits, master
-        self.params: list[Tensor] = []
-
-
 class AdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW`` on the framework's kernels.
 
@@ -84,7 +73,7 @@ class AdamW(torch.optim.Optimizer):
     """
 
     grad_norm: Tensor | None = None
-    _plan: tuple[list[list[Tensor]], list[_Kind]] | None = None
+    _plan: _Plan | None = None
 
     def __init__(self, params, lr: float | Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, master_weights: bool = False,
@@ -209,24 +198,26 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        active = [[p for p in group["params"] if p.grad is not None and p.numel()] for group in self.param_groups]
-        if not any(active):
-            return loss
+        # What stands between the calls is looked at in lists: a model has hundreds of parameters.
+        params = [p for group in self.param_groups for p in group["params"]]
+        grads = [p.grad for p in params]
         plan = self._plan
-        if plan is None or not _same(plan[0], active) or not self._current(plan[1]):
-            plan = self._plan = self._make_plan(active)
-        device = plan[1][0].params[0].device
-        hyper = (_native.OwAdamwGroup * len(self.param_groups))(*[_hyper(g, device) for g in self.param_groups])
-        if device.index != torch.cuda.current_device():
+        if plan is None or not plan.current(self, params, grads):
+            plan = self._plan = _Plan(self, params, grads)
+        if not plan.kinds:
+            return loss
+        device = plan.device
+        hyper = plan.hyper(*[_hyper(g, device) for g in self.param_groups])
+        if device.index != torch._C._cuda_getDevice():
             with torch.cuda.device(device):
-                self._launch(plan[1], hyper, device)
+                self._launch(plan.kinds, grads, hyper, device)
         else:
-            self._launch(plan[1], hyper, device)
+            self._launch(plan.kinds, grads, hyper, device)
         return loss
 
-    def _launch(self, kinds: list[_Kind], hyper, device: torch.device) -> None:
+    def _launch(self, kinds: list[_Kind], grads: list[Tensor | None], hyper, device: torch.device) -> None:
         lib, stream = _native.lib(), _stream_ptr(device)
-        keep = [_gradients(kind) for kind in kinds]  # copies of strided gradients live until the launches are queued
+        keep = [kind.set_gradients(grads) for kind in kinds]  # copies of strided ones live until the launches are queued
         partials, total, norm_ptr = None, 0, None
         if self.max_grad_norm is not None:
             total = sum(kind.partials for kind in kinds)
@@ -235,84 +226,120 @@ class AdamW(torch.optim.Optimizer):
             norm_ptr = self.grad_norm.data_ptr()
             at = 0
             for kind in kinds:
-                _native.check(lib.ow_grad_norm(kind.table.ctypes.data, len(kind.params), _DTYPE_CODE[kind.dtype],
+                _native.check(lib.ow_grad_norm(kind.pointer, kind.count, kind.code,
                                                partials.data_ptr() + 8 * at, kind.partials, stream), "ow_grad_norm")
                 at += kind.partials
         for kind in kinds:
             _native.check(
-                lib.ow_adamw_step(kind.table.ctypes.data, len(kind.params), hyper, len(hyper), _DTYPE_CODE[kind.dtype],
-                                  kind.bits, int(kind.master), None if partials is None else partials.data_ptr(), total,
+                lib.ow_adamw_step(kind.pointer, kind.count, hyper, len(hyper), kind.code, kind.bits, kind.master,
+                                  None if partials is None else partials.data_ptr(), total,
                                   self.max_grad_norm or 0.0, norm_ptr, stream), "ow_adamw_step")
             norm_ptr = None
         del keep
 
-    def _make_plan(self, active: list[list[Tensor]]) -> tuple[list[list[Tensor]], list[_Kind]]:
-        groups = {p: i for i, params in enumerate(active) for p in params}
-        first = next(iter(groups))
-        device, reason = first.device, gpu_reason(first)
-        if reason is not None:
-            raise RuntimeError(f"hip AdamW not supported: {reason}")
+
+class _Plan:
+    """What the steps of the same parameters share: their lists for the native calls.  It is made anew
+    where a parameter, a state or the set of parameters with gradients is another than it was."""
+
+    def __init__(self, opt: AdamW, params: list[Tensor], grads: list[Tensor | None]) -> None:
+        self.params, self.kinds, self.device = params, [], None
+        self.without = [g is None for g in grads]
+        self.sizes = [len(group["params"]) for group in opt.param_groups]
+        self.hyper = _native.OwAdamwGroup * len(self.sizes)
+        owner = [i for i, size in enumerate(self.sizes) for _ in range(size)]
+        active = [i for i, (p, g) in enumerate(zip(params, grads)) if g is not None and p.numel()]
+        self.lies = _Addresses(params)
         kinds: dict[tuple, _Kind] = {}
-        for p in groups:
-            if p.device != device:
-                raise ValueError(f"parameters on {device} and {p.device}: an optimizer's parameters are on one GPU")
+        if active:
+            self.device, reason = params[active[0]].device, gpu_reason(params[active[0]])
+            if reason is not None:
+                raise RuntimeError(f"hip AdamW not supported: {reason}")
+        for i in active:
+            p, g = params[i], grads[i]
+            if p.device != self.device:
+                raise ValueError(f"parameters on {self.device} and {p.device}: an optimizer's parameters are on one GPU")
             if not p.is_contiguous():
                 raise ValueError(f"a parameter of shape {tuple(p.shape)} is not contiguous")
-            if not self.state[p]:
-                self._first_state(p)
-            self._check_state(p)
-            entry = self.state[p]
-            key = (p.dtype, 8 if "exp_avg_sq_root" in self._layout(p) else 32, self.master_weights and p.dtype != torch.float32)
-            kinds.setdefault(key, _Kind(*key)).params.append(p)
-        for kind in kinds.values():
-            kind.columns = _columns(kind, self.state)
-            kind.table = np.zeros((len(kind.params), _FIELDS), dtype=np.int64)
-            kind.table[:, 0], kind.table[:, 2:8] = kind.columns[0], np.array(kind.columns[1:], dtype=np.int64).T
-            kind.table[:, 8] = [p.numel() for p in kind.params]
-            kind.table[:, 9] = [groups[p] for p in kind.params]
-            kind.partials = _native.lib().ow_grad_norm_partials(kind.table.ctypes.data, len(kind.params))
-        return active, list(kinds.values())
+            if g.layout != torch.strided:
+                raise RuntimeError("AdamW takes dense gradients")
+            if g.shape != p.shape or g.dtype != p.dtype or g.device != p.device:
+                raise ValueError(f"the gradient of a {p.dtype} parameter of shape {tuple(p.shape)} is {g.dtype} "
+                                 f"{tuple(g.shape)} on {g.device}")
+            if not opt.state[p]:
+                opt._first_state(p)
+            opt._check_state(p)
+            layout = opt._layout(p)
+            key = (p.dtype, 8 if "exp_avg_sq_root" in layout else 32, "master" in layout)
+            kinds.setdefault(key, _Kind(*key)).add(i, p, opt.state[p], owner[i])
+        self.kinds = list(kinds.values())
+        for kind in self.kinds:
+            kind.finish()
+        self.entries = list(opt.state.values())
+        self.states = _Addresses(_tensors(self.entries))
 
-    def _current(self, kinds: list[_Kind]) -> bool:
-        """Whether every parameter and state still lies where the plan has it (anything else is
-        checked and planned anew)."""
-        return all(_columns(kind, self.state) == kind.columns for kind in kinds)
-
-
-def _same(a: list[list[Tensor]], b: list[list[Tensor]]) -> bool:
-    return len(a) == len(b) and all(len(x) == len(y) and all(map(is_, x, y)) for x, y in zip(a, b))
-
-
-def _columns(kind: _Kind, state) -> list[list[int]]:
-    """Addresses of the parameters and their states, by field (the gradients' apart)."""
-    entries = [state[p] for p in kind.params]
-    none = [0] * len(entries)
-    try:
-        cols = [[p.data_ptr() for p in kind.params], [e["exp_avg"].data_ptr() for e in entries]]
-        if kind.bits == 8:
-            cols += [[e["exp_avg_sq_root"].data_ptr() for e in entries], [e["exp_avg_scale"].data_ptr() for e in entries],
-                     [e["exp_avg_sq_root_scale"].data_ptr() for e in entries]]
-        else:
-            cols += [[e["exp_avg_sq"].data_ptr() for e in entries], none, none]
-        cols += [[e["master"].data_ptr() for e in entries] if kind.master else none, [e["step"].data_ptr() for e in entries]]
-    except KeyError:
-        return []
-    return cols
+    def current(self, opt: AdamW, params: list[Tensor], grads: list[Tensor | None]) -> bool:
+        """Whether everything still lies where the plan has it."""
+        entries = list(opt.state.values())
+        return (len(params) == len(self.params) and all(map(is_, params, self.params))
+                and [g is None for g in grads] == self.without
+                and [len(group["params"]) for group in opt.param_groups] == self.sizes
+                and len(entries) == len(self.entries) and all(map(is_, entries, self.entries))
+                and self.lies.still(params) and self.states.still(_tensors(entries)))
 
 
-def _gradients(kind: _Kind) -> list[Tensor]:
-    """Writes the gradients' addresses into the kind's table; returns the tensors that hold them."""
-    grads = [p.grad for p in kind.params]
-    for i, (p, g) in enumerate(zip(kind.params, grads)):
-        if g.layout != torch.strided:
-            raise RuntimeError("AdamW takes dense gradients")
-        if not g.is_contiguous():
-            grads[i] = g = g.contiguous()
-        if g.numel() != p.numel() or g.dtype != kind.dtype or g.device != p.device:
-            raise ValueError(f"the gradient of a {p.dtype} parameter of shape {tuple(p.shape)} is {g.dtype} {tuple(g.shape)} "
-                             f"on {g.device}")
-    kind.table[:, _GRAD] = [g.data_ptr() for g in grads]
-    return grads
+def _tensors(entries: list[dict]) -> list[Tensor]:
+    return [t for e in entries for t in e.values()]
+
+
+class _Addresses:
+    """Where a list of tensors lies, to be compared with later in one call."""
+
+    def __init__(self, tensors: list) -> None:
+        self.of = [t.data_ptr() if isinstance(t, Tensor) else 0 for t in tensors]
+        self.places = list(range(len(self.of)))
+
+    def still(self, tensors: list) -> bool:
+        try:
+            return len(tensors) == len(self.of) and torch._C._tensors_data_ptrs_at_indices_equal(tensors, self.of, self.places)
+        except TypeError:  # not all of them are tensors
+            return False
+
+
+class _Kind:
+    """Tensors of one dtype and state layout: one list for the native calls."""
+
+    def __init__(self, dtype: torch.dtype, bits: int, master: bool) -> None:
+        self.dtype, self.bits, self.master = dtype, bits, master
+        self.at: list[int] = []  # places among the parameters
+        self.rows: list[list[int]] = []
+        self.lie: _Addresses | None = None  # the gradients
+
+    def add(self, i: int, p: Tensor, entry: dict[str, Tensor], group: int) -> None:
+        second = ("exp_avg_sq_root", "exp_avg_scale", "exp_avg_sq_root_scale") if self.bits == 8 else ("exp_avg_sq",)
+        ptr = [entry[k].data_ptr() for k in ("exp_avg", *second)] + [0] * (3 - len(second))
+        self.at.append(i)
+        self.rows.append([p.data_ptr(), 0, *ptr, entry["master"].data_ptr() if self.master else 0, entry["step"].data_ptr(),
+                          p.numel(), group])
+
+    def finish(self) -> None:
+        self.table = np.array(self.rows, dtype=np.int64)
+        self.sizes = [row[8] for row in self.rows]
+        self.pointer, self.count, self.code = self.table.ctypes.data, len(self.rows), _DTYPE_CODE[self.dtype]
+        self.partials = _native.lib().ow_grad_norm_partials(self.pointer, self.count)
+
+    def set_gradients(self, grads: list[Tensor | None]) -> list[Tensor]:
+        """Writes the gradients' addresses into the table; returns the tensors that hold them.  (Torch
+        keeps a gradient in its parameter's dtype and on its device; its strides may differ.)"""
+        mine = [grads[i] for i in self.at]
+        if not all([g.is_contiguous() for g in mine]):
+            mine = [g.contiguous() for g in mine]
+        if self.lie is None or not self.lie.still(mine):
+            if [g.numel() for g in mine] != self.sizes:
+                raise ValueError("a gradient has not its parameter's shape")
+            self.lie = _Addresses(mine)
+            self.table[:, _GRAD] = self.lie.of
+        return mine
 
 
 def _hyper(group: dict, device: torch.device | None = None) -> tuple:
