@@ -35,8 +35,8 @@ constexpr int kChunk = OW_ADAMW_CHUNK;  // values of a workgroup
 constexpr int kBlock = OW_ADAMW_BLOCK;  // values that share a scale: 64 lanes x 4
 constexpr int kThreads = 256;
 constexpr int kIters = kChunk / (4 * kThreads);
-constexpr int kGroups = 8;              // hyperparameter sets of a launch
-constexpr int kArgBytes = 4096 - 256;   // of the tensor and hyperparameter tables
+constexpr int kGroups = 6;              // hyperparameter sets of a launch
+constexpr int kArgBytes = 4096 - 64;    // of the tensor and hyperparameter tables
 constexpr float kFp8Most = 448.f;
 constexpr float kFp8Least = 0x1p-9f;    // the least e4m3fn number above zero
 constexpr float kLeastScale = 1.17549435e-38f;  // smaller (subnormal) scales: a block of zeros

@@ -8,7 +8,7 @@
 // with w the upstream gradient, divided by the number of counted rows for their mean, and 0 for rows
 // left out.  Forward and backward read the logits once each; they are bound by memory where there are many
 // and by the launches where there are few.  A thread of the forward keeps a running maximum, the sum of
-// exponentials below it and the sum of the logits, so a row of any length is one pass; a row belongs to
+// exponentials below it and the sum of the logits, four vectors at a time, so a row of any length is one pass; a row belongs to
 // a wave, or to a workgroup where it is long, and where rows are too few to fill the chip each is cut
 // into parts whose numbers the second kernel joins.  That kernel also sums the rows' losses, in a fixed
 // order.  The backward needs m and z of a row alone, so it is cut into workgroups at will.  m and z are
@@ -55,115 +55,137 @@ __device__ __forceinline__ void join_lanes(float& m, float& z, float& total) {
   m = top;
 }
 
-// Writes a row's statistics and loss; false for rows left out.
-__device__ __forceinline__ void finish_row(const XentArgs& a, int64_t row, float m, float z, float total) {
+// A row's labels and their logits, which a row's kernel asks for before it reads the row.
+struct Labels {
+  float l, x_a, x_b;
+  bool counted, known;
+  __device__ __forceinline__ Labels() {}
+  __device__ __forceinline__ Labels(const XentArgs& a, int64_t row) {
+    const int64_t la = a.c.target[row], k = a.c.classes, off = row * a.c.row_stride;
+    l = a.c.target_b == nullptr ? 1.f : a.c.mix != nullptr ? a.c.mix[row] : a.c.mix_value;
+    const int64_t lb = a.c.target_b != nullptr && l != 1.f ? a.c.target_b[row] : la;
+    counted = la != a.c.ignore_index;
+    known = la >= 0 && la < k && lb >= 0 && lb < k;
+    x_a = known ? load_any(a.c.logits, a.c.dtype, off + la) : 0.f;
+    x_b = known ? load_any(a.c.logits, a.c.dtype, off + lb) : 0.f;
+  }
+};
+
+// Writes a row's statistics and loss.
+__device__ __forceinline__ void finish_row(const XentArgs& a, int64_t row, const Labels& y, float m, float z, float total) {
   a.stats[2 * row] = m;
   a.stats[2 * row + 1] = 1.f / z;
-  const int64_t la = a.c.target[row], k = a.c.classes;
   float loss = 0.f;
-  if (la != a.c.ignore_index) {
-    const int64_t off = row * a.c.row_stride;
-    const float l = a.c.target_b == nullptr ? 1.f : a.c.mix != nullptr ? a.c.mix[row] : a.c.mix_value;
-    const int64_t lb = a.c.target_b != nullptr && l != 1.f ? a.c.target_b[row] : la;
-    if (la < 0 || la >= k || lb < 0 || lb >= k) {
-      loss = __builtin_nanf("");  // no such class
-    } else {
-      const float ln_z = logf(z), s = a.c.smoothing;
-      if (s != 1.f) {
-        float picked = 0.f;
-        if (l != 0.f) picked += l * (m - load_any(a.c.logits, a.c.dtype, off + la));
-        if (l != 1.f) picked += (1.f - l) * (m - load_any(a.c.logits, a.c.dtype, off + lb));
-        loss = (1.f - s) * (picked + ln_z);
-      }
-      if (s != 0.f) loss += s * (m - total / static_cast<float>(k) + ln_z);
+  if (y.counted) {
+    const float ln_z = logf(z), s = a.c.smoothing;
+    if (s != 1.f) {  // a term of weight zero is left out, whatever its logit
+      float picked = 0.f;
+      if (y.l != 0.f) picked += y.l * (m - y.x_a);
+      if (y.l != 1.f) picked += (1.f - y.l) * (m - y.x_b);
+      loss = (1.f - s) * (picked + ln_z);
     }
+    if (s != 0.f) loss += s * (m - total / static_cast<float>(a.c.classes) + ln_z);
+    if (!y.known) loss = __builtin_nanf("");  // no such class
   }
   a.losses[row] = loss;
 }
+
+// Numbers of logits begin .. end - 1 of a row that a thread takes, T of them apart by a vector.
+struct Numbers {
+  float m = -__builtin_inff(), z = 0.f, total = 0.f;
+  // N vectors, of which the last may have only n values.
+  template <class R, int N, bool WHOLE>
+  __device__ __forceinline__ void add(const typename R::Raw (&raw)[N], int n) {
+    constexpr int V = R::kVec;
+    float v[N][V], top = m;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      R::widen(raw[u], v[u]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if (WHOLE || j < n) total += v[u][j];
+        if (!WHOLE && j >= n) v[u][j] = -__builtin_inff();
+        top = fmaxf(top, v[u][j]);
+      }
+    }
+    z *= exp_below(m, top);
+    m = top;
+    if (top == -__builtin_inff()) return;
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+#pragma unroll
+      for (int j = 0; j < V; ++j) z += __builtin_amdgcn_exp2f((v[u][j] - top) * kLog2e);
+  }
+  template <class R, int T>
+  __device__ __forceinline__ void scan(const typename R::Elem* x, int64_t begin, int64_t end, int t) {
+    constexpr int V = R::kVec, U = 4;  // vectors in flight
+    int64_t i = begin + t * V;
+    for (; i + (U - 1) * T * V + V <= end; i += U * T * V) {
+      typename R::Raw raw[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = R::raw(x + i + u * T * V);
+      add<R, U, true>(raw, V);
+    }
+    for (; i < end; i += T * V) {
+      const int n = end - i < V ? static_cast<int>(end - i) : V;
+      typename R::Raw raw[1] = {R::zero()};
+      if (n == V) {
+        raw[0] = R::raw(x + i);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (j < n) R::set(raw[0], j, x[i + j]);
+      }
+      add<R, 1, false>(raw, n);
+    }
+  }
+  __device__ __forceinline__ void join_wave() { join_lanes<64>(m, z, total); }
+};
 
 // T threads a (row, part).
 template <class Ty, int T>
 __global__ void __launch_bounds__(256) xent_fwd_kernel(XentArgs a) {
   typedef Row<Ty> R;
-  constexpr int V = R::kVec, UNITS = 256 / T;
+  constexpr int UNITS = 256 / T;
   const int t = threadIdx.x % T;
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * UNITS + threadIdx.x / T;
   const int64_t row = unit / a.n_parts;
   const int part = static_cast<int>(unit % a.n_parts);
   const bool valid = row < a.c.rows;  // uniform over a unit
-  float m = -__builtin_inff(), z = 0.f, total = 0.f;
+  Labels y;
+  if (valid && t == 0 && a.n_parts == 1) y = Labels(a, row);
+  Numbers s;
   if (valid) {
-    const typename R::Elem* x = static_cast<const typename R::Elem*>(a.c.logits) + row * a.c.row_stride;
     const int64_t begin = static_cast<int64_t>(part) * a.part_len, stop = begin + a.part_len;
-    const int64_t end = stop < a.c.classes ? stop : a.c.classes;
-    for (int64_t i = begin + t * V; i < end; i += T * V) {
-      float v[V];
-      const int n = end - i < V ? static_cast<int>(end - i) : V;
-      if (n == V) {
-        R::load(x + i, v);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = j < n ? R::to_f32(x[i + j]) : -__builtin_inff();
-      }
-      float top = m;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (j < n) total += v[j];
-        top = fmaxf(top, v[j]);
-      }
-      z *= exp_below(m, top);
-      m = top;
-      if (top != -__builtin_inff()) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) z += __builtin_amdgcn_exp2f((v[j] - top) * kLog2e);
-      }
-    }
+    s.scan<R, T>(static_cast<const typename R::Elem*>(a.c.logits) + row * a.c.row_stride, begin,
+                 stop < a.c.classes ? stop : a.c.classes, t);
   }
-  join_lanes<64>(m, z, total);
+  s.join_wave();
   if constexpr (T == 256) {
     __shared__ float lds[3][4];
     const int wave = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) lds[0][wave] = m, lds[1][wave] = z, lds[2][wave] = total;
+    if ((threadIdx.x & 63) == 0) lds[0][wave] = s.m, lds[1][wave] = s.z, lds[2][wave] = s.total;
     __syncthreads();
-    m = lds[0][0], z = lds[1][0], total = lds[2][0];
+    s.m = lds[0][0], s.z = lds[1][0], s.total = lds[2][0];
 #pragma unroll
     for (int w = 1; w < 4; ++w) {
-      join(m, z, lds[0][w], lds[1][w]);
-      total += lds[2][w];
+      join(s.m, s.z, lds[0][w], lds[1][w]);
+      s.total += lds[2][w];
     }
   }
   if (t != 0 || !valid) return;
   if (a.n_parts == 1) {
-    finish_row(a, row, m, z, total);
+    finish_row(a, row, y, s.m, s.z, s.total);
   } else {
     float* p = a.parts + unit * 3;
-    p[0] = m, p[1] = z, p[2] = total;
+    p[0] = s.m, p[1] = s.z, p[2] = s.total;
   }
 }
 
-// Joins the parts of rows, 16 lanes a row (n_parts > 1), and sums the losses (one workgroup then).
-__global__ void __launch_bounds__(kSumThreads) xent_sum_kernel(XentArgs a) {
-  constexpr int ROWS = kSumThreads / kSumLanes;
+// The rows' losses, which this workgroup's threads see, as their sum or mean.
+__device__ __forceinline__ void sum_rows(const XentArgs& a) {
   __shared__ double sums[kSumThreads / 64];
   __shared__ int64_t counts[kSumThreads / 64];
-  if (a.n_parts > 1) {
-    const int lane = threadIdx.x % kSumLanes;
-    for (int64_t base = static_cast<int64_t>(blockIdx.x) * ROWS; base < a.c.rows; base += static_cast<int64_t>(gridDim.x) * ROWS) {
-      const int64_t row = base + threadIdx.x / kSumLanes;
-      float m = -__builtin_inff(), z = 0.f, total = 0.f;
-      if (row < a.c.rows) {
-        const float* p = a.parts + row * a.n_parts * 3;
-        for (int i = lane; i < a.n_parts; i += kSumLanes) {
-          join(m, z, p[3 * i], p[3 * i + 1]);
-          total += p[3 * i + 2];
-        }
-      }
-      join_lanes<kSumLanes>(m, z, total);
-      if (lane == 0 && row < a.c.rows) finish_row(a, row, m, z, total);
-    }
-    __syncthreads();  // the losses of this workgroup's rows, which are all rows where they are summed
-  }
-  if (a.loss == nullptr) return;
   double sum = 0.0;
   int64_t count = 0;
 #pragma unroll 4
@@ -184,6 +206,48 @@ __global__ void __launch_bounds__(kSumThreads) xent_sum_kernel(XentArgs a) {
     *a.loss = static_cast<float>(count ? sum * weight : a.c.reduction == OW_REDUCE_MEAN ? __builtin_nan("") : 0.0);
     *a.weight = static_cast<float>(weight);
   }
+}
+
+// Few short rows and their sum in one launch: one workgroup, a wave a row.
+template <class Ty>
+__global__ void __launch_bounds__(kSumThreads) xent_few_kernel(XentArgs a) {
+  typedef Row<Ty> R;
+  const int lane = threadIdx.x & 63;
+  for (int64_t row = threadIdx.x >> 6; row < a.c.rows; row += kSumThreads / 64) {
+    Labels y;
+    if (lane == 0) y = Labels(a, row);
+    Numbers s;
+    s.scan<R, 64>(static_cast<const typename R::Elem*>(a.c.logits) + row * a.c.row_stride, 0, a.c.classes, lane);
+    s.join_wave();
+    if (lane == 0) finish_row(a, row, y, s.m, s.z, s.total);
+  }
+  __syncthreads();
+  sum_rows(a);
+}
+
+// Joins the parts of rows, 16 lanes a row (n_parts > 1), and sums the losses (one workgroup then).
+__global__ void __launch_bounds__(kSumThreads) xent_sum_kernel(XentArgs a) {
+  constexpr int ROWS = kSumThreads / kSumLanes;
+  if (a.n_parts > 1) {
+    const int lane = threadIdx.x % kSumLanes;
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * ROWS; base < a.c.rows; base += static_cast<int64_t>(gridDim.x) * ROWS) {
+      const int64_t row = base + threadIdx.x / kSumLanes;
+      float m = -__builtin_inff(), z = 0.f, total = 0.f;
+      Labels y;
+      if (row < a.c.rows) {
+        if (lane == 0) y = Labels(a, row);
+        const float* p = a.parts + row * a.n_parts * 3;
+        for (int i = lane; i < a.n_parts; i += kSumLanes) {
+          join(m, z, p[3 * i], p[3 * i + 1]);
+          total += p[3 * i + 2];
+        }
+      }
+      join_lanes<kSumLanes>(m, z, total);
+      if (lane == 0 && row < a.c.rows) finish_row(a, row, y, m, z, total);
+    }
+    __syncthreads();  // the losses of this workgroup's rows, which are all rows where they are summed
+  }
+  if (a.loss != nullptr) sum_rows(a);
 }
 
 struct XentBwdArgs {
@@ -278,10 +342,17 @@ int check(const OwCrossEntropy* c) {
   return OW_OK;
 }
 
+// Rows that one workgroup takes with their sum: two a wave, below which a second launch costs more than
+// the rows gain from more workgroups.
+constexpr int kFewRows = 2 * kSumThreads / 64;
+bool few_rows(const XentArgs& a) { return a.loss != nullptr && a.c.rows <= kFewRows && a.c.classes <= kLong; }
+
 template <class Ty>
 void launch_fwd(const XentArgs& a, hipStream_t s) {
   const int64_t units = a.c.rows * a.n_parts;
-  if (a.c.classes <= kLong)
+  if (few_rows(a))
+    hipLaunchKernelGGL((xent_few_kernel<Ty>), dim3(1), dim3(kSumThreads), 0, s, a);
+  else if (a.c.classes <= kLong)
     hipLaunchKernelGGL((xent_fwd_kernel<Ty, 64>), dim3(static_cast<unsigned>((units + 3) / 4)), dim3(256), 0, s, a);
   else
     hipLaunchKernelGGL((xent_fwd_kernel<Ty, 256>), dim3(static_cast<unsigned>(units)), dim3(256), 0, s, a);
@@ -339,7 +410,7 @@ int ow_cross_entropy_fwd(const OwCrossEntropy* ce, float* stats, float* losses, 
     else ow::launch_fwd<ow::F16>(a, s);
     if (int rc = ow::hip_status(hipGetLastError(), "xent_fwd_kernel launch")) return rc;
   }
-  if (reduced || a.n_parts > 1) {
+  if ((reduced && (ce->rows == 0 || !ow::few_rows(a))) || a.n_parts > 1) {
     const int64_t rows_at_once = ow::kSumThreads / ow::kSumLanes;
     const int64_t groups = reduced ? 1 : (ce->rows + rows_at_once - 1) / rows_at_once;
     hipLaunchKernelGGL(ow::xent_sum_kernel, dim3(static_cast<unsigned>(groups)), dim3(ow::kSumThreads), 0, s, a);
