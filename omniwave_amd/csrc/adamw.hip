@@ -19,8 +19,8 @@
 // that is not zero is never held as zero, since m / (0 + eps) would be a step of m / eps.  The update
 // itself uses the unrounded m and v.  Arithmetic is not contracted to fused multiply-adds: rounding
 // after each operation is what the states' definition says, and a value next to a border of two codes
-// then falls on the same side everywhere.  Roots and the update's quotient are the hardware's, within a
-// unit in the last place each; 1 - b^t is formed as -expm1(t ln b), which keeps its relative precision
+// then falls on the same side everywhere.  The update's quotient (and a root that is not stored) is the
+// hardware's, within a unit in the last place; 1 - b^t is formed as -expm1(t ln b), which keeps its relative precision
 // where b^t is near one.
 #include <hip/hip_runtime.h>
 
@@ -152,7 +152,7 @@ __device__ __forceinline__ uint32_t encode4(const float (&v)[4], float& scale) {
     most = u > most ? u : most;
   }
   most = lanes_reduce<MaxUintOp, 64>(most);
-  scale = __uint_as_float(most) / kFp8Most;
+  scale = __uint_as_float(most) * (1.f / kFp8Most);
   if (scale < kLeastScale) scale = 0.f;
   const float inv = scale != 0.f ? 1.f / scale : 0.f;
   float y[4];
@@ -266,7 +266,8 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_kernel(StepArgs<kPtrsOf<Ty,
       const float gj = g[k][j] * coef;
       m[k][j] = m[k][j] * h.b1 + gj * h.c1;
       v[k][j] = v[k][j] * h.b2 + gj * gj * h.c2;
-      root[j] = __builtin_amdgcn_sqrtf(v[k][j]);
+      // A root that is stored is rounded correctly, as m and v are: its code is then the definition's.
+      root[j] = BITS == 8 ? sqrtf(v[k][j]) : __builtin_amdgcn_sqrtf(v[k][j]);
       p[k][j] = p[k][j] * keep - step * (m[k][j] * __builtin_amdgcn_rcpf(root[j] * unbias + h.eps));
     }
     if constexpr (MASTER) store4<F32>(a.t.ptr[PTRS - 1][i], idx, left, p[k]);

@@ -62,7 +62,7 @@ def _run_forward(logits, target, target_b, mix, mix_value, label_smoothing, igno
     desc, keep = _descriptor(logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction)
     rows, lib = desc.rows, _native.lib()
     ref = ctypes.byref(desc)
-    if device.index != torch.cuda.current_device():
+    if device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):  # the size goes by the device's compute units
             ws_bytes = lib.ow_cross_entropy_workspace(ref)
     else:
@@ -81,7 +81,7 @@ def _run_forward(logits, target, target_b, mix, mix_value, label_smoothing, igno
 def _run_backward(up, aux, desc, logits, target, target_b, mix, *options) -> Tensor:
     """The logits' gradient; ``up``: the upstream gradient of the loss (a value) or the losses; ``desc``:
     the forward's descriptor, or None."""
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    grad = torch.empty_like(logits, memory_format=torch.contiguous_format)
     if not grad.numel():
         return grad
     # The forward's descriptor serves where the inputs came back as they were (hooks on saved tensors may

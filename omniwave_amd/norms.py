@@ -123,7 +123,7 @@ def _descriptor(x, delta, post_weight, gate, scale, next_weight, eps):
 
 def _on(device: torch.device, fn, *args) -> None:
     """One native call on ``device``'s current stream (the call's last argument)."""
-    if device.index != torch.cuda.current_device():
+    if device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             _native.check(fn(*args, _stream_ptr(device)), fn.__name__)
     else:
@@ -131,7 +131,7 @@ def _on(device: torch.device, fn, *args) -> None:
 
 
 def _empty(t: Tensor) -> Tensor:
-    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _run_forward(x, delta, post_weight, gate, scale, next_weight, eps):
@@ -177,7 +177,7 @@ def _run_backward(dout, dnext, desc, x, delta, post_weight, gate, scale, next_we
     lib, ref, device = _native.lib(), ctypes.byref(desc), x.device
     workspace, ws_bytes, ws_ptr = None, 0, None
     if ptr[2] or ptr[3] or ptr[4]:
-        if device.index != torch.cuda.current_device():
+        if device.index != torch._C._cuda_getDevice():
             with torch.cuda.device(device):  # the size goes by the device's compute units
                 ws_bytes = lib.ow_block_norms_bwd_workspace(ref)
         else:

@@ -135,15 +135,15 @@ class AdamW(torch.optim.Optimizer):
                 if dtype == FP8:
                     entry[name] = entry[name].view(FP8)
 
-    def _check_state(self, p: Tensor) -> None:
-        entry = self.state[p]
-        for name, (dtype, shape) in self._layout(p).items():
+    def _check_state(self, p: Tensor, layout: dict | None = None) -> None:
+        entry, device = self.state[p], p.device
+        for name, (dtype, shape) in (self._layout(p) if layout is None else layout).items():
             t = entry.get(name)
-            if not isinstance(t, Tensor) or t.dtype != dtype or t.shape != shape or t.device != p.device \
+            if not isinstance(t, Tensor) or t.dtype != dtype or t.shape != shape or t.device != device \
                     or not t.is_contiguous():
                 got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, Tensor) else repr(t)
                 raise ValueError(f"state {name!r} of a parameter of shape {tuple(p.shape)} must be {dtype} {tuple(shape)}, "
-                                 f"contiguous on {p.device}; got {got}")
+                                 f"contiguous on {device}; got {got}")
 
     def load_state_dict(self, state_dict: dict) -> None:
         """``torch.optim.Optimizer.load_state_dict``; states keep their own dtypes, and those of
@@ -268,8 +268,8 @@ class _Plan:
                                  f"{tuple(g.shape)} on {g.device}")
             if not opt.state[p]:
                 opt._first_state(p)
-            opt._check_state(p)
             layout = opt._layout(p)
+            opt._check_state(p, layout)
             key = (p.dtype, 8 if "exp_avg_sq_root" in layout else 32, "master" in layout)
             kinds.setdefault(key, _Kind(*key)).add(i, p, opt.state[p], owner[i])
         self.kinds = list(kinds.values())
