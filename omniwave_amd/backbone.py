@@ -15,8 +15,9 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch import Tensor
 
-from omniwave_amd.block import OmniWeaveBlock
+from omniwave_amd.block import RMS_EPS, OmniWeaveBlock
 from omniwave_amd.hip import stem_hip, stem_is_supported
+from omniwave_amd.norms import rms_norm_hip
 from omniwave_amd.routing import build_stage_schedule
 
 
@@ -34,7 +35,7 @@ class _Stage(nn.Module):
     """Optional anchor Linear, then blocks on the stage schedule (backbone.py:30-80)."""
 
     def __init__(self, height, width, dim, depth, channel_tile, expansion, layer_scale_init, spatial_tile,
-                 use_anchor, backend, drop_path_rates) -> None:
+                 use_anchor, backend, drop_path_rates, post_norm=False) -> None:
         super().__init__()
         self.anchor: nn.Linear | None = nn.Linear(dim, dim, bias=False) if use_anchor else None
         self.blocks = nn.ModuleList()
@@ -42,20 +43,35 @@ class _Stage(nn.Module):
             self.blocks.append(OmniWeaveBlock(
                 height=height, width=width, dim=dim, channel_tile=channel_tile, route=route,
                 radix_level=radix_level, expansion=expansion, layer_scale_init=layer_scale_init,
-                spatial_tile=spatial_tile, backend=backend, drop_path_rate=rate,
+                spatial_tile=spatial_tile, backend=backend, drop_path_rate=rate, post_norm=post_norm,
             ))
 
     def forward(self, x: Tensor) -> Tensor:
         if self.anchor is not None:
             x = self.anchor(x)
+        if self._takes_normed(x):
+            return self._forward_normed(x)
         for block in self.blocks:
             x = block(x)
+        return x
+
+    def _takes_normed(self, x: Tensor) -> bool:
+        return len(self.blocks) > 0 and all(block.takes_normed(x) for block in self.blocks)
+
+    def _forward_normed(self, x: Tensor) -> Tensor:
+        """The blocks with ``post_norm`` in a row: the norm before the first one, then each block's kernel
+        behind its BiGEMM forms the norm before the next."""
+        normed = rms_norm_hip(x, self.blocks[0].norm_weight, RMS_EPS)
+        for block, following in zip(self.blocks, [*self.blocks[1:], None]):
+            x, normed = block.forward_normed(x, normed, None if following is None else following.norm_weight)
         return x
 
     def forward_blocks_s2d(self, x: Tensor, factor: int) -> Tensor:
         """``space_to_depth`` of the blocks' output (the anchor is the caller's); the last block
         writes that layout itself when it can, and each block hands the next its RMSNorm
         statistics when it can (``OmniWeaveBlock.forward_chain``)."""
+        if self._takes_normed(x):
+            return space_to_depth_nhwc(self._forward_normed(x), factor)
         x, stats = self._chain(self.blocks[:-1], x)
         r = self.blocks[-1].forward_chain(x, stats, factor)
         if r is not None:
@@ -65,6 +81,8 @@ class _Stage(nn.Module):
 
     def forward_blocks(self, x: Tensor) -> Tensor:
         """The blocks (the anchor is the caller's), chained as in ``forward_blocks_s2d``."""
+        if self._takes_normed(x):
+            return self._forward_normed(x)
         return self._chain(self.blocks, x)[0]
 
     @staticmethod
@@ -80,7 +98,8 @@ class _Stage(nn.Module):
 
 
 class OmniWeaveBackbone(nn.Module):
-    """Input ``[B, 3, H, W]`` (NCHW) -> logits ``[B, num_classes]``."""
+    """Input ``[B, 3, H, W]`` (NCHW) -> logits ``[B, num_classes]``.  ``post_norm``: every block also
+    normalises what it adds (``OmniWeaveBlock``)."""
 
     def __init__(
         self,
@@ -95,6 +114,7 @@ class OmniWeaveBackbone(nn.Module):
         backend: str = "auto",
         input_size: int = 224,
         drop_path_rate: float = 0.0,
+        post_norm: bool = False,
     ) -> None:
         super().__init__()
         widths = widths or [128, 256, 512, 1024]
@@ -121,7 +141,7 @@ class OmniWeaveBackbone(nn.Module):
                 height=resolutions[i], width=resolutions[i], dim=widths[i], depth=depths[i],
                 channel_tile=channel_tiles[i], expansion=expansion, layer_scale_init=layer_scale_init,
                 spatial_tile=spatial_tile, use_anchor=(i + 1) in anchor_stages, backend=backend,
-                drop_path_rates=rates[offset:offset + depths[i]],
+                drop_path_rates=rates[offset:offset + depths[i]], post_norm=post_norm,
             ))
             offset += depths[i]
         self.head = nn.Linear(widths[-1], num_classes)

@@ -4,6 +4,11 @@ Parameter names, shapes and initialisation match the reference so state_dicts in
 When the resolved backend is ``hip`` the whole block runs as one fused kernel
 (``bigemm_block_hip``); otherwise RMSNorm runs here and ``bigemm`` (a module-level import, so
 callers can patch ``omniwave_amd.block.bigemm``) computes the delta.
+
+With ``post_norm`` (no counterpart in the reference) the delta is normalised too, by a weight of its own,
+before LayerScale: ``x + drop * gamma * RMSNorm(BiGEMM(RMSNorm(x)))``.  On the hip backend the BiGEMM kernel
+is then followed by ``block_norms_hip``, which also forms the next block's normalised input where a
+stage runs its blocks in a row.
 """
 
 from __future__ import annotations
@@ -15,10 +20,18 @@ import torch.nn as nn
 from torch import Tensor
 
 from omniwave_amd.bigemm import bigemm
-from omniwave_amd.hip import _block, _chain, bigemm_block_s2d_hip, drop_path_scale, hip_is_supported
+from omniwave_amd.hip import (_block, _chain, bigemm_block_s2d_hip, bigemm_delta_hip, drop_path_scale,
+                              hip_is_supported)
+from omniwave_amd.norms import MAX_CHANNELS, block_norms_hip
 from omniwave_amd.routing import RoutePlan, build_route_plan
 
 RMS_EPS = 1e-6  # omniweave/models/block.py:84
+
+
+def _rms_norm(x: Tensor, weight: Tensor) -> Tensor:
+    """RMSNorm in fp32, for backends without ``block_norms_hip``."""
+    x = x.float()
+    return x * torch.rsqrt(x.square().mean(dim=-1, keepdim=True) + RMS_EPS) * weight.float()
 
 
 class OmniWeaveBlock(nn.Module):
@@ -37,6 +50,7 @@ class OmniWeaveBlock(nn.Module):
         spatial_tile: int = 16,
         backend: str = "auto",
         drop_path_rate: float = 0.0,
+        post_norm: bool = False,
     ) -> None:
         super().__init__()
         if not 0.0 <= drop_path_rate < 1.0:
@@ -59,6 +73,11 @@ class OmniWeaveBlock(nn.Module):
         self.b_v = nn.Parameter(torch.empty(q_c, d, rd))
         self.b_o = nn.Parameter(torch.empty(q_c, rd, d))
         self.gamma = nn.Parameter(torch.full((dim,), layer_scale_init))
+        self.post_norm = post_norm
+        if post_norm:
+            self.post_norm_weight = nn.Parameter(torch.ones(dim))
+            # LayerScale follows the norm, so the BiGEMM itself has none.
+            self.register_buffer("_ones", torch.ones(dim), persistent=False)
         self.fp8 = False  # e4m3fn channel side (inference with the hip backend); see enable_fp8
         self._init_weights()
 
@@ -86,12 +105,51 @@ class OmniWeaveBlock(nn.Module):
         mask = torch.empty(shape, dtype=delta.dtype, device=delta.device).bernoulli_(keep)
         return delta * mask / keep
 
+    def _drop_scale(self, x: Tensor) -> Tensor | None:
+        """Drop-path factors of the images (training), None where nothing is dropped."""
+        if not (self.training and self.drop_path_rate > 0):
+            return None
+        return drop_path_scale(x.shape[0], self.drop_path_rate, x.dtype, x.device)
+
+    def takes_normed(self, x: Tensor) -> bool:
+        """Whether ``forward_normed`` can run ``x``: a block with ``post_norm`` on the hip backend, not in fp8
+        (whose kernel wants the norm fused)."""
+        return self.post_norm and not self.fp8 and self.dim <= MAX_CHANNELS and self._fused(x)
+
+    def forward_normed(self, x: Tensor, normed: Tensor, next_weight: Tensor | None) -> tuple[Tensor, Tensor | None]:
+        """(``self(x)``, the same under the next block's norm), given ``normed``, x under this block's norm:
+        the BiGEMM on it, then one kernel for the norm after the block, LayerScale, drop-path, the
+        residual and the norm with ``next_weight`` (None: no second output)."""
+        delta = bigemm_delta_hip(x=normed, plan=self.plan, a_u=self.a_u, a_v=self.a_v, a_o=self.a_o, b_u=self.b_u,
+                                 b_v=self.b_v, b_o=self.b_o, gamma=self._ones)
+        return block_norms_hip(x, delta, post_weight=self.post_norm_weight, gate=self.gamma, scale=self._drop_scale(x),
+                               next_weight=next_weight, eps=RMS_EPS)
+
+    def _forward_post_norm(self, x: Tensor) -> Tensor:
+        ops = (self.a_u, self.a_v, self.a_o, self.b_u, self.b_v, self.b_o, self._ones)
+        fused = self.dim <= MAX_CHANNELS and self._fused(x)
+        if self.fp8 and self.training:
+            raise RuntimeError("the fp8 BiGEMM variant is inference-only; call model.eval()")
+        if self.fp8 and not fused:
+            raise RuntimeError("the fp8 BiGEMM variant needs the hip backend on a gfx950 GPU")
+        if fused:
+            delta = _block(x, self.norm_weight, self.plan, *ops, RMS_EPS, residual=False, fp8=self.fp8)
+            return block_norms_hip(x, delta, post_weight=self.post_norm_weight, gate=self.gamma,
+                                   scale=self._drop_scale(x), eps=RMS_EPS)[0]
+        delta = bigemm(x=_rms_norm(x, self.norm_weight).to(x.dtype), plan=self.plan,
+                       **dict(zip(("a_u", "a_v", "a_o", "b_u", "b_v", "b_o", "gamma"), ops)), backend=self.backend)
+        branch = self.gamma * _rms_norm(delta, self.post_norm_weight)
+        scale = self._drop_scale(x)
+        if scale is not None:
+            branch = branch * scale.reshape(-1, 1, 1, 1)
+        return (x.float() + branch).to(x.dtype)
+
     def forward_s2d(self, x: Tensor, factor: int = 2) -> Tensor | None:
         """``space_to_depth(self(x), factor)`` as one kernel — the block writes its output rows
         straight into the ``[B, H/f, W/f, C f^2]`` layout (omniweave/models/backbone.py:14-27,
         183-186) — when nothing needs a gradient and the fused hip path takes ``x`` (bf16 /
         fp16); ``None`` otherwise, and the caller composes the two."""
-        if torch.is_grad_enabled() or (self.training and (self.drop_path_rate > 0 or self.fp8)):
+        if self.post_norm or torch.is_grad_enabled() or (self.training and (self.drop_path_rate > 0 or self.fp8)):
             return None
         if x.dtype not in (torch.bfloat16, torch.float16) or not self._fused(x):
             return None
@@ -106,7 +164,7 @@ class OmniWeaveBlock(nn.Module):
         (inference): returns ``(y, stats)``, ``stats`` being the RMSNorm statistics of ``y`` for
         the next block (or None), given ``stats`` of ``x`` from the previous block; ``None``
         when the chained hip path does not apply and the caller uses the plain calls."""
-        if torch.is_grad_enabled() or (self.training and (self.drop_path_rate > 0 or self.fp8)):
+        if self.post_norm or torch.is_grad_enabled() or (self.training and (self.drop_path_rate > 0 or self.fp8)):
             return None
         if x.dtype not in (torch.bfloat16, torch.float16) or not self._fused(x):
             return None
@@ -117,6 +175,8 @@ class OmniWeaveBlock(nn.Module):
 
     def forward(self, x: Tensor) -> Tensor:
         """``x``: ``[B, H, W, C]`` -> ``[B, H, W, C]``."""
+        if self.post_norm:
+            return self._forward_post_norm(x)
         params = (self.a_u, self.a_v, self.a_o, self.b_u, self.b_v, self.b_o, self.gamma)
         dropping = self.training and self.drop_path_rate > 0
         fused = self._fused(x)

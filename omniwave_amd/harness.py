@@ -10,6 +10,8 @@ Mirrors the reference's harness so its result files and gates read the same:
 * ``run_benchmark`` — scripts/benchmark.py:120-320 with the same row schema
   (scripts/benchmark.py:194-217, 288-310), every route of the block schedule rather than only
   ``local``, plus ``"route"`` in each row;
+* ``run_training_benchmark`` — rows of whole training steps (forward, cross-entropy, backward, AdamW step;
+  the loop body of omniweave/training/engine.py:193-258) for the configured ``train_batch_sizes``;
 * ``evaluate_operator_gates`` / ``pair_operator_rows`` — scripts/check_gates.py:12-132, with
   ``hip`` rows paired against the fastest ``reference`` / ``compile`` row of the same shape,
   batch, dtype and route (``triton`` rows pair as before).
@@ -245,10 +247,78 @@ def run_model_benchmark(config: dict[str, Any], device: torch.device) -> list[di
     return rows
 
 
+class TrainingStep:
+    """One training step of a model as the framework runs it: ``step(images, labels)`` returns the loss.
+
+    ``labels_b`` / ``mix``: the second labels and the weight of the first ones of mixed images."""
+
+    def __init__(self, model: nn.Module, *, lr: float = 1e-3, weight_decay: float = 0.05, state_bits: int = 32,
+                 master_weights: bool = True, max_grad_norm: float | None = 1.0, label_smoothing: float = 0.1) -> None:
+        from omniwave_amd.optim import AdamW
+
+        self.model, self.label_smoothing = model, label_smoothing
+        matrices = [p for p in model.parameters() if p.requires_grad and p.dim() >= 2]
+        vectors = [p for p in model.parameters() if p.requires_grad and p.dim() < 2]
+        groups = [{"params": matrices, "weight_decay": weight_decay}, {"params": vectors, "weight_decay": 0.0}]
+        self.optimizer = AdamW([g for g in groups if g["params"]], lr=lr, state_bits=state_bits,
+                               master_weights=master_weights, max_grad_norm=max_grad_norm)
+
+    def step(self, images: torch.Tensor, labels: torch.Tensor, labels_b: torch.Tensor | None = None,
+             mix: torch.Tensor | float | None = None) -> torch.Tensor:
+        from omniwave_amd.loss import cross_entropy_hip
+
+        self.optimizer.zero_grad(set_to_none=True)
+        loss = cross_entropy_hip(self.model(images), labels, target_b=labels_b, mix=mix,
+                                 label_smoothing=self.label_smoothing)
+        loss.backward()
+        self.optimizer.step()
+        return loss.detach()
+
+
+def run_training_benchmark(config: dict[str, Any], device: torch.device) -> list[dict[str, Any]]:
+    """Rows of training steps: ``models`` x ``resolutions`` x ``train_dtypes`` x ``train_batch_sizes``, with
+    ``training`` (``TrainingStep``'s options) and ``model_options`` (the model's)."""
+    from omniwave_amd.registry import create_model
+
+    rows: list[dict[str, Any]] = []
+    for model_name in config.get("models", ["omniweave_t"]):
+        for resolution in config["resolutions"]:
+            for dtype_name in config.get("train_dtypes", ["bfloat16"]):
+                for batch in config["train_batch_sizes"]:
+                    base = {"kind": "train", "model": model_name, "resolution": resolution, "dtype": dtype_name,
+                            "batch_size": batch, "backend": "hip"}
+                    try:
+                        dtype = getattr(torch, dtype_name)
+                        model = create_model(model_name, backend="hip", input_size=resolution,
+                                             **config.get("model_options", {})).to(device=device, dtype=dtype).train()
+                        training = TrainingStep(model, **config.get("training", {}))
+                        images = torch.randn(batch, 3, resolution, resolution, device=device).to(dtype)
+                        labels = torch.randint(0, model.head.out_features, (batch,), device=device)
+                        losses = []
+                        res = benchmark_fn(lambda: losses.append(training.step(images, labels)),
+                                           warmup=config.get("warmup", 100), iterations=config.get("iterations", 1000))
+                        if not torch.isfinite(losses[-1]):
+                            raise RuntimeError("the training step's loss is not finite")
+                        rows.append({
+                            **base,
+                            "p50_ms": res.p50_seconds * 1000, "p90_ms": res.p90_seconds * 1000,
+                            "p99_ms": res.p99_seconds * 1000, "mean_ms": res.mean_seconds * 1000,
+                            "images_per_second": batch * res.throughput_per_second,
+                            "first_loss": float(losses[0]), "last_loss": float(losses[-1]),
+                            "peak_allocated_mb": res.peak_allocated_bytes / 2 ** 20,
+                            "peak_reserved_mb": res.peak_reserved_bytes / 2 ** 20,
+                        })
+                    except (ValueError, RuntimeError) as exc:
+                        rows.append({**base, "error": str(exc)})
+    return rows
+
+
 def run_benchmark(config: dict[str, Any], device: torch.device) -> list[dict[str, Any]]:
     rows = run_operator_benchmark(config, device) if "shapes" in config else []
     if "resolutions" in config:
         rows += run_model_benchmark(config, device)
+        if "train_batch_sizes" in config:
+            rows += run_training_benchmark(config, device)
     return rows
 
 

@@ -64,7 +64,8 @@ class AdamW(torch.optim.Optimizer):
     Parameters: contiguous, of fp32, bf16 or fp16, on one gfx950 GPU; gradients of the same dtype, dense.
     ``lr`` may be a 0-dim fp32 tensor on the GPU, which a captured step reads anew; other
     hyperparameters of a captured step are those of its capture.  States are made by the first step, which
-    therefore is not captured.
+    therefore is not captured.  A step raises the parameters' version counters; the replay of a captured one
+    cannot, so before an eager forward that follows replays call ``omniwave_amd.hip.clear_pack_cache()``.
 
     ``state[p]``: ``step`` (int32, the steps done, one for every 4,096 values), ``exp_avg`` and
     ``exp_avg_sq`` (fp32), or ``exp_avg`` and ``exp_avg_sq_root`` (e4m3fn) with ``exp_avg_scale`` and
@@ -213,6 +214,8 @@ class AdamW(torch.optim.Optimizer):
                 self._launch(plan.kinds, grads, hyper, device)
         else:
             self._launch(plan.kinds, grads, hyper, device)
+        # The kernels write past autograd's notice: what goes by a parameter's version has to see the change.
+        torch.autograd.graph.increment_version(plan.active)
         return loss
 
     def _launch(self, kinds: list[_Kind], grads: list[Tensor | None], hyper, device: torch.device) -> None:
@@ -275,6 +278,7 @@ class _Plan:
         self.kinds = list(kinds.values())
         for kind in self.kinds:
             kind.finish()
+        self.active = [params[i] for i in active]
         self.entries = list(opt.state.values())
         self.states = _Addresses(_tensors(self.entries))
 
