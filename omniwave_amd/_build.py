@@ -2,7 +2,8 @@
 
 The library is a plain C-ABI shared object (include/omniwave_amd.h): host route tables
 (route.cpp) and the HIP kernels + launchers (bigemm_fwd.hip).  It is written next to this
-file so it travels with the source tree.
+file so it travels with the source tree, as is the Python module _glue.so (torch_glue.cpp): the
+small operators' calls and autograd nodes over that library, host code against torch's headers.
 """
 
 from __future__ import annotations
@@ -10,6 +11,7 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+import sysconfig
 import tempfile
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
@@ -21,6 +23,8 @@ INCLUDE = REPO_DIR / "include"
 LIB_PATH = PKG_DIR / "libomniwave_amd.so"
 SOURCES = ["route.cpp", "bigemm_fwd.hip", "bigemm_fwd_resident.hip", "bigemm_fwd_wave16.hip", "bigemm_fwd_persist.hip", "bigemm_fwd_split.hip", "bigemm_fwd_f32.hip", "bigemm_fwd_x3.hip", "bigemm_bwd.hip", "bigemm_bwd_f32.hip", "bigemm_bwd_x3.hip", "bwd_block.hip", "stem.hip", "fwd_noalloc.hip",
            "block_norms.hip", "adamw.hip", "cross_entropy.hip"]
+GLUE_PATH = PKG_DIR / "_glue.so"
+GLUE_SOURCE = "torch_glue.cpp"
 ARCH = "gfx950"
 
 
@@ -48,12 +52,34 @@ def compile_flags() -> list[str]:
     ]
 
 
+def glue_commands(obj: str, out: str, lib_dir: str) -> tuple[list[str], list[str]]:
+    """Compile and link commands of the Python module (host compiler, torch's headers and libraries)."""
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    rocm = Path(hipcc()).resolve().parent.parent
+    if not (rocm / "include" / "hip").exists():
+        rocm = Path("/opt/rocm")
+    include = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", rocm / "include", INCLUDE,
+               sysconfig.get_paths()["include"]]
+    cc = shutil.which("g++") or "g++"
+    compile_cmd = [cc, "-O2", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+                   f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *[f"-I{p}" for p in include], "-c",
+                   str(CSRC / GLUE_SOURCE), "-o", obj]
+    link_cmd = [cc, "-shared", obj, "-o", out, f"-L{root / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
+                "-lc10_hip", f"-L{rocm / 'lib'}", "-lamdhip64", f"-L{lib_dir}", f"-l:{LIB_PATH.name}", "-Wl,-rpath,$ORIGIN"]
+    return compile_cmd, link_cmd
+
+
 def build(verbose: bool = False) -> Path:
-    """Compile every source into LIB_PATH (always recompiles); returns the library path."""
+    """Compile every source into LIB_PATH and GLUE_PATH (always recompiles); returns the library path."""
     cc = hipcc()
     with tempfile.TemporaryDirectory(prefix="ow_build_") as tmp:
         objs = [str(Path(tmp) / (Path(src).stem + ".o")) for src in SOURCES]
         cmds = [[cc, *compile_flags(), "-c", str(CSRC / src), "-o", obj] for src, obj in zip(SOURCES, objs)]
+        glue_out = str(Path(tmp) / GLUE_PATH.name)
+        glue_compile, glue_link = glue_commands(str(Path(tmp) / "torch_glue.o"), glue_out, tmp)
+        cmds.append(glue_compile)
         if verbose:
             for cmd in cmds:
                 print(" ".join(cmd), flush=True)
@@ -65,9 +91,13 @@ def build(verbose: bool = False) -> Path:
         if verbose:
             print(" ".join(cmd), flush=True)
         _run(cmd)
-        staged = LIB_PATH.with_suffix(".so.tmp")
-        shutil.copyfile(out_tmp, staged)
-        os.replace(staged, LIB_PATH)
+        if verbose:
+            print(" ".join(glue_link), flush=True)
+        _run(glue_link)
+        for built, path in ((out_tmp, LIB_PATH), (glue_out, GLUE_PATH)):
+            staged = path.with_suffix(".so.tmp")
+            shutil.copyfile(built, staged)
+            os.replace(staged, path)
     return LIB_PATH
 
 

@@ -349,6 +349,31 @@ def lib() -> ctypes.CDLL:
     return handle
 
 
+_glue = None
+_glue_error: str | None = None
+
+
+def glue():
+    """The module of the small operators' native calls, or None (``glue_error`` says why)."""
+    global _glue, _glue_error
+    if _glue is None and _glue_error is None:
+        if _load() is None:
+            _glue_error = _load_error
+            return None
+        try:
+            from omniwave_amd import _glue as module
+        except ImportError as exc:
+            _glue_error = f"cannot load _glue.so (run omniwave_amd._build.build()): {exc}"
+            return None
+        _glue = module
+    return _glue
+
+
+def glue_error() -> str | None:
+    glue()
+    return _glue_error
+
+
 def check(rc: int, what: str) -> None:
     """Raise the library's error text for a non-zero status."""
     if rc != OW_OK:

@@ -1,4 +1,8 @@
-"""Softmax cross-entropy of logits with its gradient, as HIP kernels (``cross_entropy.hip``)."""
+"""Softmax cross-entropy of logits with its gradient, as HIP kernels (``cross_entropy.hip``).
+
+A plain call is native, its autograd node included (``torch_glue.cpp``); the operator
+``omniwave_amd::cross_entropy_fwd`` takes the others (compilation, tracing, transforms, tensors to copy first).
+"""
 
 from __future__ import annotations
 
@@ -7,11 +11,10 @@ import math
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from omniwave_amd import _native
 from omniwave_amd.hip import _DTYPE_CODE, SUPPORTED_DTYPES, _plain
-from omniwave_amd.norms import _lies, _on, _rows, gpu_reason
+from omniwave_amd.norms import _on, _rows, gpu_reason
 
 
 def _check(logits, target, target_b, mix, label_smoothing, ignore_index, reduction) -> None:
@@ -54,81 +57,45 @@ def _descriptor(logits, target, target_b, mix, mix_value, label_smoothing, ignor
                                   _DTYPE_CODE[logits.dtype], reduction), keep
 
 
-def _run_forward(logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction):
-    """(the loss, or the losses of the rows; what the backward needs beside the inputs; the descriptor and
-    whether it points at the inputs themselves).  The second: the statistics of the rows, a row's weight in
-    the loss and, with a reduction, the losses."""
+def _run_forward(logits, target, target_b, mix, mix_value, label_smoothing, ignore_index,
+                 reduction) -> tuple[Tensor, Tensor]:
+    """(the loss, or the losses of the rows; what the backward needs beside the inputs: the statistics of the
+    rows, a row's weight in the loss and, with a reduction, the losses)."""
     device, reduced = logits.device, reduction != 0
-    desc, keep = _descriptor(logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction)
+    desc, _keep = _descriptor(logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction)
     rows, lib = desc.rows, _native.lib()
-    ref = ctypes.byref(desc)
-    if device.index != torch._C._cuda_getDevice():
-        with torch.cuda.device(device):  # the size goes by the device's compute units
-            ws_bytes = lib.ow_cross_entropy_workspace(ref)
-    else:
-        ws_bytes = lib.ow_cross_entropy_workspace(ref)
+    with torch.cuda.device(device):  # the size goes by the device's compute units
+        ws_bytes = lib.ow_cross_entropy_workspace(ctypes.byref(desc))
     aux = torch.empty(2 * rows + 1 + (rows if reduced else 0), dtype=torch.float32, device=device)
     loss = torch.empty(() if reduced else target.shape, dtype=torch.float32, device=device)
     workspace = torch.empty(ws_bytes // 4, dtype=torch.float32, device=device) if ws_bytes else None
     at, out = aux.data_ptr(), loss.data_ptr()
     weight = at + 8 * rows
-    _on(device, lib.ow_cross_entropy_fwd, ref, at, weight + 4 if reduced else out, out if reduced else None,
+    _on(device, lib.ow_cross_entropy_fwd, ctypes.byref(desc), at, weight + 4 if reduced else out, out if reduced else None,
         weight if reduced else None, None if workspace is None else workspace.data_ptr(), ws_bytes)
-    inputs = keep[0] is logits and keep[1] is target and keep[2] is target_b and keep[3] is mix
-    return loss, aux, desc if inputs else None
+    return loss, aux
 
 
-def _run_backward(up, aux, desc, logits, target, target_b, mix, *options) -> Tensor:
-    """The logits' gradient; ``up``: the upstream gradient of the loss (a value) or the losses; ``desc``:
-    the forward's descriptor, or None."""
+def _run_backward(up, aux, logits, target, target_b, mix, *options) -> Tensor:
+    """The logits' gradient; ``up``: the upstream gradient of the loss (a value) or the losses."""
     grad = torch.empty_like(logits, memory_format=torch.contiguous_format)
     if not grad.numel():
         return grad
-    # The forward's descriptor serves where the inputs came back as they were (hooks on saved tensors may
-    # hand out copies).
-    if desc is None or logits.data_ptr() != desc.logits or target.data_ptr() != desc.target \
-            or (target_b is not None and target_b.data_ptr() != desc.target_b) \
-            or (mix is not None and mix.data_ptr() != desc.mix) or not _lies(logits, desc.row_stride):
-        desc, _keep = _descriptor(logits, target, target_b, mix, *options)
-    if up.dtype != torch.float32 or not up.is_contiguous():
-        up = up.to(torch.float32).contiguous()
-    at = aux.data_ptr()
+    desc, _keep = _descriptor(logits, target, target_b, mix, *options)
+    up, at = up.to(torch.float32).contiguous(), aux.data_ptr()
     _on(logits.device, _native.lib().ow_cross_entropy_bwd, ctypes.byref(desc), at,
         at + 8 * desc.rows if desc.reduction else None, up.data_ptr(), grad.data_ptr())
     return grad
 
 
-class _PlainLoss(torch.autograd.Function):
-    """``cross_entropy_fwd`` with its gradient, without the dispatcher's cost."""
-
-    @staticmethod
-    def forward(ctx, logits, target, target_b, mix, *options):
-        loss, aux, ctx.desc = _run_forward(logits, target, target_b, mix, *options)
-        ctx.save_for_backward(logits, target, target_b, mix, aux)
-        ctx.options = options
-        return loss
-
-    @staticmethod
-    def backward(ctx, up):
-        if torch.is_grad_enabled():
-            return _PlainLoss._once(ctx, up)
-        logits, target, target_b, mix, aux = ctx.saved_tensors
-        return _run_backward(up, aux, ctx.desc, logits, target, target_b, mix, *ctx.options), *_NO_GRADS
-
-    @staticmethod
-    @once_differentiable
-    def _once(ctx, up):
-        return _PlainLoss.backward(ctx, up)
-
-
-_NO_GRADS = (None,) * 7  # of the other arguments
+_NO_GRADS = (None,) * 7  # of the arguments after the logits
 
 
 @torch.library.custom_op("omniwave_amd::cross_entropy_fwd", mutates_args=())
 def cross_entropy_fwd(logits: Tensor, target: Tensor, target_b: Tensor | None, mix: Tensor | None, mix_value: float,
                       label_smoothing: float, ignore_index: int, reduction: int) -> tuple[Tensor, Tensor]:
     """(the loss, or the losses of the rows; what the backward needs) of ``cross_entropy_hip``."""
-    return _run_forward(logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction)[:2]
+    return _run_forward(logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction)
 
 
 @cross_entropy_fwd.register_fake
@@ -143,7 +110,7 @@ def cross_entropy_bwd(up: Tensor, aux: Tensor, logits: Tensor, target: Tensor, t
                       mix: Tensor | None, mix_value: float, label_smoothing: float, ignore_index: int,
                       reduction: int) -> Tensor:
     """The logits' gradient."""
-    return _run_backward(up, aux, None, logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction)
+    return _run_backward(up, aux, logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction)
 
 
 @cross_entropy_bwd.register_fake
@@ -179,16 +146,18 @@ def cross_entropy_hip(logits: Tensor, target: Tensor, *, target_b: Tensor | None
     gradient; a mean of no rows is NaN.  A label outside ``[0, classes)`` makes its row NaN.
     ``reduction``: ``"mean"``, ``"sum"`` or ``"none"``.  Differentiable once in the logits.
     """
+    glue, code = _native.glue(), _native.OW_REDUCE.get(reduction)
+    number = mix is None or not isinstance(mix, Tensor)  # mix for all rows, or none
+    if glue is not None and code is not None and (target_b is None) == (mix is None) \
+            and _plain(logits, target, target_b, None if number else mix):
+        loss = glue.cross_entropy(logits, target, target_b, None if number else mix, 1.0 if mix is None or not number else mix,
+                                  label_smoothing, ignore_index, code)
+        if loss is not None:
+            return loss
+    # Everything else is checked, and goes through the operator.
     _check(logits, target, target_b, mix, label_smoothing, ignore_index, reduction)
     reason = gpu_reason(logits)
     if reason is not None:
         raise RuntimeError(f"hip cross-entropy not supported: {reason}")
-    mix_value = 1.0
-    if mix is not None and not isinstance(mix, Tensor):
-        mix, mix_value = None, float(mix)
-    args = (logits, target, target_b, mix, mix_value, float(label_smoothing), ignore_index, _native.OW_REDUCE[reduction])
-    if not _plain(logits, target, target_b, mix):
-        return cross_entropy_fwd(*args)[0]
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _PlainLoss.apply(*args)
-    return _run_forward(*args)[0]
+    return cross_entropy_fwd(logits, target, target_b, None if number else mix, 1.0 if mix is None or not number else float(mix),
+                             float(label_smoothing), ignore_index, code)[0]

@@ -9,17 +9,18 @@ Both are differentiable.  The reference has the norm before the block, the Layer
 scale and the residual as eager steps (omniweave/models/block.py:83-108) and no norm after the block;
 ``OmniWeaveBlock(post_norm=True)`` is the block that has one.  All sums are fp32 and each output is rounded
 once from fp32.
+
+A plain call is native, its autograd node included (``torch_glue.cpp``); the operator
+``omniwave_amd::block_norms_fwd`` takes the others (compilation, tracing, transforms, tensors to copy first).
 """
 
 from __future__ import annotations
 
 import ctypes
 import math
-from operator import is_
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from omniwave_amd import _native
 from omniwave_amd.hip import _DTYPE_CODE, SUPPORTED_DTYPES, _device_arch, _plain, _stream_ptr
@@ -29,7 +30,7 @@ MAX_CHANNELS = 8192
 
 def gpu_reason(t: Tensor) -> str | None:
     """Why the kernels cannot run on ``t``'s device, or None."""
-    err = _native.load_error()
+    err = _native.load_error() or _native.glue_error()
     if err is not None:
         return f"native library unavailable: {err}"
     if not t.is_cuda:
@@ -93,14 +94,6 @@ def _rows(t: Tensor) -> tuple[Tensor, int]:
     return t.contiguous(), c
 
 
-def _lies(t: Tensor, stride: int) -> bool:
-    """Whether ``_rows(t)`` is ``t`` itself with this distance."""
-    if t.is_contiguous():
-        return stride == t.shape[-1]
-    r, got = _rows(t)
-    return r is t and got == stride
-
-
 def _descriptor(x, delta, post_weight, gate, scale, next_weight, eps):
     """The C descriptor and the tensors it points into."""
     keep = [x, delta, post_weight, gate, scale, next_weight]
@@ -134,23 +127,19 @@ def _empty(t: Tensor) -> Tensor:
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
-def _run_forward(x, delta, post_weight, gate, scale, next_weight, eps):
-    """(out or None, next or None, the descriptor where it points at the inputs themselves, else None)."""
+def _run_forward(x, delta, post_weight, gate, scale, next_weight, eps) -> tuple[Tensor | None, Tensor | None]:
     out = _empty(x) if delta is not None else None
     nxt = _empty(x) if next_weight is not None else None
-    if not x.numel():
-        return out, nxt, None
-    desc, keep = _descriptor(x, delta, post_weight, gate, scale, next_weight, eps)
-    _on(x.device, _native.lib().ow_block_norms_fwd, ctypes.byref(desc), None if out is None else out.data_ptr(),
-        None if nxt is None else nxt.data_ptr())
-    inputs = all(map(is_, keep, (x, delta, post_weight, gate, scale, next_weight)))
-    return out, nxt, desc if inputs else None
+    if x.numel():
+        desc, _keep = _descriptor(x, delta, post_weight, gate, scale, next_weight, eps)
+        _on(x.device, _native.lib().ow_block_norms_fwd, ctypes.byref(desc), None if out is None else out.data_ptr(),
+            None if nxt is None else nxt.data_ptr())
+    return out, nxt
 
 
-def _run_backward(dout, dnext, desc, x, delta, post_weight, gate, scale, next_weight, eps, want) -> list[Tensor | None]:
+def _run_backward(dout, dnext, x, delta, post_weight, gate, scale, next_weight, eps, want) -> list[Tensor | None]:
     """Gradients of x, delta, post_weight, gate and next_weight where ``want`` asks for them and they
-    exist; ``dout`` / ``dnext`` None: that output has no upstream gradient; ``desc``: the forward's
-    descriptor, or None."""
+    exist; ``dout`` / ``dnext`` None: that output has no upstream gradient."""
     grads = [_empty(t) if w and t is not None else None for t, w in zip((x, delta, post_weight, gate, next_weight), want)]
     if x.numel() == 0 or (dout is None and dnext is None):
         return [None if g is None else g.zero_() for g in grads]
@@ -158,59 +147,19 @@ def _run_backward(dout, dnext, desc, x, delta, post_weight, gate, scale, next_we
     if dnext is None and grads[4] is not None:
         grads[4].zero_()
         ptr[4] = None
-    # The forward's descriptor serves where the inputs came back as they were (hooks on saved tensors may
-    # hand out copies).
-    if desc is None or x.data_ptr() != desc.x or not _lies(x, desc.x_stride) \
-            or (delta is not None and (delta.data_ptr() != desc.delta or not _lies(delta, desc.delta_stride))) \
-            or (post_weight is not None and post_weight.data_ptr() != desc.post_weight) \
-            or (gate is not None and gate.data_ptr() != desc.gate) \
-            or (scale is not None and scale.data_ptr() != desc.scale) \
-            or (next_weight is not None and next_weight.data_ptr() != desc.next_weight):
-        desc, _keep = _descriptor(x, delta, post_weight, gate, scale, next_weight, eps)
-    out_ptr, out_stride, next_ptr, next_stride = None, 0, None, 0
-    if dout is not None:
-        dout, out_stride = _rows(dout)
-        out_ptr = dout.data_ptr()
-    if dnext is not None:
-        dnext, next_stride = _rows(dnext)
-        next_ptr = dnext.data_ptr()
-    lib, ref, device = _native.lib(), ctypes.byref(desc), x.device
-    workspace, ws_bytes, ws_ptr = None, 0, None
-    if ptr[2] or ptr[3] or ptr[4]:
-        if device.index != torch._C._cuda_getDevice():
-            with torch.cuda.device(device):  # the size goes by the device's compute units
-                ws_bytes = lib.ow_block_norms_bwd_workspace(ref)
-        else:
-            ws_bytes = lib.ow_block_norms_bwd_workspace(ref)
-        workspace = torch.empty(ws_bytes // 4, dtype=torch.float32, device=device)
-        ws_ptr = workspace.data_ptr()
-    _on(device, lib.ow_block_norms_bwd, ref, out_ptr, out_stride, next_ptr, next_stride, *ptr, ws_ptr, ws_bytes)
+    desc, _keep = _descriptor(x, delta, post_weight, gate, scale, next_weight, eps)
+    upstream = []
+    for g in (dout, dnext):
+        upstream.append((None, 0) if g is None else _rows(g))
+    args = [v for g, stride in upstream for v in (None if g is None else g.data_ptr(), stride)]
+    lib, ws_bytes, workspace = _native.lib(), 0, None
+    if any(ptr[2:]):
+        with torch.cuda.device(x.device):  # the size goes by the device's compute units
+            ws_bytes = lib.ow_block_norms_bwd_workspace(ctypes.byref(desc))
+        workspace = torch.empty(ws_bytes // 4, dtype=torch.float32, device=x.device)
+    _on(x.device, lib.ow_block_norms_bwd, ctypes.byref(desc), *args, *ptr,
+        None if workspace is None else workspace.data_ptr(), ws_bytes)
     return grads
-
-
-class _PlainNorms(torch.autograd.Function):
-    """``block_norms_fwd`` with its gradient, without the dispatcher's cost."""
-
-    @staticmethod
-    def forward(ctx, x, delta, post_weight, gate, scale, next_weight, eps):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x, delta, post_weight, gate, scale, next_weight)
-        out, nxt, ctx.desc = _run_forward(x, delta, post_weight, gate, scale, next_weight, eps)
-        ctx.eps = eps
-        return out, nxt
-
-    @staticmethod
-    def backward(ctx, dout, dnext):
-        if torch.is_grad_enabled():
-            return _PlainNorms._once(ctx, dout, dnext)
-        need = ctx.needs_input_grad
-        grads = _run_backward(dout, dnext, ctx.desc, *ctx.saved_tensors, ctx.eps, (need[0], need[1], need[2], need[3], need[5]))
-        return grads[0], grads[1], grads[2], grads[3], None, grads[4], None
-
-    @staticmethod
-    @once_differentiable
-    def _once(ctx, dout, dnext):
-        return _PlainNorms.backward(ctx, dout, dnext)
 
 
 @torch.library.custom_op("omniwave_amd::block_norms_fwd", mutates_args=())
@@ -218,7 +167,7 @@ def block_norms_fwd(x: Tensor, delta: Tensor | None, post_weight: Tensor | None,
                     scale: Tensor | None, next_weight: Tensor | None, eps: float) -> tuple[Tensor, Tensor]:
     """(out, next) of ``block_norms_hip``; empty where there is none (``out`` without ``delta``, ``next``
     without ``next_weight``)."""
-    out, nxt, _ = _run_forward(x, delta, post_weight, gate, scale, next_weight, eps)
+    out, nxt = _run_forward(x, delta, post_weight, gate, scale, next_weight, eps)
     return x.new_empty(0) if out is None else out, x.new_empty(0) if nxt is None else nxt
 
 
@@ -233,7 +182,7 @@ def block_norms_bwd(dout: Tensor | None, dnext: Tensor | None, x: Tensor, delta:
                     post_weight: Tensor | None, gate: Tensor | None, scale: Tensor | None, next_weight: Tensor | None,
                     eps: float, want: list[bool]) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
     """Gradients of x, delta, post_weight, gate and next_weight; empty where ``want`` is false."""
-    grads = _run_backward(dout, dnext, None, x, delta, post_weight, gate, scale, next_weight, eps, want)
+    grads = _run_backward(dout, dnext, x, delta, post_weight, gate, scale, next_weight, eps, want)
     return tuple(x.new_empty(0) if g is None else g for g in grads)
 
 
@@ -266,18 +215,19 @@ block_norms_fwd.register_autograd(_norms_backward, setup_context=_norms_setup_co
 
 
 def _norms(x, delta, post_weight, gate, scale, next_weight, eps) -> tuple[Tensor | None, Tensor | None]:
+    glue = _native.glue()
+    if glue is not None and _plain(x, delta, post_weight, gate, scale, next_weight):
+        both = glue.norms(x, delta, post_weight, gate, scale, next_weight, eps)
+        if both is not None:
+            return both
+    # Everything else is checked, and goes through the operator.
     eps = float(eps)
     _check(x, delta, post_weight, gate, scale, next_weight, eps)
     reason = gpu_reason(x)
     if reason is not None:
         raise RuntimeError(f"hip norms not supported: {reason}")
-    tensors = (x, delta, post_weight, gate, scale, next_weight)
-    if not _plain(*tensors):
-        out, nxt = block_norms_fwd(*tensors, eps)
-        return (None if delta is None else out), (None if next_weight is None else nxt)
-    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors]):
-        return _PlainNorms.apply(*tensors, eps)
-    return _run_forward(*tensors, eps)[:2]
+    out, nxt = block_norms_fwd(x, delta, post_weight, gate, scale, next_weight, eps)
+    return (None if delta is None else out), (None if next_weight is None else nxt)
 
 
 def block_norms_hip(x: Tensor, delta: Tensor, *, post_weight: Tensor | None = None, gate: Tensor | None = None,
