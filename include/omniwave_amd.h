@@ -562,7 +562,8 @@ int ow_bwd_block(const void* grad, const void* x, const void* const* small, cons
  * The backward takes dout and dnext (each NULL where it has none, with row strides) and writes those of
  * dx, ddelta (contiguous, `dtype`), dpost_weight, dgate and dnext_weight (in their weights' dtypes) that
  * are not NULL.  Weight gradients are summed in a fixed order over ow_block_norms_bwd_workspace bytes of
- * workspace (not needed, and NULL, where no weight gradient is asked for).  rows, channels >= 1 there.
+ * workspace (0 for few rows; not needed, and NULL, where no weight gradient is asked for).  rows,
+ * channels >= 1 there.
  */
 typedef struct OwBlockNorms {
   int64_t rows;

@@ -42,6 +42,8 @@ struct NormsArgs {
   void* dx;
   void* ddelta;
   void* dgate;          // written here where a segment has one workgroup
+  void* dpost;          // written here where there is one workgroup
+  void* dnextw;
   float* partial;       // [3][n_part][C]: dpost, dnext_weight, dgate
   int32_t want;         // bits: dpost, dnext_weight, dgate
   int32_t n_part;       // workgroups
@@ -387,13 +389,20 @@ __global__ void __launch_bounds__(kThreads<T>, bwd_waves(Row<Ty>::kVec)) block_n
     }
   }
   }
+  const bool alone = a.n_part == 1;  // these sums are the gradients
   if (a.want & kWantPost) {
     float* dst = partial_row(0);
-    each_sum(s_post, [&](int col, float sum) { dst[col] = sum; });
+    each_sum(s_post, [&](int col, float sum) {
+      if (alone) store_any(a.dpost, a.n.post_dtype, col, sum);
+      else dst[col] = sum;
+    });
   }
   if (a.want & kWantNext) {
     float* dst = partial_row(1);
-    each_sum(s_next, [&](int col, float sum) { dst[col] = sum; });
+    each_sum(s_next, [&](int col, float sum) {
+      if (alone) store_any(a.dnextw, a.n.next_dtype, col, sum);
+      else dst[col] = sum;
+    });
   }
 }
 
@@ -448,7 +457,9 @@ struct Parts {
 
 // How the backward's rows are shared out: segments (images where the gate is per image, else one), each
 // to seg_parts workgroups, as many in all as run at once and none without a row group; more segments
-// than that go several to a workgroup.
+// than that go several to a workgroup.  Few rows go to one workgroup, which writes the weights' gradients
+// itself: a second launch costs more than the rows gain from more workgroups.
+constexpr int kFewGroups = 8;
 Parts backward_parts(const OwBlockNorms& n) {
   const int vec = n.dtype == OW_DTYPE_F32 ? 4 : 8, threads = threads_of(n.channels, vec);
   const int at_once = rows_at_once(n.channels, vec);
@@ -457,6 +468,10 @@ Parts backward_parts(const OwBlockNorms& n) {
   p.segments = n.gate != nullptr && n.gate_per_image ? n.rows / n.rows_per_image : 1;
   p.seg_rows = n.rows / p.segments;
   const int64_t groups = (p.seg_rows + at_once - 1) / at_once, parts = most / p.segments;
+  if (p.segments * groups <= kFewGroups) {
+    p.seg_parts = p.n_part = 1;
+    return p;
+  }
   p.seg_parts = static_cast<int32_t>(parts < 1 ? 1 : parts < groups ? parts : groups);
   p.n_part = static_cast<int32_t>(p.segments < most ? p.segments * p.seg_parts : most);
   return p;
@@ -552,7 +567,8 @@ int ow_block_norms_fwd(const OwBlockNorms* norms, void* out, void* next, void* s
 
 size_t ow_block_norms_bwd_workspace(const OwBlockNorms* norms) {
   if (norms == nullptr || norms->rows <= 0 || norms->channels <= 0 || norms->rows_per_image <= 0) return 0;
-  return static_cast<size_t>(3) * ow::backward_parts(*norms).n_part * norms->channels * sizeof(float);
+  const int32_t parts = ow::backward_parts(*norms).n_part;
+  return parts > 1 ? static_cast<size_t>(3) * parts * norms->channels * sizeof(float) : 0;
 }
 
 int ow_block_norms_bwd(const OwBlockNorms* norms, const void* dout, int64_t dout_stride, const void* dnext,
@@ -576,6 +592,8 @@ int ow_block_norms_bwd(const OwBlockNorms* norms, const void* dout, int64_t dout
   a.want = (dpost_weight ? ow::kWantPost : 0) | (dnext_weight ? ow::kWantNext : 0) | (dgate ? ow::kWantGate : 0);
   a.inv_c = 1.f / static_cast<float>(norms->channels);
   a.dgate = dgate;
+  a.dpost = dpost_weight;
+  a.dnextw = dnext_weight;
   const ow::Parts p = ow::backward_parts(*norms);
   a.segments = p.segments;
   a.seg_rows = p.seg_rows;
@@ -590,7 +608,7 @@ int ow_block_norms_bwd(const OwBlockNorms* norms, const void* dout, int64_t dout
   ow::run(a, true, s);
   if (int rc = ow::hip_status(hipGetLastError(), "block_norms_bwd_kernel launch")) return rc;
   const bool gate_sums = dgate != nullptr && a.seg_parts > 1;  // else the kernel wrote dgate
-  if (dpost_weight || dnext_weight || gate_sums) {
+  if (gate_sums || ((dpost_weight || dnext_weight) && a.n_part > 1)) {
     ow::SumArgs m{};
     m.partial = a.partial;
     m.dst[0] = dpost_weight, m.dst[1] = dnext_weight, m.dst[2] = dgate;

@@ -234,7 +234,7 @@ class NormsNode : public torch::autograd::Function<NormsNode> {
       Tensor workspace;
       if (grads[2].defined() || grads[3].defined() || next_weight_grad != nullptr) {
         bytes = ow_block_norms_bwd_workspace(&d);
-        workspace = at::empty({static_cast<int64_t>(bytes)}, n.x.options().dtype(at::kByte));
+        if (bytes) workspace = at::empty({static_cast<int64_t>(bytes)}, n.x.options().dtype(at::kByte));
       }
       check(ow_block_norms_bwd(&d, ptr(dout), out_stride, ptr(dnext), next_stride, out_ptr(grads[0]), out_ptr(grads[1]),
                                out_ptr(grads[2]), out_ptr(grads[3]), next_weight_grad, out_ptr(workspace), bytes,

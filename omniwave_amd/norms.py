@@ -156,7 +156,7 @@ def _run_backward(dout, dnext, x, delta, post_weight, gate, scale, next_weight, 
     if any(ptr[2:]):
         with torch.cuda.device(x.device):  # the size goes by the device's compute units
             ws_bytes = lib.ow_block_norms_bwd_workspace(ctypes.byref(desc))
-        workspace = torch.empty(ws_bytes // 4, dtype=torch.float32, device=x.device)
+        workspace = torch.empty(ws_bytes // 4, dtype=torch.float32, device=x.device) if ws_bytes else None
     _on(x.device, lib.ow_block_norms_bwd, ctypes.byref(desc), *args, *ptr,
         None if workspace is None else workspace.data_ptr(), ws_bytes)
     return grads

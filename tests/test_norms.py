@@ -106,7 +106,9 @@ def test_c_entry_points_check_their_arguments() -> None:
     refused(lib.ow_block_norms_fwd(desc(delta=None), None, None, None), b"neither")
     assert lib.ow_block_norms_fwd(desc(rows=0), p, None, None) == 0
     assert lib.ow_block_norms_bwd_workspace(None) == 0
-    assert lib.ow_block_norms_bwd_workspace(desc()) >= 3 * 8 * 4
+    many = dict(rows=6000, rows_per_image=3000)
+    assert lib.ow_block_norms_bwd_workspace(desc()) == 0  # few rows: one workgroup
+    assert lib.ow_block_norms_bwd_workspace(desc(**many)) >= 3 * 8 * 4
 
     def bwd(d, dout=p, dnext=None, dx=p, ddelta=None, dpost=None, dgate=None, dnw=None, ws=None, n=0):
         return lib.ow_block_norms_bwd(d, dout, 8, dnext, 8, dx, ddelta, dpost, dgate, dnw, ws, n, None)
@@ -115,5 +117,5 @@ def test_c_entry_points_check_their_arguments() -> None:
     refused(bwd(desc(), dnext=p), b"next_weight")
     refused(bwd(desc(), dout=None), b"no upstream")
     refused(bwd(desc(), dgate=p), b"not given")
-    refused(bwd(desc(gate=256), dgate=p), b"workspace")
-    refused(bwd(desc(gate=256), dgate=p, ws=p, n=8), b"workspace")
+    refused(bwd(desc(gate=256, **many), dgate=p), b"workspace")
+    refused(bwd(desc(gate=256, **many), dgate=p, ws=p, n=8), b"workspace")
