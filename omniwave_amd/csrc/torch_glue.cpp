@@ -1,5 +1,6 @@
-// Calls of the small operators (norms, cross-entropy) with their autograd nodes, as the Python module
-// omniwave_amd._glue: host code only, over the C ABI of libomniwave_amd.
+// Calls of the small operators (norms, cross-entropy) with their autograd nodes, and the optimizer's look at
+// hundreds of tensors a step, as the Python module omniwave_amd._glue: host code only, over the C ABI of
+// libomniwave_amd.
 //
 // Why: a small launch takes 4 us on the GPU, and the same call through a Python autograd function costs its
 // caller 90 (cross-entropy) to 145 us (norms), most of it Python that runs cold on autograd's thread.  Here
@@ -20,6 +21,8 @@
 #include <cmath>
 #include <cstring>
 #include <string>
+#include <utility>
+#include <vector>
 
 #include "omniwave_amd.h"
 
@@ -441,7 +444,82 @@ PyObject* py_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n_args) 
   END_HANDLE_TH_ERRORS
 }
 
+// Addresses of tensors as bytes, 8 each, to be compared as a whole.
+class Addresses {
+ public:
+  explicit Addresses(Py_ssize_t n) { of_.reserve(static_cast<size_t>(n)); }
+  void add(const void* p) { of_.push_back(reinterpret_cast<int64_t>(p)); }
+  PyObject* bytes() const {
+    return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(of_.data()), static_cast<Py_ssize_t>(of_.size() * 8));
+  }
+
+ private:
+  std::vector<int64_t> of_;
+};
+
+const void* address(const Tensor& t) { return t.has_storage() ? t.const_data_ptr() : nullptr; }
+
+// addresses(tensors) -> bytes: where the tensors of a list lie
+PyObject* py_addresses(PyObject*, PyObject* list) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(PyList_Check(list), "addresses takes a list");
+  const Py_ssize_t n = PyList_GET_SIZE(list);
+  Addresses found(n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* o = PyList_GET_ITEM(list, i);
+    TORCH_CHECK_TYPE(THPVariable_Check(o), "addresses takes tensors");
+    found.add(address(THPVariable_Unpack(o)));
+  }
+  return found.bytes();
+  END_HANDLE_TH_ERRORS
+}
+
+// state_addresses(entries) -> bytes: where the tensors of a list of dictionaries lie, in their order (0 for
+// what is no tensor)
+PyObject* py_state_addresses(PyObject*, PyObject* list) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(PyList_Check(list), "state_addresses takes a list");
+  const Py_ssize_t n = PyList_GET_SIZE(list);
+  Addresses found(4 * n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject *entry = PyList_GET_ITEM(list, i), *key = nullptr, *value = nullptr;
+    TORCH_CHECK_TYPE(PyDict_Check(entry), "state_addresses takes dictionaries");
+    for (Py_ssize_t at = 0; PyDict_Next(entry, &at, &key, &value);)
+      found.add(THPVariable_Check(value) ? address(THPVariable_Unpack(value)) : nullptr);
+  }
+  return found.bytes();
+  END_HANDLE_TH_ERRORS
+}
+
+// gradients(parameters) -> bytes: where the parameters' gradients lie (0: none); None where one of them is not
+// dense and contiguous in its parameter's shape, dtype and device
+PyObject* py_gradients(PyObject*, PyObject* list) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(PyList_Check(list), "gradients takes a list");
+  const Py_ssize_t n = PyList_GET_SIZE(list);
+  Addresses found(n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* o = PyList_GET_ITEM(list, i);
+    TORCH_CHECK_TYPE(THPVariable_Check(o), "gradients takes tensors");
+    const Tensor& p = THPVariable_Unpack(o);
+    const Tensor& g = p.grad();
+    if (!g.defined()) {
+      found.add(nullptr);
+      continue;
+    }
+    if (g.layout() != at::kStrided || !g.is_contiguous() || g.sizes() != p.sizes() || g.scalar_type() != p.scalar_type() ||
+        g.device() != p.device() || g.is_neg())
+      Py_RETURN_NONE;
+    found.add(address(g));
+  }
+  return found.bytes();
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef kMethods[] = {
+    {"addresses", py_addresses, METH_O, nullptr},
+    {"state_addresses", py_state_addresses, METH_O, nullptr},
+    {"gradients", py_gradients, METH_O, nullptr},
     {"norms", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_norms)), METH_FASTCALL, nullptr},
     {"cross_entropy", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_cross_entropy)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},

@@ -16,6 +16,7 @@ from operator import is_
 import numpy as np
 import torch
 from torch import Tensor
+from torch.optim import optimizer as _base
 
 from omniwave_amd import _native
 from omniwave_amd.hip import _DTYPE_CODE, SUPPORTED_DTYPES, _stream_ptr
@@ -193,82 +194,109 @@ class AdamW(torch.optim.Optimizer):
 
     # -- the step -------------------------------------------------------------------------
 
-    @torch.no_grad()
     def step(self, closure=None):
+        # The base class's wrapper (a profiler's record, hooks) costs more than looking at the tensors does:
+        # only where something listens.
+        if (self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks or _base._global_optimizer_pre_hooks
+                or _base._global_optimizer_post_hooks or torch.autograd.profiler._is_profiler_enabled):
+            return self._heard_step(closure)
+        return self._step(closure)
+
+    step.hooked = True  # the base class leaves it as it is
+
+    def _step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        # What stands between the calls is looked at in lists: a model has hundreds of parameters.
+        # A model has hundreds of parameters, and a step takes the GPU no longer than looking at each of them
+        # takes Python: they are looked at natively, in lists.
+        glue = _native.glue()
+        if glue is None:
+            raise RuntimeError(f"hip AdamW not supported: native library unavailable: {_native.glue_error()}")
         params = [p for group in self.param_groups for p in group["params"]]
-        grads = [p.grad for p in params]
+        lie = glue.gradients(params)
+        keep = None  # copies of strided gradients live until the launches are queued
+        if lie is None:
+            keep = [None if p.grad is None else _dense(p) for p in params]
+            lie = np.array([0 if g is None else g.data_ptr() for g in keep], dtype=np.int64).tobytes()
         plan = self._plan
-        if plan is None or not plan.current(self, params, grads):
-            plan = self._plan = _Plan(self, params, grads)
+        if plan is None or not plan.current(self, glue, params, lie):
+            plan = self._plan = _Plan(self, glue, params, lie)
         if not plan.kinds:
             return loss
+        plan.set_gradients(lie)
         device = plan.device
         hyper = plan.hyper(*[_hyper(g, device) for g in self.param_groups])
         if device.index != torch._C._cuda_getDevice():
             with torch.cuda.device(device):
-                self._launch(plan.kinds, grads, hyper, device)
+                self._launch(plan.kinds, hyper, device)
         else:
-            self._launch(plan.kinds, grads, hyper, device)
+            self._launch(plan.kinds, hyper, device)
+        del keep
         # The kernels write past autograd's notice: what goes by a parameter's version has to see the change.
         torch.autograd.graph.increment_version(plan.active)
         return loss
 
-    def _launch(self, kinds: list[_Kind], grads: list[Tensor | None], hyper, device: torch.device) -> None:
+    _heard_step = torch.optim.Optimizer.profile_hook_step(_step)
+
+    def _launch(self, kinds: list[_Kind], hyper, device: torch.device) -> None:
         lib, stream = _native.lib(), _stream_ptr(device)
-        keep = [kind.set_gradients(grads) for kind in kinds]  # copies of strided ones live until the launches are queued
-        partials, total, norm_ptr = None, 0, None
+        partials, total, norm_ptr, at = None, 0, None, None
         if self.max_grad_norm is not None:
             total = sum(kind.partials for kind in kinds)
             partials = torch.empty(total, dtype=torch.float64, device=device)
             self.grad_norm = torch.empty((), dtype=torch.float32, device=device)
+            at = first = partials.data_ptr()
             norm_ptr = self.grad_norm.data_ptr()
-            at = 0
             for kind in kinds:
-                _native.check(lib.ow_grad_norm(kind.pointer, kind.count, kind.code,
-                                               partials.data_ptr() + 8 * at, kind.partials, stream), "ow_grad_norm")
-                at += kind.partials
+                _native.check(lib.ow_grad_norm(kind.pointer, kind.count, kind.code, first, kind.partials, stream),
+                              "ow_grad_norm")
+                first += 8 * kind.partials
         for kind in kinds:
-            _native.check(
-                lib.ow_adamw_step(kind.pointer, kind.count, hyper, len(hyper), kind.code, kind.bits, kind.master,
-                                  None if partials is None else partials.data_ptr(), total,
-                                  self.max_grad_norm or 0.0, norm_ptr, stream), "ow_adamw_step")
+            _native.check(lib.ow_adamw_step(kind.pointer, kind.count, hyper, len(hyper), kind.code, kind.bits, kind.master, at,
+                                            total, self.max_grad_norm or 0.0, norm_ptr, stream), "ow_adamw_step")
             norm_ptr = None
-        del keep
+
+
+def _dense(p: Tensor) -> Tensor:
+    """The gradient of ``p``, contiguous."""
+    g = p.grad
+    if g.layout != torch.strided:
+        raise RuntimeError("AdamW takes dense gradients")
+    if g.shape != p.shape or g.dtype != p.dtype or g.device != p.device:
+        raise ValueError(f"the gradient of a {p.dtype} parameter of shape {tuple(p.shape)} is {g.dtype} {tuple(g.shape)} "
+                         f"on {g.device}")
+    return g.resolve_neg().contiguous()
+
+
+def _without(lie: bytes) -> bytes:
+    """Which of the gradients there are none of."""
+    return (np.frombuffer(lie, dtype=np.int64) == 0).tobytes()
 
 
 class _Plan:
     """What the steps of the same parameters share: their lists for the native calls.  It is made anew
     where a parameter, a state or the set of parameters with gradients is another than it was."""
 
-    def __init__(self, opt: AdamW, params: list[Tensor], grads: list[Tensor | None]) -> None:
-        self.params, self.kinds, self.device = params, [], None
-        self.without = [g is None for g in grads]
+    def __init__(self, opt: AdamW, glue, params: list[Tensor], lie: bytes) -> None:
+        self.params, self.device = params, None
+        self.without, self.lie = _without(lie), None
         self.sizes = [len(group["params"]) for group in opt.param_groups]
         self.hyper = _native.OwAdamwGroup * len(self.sizes)
         owner = [i for i, size in enumerate(self.sizes) for _ in range(size)]
-        active = [i for i, (p, g) in enumerate(zip(params, grads)) if g is not None and p.numel()]
-        self.lies = _Addresses(params)
+        active = [i for i, p in enumerate(params) if not self.without[i] and p.numel()]
         kinds: dict[tuple, _Kind] = {}
         if active:
             self.device, reason = params[active[0]].device, gpu_reason(params[active[0]])
             if reason is not None:
                 raise RuntimeError(f"hip AdamW not supported: {reason}")
         for i in active:
-            p, g = params[i], grads[i]
+            p = params[i]
             if p.device != self.device:
                 raise ValueError(f"parameters on {self.device} and {p.device}: an optimizer's parameters are on one GPU")
             if not p.is_contiguous():
                 raise ValueError(f"a parameter of shape {tuple(p.shape)} is not contiguous")
-            if g.layout != torch.strided:
-                raise RuntimeError("AdamW takes dense gradients")
-            if g.shape != p.shape or g.dtype != p.dtype or g.device != p.device:
-                raise ValueError(f"the gradient of a {p.dtype} parameter of shape {tuple(p.shape)} is {g.dtype} "
-                                 f"{tuple(g.shape)} on {g.device}")
             if not opt.state[p]:
                 opt._first_state(p)
             layout = opt._layout(p)
@@ -279,35 +307,26 @@ class _Plan:
         for kind in self.kinds:
             kind.finish()
         self.active = [params[i] for i in active]
+        self.addresses = glue.addresses(params)
         self.entries = list(opt.state.values())
-        self.states = _Addresses(_tensors(self.entries))
+        self.states = glue.state_addresses(self.entries)
 
-    def current(self, opt: AdamW, params: list[Tensor], grads: list[Tensor | None]) -> bool:
-        """Whether everything still lies where the plan has it."""
+    def current(self, opt: AdamW, glue, params: list[Tensor], lie: bytes) -> bool:
+        """Whether everything but the gradients still lies where the plan has it."""
         entries = list(opt.state.values())
         return (len(params) == len(self.params) and all(map(is_, params, self.params))
-                and [g is None for g in grads] == self.without
+                and (lie == self.lie or _without(lie) == self.without)
                 and [len(group["params"]) for group in opt.param_groups] == self.sizes
                 and len(entries) == len(self.entries) and all(map(is_, entries, self.entries))
-                and self.lies.still(params) and self.states.still(_tensors(entries)))
+                and glue.addresses(params) == self.addresses and glue.state_addresses(entries) == self.states)
 
-
-def _tensors(entries: list[dict]) -> list[Tensor]:
-    return [t for e in entries for t in e.values()]
-
-
-class _Addresses:
-    """Where a list of tensors lies, to be compared with later in one call."""
-
-    def __init__(self, tensors: list) -> None:
-        self.of = [t.data_ptr() if isinstance(t, Tensor) else 0 for t in tensors]
-        self.places = list(range(len(self.of)))
-
-    def still(self, tensors: list) -> bool:
-        try:
-            return len(tensors) == len(self.of) and torch._C._tensors_data_ptrs_at_indices_equal(tensors, self.of, self.places)
-        except TypeError:  # not all of them are tensors
-            return False
+    def set_gradients(self, lie: bytes) -> None:
+        """Writes the gradients' addresses into the lists."""
+        if lie != self.lie:
+            where = np.frombuffer(lie, dtype=np.int64)
+            for kind in self.kinds:
+                kind.table[:, _GRAD] = where[kind.at]
+            self.lie = lie
 
 
 class _Kind:
@@ -317,7 +336,6 @@ class _Kind:
         self.dtype, self.bits, self.master = dtype, bits, master
         self.at: list[int] = []  # places among the parameters
         self.rows: list[list[int]] = []
-        self.lie: _Addresses | None = None  # the gradients
 
     def add(self, i: int, p: Tensor, entry: dict[str, Tensor], group: int) -> None:
         second = ("exp_avg_sq_root", "exp_avg_scale", "exp_avg_sq_root_scale") if self.bits == 8 else ("exp_avg_sq",)
@@ -328,22 +346,8 @@ class _Kind:
 
     def finish(self) -> None:
         self.table = np.array(self.rows, dtype=np.int64)
-        self.sizes = [row[8] for row in self.rows]
         self.pointer, self.count, self.code = self.table.ctypes.data, len(self.rows), _DTYPE_CODE[self.dtype]
         self.partials = _native.lib().ow_grad_norm_partials(self.pointer, self.count)
-
-    def set_gradients(self, grads: list[Tensor | None]) -> list[Tensor]:
-        """Writes the gradients' addresses into the table; returns the tensors that hold them.  (Torch
-        keeps a gradient in its parameter's dtype and on its device; its strides may differ.)"""
-        mine = [grads[i] for i in self.at]
-        if not all([g.is_contiguous() for g in mine]):
-            mine = [g.contiguous() for g in mine]
-        if self.lie is None or not self.lie.still(mine):
-            if [g.numel() for g in mine] != self.sizes:
-                raise ValueError("a gradient has not its parameter's shape")
-            self.lie = _Addresses(mine)
-            self.table[:, _GRAD] = self.lie.of
-        return mine
 
 
 def _hyper(group: dict, device: torch.device | None = None) -> tuple:

@@ -385,3 +385,32 @@ def test_a_model_follows_torch() -> None:
         # 3 steps of at most lr each way: 24 U of the updates and 3 U of the parameter per step and side
         bound = 6 * (24 * U * 1.1e-3 + 3 * U * p.detach().abs())
         assert ((p - q).detach().abs() <= bound).all(), name
+
+
+def test_hooks_schedulers_closures_and_profiles_see_the_step() -> None:
+    announce("adamw hooks, scheduler, closure, profiler")
+    p = torch.nn.Parameter(torch.ones(300, device=DEV))
+    opt = AdamW([p], lr=1e-2, weight_decay=0.0)
+    schedule = torch.optim.lr_scheduler.StepLR(opt, 1, gamma=0.5)
+    seen = []
+    before = opt.register_step_pre_hook(lambda o, args, kwargs: seen.append("before"))
+    after = opt.register_step_post_hook(lambda o, args, kwargs: seen.append("after"))
+    p.grad = torch.ones_like(p)
+    check_step(opt, [p], [(1e-2, 0.0)])
+    assert seen == ["before", "after"]
+    before.remove(), after.remove()
+    schedule.step()
+    check_step(opt, [p], [(5e-3, 0.0)])
+    assert seen == ["before", "after"]
+
+    def closure():
+        opt.zero_grad()
+        loss = (p * p).sum()
+        loss.backward()
+        return loss
+
+    assert opt.step(closure).item() > 0 and (opt.state[p]["step"] == 3).all()
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as profile:
+        opt.step()
+    assert any("Optimizer.step#AdamW" in e.key for e in profile.key_averages())
+    assert (opt.state[p]["step"] == 4).all()
