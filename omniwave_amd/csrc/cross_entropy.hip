@@ -92,51 +92,63 @@ __device__ __forceinline__ void finish_row(const XentArgs& a, int64_t row, const
 
 // Numbers of logits begin .. end - 1 of a row that a thread takes, T of them apart by a vector.
 struct Numbers {
+  static constexpr int U = 4;  // vectors in flight, beside as many that are computed
   float m = -__builtin_inff(), z = 0.f, total = 0.f;
-  // N vectors, of which the last may have only n values.
-  template <class R, int N, bool WHOLE>
-  __device__ __forceinline__ void add(const typename R::Raw (&raw)[N], int n) {
+  // Vectors u < count (WHOLE: all).
+  template <class R, bool WHOLE>
+  __device__ __forceinline__ void add(const typename R::Raw (&raw)[U], int count) {
     constexpr int V = R::kVec;
-    float v[N][V], top = m;
+    float v[U][V], top = m;
 #pragma unroll
-    for (int u = 0; u < N; ++u) {
+    for (int u = 0; u < U; ++u) {
       R::widen(raw[u], v[u]);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        if (WHOLE || j < n) total += v[u][j];
-        if (!WHOLE && j >= n) v[u][j] = -__builtin_inff();
+        if (!WHOLE && u >= count) v[u][j] = -__builtin_inff();
+        else total += v[u][j];
         top = fmaxf(top, v[u][j]);
       }
     }
-    z *= exp_below(m, top);
-    m = top;
+    scale_to(top);
     if (top == -__builtin_inff()) return;
 #pragma unroll
-    for (int u = 0; u < N; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int j = 0; j < V; ++j) z += __builtin_amdgcn_exp2f((v[u][j] - top) * kLog2e);
   }
+  __device__ __forceinline__ void scale_to(float top) {
+    z *= exp_below(m, top);
+    m = top;
+  }
   template <class R, int T>
   __device__ __forceinline__ void scan(const typename R::Elem* x, int64_t begin, int64_t end, int t) {
-    constexpr int V = R::kVec, U = 4;  // vectors in flight
-    int64_t i = begin + t * V;
-    for (; i + (U - 1) * T * V + V <= end; i += U * T * V) {
+    constexpr int V = R::kVec;
+    const int64_t vectors = (end - begin) / V;
+    x += begin;
+    // Vectors of this thread: t, t + T, ...
+    typename R::Raw next[U];
+    auto load = [&](int64_t at) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) next[u] = at + u * T < vectors ? R::raw(x + (at + u * T) * V) : R::zero();
+    };
+    load(t);
+    for (int64_t at = t; at < vectors; at += U * T) {
       typename R::Raw raw[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) raw[u] = R::raw(x + i + u * T * V);
-      add<R, U, true>(raw, V);
+      for (int u = 0; u < U; ++u) raw[u] = next[u];
+      load(at + U * T);
+      const int64_t left = (vectors - at + T - 1) / T;
+      if (left >= U) add<R, true>(raw, U);
+      else add<R, false>(raw, static_cast<int>(left));
     }
-    for (; i < end; i += T * V) {
-      const int n = end - i < V ? static_cast<int>(end - i) : V;
-      typename R::Raw raw[1] = {R::zero()};
-      if (n == V) {
-        raw[0] = R::raw(x + i);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (j < n) R::set(raw[0], j, x[i + j]);
-      }
-      add<R, 1, false>(raw, n);
+    // What fills no vector, a value each.
+    const int64_t i = vectors * V + t;
+    if (t < V && begin + i < end) {
+      const float v = R::to_f32(x[i]);
+      total += v;
+      const float top = fmaxf(m, v);
+      scale_to(top);
+      if (top != -__builtin_inff()) z += __builtin_amdgcn_exp2f((v - top) * kLog2e);
     }
   }
   __device__ __forceinline__ void join_wave() { join_lanes<64>(m, z, total); }
