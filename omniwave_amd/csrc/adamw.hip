@@ -40,7 +40,7 @@ constexpr int kArgBytes = 4096 - 64;    // of the tensor and hyperparameter tabl
 constexpr float kFp8Most = 448.f;
 constexpr float kFp8Least = 0x1p-9f;    // the least e4m3fn number above zero
 constexpr float kLeastScale = 1.17549435e-38f;  // smaller (subnormal) scales: a block of zeros
-static_assert(kBlock == 4 * 64, "a wave's vectors are a block");
+static_assert(kBlock == 4 * 64 && kIters == 4, "a wave's vector is a block, and its blocks' scales a vector");
 
 struct Hyper {
   const float* lr_device;  // NULL: lr
@@ -201,31 +201,35 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_kernel(StepArgs<kPtrsOf<Ty,
   const uint32_t next = i + 1 < a.count ? a.t.first[i + 1] : gridDim.x;
   const int n = chunk + 1 == next ? a.t.last[i] + 1 : kChunk;  // values of this chunk
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t base = static_cast<int64_t>(local) * kChunk, block0 = static_cast<int64_t>(local) * (kChunk / kBlock);
+  const int64_t base = static_cast<int64_t>(local) * kChunk;
 
   // Everything is read before anything is written: a vector's loads do not wait for the stores of the
-  // one before it, nor for the counter and the norm.
+  // one before it, nor for the counter and the norm.  A wave has four blocks in a row, whose scales are one
+  // vector.
   float p[kIters][4], g[kIters][4], m[kIters][4], v[kIters][4];
   uint32_t mw[kIters], vw[kIters];
   float ms[kIters], vs[kIters];
 #pragma unroll
   for (int k = 0; k < kIters; ++k) {
-    const int block = wave + k * (kThreads / 64), at = block * kBlock + 4 * lane;
+    const int at = (wave * kIters + k) * kBlock + 4 * lane;
     const int left = n - at;
     const int64_t idx = base + at;
     if constexpr (MASTER) load4<F32>(a.t.ptr[PTRS - 1][i], idx, left, p[k]);
     else load4<Ty>(a.t.ptr[kParam][i], idx, left, p[k]);
     load4<Ty>(a.t.ptr[kGrad][i], idx, left, g[k]);
     if constexpr (BITS == 8) {
-      const bool held = block * kBlock < n;  // wave-uniform: the block has values
-      ms[k] = held ? static_cast<const float*>(a.t.ptr[kMScale][i])[block0 + block] : 0.f;
-      vs[k] = held ? static_cast<const float*>(a.t.ptr[kVScale][i])[block0 + block] : 0.f;
       mw[k] = load_codes(a.t.ptr[kM][i], idx, left);
       vw[k] = load_codes(a.t.ptr[kV][i], idx, left);
     } else {
       load4<F32>(a.t.ptr[kM][i], idx, left, m[k]);
       load4<F32>(a.t.ptr[kV][i], idx, left, v[k]);
     }
+  }
+  const int64_t block0 = static_cast<int64_t>(local) * (kChunk / kBlock) + wave * kIters;
+  const int blocks = (n + kBlock - 1) / kBlock - wave * kIters;  // of this wave, where below kIters
+  if constexpr (BITS == 8) {
+    load4<F32>(a.t.ptr[kMScale][i], block0, blocks, ms);
+    load4<F32>(a.t.ptr[kVScale][i], block0, blocks, vs);
   }
 
   float coef = 1.f;
@@ -250,8 +254,8 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_kernel(StepArgs<kPtrsOf<Ty,
 
 #pragma unroll
   for (int k = 0; k < kIters; ++k) {
-    const int block = wave + k * (kThreads / 64), at = block * kBlock + 4 * lane;
-    if (block * kBlock >= n) break;  // wave-uniform
+    if (k >= blocks) break;  // wave-uniform
+    const int at = (wave * kIters + k) * kBlock + 4 * lane;
     const int left = n - at;
     const int64_t idx = base + at;
     if constexpr (BITS == 8) {
@@ -277,14 +281,14 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_kernel(StepArgs<kPtrsOf<Ty,
       vw[k] = encode4<true>(root, vs[k]);
       store_codes(a.t.ptr[kM][i], idx, left, mw[k]);
       store_codes(a.t.ptr[kV][i], idx, left, vw[k]);
-      if (lane == 0) {
-        static_cast<float*>(a.t.ptr[kMScale][i])[block0 + block] = ms[k];
-        static_cast<float*>(a.t.ptr[kVScale][i])[block0 + block] = vs[k];
-      }
     } else {
       store4<F32>(a.t.ptr[kM][i], idx, left, m[k]);
       store4<F32>(a.t.ptr[kV][i], idx, left, v[k]);
     }
+  }
+  if (BITS == 8 && lane == 0) {
+    store4<F32>(a.t.ptr[kMScale][i], block0, blocks, ms);
+    store4<F32>(a.t.ptr[kVScale][i], block0, blocks, vs);
   }
 }
 
