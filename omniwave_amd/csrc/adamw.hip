@@ -303,25 +303,50 @@ struct NormArgs {
   int32_t count;
 };
 
+// A workgroup takes a range of chunks and walks the tensors that they are of, so that it looks a tensor up
+// once and has four vectors of 16 bytes a thread in flight.
 template <class Ty>
 __global__ void __launch_bounds__(kThreads) grad_norm_kernel(NormArgs a) {
+  typedef Row<Ty> R;
+  constexpr int V = R::kVec, U = 4;
   __shared__ double lds[kThreads / 64];
   double sum = 0.0;
-  for (uint32_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
-    const int i = tensor_of<NormArgs::N>(a, a.count, chunk);
-    const uint32_t local = chunk - a.first[i];
-    const uint32_t next = i + 1 < a.count ? a.first[i + 1] : a.chunks;
-    const int n = chunk + 1 == next ? a.last[i] + 1 : kChunk;
+  uint32_t chunk = static_cast<uint32_t>(static_cast<uint64_t>(a.chunks) * blockIdx.x / gridDim.x);
+  const uint32_t stop = static_cast<uint32_t>(static_cast<uint64_t>(a.chunks) * (blockIdx.x + 1) / gridDim.x);
+  int i = chunk < stop ? tensor_of<NormArgs::N>(a, a.count, chunk) : 0;
+  for (; chunk < stop; ++i) {
+    const uint32_t first = a.first[i], next = i + 1 < a.count ? a.first[i + 1] : a.chunks;
+    const int64_t numel = static_cast<int64_t>(next - first - 1) * kChunk + a.last[i] + 1;
+    const uint32_t until = next < stop ? next : stop;
+    const int64_t limit = static_cast<int64_t>(until - first) * kChunk, end = limit < numel ? limit : numel;
+    const typename R::Elem* g = static_cast<const typename R::Elem*>(a.grad[i]);
+    auto add = [&](const float (&v)[V]) {
 #pragma unroll
-    for (int k = 0; k < kIters; ++k) {
-      const int at = (k * kThreads + threadIdx.x) * 4;
-      if (at < n) {
-        float g[4];
-        load4<Ty>(a.grad[i], static_cast<int64_t>(local) * kChunk + at, n - at, g);
+      for (int j = 0; j < V; ++j) sum += static_cast<double>(v[j]) * v[j];
+    };
+    int64_t at = static_cast<int64_t>(chunk - first) * kChunk + threadIdx.x * V;
+    for (; at + (U - 1) * kThreads * V + V <= end; at += U * kThreads * V) {
+      typename R::Raw raw[U];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sum += static_cast<double>(g[j]) * g[j];
+      for (int u = 0; u < U; ++u) raw[u] = R::raw(g + at + u * kThreads * V);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float v[V];
+        R::widen(raw[u], v);
+        add(v);
       }
     }
+    for (; at < end; at += kThreads * V) {
+      float v[V];
+      if (at + V <= end) {
+        R::load(g + at, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = at + j < end ? R::to_f32(g[at + j]) : 0.f;
+      }
+      add(v);
+    }
+    chunk = until;
   }
   sum = workgroup_sum<kThreads / 64>(sum, lds);
   if (threadIdx.x == 0) a.partials[blockIdx.x] = sum;
