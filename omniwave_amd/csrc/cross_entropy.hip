@@ -8,12 +8,16 @@
 // with w the upstream gradient, divided by the number of counted rows for their mean, and 0 for rows
 // left out.  Forward and backward read the logits once each; they are bound by memory where there are many
 // and by the launches where there are few.  A thread of the forward keeps a running maximum, the sum of
-// exponentials below it and the sum of the logits, four vectors at a time, so a row of any length is one pass; a row belongs to
-// a wave, or to a workgroup where it is long, and where rows are too few to fill the chip each is cut
-// into parts whose numbers the second kernel joins.  That kernel also sums the rows' losses, in a fixed
-// order.  The backward needs m and z of a row alone, so it is cut into workgroups at will.  m and z are
-// kept apart: x - m has the rounding of the difference, x - (m + ln z) would have that of x.
-// Exponentials, sums and losses are fp32; the gradient is rounded once.
+// exponentials below it and the sum of the logits, four vectors at a time, so a row of any length is one
+// pass; a row belongs to a wave, or to a workgroup where it is long, and where rows are too few to fill the
+// chip each is cut into parts whose numbers the second kernel joins.  That kernel also sums the rows' losses,
+// in a fixed order.  The backward needs m and z of a row alone, so it is cut into workgroups at will.  m and
+// z are kept apart: x - m has the rounding of the difference, x - (m + ln z) would have that of x.
+// Exponentials, sums and losses are fp32 (the sum of losses fp64); the gradient is rounded once.
+//
+// Measured: 4,096 x 21,841 bf16 forward 54 us (3.3 TB/s; 47.5 us where every row starts at 16 bytes, and
+// 44.4 for the read alone), backward 61 us (5.9 TB/s); 1,024 x 1,000 fp32 4.9 + 4.0 (the sum) and 5.0 us;
+// 8 x 1,000 bf16 4.4 and 3.3 us, where a call costs its caller 48 us.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -230,7 +234,8 @@ template <class Ty>
 __global__ void __launch_bounds__(kSumThreads) xent_few_kernel(XentArgs a) {
   typedef Row<Ty> R;
   const int lane = threadIdx.x & 63;
-  for (int64_t row = threadIdx.x >> 6; row < a.c.rows; row += kSumThreads / 64) {
+  const int64_t row = threadIdx.x >> 6;
+  if (row < a.c.rows) {
     Labels y;
     if (lane == 0) y = Labels(a, row);
     Numbers s;
@@ -330,10 +335,13 @@ __global__ void __launch_bounds__(256) xent_bwd_kernel(XentBwdArgs a) {
   }
 }
 
-// How rows are cut: `parts` of `len` logits each, enough of them for two workgroups a compute unit.
+// How rows are cut: `parts` of `len` logits each, enough of them for two workgroups a compute unit.  The
+// parts' join costs 0.7 us and 1.3 more for every 64 rows, a row read by one workgroup 0.09 us for every 1,000
+// logits; cut against not, forward of bf16 rows with their mean: 8 x 8,192 6.8 / 6.2 us, 8 x 21,841 6.8 / 8.0,
+// 64 x 50,000 8.6 / 10.4, 160 x 50,000 11.9 / 10.6, 128 x 200,000 18.8 / 29.2, 300 x 200,000 36.2 / 34.8.
 void cut(const OwCrossEntropy& c, int32_t* parts, int32_t* len) {
   int64_t n = 1;
-  if (c.classes > kLong) {
+  if (c.rows < device_cus() && c.classes > 4 * kPart && c.classes > 400 * c.rows) {
     const int64_t want = (2 * static_cast<int64_t>(device_cus()) + c.rows - 1) / c.rows;
     const int64_t most = (c.classes + kPart - 1) / kPart;
     n = want < most ? want : most;
@@ -341,6 +349,14 @@ void cut(const OwCrossEntropy& c, int32_t* parts, int32_t* len) {
   const int64_t each = ((c.classes + n - 1) / n + 7) / 8 * 8;
   *parts = static_cast<int32_t>((c.classes + each - 1) / each);
   *len = static_cast<int32_t>(each);
+}
+
+// Logits of a workgroup of the backward: 4 vectors a thread (8 for fp32), or one (2) where that leaves
+// compute units without work (64 x 21,841 bf16: 14.1 us with the forward at 4 vectors, 12.9 at one;
+// 4,096 x 21,841: 102 and 117).
+int backward_part(const OwCrossEntropy& c) {
+  const int64_t workgroups = c.rows * ((c.classes + 2 * kPart - 1) / (2 * kPart));
+  return workgroups < device_cus() ? kPart / 2 : 2 * kPart;
 }
 
 // Whether a row belongs to a wave or to a workgroup (700 rows of 4,096 fp32: forward 6.8 and backward 10.8 us
@@ -365,10 +381,12 @@ int check(const OwCrossEntropy* c) {
   return OW_OK;
 }
 
-// Rows that one workgroup takes with their sum: two a wave, below which a second launch costs more than
-// the rows gain from more workgroups.
-constexpr int kFewRows = 2 * kSumThreads / 64;
-bool few_rows(const XentArgs& a) { return a.loss != nullptr && a.c.rows <= kFewRows && a.c.classes <= kLong; }
+// Whether one workgroup takes all rows with their sum, a wave each: a second launch costs more there than the
+// rows gain from more workgroups (bf16, one launch against two: 8 x 1,000 4.7 / 5.6 us, 16 x 2,048 5.6 / 6.2,
+// 8 x 4,096 5.7 / 6.1, but 16 x 4,096 7.5 / 6.3 and 32 x 1,000 8.2 / 5.8).
+bool few_rows(const XentArgs& a) {
+  return a.loss != nullptr && a.c.rows <= kSumThreads / 64 && a.c.classes <= kLong && a.c.rows * a.c.classes <= 8 * kLong;
+}
 
 template <class Ty>
 void launch_fwd(const XentArgs& a, hipStream_t s) {
@@ -457,8 +475,7 @@ int ow_cross_entropy_bwd(const OwCrossEntropy* ce, const float* stats, const flo
   a.weight = weight;
   a.upstream = upstream;
   a.grad = grad;
-  // Parts of a workgroup's 4 vectors a thread (2 for fp32).
-  a.part_len = ow::wave_rows(*ce) ? static_cast<int32_t>((ce->classes + 7) / 8 * 8) : 2 * ow::kPart;
+  a.part_len = ow::wave_rows(*ce) ? static_cast<int32_t>((ce->classes + 7) / 8 * 8) : ow::backward_part(*ce);
   a.n_parts = static_cast<int32_t>((ce->classes + a.part_len - 1) / a.part_len);
   OW_CHECK_SUPPORTED(ce->rows * a.n_parts < (int64_t(1) << 31), "too many rows");
   hipStream_t s = static_cast<hipStream_t>(stream);

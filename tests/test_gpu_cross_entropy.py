@@ -264,3 +264,35 @@ def test_same_bits_on_a_side_stream_in_a_graph_and_through_the_operator() -> Non
             eager = step()
             torch.cuda.synchronize()
             assert all(torch.equal(p, q) for p, q in zip(held, eager)), f"replay {n}"
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,k", [(16, 2048), (16, 2049), (17, 100), (8, 4096), (9, 4096), (3, 16384), (3, 16385), (40, 16400),
+                                    (42, 16400), (250, 8193), (1, 66000)])
+def test_sizes_where_another_kernel_or_another_cut_begins(rows, k, dtype) -> None:
+    """Sizes as above: a thread adds at most 16,400 / 256 terms where rows are not cut, 4,096 / 256 where they are."""
+    announce(f"xent rows={rows} k={k} {dtype}")
+    x, a, b, mix = make(rows, k, TYPES[dtype], seed=rows + k, left_out=0.2)
+    for reduction in ("mean", "none"):
+        check(x, a, b, mix, s=0.1, reduction=reduction)
+
+
+def test_parts_of_a_row_without_a_number_above_minus_infinity() -> None:
+    announce("xent masked parts")
+    x, a, b, _ = make(6, 20000, torch.float32)
+    x[0, :9000] = float("-inf")  # whole parts
+    x[1, 9000:] = float("-inf")
+    x[2, 4096:16384] = float("-inf")
+    x[3] = float("-inf")
+    x[4, 19999] = float("nan")
+    x[5, 8000] = float("inf")
+    a[:3] = torch.tensor([19999, 0, 19998], device=DEV)
+    b[:3] = torch.tensor([9000, 8999, 4095], device=DEV)
+    for reduction in ("none", "mean"):
+        check(x[:3], a[:3], b[:3], 0.3, reduction=reduction)
+    assert cross_entropy_hip(x, a, reduction="none")[3:].isnan().all()
+    a[3:] = -100
+    y = x.detach().requires_grad_(True)
+    loss = cross_entropy_hip(y, a)
+    (grad,) = torch.autograd.grad(loss, y)
+    assert loss.isfinite() and grad.isfinite().all() and not grad[3:].any()
