@@ -238,7 +238,13 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_kernel(StepArgs<kPtrsOf<Ty,
   float coef = 1.f;
   if (a.partials != nullptr) {
     double sum = 0.0;  // in a fixed order, every workgroup alike
-    for (int k = threadIdx.x; k < a.n_partials; k += kThreads) sum += a.partials[k];
+    for (int k = threadIdx.x; k < a.n_partials; k += 8 * kThreads) {  // eight loads in flight, not one
+      double part[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) part[u] = k + u * kThreads < a.n_partials ? a.partials[k + u * kThreads] : 0.0;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) sum += part[u];
+    }
     const float norm = static_cast<float>(sqrt(workgroup_sum<kThreads / 64>(sum, lds)));
     if (chunk == 0 && threadIdx.x == 0 && a.norm_out != nullptr) *a.norm_out = norm;
     if (!(norm < __builtin_inff())) return;  // the step is skipped

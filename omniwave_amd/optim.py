@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from itertools import chain
+from itertools import chain, groupby
 from operator import is_
 
 import numpy as np
@@ -230,9 +230,9 @@ class AdamW(torch.optim.Optimizer):
         hyper = plan.hyper(*[_hyper(g, device) for g in self.param_groups])
         if device.index != torch._C._cuda_getDevice():
             with torch.cuda.device(device):
-                self._launch(plan.kinds, hyper, device)
+                self._launch(plan, hyper, device)
         else:
-            self._launch(plan.kinds, hyper, device)
+            self._launch(plan, hyper, device)
         del keep
         # The kernels write past autograd's notice: what goes by a parameter's version has to see the change.
         torch.autograd.graph.increment_version(plan.active)
@@ -240,20 +240,19 @@ class AdamW(torch.optim.Optimizer):
 
     _heard_step = torch.optim.Optimizer.profile_hook_step(_step)
 
-    def _launch(self, kinds: list[_Kind], hyper, device: torch.device) -> None:
+    def _launch(self, plan: _Plan, hyper, device: torch.device) -> None:
         lib, stream = _native.lib(), _stream_ptr(device)
         partials, total, norm_ptr, at = None, 0, None, None
         if self.max_grad_norm is not None:
-            total = sum(kind.partials for kind in kinds)
+            total = sum(partials for *_, partials in plan.norms)
             partials = torch.empty(total, dtype=torch.float64, device=device)
             self.grad_norm = torch.empty((), dtype=torch.float32, device=device)
             at = first = partials.data_ptr()
             norm_ptr = self.grad_norm.data_ptr()
-            for kind in kinds:
-                _native.check(lib.ow_grad_norm(kind.pointer, kind.count, kind.code, first, kind.partials, stream),
-                              "ow_grad_norm")
-                first += 8 * kind.partials
-        for kind in kinds:
+            for pointer, count, code, n in plan.norms:
+                _native.check(lib.ow_grad_norm(pointer, count, code, first, n, stream), "ow_grad_norm")
+                first += 8 * n
+        for kind in plan.kinds:
             _native.check(lib.ow_adamw_step(kind.pointer, kind.count, hyper, len(hyper), kind.code, kind.bits, kind.master, at,
                                             total, self.max_grad_norm or 0.0, norm_ptr, stream), "ow_adamw_step")
             norm_ptr = None
@@ -303,9 +302,19 @@ class _Plan:
             opt._check_state(p, layout)
             key = (p.dtype, 8 if "exp_avg_sq_root" in layout else 32, "master" in layout)
             kinds.setdefault(key, _Kind(*key)).add(i, p, opt.state[p], owner[i])
-        self.kinds = list(kinds.values())
-        for kind in self.kinds:
-            kind.finish()
+        # One list, kinds of a dtype next to each other: their gradients' norm is one call.
+        self.kinds = sorted(kinds.values(), key=lambda kind: kind.code)
+        self.table = np.array([row for kind in self.kinds for row in kind.rows], dtype=np.int64)
+        self.at = [i for kind in self.kinds for i in kind.at]
+        self.norms: list[tuple[int, int, int, int]] = []  # address, tensors, dtype, partial sums
+        first = 0
+        for code, same in groupby(self.kinds, key=lambda kind: kind.code):
+            start = first
+            for kind in same:
+                kind.pointer, kind.count = self.table[first:].ctypes.data, len(kind.rows)
+                first += kind.count
+            pointer, count = self.table[start:].ctypes.data, first - start
+            self.norms.append((pointer, count, code, _native.lib().ow_grad_norm_partials(pointer, count)))
         self.active = [params[i] for i in active]
         self.addresses = glue.addresses(params)
         self.entries = list(opt.state.values())
@@ -324,8 +333,7 @@ class _Plan:
         """Writes the gradients' addresses into the lists."""
         if lie != self.lie:
             where = np.frombuffer(lie, dtype=np.int64)
-            for kind in self.kinds:
-                kind.table[:, _GRAD] = where[kind.at]
+            self.table[:, _GRAD] = where[self.at]
             self.lie = lie
 
 
@@ -333,7 +341,7 @@ class _Kind:
     """Tensors of one dtype and state layout: one list for the native calls."""
 
     def __init__(self, dtype: torch.dtype, bits: int, master: bool) -> None:
-        self.dtype, self.bits, self.master = dtype, bits, master
+        self.code, self.bits, self.master = _DTYPE_CODE[dtype], bits, master
         self.at: list[int] = []  # places among the parameters
         self.rows: list[list[int]] = []
 
@@ -343,11 +351,6 @@ class _Kind:
         self.at.append(i)
         self.rows.append([p.data_ptr(), 0, *ptr, entry["master"].data_ptr() if self.master else 0, entry["step"].data_ptr(),
                           p.numel(), group])
-
-    def finish(self) -> None:
-        self.table = np.array(self.rows, dtype=np.int64)
-        self.pointer, self.count, self.code = self.table.ctypes.data, len(self.rows), _DTYPE_CODE[self.dtype]
-        self.partials = _native.lib().ow_grad_norm_partials(self.pointer, self.count)
 
 
 def _hyper(group: dict, device: torch.device | None = None) -> tuple:
