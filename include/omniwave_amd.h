@@ -659,9 +659,10 @@ int ow_adamw_step(const OwAdamwTensor* tensors, int32_t count, const OwAdamwGrou
  * mix is NULL.  Labels outside [0, classes) make the row's loss and gradient NaN.  row_stride: values between
  * rows (any alignment; value stride 1).
  *
- * Forward: stats [rows][2] (what the backward needs), losses [rows], and with a reduction loss [1],
- * the result, and weight [1], a row's weight in it (both NULL without).  Backward: the forward's stats and
- * weight, upstream [1] or, without a reduction, [rows]; grad [rows][classes] of the logits' dtype.
+ * Forward: stats [rows][2] (what the backward needs), losses [rows], a workspace (8-byte aligned) of
+ * ow_cross_entropy_workspace bytes, and with a reduction loss [1], the result, and weight [1], a row's weight
+ * in it (both NULL without).  Backward: the forward's stats and weight, upstream [1] or, without a reduction,
+ * [rows]; grad [rows][classes] of the logits' dtype.
  */
 #define OW_REDUCE_NONE 0
 #define OW_REDUCE_SUM 1

@@ -296,3 +296,53 @@ def test_parts_of_a_row_without_a_number_above_minus_infinity() -> None:
     loss = cross_entropy_hip(y, a)
     (grad,) = torch.autograd.grad(loss, y)
     assert loss.isfinite() and grad.isfinite().all() and not grad[3:].any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,k", [(2047, 40), (2048, 40), (8192, 3), (8193, 3), (8195, 9), (9000, 130), (9000, 260), (9001, 600),
+                                    (9000, 1100), (140001, 7), (8200, 4097)])
+def test_many_rows(rows, k, dtype) -> None:
+    """Several rows a wave and a workgroup; a thread adds at most 4,097 / 64 terms."""
+    announce(f"xent rows={rows} k={k} {dtype}")
+    x, a, b, mix = make(rows, k, TYPES[dtype], seed=rows + k, left_out=0.2)
+    first = check(x, a, b, mix, s=0.1)
+    again = check(x, a, b, mix, s=0.1, up=torch.ones((), device=DEV))
+    assert torch.equal(first[0], again[0])
+    check(x, a, reduction="sum")
+    check(x, a, b, mix, s=0.1, reduction="none")
+    a[:] = -100
+    y = x.detach().requires_grad_(True)
+    loss = cross_entropy_hip(y, a)
+    assert loss.isnan() and not torch.autograd.grad(loss, y)[0].any()
+
+
+def test_many_rows_in_strides_with_bad_ones_and_in_a_graph() -> None:
+    announce("xent many rows, strides, bad rows, graph")
+    x, a, b, mix = make(10000, 61, torch.float32)
+    wide = torch.zeros(10000, 70, device=DEV)
+    wide[:, 5:66] = x
+    wide.requires_grad_(True)
+
+    def step():
+        loss = cross_entropy_hip(wide[:, 5:66], a, target_b=b, mix=mix)
+        return loss.detach(), torch.autograd.grad(loss, wide)[0]
+
+    check(wide[:, 5:66], a, b, mix)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for n in range(3):
+        with torch.no_grad():
+            wide.mul_(0.9)
+            a.copy_(a.roll(1))
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(held, eager)), f"replay {n}"
+    x[77, 3], a[78] = float("nan"), 61
+    losses = cross_entropy_hip(x, a, reduction="none")
+    bad = losses.isnan()
+    assert bad[77:79].all() and bad.sum() == 2 and cross_entropy_hip(x, a).isnan()
+    a[77:79] = -100
+    assert cross_entropy_hip(x, a).isfinite()
