@@ -344,3 +344,25 @@ def test_the_operator_is_the_plain_call() -> None:
     assert torch.equal(out, plain[0]) and torch.equal(nxt, plain[1])
     grads = torch.autograd.grad((out, nxt), [t[n] for n in LEAVES], (t["dout"], t["dnext"]))
     assert all(torch.equal(g, plain[2][n]) for g, n in zip(grads, LEAVES))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", [(3, 7, 96), (2, 5, 1024), (5, 1, 33)])
+def test_rows_that_fill_no_workgroup_without_eps(shape, dtype) -> None:
+    """eps = 0: what a workgroup holds beside its last rows adds nothing to the weights' gradients."""
+    announce(f"norms eps=0 {shape} {dtype}")
+    check(make(shape, dtype, torch.float32, scale=True), eps=0.0)
+    t = make(shape, dtype, torch.float32, scale=True, gate="image")
+    check(dict(t), eps=0.0)
+    for n in LEAVES:
+        t[n] = t[n].detach().requires_grad_(True)
+    t["scale"][0] = float("inf")  # an image's scale stays with it
+    (g,) = torch.autograd.grad(call(t, eps=0.0), [t["gate"]], (t["dout"], t["dnext"]))
+    assert g[1:].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("c", [4096, 5000, 8192, 8190])
+def test_wide_rows(c, dtype) -> None:
+    announce(f"norms 2x400x{c} {dtype}")
+    check(make((2, 400, c), dtype, torch.float32, scale=True))
