@@ -62,7 +62,9 @@ class AdamW(torch.optim.Optimizer):
     at most this, and skip the step (parameters, states and counters) where the norm is not finite;
     ``grad_norm`` is then the last step's norm, on the device.
 
-    Parameters: contiguous, of fp32, bf16 or fp16, on one gfx950 GPU; gradients of the same dtype, dense.
+    Parameters: contiguous, of fp32, bf16 or fp16, on one gfx950 GPU, no two in the same memory; gradients of
+    the same dtype, dense.  With ``master_weights`` a step starts from the fp32 copy: a parameter that is
+    changed otherwise (weights loaded or averaged in) has ``state[p]["master"]`` to be changed alike.
     ``lr`` may be a 0-dim fp32 tensor on the GPU, which a captured step reads anew; other
     hyperparameters of a captured step are those of its capture.  States are made by the first step, which
     therefore is not captured.  A step raises the parameters' version counters; the replay of a captured one
@@ -302,6 +304,7 @@ class _Plan:
             opt._check_state(p, layout)
             key = (p.dtype, 8 if "exp_avg_sq_root" in layout else 32, "master" in layout)
             kinds.setdefault(key, _Kind(*key)).add(i, p, opt.state[p], owner[i])
+        _refuse_overlap([params[i] for i in active])
         # One list, kinds of a dtype next to each other: their gradients' norm is one call.
         self.kinds = sorted(kinds.values(), key=lambda kind: kind.code)
         self.table = np.array([row for kind in self.kinds for row in kind.rows], dtype=np.int64)
@@ -351,6 +354,14 @@ class _Kind:
         self.at.append(i)
         self.rows.append([p.data_ptr(), 0, *ptr, entry["master"].data_ptr() if self.master else 0, entry["step"].data_ptr(),
                           p.numel(), group])
+
+
+def _refuse_overlap(params: list[Tensor]) -> None:
+    """Tensors that share memory would be updated by two workgroups at once."""
+    spans = sorted((p.data_ptr(), p.numel() * p.element_size(), tuple(p.shape)) for p in params)
+    for (at, size, shape), (other, _, other_shape) in zip(spans, spans[1:]):
+        if at + size > other:
+            raise ValueError(f"parameters of shapes {shape} and {other_shape} share memory")
 
 
 def _hyper(group: dict, device: torch.device | None = None) -> tuple:

@@ -137,3 +137,29 @@ def test_half_precision_mix_and_numbers_of_other_kinds() -> None:
         block_norms_hip(x, x, post_weight=torch.ones(50))
     with pytest.raises(ValueError, match="eps"):
         rms_norm_hip(x, torch.ones(50, device=DEV), eps=-1)
+
+
+def test_parameters_in_the_same_memory_are_refused() -> None:
+    announce("adamw overlapping parameters")
+    flat = torch.zeros(10000, device=DEV)
+    p, q, r = (torch.nn.Parameter(flat[a:b]) for a, b in ((0, 5000), (5000, 10000), (4999, 6000)))
+    for t in (p, q, r):
+        t.grad = torch.ones_like(t)
+    AdamW([p, q]).step()  # beside each other
+    kept = flat.clone()
+    with pytest.raises(ValueError, match="share memory"):
+        AdamW([p, r]).step()
+    assert torch.equal(flat, kept)
+
+
+def test_a_master_copy_is_what_a_step_starts_from() -> None:
+    announce("adamw master copy")
+    p = torch.nn.Parameter(torch.ones(300, device=DEV).bfloat16())
+    opt = AdamW([p], lr=0.0, weight_decay=0.0, master_weights=True)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    with torch.no_grad():
+        p.fill_(2.0)
+        opt.state[p]["master"].fill_(2.0)
+    opt.step()
+    assert (p == 2).all()
