@@ -56,7 +56,9 @@ class _Stage(nn.Module):
         return x
 
     def _takes_normed(self, x: Tensor) -> bool:
-        return len(self.blocks) > 0 and all(block.takes_normed(x) for block in self.blocks)
+        # A block may have been wrapped, and is then called like any module.
+        return len(self.blocks) > 0 and all(isinstance(block, OmniWeaveBlock) and block.takes_normed(x)
+                                            for block in self.blocks)
 
     def _forward_normed(self, x: Tensor) -> Tensor:
         """The blocks with ``post_norm`` in a row: the norm before the first one, then each block's kernel

@@ -18,6 +18,7 @@ import math
 import torch
 import torch.nn as nn
 from torch import Tensor
+from torch.nn.modules.module import _has_any_global_hook
 
 from omniwave_amd.bigemm import bigemm
 from omniwave_amd.hip import (_block, _chain, bigemm_block_s2d_hip, bigemm_delta_hip, drop_path_scale,
@@ -113,8 +114,11 @@ class OmniWeaveBlock(nn.Module):
 
     def takes_normed(self, x: Tensor) -> bool:
         """Whether ``forward_normed`` can run ``x``: a block with ``post_norm`` on the hip backend, not in fp8
-        (whose kernel wants the norm fused)."""
-        return self.post_norm and not self.fp8 and self.dim <= MAX_CHANNELS and self._fused(x)
+        (whose kernel wants the norm fused), whose own call nothing listens to or replaces."""
+        return (self.post_norm and not self.fp8 and self.dim <= MAX_CHANNELS and self._fused(x)
+                and type(self).forward is OmniWeaveBlock.forward and "forward" not in vars(self)
+                and not (self._forward_hooks or self._forward_pre_hooks or self._backward_hooks
+                         or self._backward_pre_hooks or _has_any_global_hook()))
 
     def forward_normed(self, x: Tensor, normed: Tensor, next_weight: Tensor | None) -> tuple[Tensor, Tensor | None]:
         """(``self(x)``, the same under the next block's norm), given ``normed``, x under this block's norm:

@@ -255,3 +255,26 @@ def test_training_rows() -> None:
                           "model_options": options, "training": {"state_bits": 8}, "warmup": 1, "iterations": 2}, DEV)
     assert len(rows) == 2 and all("error" not in r for r in rows), rows
     assert all(r["kind"] == "train" and r["images_per_second"] > 0 for r in rows)
+
+
+def test_hooks_and_wrappers_of_blocks_are_called() -> None:
+    """The stage runs its blocks one by one where something listens; the two ways differ by roundings of the
+    normalised inputs (half a step of bf16 each, through two blocks)."""
+    announce("post-norm stage with hooks")
+    torch.manual_seed(0)
+    model = create_model("omniweave_t", backend="hip", post_norm=True).to(DEV, torch.bfloat16).train()
+    stage = model.stages[2]
+    x = torch.randn(2, 14, 14, stage.blocks[0].dim, device=DEV).bfloat16()
+    assert stage._takes_normed(x)
+    want = stage(x)
+    seen = []
+    handle = stage.blocks[1].register_forward_hook(lambda *_: seen.append(1))
+    assert not stage._takes_normed(x)
+    got = stage(x)
+    assert seen == [1]
+    assert (got.float() - want.float()).norm() <= 2e-2 * want.float().norm()
+    handle.remove()
+    assert stage._takes_normed(x) and torch.equal(stage(x), want)
+    inner = stage.blocks[0]
+    stage.blocks[0] = torch.nn.Sequential(inner)
+    assert not stage._takes_normed(x) and torch.equal(stage(x), got)

@@ -98,3 +98,25 @@ def test_training_rows_say_why_there_are_none() -> None:
                          torch.device("cpu"))
     assert [r["kind"] for r in rows] == ["train"]
     assert "error" in rows[0] and rows[0]["batch_size"] == 2
+
+
+class Wrapped(torch.nn.Module):
+    def __init__(self, inner) -> None:
+        super().__init__()
+        self.inner, self.calls = inner, 0
+
+    def forward(self, x):
+        self.calls += 1
+        return self.inner(x)
+
+
+@pytest.mark.parametrize("post_norm", [False, True])
+def test_wrapped_blocks_and_hooks_are_called(oracle_backend, post_norm) -> None:
+    model = create_model("omniweave_t", backend="reference", post_norm=post_norm, **SMALL)
+    stage = model.stages[2]
+    x = torch.randn(1, stage.blocks[0].plan.height, stage.blocks[0].plan.width, 128)
+    want = stage(x)
+    seen = []
+    stage.blocks[0].register_forward_hook(lambda *_: seen.append(0))
+    stage.blocks[1] = Wrapped(stage.blocks[1])
+    assert torch.equal(stage(x), want) and seen == [0] and stage.blocks[1].calls == 1
