@@ -15,9 +15,9 @@
 // z are kept apart: x - m has the rounding of the difference, x - (m + ln z) would have that of x.
 // Exponentials, sums and losses are fp32 (the sum of losses fp64); the gradient is rounded once.
 //
-// Measured: 4,096 x 21,841 bf16 forward 54 us (3.3 TB/s; 47.5 us where every row starts at 16 bytes, and
-// 44.4 for the read alone), backward 61 us (5.9 TB/s); 1,024 x 1,000 fp32 4.9 + 4.0 (the sum) and 5.0 us;
-// 8 x 1,000 bf16 4.4 and 3.3 us, where a call costs its caller 48 us.
+// Measured: 4,096 x 21,841 bf16 forward 50 us (179 MB; 55 where vectors began with the row, at any address),
+// backward 61 us (358 MB, 5.9 TB/s); 1,024 x 1,000 fp32 4.9 + 4.0 (the sum) and 5.0 us; 8 x 1,000 bf16 4.4 and
+// 3.3 us, where a call costs its caller 48 us.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -141,13 +141,21 @@ struct Numbers {
   template <class R, int T>
   __device__ __forceinline__ void scan(const typename R::Elem* x, int64_t begin, int64_t end, int t) {
     constexpr int V = R::kVec;
-    const int64_t vectors = (end - begin) / V;
     x += begin;
+    // Vectors of a long row begin at 16 bytes: the values before and behind them are taken one by one.
+    const int64_t n = end - begin;
+    int head = 0;
+    if (T > 64) {
+      head = static_cast<int>((0 - reinterpret_cast<uintptr_t>(x)) % 16 / sizeof(typename R::Elem));
+      head = head < n ? head : static_cast<int>(n);
+    }
+    const typename R::Elem* body = x + head;
+    const int64_t vectors = (n - head) / V;
     // Vectors of this thread: t, t + T, ...
     typename R::Raw next[U];
     auto load = [&](int64_t at) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) next[u] = at + u * T < vectors ? R::raw(x + (at + u * T) * V) : R::zero();
+      for (int u = 0; u < U; ++u) next[u] = at + u * T < vectors ? R::raw(body + (at + u * T) * V) : R::zero();
     };
     // A long row's next block is read while one is computed; a wave's short rows have few blocks, and more
     // waves instead (30,000 rows of 300 fp32: 22.3 us with, 18.5 without).
@@ -163,9 +171,9 @@ struct Numbers {
       if (left >= U) add<R, true>(raw, U);
       else add<R, false>(raw, left);
     }
-    // What fills no vector, a value each.
-    const int64_t i = vectors * V + t;
-    if (t < V && begin + i < end) {
+    // What fills no vector, a value each (fewer than V before and behind: 2 V <= T where both may be).
+    const int64_t i = t < head ? t : vectors * V + t;
+    if (t < head + V && i < n) {
       const float v = R::to_f32(x[i]);
       total += v;
       const float top = fmaxf(m, v);
