@@ -128,16 +128,27 @@ struct Numbers {
       }
     }
     scale_to(top);
-    if (top == -__builtin_inff()) return;
+    // Blocks that are not whole, a row's last ones, are left early (200,000 rows of 1,000 bf16: 88.5 us, 92.9 without;
+    // whole ones, 4,096 of 21,841, lose 0.3 by it).
+    if (!WHOLE && top == -__builtin_inff()) {
+      if (total != total) z = total;
+      return;
+    }
+    const float from = WHOLE ? floor_of(top) : top;
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int j = 0; j < V; ++j) z += __builtin_amdgcn_exp2f((v[u][j] - top) * kLog2e);
+      for (int j = 0; j < V; ++j) z += __builtin_amdgcn_exp2f((v[u][j] - from) * kLog2e);
   }
   __device__ __forceinline__ void scale_to(float top) {
     z *= exp_below(m, top);
     m = top;
   }
+  // What is subtracted from a logit before its exponential is added to z: the maximum, and the lowest finite number
+  // while nothing above -inf has been seen: -inf then adds 0, and a NaN, which a maximum passes over, is in z all
+  // the same.  (`total` is NaN then, too, and only then: it is a sum of -inf otherwise.)  Every join keeps a NaN z,
+  // and the row's loss and gradient get it from there.
+  static __device__ __forceinline__ float floor_of(float m) { return fmaxf(m, -3.402823466e38f); }
   template <class R, int T>
   __device__ __forceinline__ void scan(const typename R::Elem* x, int64_t begin, int64_t end, int t) {
     constexpr int V = R::kVec;
@@ -178,7 +189,7 @@ struct Numbers {
       total += v;
       const float top = fmaxf(m, v);
       scale_to(top);
-      if (top != -__builtin_inff()) z += __builtin_amdgcn_exp2f((v - top) * kLog2e);
+      z += __builtin_amdgcn_exp2f((v - floor_of(top)) * kLog2e);
     }
   }
   template <int T>
