@@ -444,11 +444,12 @@ PyObject* py_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n_args) 
   END_HANDLE_TH_ERRORS
 }
 
-// Addresses of tensors as bytes, 8 each, to be compared as a whole.
-class Addresses {
+// Numbers (addresses of tensors and what lies there) as bytes, 8 each, to be compared as a whole.
+class Numbers {
  public:
-  explicit Addresses(Py_ssize_t n) { of_.reserve(static_cast<size_t>(n)); }
+  explicit Numbers(Py_ssize_t n) { of_.reserve(static_cast<size_t>(n)); }
   void add(const void* p) { of_.push_back(reinterpret_cast<int64_t>(p)); }
+  void add(int64_t v) { of_.push_back(v); }
   PyObject* bytes() const {
     return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(of_.data()), static_cast<Py_ssize_t>(of_.size() * 8));
   }
@@ -459,16 +460,40 @@ class Addresses {
 
 const void* address(const Tensor& t) { return t.has_storage() ? t.const_data_ptr() : nullptr; }
 
+// Where a tensor lies and what lies there: values, type and whether they are dense in their order.
+void add_layout(Numbers& found, const Tensor& t) {
+  found.add(address(t));
+  const bool dense = t.layout() == at::kStrided && t.is_contiguous() && !t.is_neg();
+  found.add(t.numel() << 16 | int64_t(dense) << 8 | static_cast<int64_t>(t.scalar_type()));
+}
+
 // addresses(tensors) -> bytes: where the tensors of a list lie
 PyObject* py_addresses(PyObject*, PyObject* list) {
   HANDLE_TH_ERRORS
   TORCH_CHECK_TYPE(PyList_Check(list), "addresses takes a list");
   const Py_ssize_t n = PyList_GET_SIZE(list);
-  Addresses found(n);
+  Numbers found(n);
   for (Py_ssize_t i = 0; i < n; ++i) {
     PyObject* o = PyList_GET_ITEM(list, i);
     TORCH_CHECK_TYPE(THPVariable_Check(o), "addresses takes tensors");
     found.add(address(THPVariable_Unpack(o)));
+  }
+  return found.bytes();
+  END_HANDLE_TH_ERRORS
+}
+
+// layouts(tensors) -> bytes: where the tensors of a list lie, what lies there and their sizes
+PyObject* py_layouts(PyObject*, PyObject* list) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(PyList_Check(list), "layouts takes a list");
+  const Py_ssize_t n = PyList_GET_SIZE(list);
+  Numbers found(4 * n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* o = PyList_GET_ITEM(list, i);
+    TORCH_CHECK_TYPE(THPVariable_Check(o), "layouts takes tensors");
+    const Tensor& t = THPVariable_Unpack(o);
+    add_layout(found, t);
+    for (const int64_t size : t.sizes()) found.add(size);
   }
   return found.bytes();
   END_HANDLE_TH_ERRORS
@@ -480,12 +505,31 @@ PyObject* py_state_addresses(PyObject*, PyObject* list) {
   HANDLE_TH_ERRORS
   TORCH_CHECK_TYPE(PyList_Check(list), "state_addresses takes a list");
   const Py_ssize_t n = PyList_GET_SIZE(list);
-  Addresses found(4 * n);
+  Numbers found(4 * n);
   for (Py_ssize_t i = 0; i < n; ++i) {
     PyObject *entry = PyList_GET_ITEM(list, i), *key = nullptr, *value = nullptr;
     TORCH_CHECK_TYPE(PyDict_Check(entry), "state_addresses takes dictionaries");
     for (Py_ssize_t at = 0; PyDict_Next(entry, &at, &key, &value);)
       found.add(THPVariable_Check(value) ? address(THPVariable_Unpack(value)) : nullptr);
+  }
+  return found.bytes();
+  END_HANDLE_TH_ERRORS
+}
+
+// state_layouts(entries) -> bytes: the same without sizes of the tensors of a list of dictionaries, in their order
+// (-1: no tensor)
+PyObject* py_state_layouts(PyObject*, PyObject* list) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(PyList_Check(list), "state_layouts takes a list");
+  const Py_ssize_t n = PyList_GET_SIZE(list);
+  Numbers found(8 * n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject *entry = PyList_GET_ITEM(list, i), *key = nullptr, *value = nullptr;
+    TORCH_CHECK_TYPE(PyDict_Check(entry), "state_layouts takes dictionaries");
+    for (Py_ssize_t at = 0; PyDict_Next(entry, &at, &key, &value);) {
+      if (THPVariable_Check(value)) add_layout(found, THPVariable_Unpack(value));
+      else found.add(int64_t(-1));
+    }
   }
   return found.bytes();
   END_HANDLE_TH_ERRORS
@@ -497,7 +541,7 @@ PyObject* py_gradients(PyObject*, PyObject* list) {
   HANDLE_TH_ERRORS
   TORCH_CHECK_TYPE(PyList_Check(list), "gradients takes a list");
   const Py_ssize_t n = PyList_GET_SIZE(list);
-  Addresses found(n);
+  Numbers found(n);
   for (Py_ssize_t i = 0; i < n; ++i) {
     PyObject* o = PyList_GET_ITEM(list, i);
     TORCH_CHECK_TYPE(THPVariable_Check(o), "gradients takes tensors");
@@ -518,7 +562,9 @@ PyObject* py_gradients(PyObject*, PyObject* list) {
 
 PyMethodDef kMethods[] = {
     {"addresses", py_addresses, METH_O, nullptr},
+    {"layouts", py_layouts, METH_O, nullptr},
     {"state_addresses", py_state_addresses, METH_O, nullptr},
+    {"state_layouts", py_state_layouts, METH_O, nullptr},
     {"gradients", py_gradients, METH_O, nullptr},
     {"norms", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_norms)), METH_FASTCALL, nullptr},
     {"cross_entropy", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_cross_entropy)), METH_FASTCALL, nullptr},

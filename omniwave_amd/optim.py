@@ -97,10 +97,7 @@ class AdamW(torch.optim.Optimizer):
             if len(set(group["params"])) != len(group["params"]):
                 raise ValueError("a parameter is in its group twice")
             for p in group["params"]:
-                if p.dtype not in SUPPORTED_DTYPES:
-                    raise ValueError(f"unsupported parameter dtype {p.dtype}; expected float32, bfloat16 or float16")
-                if p.layout != torch.strided or not p.is_contiguous():
-                    raise ValueError(f"a parameter of shape {tuple(p.shape)} is not contiguous")
+                _check_parameter(p)
         except ValueError:
             self.param_groups.pop()
             raise
@@ -144,7 +141,7 @@ class AdamW(torch.optim.Optimizer):
         for name, (dtype, shape) in (self._layout(p) if layout is None else layout).items():
             t = entry.get(name)
             if not isinstance(t, Tensor) or t.dtype != dtype or t.shape != shape or t.device != device \
-                    or not t.is_contiguous():
+                    or not t.is_contiguous() or t.is_neg():
                 got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, Tensor) else repr(t)
                 raise ValueError(f"state {name!r} of a parameter of shape {tuple(p.shape)} must be {dtype} {tuple(shape)}, "
                                  f"contiguous on {device}; got {got}")
@@ -260,6 +257,15 @@ class AdamW(torch.optim.Optimizer):
             norm_ptr = None
 
 
+def _check_parameter(p: Tensor) -> None:
+    if p.dtype not in SUPPORTED_DTYPES:
+        raise ValueError(f"unsupported parameter dtype {p.dtype}; expected float32, bfloat16 or float16")
+    if p.layout != torch.strided or not p.is_contiguous():
+        raise ValueError(f"a parameter of shape {tuple(p.shape)} is not contiguous")
+    if p.is_neg():
+        raise ValueError(f"a parameter of shape {tuple(p.shape)} is a negated view")
+
+
 def _dense(p: Tensor) -> Tensor:
     """The gradient of ``p``, contiguous."""
     g = p.grad
@@ -277,13 +283,15 @@ def _without(lie: bytes) -> bytes:
 
 
 class _Plan:
-    """What the steps of the same parameters share: their lists for the native calls.  It is made anew
-    where a parameter, a state or the set of parameters with gradients is another than it was."""
+    """What the steps of the same parameters share: their lists for the native calls.  It is made anew, with
+    all its checks, where a parameter, a state or the set of parameters with gradients is another than it was:
+    another tensor, at another address, or of another type, size or order at the same one."""
 
     def __init__(self, opt: AdamW, glue, params: list[Tensor], lie: bytes) -> None:
         self.params, self.device = params, None
         self.without, self.lie = _without(lie), None
         self.sizes = [len(group["params"]) for group in opt.param_groups]
+        self.options = (opt.state_bits, opt.master_weights)
         self.hyper = _native.OwAdamwGroup * len(self.sizes)
         owner = [i for i, size in enumerate(self.sizes) for _ in range(size)]
         active = [i for i, p in enumerate(params) if not self.without[i] and p.numel()]
@@ -296,15 +304,15 @@ class _Plan:
             p = params[i]
             if p.device != self.device:
                 raise ValueError(f"parameters on {self.device} and {p.device}: an optimizer's parameters are on one GPU")
-            if not p.is_contiguous():
-                raise ValueError(f"a parameter of shape {tuple(p.shape)} is not contiguous")
+            _check_parameter(p)
             if not opt.state[p]:
                 opt._first_state(p)
             layout = opt._layout(p)
             opt._check_state(p, layout)
             key = (p.dtype, 8 if "exp_avg_sq_root" in layout else 32, "master" in layout)
             kinds.setdefault(key, _Kind(*key)).add(i, p, opt.state[p], owner[i])
-        _refuse_overlap([params[i] for i in active])
+        self.active = [params[i] for i in active]
+        _refuse_overlap(glue, self.active, [opt.state[p] for p in self.active])
         # One list, kinds of a dtype next to each other: their gradients' norm is one call.
         self.kinds = sorted(kinds.values(), key=lambda kind: kind.code)
         self.table = np.array([row for kind in self.kinds for row in kind.rows], dtype=np.int64)
@@ -318,10 +326,9 @@ class _Plan:
                 first += kind.count
             pointer, count = self.table[start:].ctypes.data, first - start
             self.norms.append((pointer, count, code, _native.lib().ow_grad_norm_partials(pointer, count)))
-        self.active = [params[i] for i in active]
-        self.addresses = glue.addresses(params)
+        self.layouts = glue.layouts(params)
         self.entries = list(opt.state.values())
-        self.states = glue.state_addresses(self.entries)
+        self.states = glue.state_layouts(self.entries)
 
     def current(self, opt: AdamW, glue, params: list[Tensor], lie: bytes) -> bool:
         """Whether everything but the gradients still lies where the plan has it."""
@@ -329,8 +336,9 @@ class _Plan:
         return (len(params) == len(self.params) and all(map(is_, params, self.params))
                 and (lie == self.lie or _without(lie) == self.without)
                 and [len(group["params"]) for group in opt.param_groups] == self.sizes
+                and (opt.state_bits, opt.master_weights) == self.options
                 and len(entries) == len(self.entries) and all(map(is_, entries, self.entries))
-                and glue.addresses(params) == self.addresses and glue.state_addresses(entries) == self.states)
+                and glue.layouts(params) == self.layouts and glue.state_layouts(entries) == self.states)
 
     def set_gradients(self, lie: bytes) -> None:
         """Writes the gradients' addresses into the lists."""
@@ -356,12 +364,17 @@ class _Kind:
                           p.numel(), group])
 
 
-def _refuse_overlap(params: list[Tensor]) -> None:
+def _refuse_overlap(glue, params: list[Tensor], entries: list[dict]) -> None:
     """Tensors that share memory would be updated by two workgroups at once."""
-    spans = sorted((p.data_ptr(), p.numel() * p.element_size(), tuple(p.shape)) for p in params)
+    lie = np.frombuffer(glue.addresses(params), dtype=np.int64).tolist()
+    spans = sorted((at, p.numel() * p.element_size(), tuple(p.shape)) for at, p in zip(lie, params))
     for (at, size, shape), (other, _, other_shape) in zip(spans, spans[1:]):
         if at + size > other:
             raise ValueError(f"parameters of shapes {shape} and {other_shape} share memory")
+    states = np.frombuffer(glue.state_addresses(entries), dtype=np.int64)
+    states = states[states != 0]
+    if len(np.unique(states)) != len(states):
+        raise ValueError("states of parameters share memory")
 
 
 def _hyper(group: dict, device: torch.device | None = None) -> tuple:
