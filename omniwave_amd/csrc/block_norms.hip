@@ -61,7 +61,7 @@ constexpr int kWantPost = 1, kWantNext = 2, kWantGate = 4;
 
 // Waves per SIMD that the kernels' registers leave room for (vectors of `vec` values, t threads a row; a
 // workgroup of 1,024 threads is four): grids are as many workgroups as run at once.
-constexpr int fwd_waves(int vec, bool ragged, int t) { return t == 1024 ? 4 : vec == 8 && ragged ? 5 : 6; }
+constexpr int fwd_waves(int t) { return t == 1024 ? 4 : 6; }
 constexpr int bwd_waves(int vec, int t) { return t == 1024 ? 4 : vec == 8 ? 3 : 4; }
 
 template <int T>
@@ -126,12 +126,13 @@ struct Place {
   }
 };
 
-// a b where the value counts in its row's sums, else 0 (a mask of ones and zeros; whole vectors need none).
+// A value as it enters its row's sums, 0 where another lane counts it (whole vectors need no mask).  Chosen, not
+// multiplied by 0 or 1: 0 times an infinity would make the whole row NaN.
 template <bool RAGGED>
-__device__ __forceinline__ float counted(float a, float mask) { return RAGGED ? a * mask : a; }
+__device__ __forceinline__ float counted(float a, bool counts) { return !RAGGED || counts ? a : 0.f; }
 
 template <class Ty, int T, int K, bool RAGGED>
-__global__ void __launch_bounds__(kThreads<T>, fwd_waves(Row<Ty>::kVec, RAGGED, T)) block_norms_fwd_kernel(NormsArgs a) {
+__global__ void __launch_bounds__(kThreads<T>, fwd_waves(T)) block_norms_fwd_kernel(NormsArgs a) {
   typedef Row<Ty> R;
   typedef typename R::Elem Elem;
   constexpr int V = R::kVec, ROWS = kThreads<T> / T;
@@ -149,11 +150,11 @@ __global__ void __launch_bounds__(kThreads<T>, fwd_waves(Row<Ty>::kVec, RAGGED, 
     at.weight(per_image ? nullptr : a.n.gate, a.n.gate_dtype, 0, k, 1.f, gate[k]);
     at.weight(a.n.next_weight, a.n.next_dtype, 0, k, 1.f, nextw[k]);
   }
-  float mask[K][V];
+  bool mask[K][V];
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
-    for (int j = 0; j < V; ++j) mask[k][j] = at.counts(k, j) ? 1.f : 0.f;
+    for (int j = 0; j < V; ++j) mask[k][j] = at.counts(k, j);
 
   // A row is read while the one before it is computed.
   typename R::Raw xn[K], dn[K];
@@ -192,7 +193,10 @@ __global__ void __launch_bounds__(kThreads<T>, fwd_waves(Row<Ty>::kVec, RAGGED, 
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-          for (int j = 0; j < V; ++j) ss[0] += d[k][j] * counted<RAGGED>(d[k][j], mask[k][j]);
+          for (int j = 0; j < V; ++j) {
+            const float w = counted<RAGGED>(d[k][j], mask[k][j]);
+            ss[0] += w * w;
+          }
         row_sums<T>(ss, red, turn);
         const float r1 = rsqrtf(ss[0] * a.inv_c + a.n.eps);
 #pragma unroll
@@ -212,7 +216,10 @@ __global__ void __launch_bounds__(kThreads<T>, fwd_waves(Row<Ty>::kVec, RAGGED, 
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int j = 0; j < V; ++j) ss[0] += x[k][j] * counted<RAGGED>(x[k][j], mask[k][j]);
+        for (int j = 0; j < V; ++j) {
+          const float w = counted<RAGGED>(x[k][j], mask[k][j]);
+          ss[0] += w * w;
+        }
       row_sums<T>(ss, red, turn);
       const float r2 = rsqrtf(ss[0] * a.inv_c + a.n.eps);
 #pragma unroll
@@ -246,7 +253,8 @@ __global__ void __launch_bounds__(kThreads<T>, bwd_waves(Row<Ty>::kVec, T)) bloc
   const int64_t seg_last = parted ? seg_first + 1 : (static_cast<int64_t>(blockIdx.x) + 1) * a.segments / a.n_part;
 
   float post[K][V], gate[K][V], nextw[K][V];
-  float s_post[K][V], s_next[K][V], s_gate[K][V], mask[K][V];
+  float s_post[K][V], s_next[K][V], s_gate[K][V];
+  bool mask[K][V];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     at.weight(a.n.post_weight, a.n.post_dtype, 0, k, 1.f, post[k]);
@@ -254,7 +262,7 @@ __global__ void __launch_bounds__(kThreads<T>, bwd_waves(Row<Ty>::kVec, T)) bloc
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       s_post[k][j] = s_next[k][j] = 0.f;
-      mask[k][j] = at.counts(k, j) ? 1.f : 0.f;
+      mask[k][j] = at.counts(k, j);
     }
   }
   // put(column, sum over the workgroup's rows) of a thread's sums.
@@ -330,7 +338,10 @@ __global__ void __launch_bounds__(kThreads<T>, bwd_waves(Row<Ty>::kVec, T)) bloc
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-          for (int j = 0; j < V; ++j) ss[0] += d[k][j] * counted<RAGGED>(d[k][j], mask[k][j]);
+          for (int j = 0; j < V; ++j) {
+            const float w = counted<RAGGED>(d[k][j], mask[k][j]);
+            ss[0] += w * w;
+          }
         row_sums<T>(ss, red, turn);
         r1 = valid ? rsqrtf(ss[0] * a.inv_c + a.n.eps) : 0.f;  // no row adds nothing, also where eps is 0
       }
@@ -343,8 +354,8 @@ __global__ void __launch_bounds__(kThreads<T>, bwd_waves(Row<Ty>::kVec, T)) bloc
         for (int j = 0; j < V; ++j) {
           if (has_delta) x[k][j] += f * gate[k][j] * (d[k][j] * (r1 * post[k][j]));  // out
           const float w = counted<RAGGED>(x[k][j], mask[k][j]);
-          ss[0] += w * x[k][j];
-          ss[1] += w * (h[k][j] * nextw[k][j]);
+          ss[0] += w * w;
+          ss[1] += w * counted<RAGGED>(h[k][j] * nextw[k][j], mask[k][j]);
         }
       row_sums<T>(ss, red, turn);
       const float r2 = valid ? rsqrtf(ss[0] * a.inv_c + a.n.eps) : 0.f;
@@ -372,7 +383,7 @@ __global__ void __launch_bounds__(kThreads<T>, bwd_waves(Row<Ty>::kVec, T)) bloc
           const float q = e * gate[k][j];
           s_post[k][j] += q * u;
           g[k][j] = q * post[k][j];
-          ss[0] += g[k][j] * counted<RAGGED>(d[k][j], mask[k][j]);
+          ss[0] += counted<RAGGED>(g[k][j] * d[k][j], mask[k][j]);
         }
       if (has_post) {
         row_sums<T>(ss, red, turn);
@@ -496,7 +507,7 @@ void launch(const NormsArgs& a, bool backward, hipStream_t s) {
     return;
   }
   const int64_t groups = (a.n.rows + ROWS - 1) / ROWS;
-  const int64_t most = at_once_of(fwd_waves(Row<Ty>::kVec, RAGGED, T), T);
+  const int64_t most = at_once_of(fwd_waves(T), T);
   hipLaunchKernelGGL((block_norms_fwd_kernel<Ty, T, K, RAGGED>), dim3(static_cast<unsigned>(groups < most ? groups : most)),
                      dim3(kThreads<T>), 0, s, a);
 }
