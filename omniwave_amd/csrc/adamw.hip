@@ -22,8 +22,8 @@
 // that is not zero is never held as zero, since m / (0 + eps) would be a step of m / eps.  The update
 // itself uses the unrounded m and v.  Arithmetic is not contracted to fused multiply-adds: rounding
 // after each operation is what the states' definition says, and a value next to a border of two codes
-// then falls on the same side everywhere.  The update's quotient (and a root that is not stored) is the
-// hardware's, within a unit in the last place; 1 - b^t is formed as -expm1(t ln b), which keeps its relative
+// then falls on the same side everywhere.  The update's quotient (and a root that is not stored, of normal
+// numbers) is the hardware's, within a unit in the last place; 1 - b^t is formed as -expm1(t ln b), which keeps its relative
 // precision where b^t is near one.
 #include <hip/hip_runtime.h>
 
@@ -42,7 +42,7 @@ constexpr int kGroups = 6;              // hyperparameter sets of a launch
 constexpr int kArgBytes = 4096 - 64;    // of the tensor and hyperparameter tables
 constexpr float kFp8Most = 448.f;
 constexpr float kFp8Least = 0x1p-9f;    // the least e4m3fn number above zero
-constexpr float kLeastScale = 1.17549435e-38f;  // smaller (subnormal) scales: a block of zeros
+constexpr float kLeastNormal = 0x1p-126f;  // a scale below it is held as zero, and its block of zeros
 static_assert(kBlock == 4 * 64 && kIters == 4, "a wave's vector is a block, and its blocks' scales a vector");
 
 struct Hyper {
@@ -156,7 +156,7 @@ __device__ __forceinline__ uint32_t encode4(const float (&v)[4], float& scale) {
   }
   most = lanes_reduce<MaxUintOp, 64>(most);
   scale = __uint_as_float(most) * (1.f / kFp8Most);
-  if (scale < kLeastScale) scale = 0.f;
+  if (scale < kLeastNormal) scale = 0.f;
   const float inv = scale != 0.f ? 1.f / scale : 0.f;
   float y[4];
 #pragma unroll
@@ -281,8 +281,15 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_kernel(StepArgs<kPtrsOf<Ty,
       v[k][j] = v[k][j] * h.b2 + gj * gj * h.c2;
       // A root that is stored is rounded correctly, as m and v are: its code is then the definition's.
       root[j] = BITS == 8 ? sqrtf(v[k][j]) : __builtin_amdgcn_sqrtf(v[k][j]);
-      p[k][j] = p[k][j] * keep - step * (m[k][j] * __builtin_amdgcn_rcpf(root[j] * unbias + h.eps));
     }
+    // The hardware's root takes subnormal numbers for zero, which a small eps would not hide.
+    if (BITS != 8 && fminf(fminf(v[k][0], v[k][1]), fminf(v[k][2], v[k][3])) < kLeastNormal) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) root[j] = sqrtf(v[k][j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      p[k][j] = p[k][j] * keep - step * (m[k][j] * __builtin_amdgcn_rcpf(root[j] * unbias + h.eps));
     if constexpr (MASTER) store4<F32>(a.t.ptr[PTRS - 1][i], idx, left, p[k]);
     store4<Ty>(a.t.ptr[kParam][i], idx, left, p[k]);
     if constexpr (BITS == 8) {
