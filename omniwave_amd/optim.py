@@ -60,7 +60,7 @@ class AdamW(torch.optim.Optimizer):
     fp16 parameters and update those, so that updates smaller than a parameter's rounding step are not
     lost.  ``max_grad_norm``: scale the gradients of each step so that their norm over all parameters is
     at most this, and skip the step (parameters, states and counters) where the norm is not finite;
-    ``grad_norm`` is then the last step's norm, on the device.
+    ``grad_norm`` is then the last step's norm, on the device (0 where nothing had a gradient).
 
     Parameters: contiguous, of fp32, bf16 or fp16, on one gfx950 GPU, no two in the same memory; gradients of
     the same dtype, dense.  With ``master_weights`` a step starts from the fp32 copy: a parameter that is
@@ -222,7 +222,9 @@ class AdamW(torch.optim.Optimizer):
         plan = self._plan
         if plan is None or not plan.current(self, glue, params, lie):
             plan = self._plan = _Plan(self, glue, params, lie)
-        if not plan.kinds:
+        if not plan.kinds:  # the norm of no gradients
+            device = params[0].device if params else None
+            self.grad_norm = None if self.max_grad_norm is None else torch.zeros((), dtype=torch.float32, device=device)
             return loss
         plan.set_gradients(lie)
         device = plan.device
@@ -242,6 +244,7 @@ class AdamW(torch.optim.Optimizer):
     def _launch(self, plan: _Plan, hyper, device: torch.device) -> None:
         lib, stream = _native.lib(), _stream_ptr(device)
         partials, total, norm_ptr, at = None, 0, None, None
+        self.grad_norm = None
         if self.max_grad_norm is not None:
             total = sum(partials for *_, partials in plan.norms)
             partials = torch.empty(total, dtype=torch.float64, device=device)
