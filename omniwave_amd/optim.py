@@ -26,6 +26,8 @@ CHUNK, BLOCK = _native.OW_ADAMW_CHUNK, _native.OW_ADAMW_BLOCK
 FP8 = torch.float8_e4m3fn
 FP8_MOST = 448.0
 MIN_8BIT_VALUES = 4096  # smaller tensors keep 32-bit states: their bytes do not matter, their errors do
+# Options of torch.optim.AdamW's groups that make another update, with the values that do not.
+_PLAIN_UPDATE = {"maximize": False, "amsgrad": False, "differentiable": False, "decoupled_weight_decay": True}
 _GRAD = 1  # field of OwAdamwTensor, whose fields are 8 bytes each
 
 
@@ -73,7 +75,8 @@ class AdamW(torch.optim.Optimizer):
     ``state[p]``: ``step`` (int32, the steps done, one for every 4,096 values), ``exp_avg`` and
     ``exp_avg_sq`` (fp32), or ``exp_avg`` and ``exp_avg_sq_root`` (e4m3fn) with ``exp_avg_scale`` and
     ``exp_avg_sq_root_scale``, and ``master``.  ``load_state_dict`` also takes the states of
-    ``torch.optim.AdamW`` and those of another ``state_bits``.
+    ``torch.optim.AdamW`` and those of another ``state_bits``.  Groups and saved groups with ``maximize``, ``amsgrad``
+    or ``differentiable``, or without ``decoupled_weight_decay``, are refused: their update is another one.
     """
 
     grad_norm: Tensor | None = None
@@ -149,6 +152,8 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict: dict) -> None:
         """``torch.optim.Optimizer.load_state_dict``; states keep their own dtypes, and those of
         ``torch.optim.AdamW`` or another ``state_bits`` are converted."""
+        for group in state_dict["param_groups"]:
+            _refuse_other_updates(group)
         super().load_state_dict(state_dict)
         saved = state_dict["state"]
         ids = chain.from_iterable(g["params"] for g in state_dict["param_groups"])
@@ -380,8 +385,15 @@ def _refuse_overlap(glue, params: list[Tensor], entries: list[dict]) -> None:
         raise ValueError("states of parameters share memory")
 
 
+def _refuse_other_updates(group: dict) -> None:
+    for name, plain in _PLAIN_UPDATE.items():
+        if bool(group.get(name, plain)) != plain:
+            raise ValueError(f"{name}={group[name]!r} is not supported")
+
+
 def _hyper(group: dict, device: torch.device | None = None) -> tuple:
     """A group's hyperparameters as OwAdamwGroup's fields."""
+    _refuse_other_updates(group)
     lr, (beta1, beta2), eps, decay = group["lr"], group["betas"], group["eps"], group["weight_decay"]
     lr_device = None
     if isinstance(lr, Tensor):
