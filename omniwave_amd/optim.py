@@ -151,17 +151,27 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict: dict) -> None:
         """``torch.optim.Optimizer.load_state_dict``; states keep their own dtypes, and those of
-        ``torch.optim.AdamW`` or another ``state_bits`` are converted."""
-        for group in state_dict["param_groups"]:
-            _refuse_other_updates(group)
-        super().load_state_dict(state_dict)
-        saved = state_dict["state"]
-        ids = chain.from_iterable(g["params"] for g in state_dict["param_groups"])
-        params = chain.from_iterable(g["params"] for g in self.param_groups)
-        for i, p in zip(ids, params):
-            if i in saved:
-                self.state[p] = self._adopt(p, saved[i])
-        self._plan = None
+        ``torch.optim.AdamW`` or another ``state_bits`` are converted.  A dictionary that is refused changes nothing."""
+        adopted: dict[Tensor, dict] = {}
+
+        def before(_opt, loaded: dict) -> None:  # behind the other hooks: this is what is loaded
+            for group in loaded["param_groups"]:
+                _refuse_other_updates(group)
+            ids = chain.from_iterable(g["params"] for g in loaded["param_groups"])
+            params = chain.from_iterable(g["params"] for g in self.param_groups)
+            adopted.update((p, self._adopt(p, loaded["state"][i])) for i, p in zip(ids, params) if i in loaded["state"])
+
+        def after(_opt) -> None:  # before the other hooks; the base class has cast the states to the parameters' dtypes
+            self.state.update(adopted)
+            self._plan = None
+
+        hooks = (self.register_load_state_dict_pre_hook(before),
+                 self.register_load_state_dict_post_hook(after, prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
 
     @torch.no_grad()
     def _adopt(self, p: Tensor, saved: dict) -> dict:
