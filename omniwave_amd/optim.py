@@ -201,9 +201,9 @@ class AdamW(torch.optim.Optimizer):
                 entry["exp_avg"], entry["exp_avg_scale"] = _encode(m, False)
                 entry["exp_avg_sq_root"], entry["exp_avg_sq_root_scale"] = _encode(root, True)
             else:
-                entry["exp_avg"], entry["exp_avg_sq"] = m.contiguous(), v.contiguous()
+                entry["exp_avg"], entry["exp_avg_sq"] = (t.clone(memory_format=torch.contiguous_format) for t in (m, v))
         if "master" in layout:
-            entry["master"] = own["master"].float().clone() if "master" in own else p.detach().float()
+            entry["master"] = own["master"].float().clone(memory_format=torch.contiguous_format) if "master" in own else p.detach().float()
         return entry
 
     # -- the step -------------------------------------------------------------------------

@@ -84,3 +84,17 @@ def test_a_refused_dictionary_changes_nothing() -> None:
         opt.load_state_dict(short)
     opt.load_state_dict(source.state_dict())
     assert not torch.equal(opt.state[params[0]]["exp_avg"], before[0]["exp_avg"])
+
+
+def test_loaded_states_are_copies() -> None:
+    source, theirs = optimizer()
+    opt, params = optimizer(seed=1)
+    saved = source.state_dict()
+    saved["state"][0]["exp_avg_sq"] = saved["state"][0]["exp_avg_sq"].bfloat16()
+    opt.load_state_dict(saved)
+    kept = theirs[0], source.state[theirs[0]]["exp_avg"].clone()
+    for entry in opt.state.values():
+        for t in entry.values():
+            t.zero_()
+    assert torch.equal(source.state[kept[0]]["exp_avg"], kept[1])
+    assert (source.state[theirs[1]]["step"] == 7).all()
