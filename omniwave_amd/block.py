@@ -82,6 +82,12 @@ class OmniWeaveBlock(nn.Module):
         self.fp8 = False  # e4m3fn channel side (inference with the hip backend); see enable_fp8
         self._init_weights()
 
+    def _apply(self, fn, recurse: bool = True):
+        super()._apply(fn, recurse)
+        if self.post_norm:  # no parameter, in no state_dict: made anew without their values (to_empty), they are these
+            self._ones.fill_(1.0)
+        return self
+
     def _init_weights(self) -> None:
         """omniweave/models/block.py:72-78."""
         nn.init.orthogonal_(self.a_u)
