@@ -13,6 +13,7 @@ import shutil
 import subprocess
 import sysconfig
 import tempfile
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -72,36 +73,48 @@ def glue_commands(obj: str, out: str, lib_dir: str) -> tuple[list[str], list[str
 
 
 def build(verbose: bool = False) -> Path:
-    """Compile every source into LIB_PATH and GLUE_PATH (always recompiles); returns the library path."""
+    """Compile every source into LIB_PATH and GLUE_PATH (always recompiles); returns the library path.
+
+    The module needs more than the library does (a host compiler, Python's and torch's headers).  Where it cannot
+    be built, a warning says why and there is none: the norms and the loss then run through their operators, and
+    only ``AdamW`` is refused."""
     cc = hipcc()
     with tempfile.TemporaryDirectory(prefix="ow_build_") as tmp:
         objs = [str(Path(tmp) / (Path(src).stem + ".o")) for src in SOURCES]
         cmds = [[cc, *compile_flags(), "-c", str(CSRC / src), "-o", obj] for src, obj in zip(SOURCES, objs)]
-        glue_out = str(Path(tmp) / GLUE_PATH.name)
-        glue_compile, glue_link = glue_commands(str(Path(tmp) / "torch_glue.o"), glue_out, tmp)
-        cmds.append(glue_compile)
-        if verbose:
-            for cmd in cmds:
-                print(" ".join(cmd), flush=True)
-        with ThreadPoolExecutor(max_workers=min(len(cmds), os.cpu_count() or 1)) as pool:
-            for fut in [pool.submit(_run, cmd) for cmd in cmds]:
-                fut.result()
-        out_tmp = Path(tmp) / LIB_PATH.name
-        cmd = [cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", str(out_tmp)]
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        _run(cmd)
-        if verbose:
-            print(" ".join(glue_link), flush=True)
-        _run(glue_link)
-        for built, path in ((out_tmp, LIB_PATH), (glue_out, GLUE_PATH)):
-            staged = path.with_suffix(".so.tmp")
-            shutil.copyfile(built, staged)
-            os.replace(staged, path)
+        out_tmp, glue_tmp = Path(tmp) / LIB_PATH.name, Path(tmp) / GLUE_PATH.name
+
+        def compile_glue() -> list[str]:
+            """Compiles the module; returns its link command, which needs the library."""
+            compile_cmd, link_cmd = glue_commands(str(Path(tmp) / "torch_glue.o"), str(glue_tmp), tmp)
+            _run(compile_cmd, verbose)
+            return link_cmd
+
+        with ThreadPoolExecutor(max_workers=min(len(cmds) + 1, os.cpu_count() or 1)) as pool:
+            futures = [pool.submit(_run, cmd, verbose) for cmd in cmds]
+            glue = pool.submit(compile_glue)
+            for future in futures:
+                future.result()
+        _run([cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", str(out_tmp)], verbose)
+        _install(out_tmp, LIB_PATH)
+        try:
+            _run(glue.result(), verbose)
+            _install(glue_tmp, GLUE_PATH)
+        except (RuntimeError, OSError, ImportError) as exc:
+            GLUE_PATH.unlink(missing_ok=True)  # one that is there is of another library
+            warnings.warn(f"{GLUE_PATH.name} was not built: {exc}", RuntimeWarning, stacklevel=2)
     return LIB_PATH
 
 
-def _run(cmd: list[str]) -> None:
+def _install(built: Path, path: Path) -> None:
+    staged = path.with_suffix(".so.tmp")
+    shutil.copyfile(built, staged)
+    os.replace(staged, path)
+
+
+def _run(cmd: list[str], verbose: bool = False) -> None:
+    if verbose:
+        print(" ".join(cmd), flush=True)
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         noise = "is not a recognized feature for this target"

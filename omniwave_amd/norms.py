@@ -30,7 +30,7 @@ MAX_CHANNELS = 8192
 
 def gpu_reason(t: Tensor) -> str | None:
     """Why the kernels cannot run on ``t``'s device, or None."""
-    err = _native.load_error() or _native.glue_error()
+    err = _native.load_error()
     if err is not None:
         return f"native library unavailable: {err}"
     if not t.is_cuda:
