@@ -18,13 +18,15 @@ import math
 import torch
 import torch.nn as nn
 from torch import Tensor
-from torch.nn.modules.module import _has_any_global_hook
 
 from omniwave_amd.bigemm import bigemm
 from omniwave_amd.hip import (_block, _chain, bigemm_block_s2d_hip, bigemm_delta_hip, drop_path_scale,
                               hip_is_supported)
 from omniwave_amd.norms import MAX_CHANNELS, block_norms_hip
 from omniwave_amd.routing import RoutePlan, build_route_plan
+
+# torch's own look at the hooks of all modules; without one there may be some.
+_has_any_global_hook = getattr(torch.nn.modules.module, "_has_any_global_hook", lambda: True)
 
 RMS_EPS = 1e-6  # omniweave/models/block.py:84
 

@@ -31,6 +31,12 @@ _PLAIN_UPDATE = {"maximize": False, "amsgrad": False, "differentiable": False, "
 _GRAD = 1  # field of OwAdamwTensor, whose fields are 8 bytes each
 
 
+# Whether torch has the names by which a step sees that nothing listens to it; without them the base class wraps it.
+_SHORTCUT = (hasattr(_base, "_global_optimizer_pre_hooks") and hasattr(_base, "_global_optimizer_post_hooks")
+             and hasattr(torch.optim.Optimizer, "profile_hook_step")
+             and hasattr(torch.autograd.profiler, "_is_profiler_enabled"))
+
+
 def _blocks(n: int) -> int:
     return -(-n // BLOCK)
 
@@ -208,16 +214,6 @@ class AdamW(torch.optim.Optimizer):
 
     # -- the step -------------------------------------------------------------------------
 
-    def step(self, closure=None):
-        # The base class's wrapper (a profiler's record, hooks) costs more than looking at the tensors does:
-        # only where something listens.
-        if (self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks or _base._global_optimizer_pre_hooks
-                or _base._global_optimizer_post_hooks or torch.autograd.profiler._is_profiler_enabled):
-            return self._heard_step(closure)
-        return self._step(closure)
-
-    step.hooked = True  # the base class leaves it as it is
-
     def _step(self, closure=None):
         loss = None
         if closure is not None:
@@ -254,7 +250,21 @@ class AdamW(torch.optim.Optimizer):
         torch.autograd.graph.increment_version(plan.active)
         return loss
 
-    _heard_step = torch.optim.Optimizer.profile_hook_step(_step)
+    if _SHORTCUT:
+        _heard_step = torch.optim.Optimizer.profile_hook_step(_step)
+
+        def step(self, closure=None):
+            # The base class's wrapper (a profiler's record, hooks) costs more than looking at the tensors does:
+            # only where something listens.
+            if (self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks or _base._global_optimizer_pre_hooks
+                    or _base._global_optimizer_post_hooks or torch.autograd.profiler._is_profiler_enabled):
+                return self._heard_step(closure)
+            return self._step(closure)
+
+        step.hooked = True  # the base class leaves it as it is
+    else:
+        def step(self, closure=None):
+            return self._step(closure)
 
     def _launch(self, plan: _Plan, hyper, device: torch.device) -> None:
         lib, stream = _native.lib(), _stream_ptr(device)
