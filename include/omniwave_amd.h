@@ -608,6 +608,8 @@ int ow_block_norms_bwd(const OwBlockNorms* norms, const void* dout, int64_t dout
  *   state_bits 8   exp_avg = m, exp_avg_sq = sqrt(v): e4m3fn codes, one fp32 scale per OW_ADAMW_BLOCK
  *                  values (largest magnitude / 448) in exp_avg_scale, exp_avg_sq_scale; value = code * scale.
  *                  A root above zero is held as 2^-9 scales at least; a scale below 2^-126 as 0.
+ *                  Codes are the nearest ones after each step: a root follows what its block has in common,
+ *                  but moves beside the block's largest one only by half a code's step (3 to 6%) at once
  *   master         with use_master: fp32 parameters, which are updated, and param is their rounding
  *   group          index into groups; lr_device: NULL, or the learning rate as one fp32 on the device
  *

@@ -19,7 +19,10 @@
 // 8-bit states: 256 consecutive values (one wave's vectors) share an fp32 scale, their largest magnitude
 // over 448; a value is held as the nearest e4m3fn number of its ratio to the scale.  The second moment is
 // held as its square root: e4m3fn reaches 2^-18 of the block's largest value, so v has 2^-36.  A root
-// that is not zero is never held as zero, since m / (0 + eps) would be a step of m / eps.  The update
+// that is not zero is never held as zero, since m / (0 + eps) would be a step of m / eps.  The nearest code is
+// also the format's limit: half a code's step is 3 to 6%, a step moves a root by (1 - b2) / 2 = 0.05%, so what a
+// value's root does beside its block's largest one is not followed unless a gradient exceeds some 8 roots (the
+// scale follows what the block has in common).  The update
 // itself uses the unrounded m and v.  Arithmetic is not contracted to fused multiply-adds: rounding
 // after each operation is what the states' definition says, and a value next to a border of two codes
 // then falls on the same side everywhere.  The update's quotient (and a root that is not stored, of normal
