@@ -158,7 +158,7 @@ class AdamW(torch.optim.Optimizer):
         for name, (dtype, shape) in (self._layout(p) if layout is None else layout).items():
             t = entry.get(name)
             if not isinstance(t, Tensor) or t.dtype != dtype or t.shape != shape or t.device != device \
-                    or not t.is_contiguous() or t.is_neg():
+                    or not t.is_contiguous():
                 got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, Tensor) else repr(t)
                 raise ValueError(f"state {name!r} of a parameter of shape {tuple(p.shape)} must be {dtype} {tuple(shape)}, "
                                  f"contiguous on {device}; got {got}")
@@ -298,8 +298,6 @@ def _check_parameter(p: Tensor) -> None:
         raise ValueError(f"unsupported parameter dtype {p.dtype}; expected float32, bfloat16 or float16")
     if p.layout != torch.strided or not p.is_contiguous():
         raise ValueError(f"a parameter of shape {tuple(p.shape)} is not contiguous")
-    if p.is_neg():
-        raise ValueError(f"a parameter of shape {tuple(p.shape)} is a negated view")
 
 
 def _dense(p: Tensor) -> Tensor:
@@ -340,13 +338,17 @@ class _Plan:
             p = params[i]
             if p.device != self.device:
                 raise ValueError(f"parameters on {self.device} and {p.device}: an optimizer's parameters are on one GPU")
-            _check_parameter(p)
+            if not p.is_contiguous():
+                raise ValueError(f"a parameter of shape {tuple(p.shape)} is not contiguous")
             if not opt.state[p]:
                 opt._first_state(p)
             layout = opt._layout(p)
             opt._check_state(p, layout)
             key = (p.dtype, 8 if "exp_avg_sq_root" in layout else 32, "master" in layout)
-            kinds.setdefault(key, _Kind(*key)).add(i, p, opt.state[p], owner[i])
+            if key not in kinds:
+                _check_parameter(p)
+                kinds[key] = _Kind(*key)
+            kinds[key].add(i, p, opt.state[p], owner[i])
         self.active = [params[i] for i in active]
         _refuse_overlap(glue, self.active, [opt.state[p] for p in self.active])
         # One list, kinds of a dtype next to each other: their gradients' norm is one call.
@@ -402,14 +404,13 @@ class _Kind:
 
 def _refuse_overlap(glue, params: list[Tensor], entries: list[dict]) -> None:
     """Tensors that share memory would be updated by two workgroups at once."""
-    lie = np.frombuffer(glue.addresses(params), dtype=np.int64).tolist()
-    spans = sorted((at, p.numel() * p.element_size(), tuple(p.shape)) for at, p in zip(lie, params))
-    for (at, size, shape), (other, _, other_shape) in zip(spans, spans[1:]):
+    lie = memoryview(glue.addresses(params)).cast("q")
+    spans = sorted((at, p.numel() * p.element_size(), i) for i, (at, p) in enumerate(zip(lie, params)))
+    for (at, size, i), (other, _, j) in zip(spans, spans[1:]):
         if at + size > other:
-            raise ValueError(f"parameters of shapes {shape} and {other_shape} share memory")
-    states = np.frombuffer(glue.state_addresses(entries), dtype=np.int64)
-    states = states[states != 0]
-    if len(np.unique(states)) != len(states):
+            raise ValueError(f"parameters of shapes {tuple(params[i].shape)} and {tuple(params[j].shape)} share memory")
+    states = [at for at in memoryview(glue.state_addresses(entries)).cast("q") if at]
+    if len(set(states)) != len(states):
         raise ValueError("states of parameters share memory")
 
 
