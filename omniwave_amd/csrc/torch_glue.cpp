@@ -460,13 +460,13 @@ class Numbers {
 
 const void* address(const Tensor& t) { return t.has_storage() ? t.const_data_ptr() : nullptr; }
 
-// Where a tensor lies and what lies there: values, type and whether they are dense in their order.  Values that stand
+// Where a tensor lies and what lies there: values, dimensions, type and whether they are dense in their order.  Values that stand
 // for their negatives are refused: a kernel reads what lies there.
 void add_layout(Numbers& found, const Tensor& t) {
   TORCH_CHECK_VALUE(!t.is_neg(), "a parameter or state of shape ", t.sizes(), " is a negated view");
   found.add(address(t));
   const bool dense = t.layout() == at::kStrided && t.is_contiguous();
-  found.add(t.numel() << 16 | int64_t(dense) << 8 | static_cast<int64_t>(t.scalar_type()));
+  found.add(t.numel() << 16 | t.dim() << 9 | int64_t(dense) << 8 | static_cast<int64_t>(t.scalar_type()));
 }
 
 // addresses(tensors) -> bytes: where the tensors of a list lie

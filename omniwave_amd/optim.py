@@ -29,8 +29,6 @@ MIN_8BIT_VALUES = 4096  # smaller tensors keep 32-bit states: their bytes do not
 # Options of torch.optim.AdamW's groups that make another update, with the values that do not.
 _PLAIN_UPDATE = {"maximize": False, "amsgrad": False, "differentiable": False, "decoupled_weight_decay": True}
 _GRAD = 1  # field of OwAdamwTensor, whose fields are 8 bytes each
-
-
 # Whether torch has the names by which a step sees that nothing listens to it; without them the base class wraps it.
 _SHORTCUT = (hasattr(_base, "_global_optimizer_pre_hooks") and hasattr(_base, "_global_optimizer_post_hooks")
              and hasattr(torch.optim.Optimizer, "profile_hook_step")
@@ -64,11 +62,12 @@ class AdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW`` on the framework's kernels.
 
     ``state_bits``: 32, or 8 for states of tensors of at least 4,096 values in e4m3fn with an fp32 scale
-    for every 256 values (the second moment as its root; see below what that costs).  ``master_weights``: keep fp32 copies of bf16 /
-    fp16 parameters and update those, so that updates smaller than a parameter's rounding step are not
-    lost.  ``max_grad_norm``: scale the gradients of each step so that their norm over all parameters is
+    for every 256 values (the second moment as its root; see below what that costs).  ``master_weights``: keep
+    fp32 copies of bf16 / fp16 parameters and update those, so that updates smaller than a parameter's rounding
+    step are not lost.  ``max_grad_norm``: scale the gradients of each step so that their norm over all parameters is
     at most this, and skip the step (parameters, states and counters) where the norm is not finite;
-    ``grad_norm`` is then the last step's norm, on the device (0 where nothing had a gradient).
+    ``grad_norm`` is then the last step's norm, on the device (0 where nothing had a gradient; replays of a captured
+    step write the tensor that it had at the capture).
 
     Parameters: contiguous, of fp32, bf16 or fp16, on one gfx950 GPU, no two in the same memory; gradients of
     the same dtype, dense.  With ``master_weights`` a step starts from the fp32 copy: a parameter that is
@@ -168,14 +167,17 @@ class AdamW(torch.optim.Optimizer):
         ``torch.optim.AdamW`` or another ``state_bits`` are converted.  A dictionary that is refused changes nothing."""
         adopted: dict[Tensor, dict] = {}
 
-        def before(_opt, loaded: dict) -> None:  # behind the other hooks: this is what is loaded
+        def before(_opt, loaded: dict) -> dict:  # behind the other hooks: this is what is loaded
             for group in loaded["param_groups"]:
                 _refuse_other_updates(group)
+            saved = dict(loaded["state"])
             ids = chain.from_iterable(g["params"] for g in loaded["param_groups"])
             params = chain.from_iterable(g["params"] for g in self.param_groups)
-            adopted.update((p, self._adopt(p, loaded["state"][i])) for i, p in zip(ids, params) if i in loaded["state"])
+            # The base class would cast the states to the parameters' dtypes, a second set of them.
+            adopted.update((p, self._adopt(p, saved.pop(i))) for i, p in zip(ids, params) if i in saved)
+            return {**loaded, "state": saved}
 
-        def after(_opt) -> None:  # before the other hooks; the base class has cast the states to the parameters' dtypes
+        def after(_opt) -> None:  # before the other hooks
             self.state.update(adopted)
             self._plan = None
 
@@ -217,7 +219,8 @@ class AdamW(torch.optim.Optimizer):
             else:
                 entry["exp_avg"], entry["exp_avg_sq"] = (t.clone(memory_format=torch.contiguous_format) for t in (m, v))
         if "master" in layout:
-            entry["master"] = own["master"].float().clone(memory_format=torch.contiguous_format) if "master" in own else p.detach().float()
+            kept = own.get("master", p.detach())
+            entry["master"] = kept.to(torch.float32, copy=True, memory_format=torch.contiguous_format)
         return entry
 
     # -- the step -------------------------------------------------------------------------

@@ -98,3 +98,19 @@ def test_loaded_states_are_copies() -> None:
             t.zero_()
     assert torch.equal(source.state[kept[0]]["exp_avg"], kept[1])
     assert (source.state[theirs[1]]["step"] == 7).all()
+
+
+def test_the_load_makes_no_second_set_of_states(monkeypatch) -> None:
+    source, _ = optimizer(bits=8)
+    opt, params = optimizer(bits=8, seed=1)
+    saved = source.state_dict()
+    saved["state"]["of the run"] = {"best": 0.5}  # what belongs to no parameter stays what it is
+    cast = []
+    real = torch.Tensor.to
+    monkeypatch.setattr(torch.Tensor, "to", lambda t, *a, **k: cast.append(k.get("dtype")) or real(t, *a, **k))
+    opt.load_state_dict(saved)
+    monkeypatch.undo()
+    assert not [d for d in cast if d is not None]  # the base class would cast states to their parameter's dtype
+    assert opt.state["of the run"] == {"best": 0.5}
+    assert all(opt.state[p]["exp_avg"].dtype == torch.float8_e4m3fn for p in params[:1])
+    assert len(saved["state"]) == 3 and saved["state"][0].keys() == source.state[next(iter(source.state))].keys()
