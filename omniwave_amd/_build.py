@@ -100,7 +100,7 @@ def build(verbose: bool = False) -> Path:
         try:
             _run(glue.result(), verbose)
             _install(glue_tmp, GLUE_PATH)
-        except (RuntimeError, OSError, ImportError) as exc:
+        except Exception as exc:  # whatever it is that is missing
             GLUE_PATH.unlink(missing_ok=True)  # one that is there is of another library
             warnings.warn(f"{GLUE_PATH.name} was not built: {exc}", RuntimeWarning, stacklevel=2)
     return LIB_PATH
