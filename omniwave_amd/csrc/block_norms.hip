@@ -24,8 +24,8 @@
 //
 // A grid is as many workgroups as run at once, and a row group is read while the one before it is computed:
 // without that 128 x 56 x 56 x 128 bf16 forward took 88.7 us, with it 76.5 (411 MB, 5.4 TB/s, a copy's rate);
-// 128 x 14 x 14 x 512 bf16 forward 20.9 us (4.9 TB/s), backward 35.6 (154 MB, 4.3 TB/s; 61 without) and 4.0 for
-// the sums of the weights' gradients over workgroups; 64 x 40 x 40 x 95 bf16, ragged, 17.8 and 38.1 us.
+// 128 x 14 x 14 x 512 bf16 forward 21.0 us (4.9 TB/s), backward 35.4 (154 MB, 4.4 TB/s; 61 without) and 4.0 for
+// the sums of the weights' gradients over workgroups; 64 x 40 x 40 x 95 bf16, ragged, 18.4 and 38.4 us.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>

@@ -143,7 +143,8 @@ def cross_entropy_hip(logits: Tensor, target: Tensor, *, target_b: Tensor | None
     ``target_b`` with ``mix``: a second label of weight ``1 - mix`` beside the first one's ``mix`` (mixed
     images; a number or one for each row).  ``label_smoothing``: the weight of the uniform distribution.
     Rows whose ``target`` is ``ignore_index`` count neither in the loss nor in the mean, and have no
-    gradient; a mean of no rows is NaN.  A label outside ``[0, classes)`` makes its row NaN.
+    gradient; a mean of no rows is NaN.  A label outside ``[0, classes)`` makes its row NaN (in ``target_b``, of a
+    weight above 0, ``ignore_index`` too), and so does a NaN logit.
     ``reduction``: ``"mean"``, ``"sum"`` or ``"none"``.  Differentiable once in the logits.
     """
     glue, code = _native.glue(), _native.OW_REDUCE.get(reduction)

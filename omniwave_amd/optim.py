@@ -77,13 +77,14 @@ class AdamW(torch.optim.Optimizer):
     therefore is not captured.  A step raises the parameters' version counters; the replay of a captured one
     cannot, so before an eager forward that follows replays call ``omniwave_amd.hip.clear_pack_cache()``.
 
-    8-bit states save memory, not steps: they are the nearest codes after each step, and half a code's step is 3 to 6%
-    where a step moves the root of the second moment by 0.05% (beta2 = 0.999).  A change that a block of 256
+    8-bit states save memory, not steps: they are the nearest codes after each step, and half a code's step is 3 to
+    6% where a step moves the root of the second moment by 0.05% (beta2 = 0.999).  A change that a block of 256
     values shares is followed by the block's scale.  A change beside the block's largest value is not, but for
     gradients above some 8 times the root: where gradients fall tenfold beside a steady one the root stays up to
-    tenfold too large (7.6 times in the median: steps too small), where they rise fourfold it reaches 0.4 to 1 of the right
-    one (steps up to 2.6 times too large); where nothing changes it is 0.7 to 1.5 times the right one.  A gradient that
-    is not finite makes its block's states so, where 32-bit states lose one value (``max_grad_norm`` skips the step).
+    tenfold too large (7.6 times in the median: steps too small), where they rise fourfold it reaches 0.4 to 1 of
+    the right one (steps up to 2.6 times too large); where nothing changes it is 0.7 to 1.5 times the right one.
+    A gradient that is not finite makes its block's states so, where 32-bit states lose one value
+    (``max_grad_norm`` skips the step).
 
     ``state[p]``: ``step`` (int32, the steps done, one for every 4,096 values), ``exp_avg`` and
     ``exp_avg_sq`` (fp32), or ``exp_avg`` and ``exp_avg_sq_root`` (e4m3fn) with ``exp_avg_scale`` and
