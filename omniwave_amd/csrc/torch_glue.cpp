@@ -100,6 +100,11 @@ const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nul
 void* out_ptr(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 Tensor like(const Tensor& t) { return at::empty_like(t, at::MemoryFormat::Contiguous); }
 
+// Hooks on saved tensors may hand out others than were saved: a kernel gets only what fits.
+void check_unpacked(bool ok) {
+  TORCH_CHECK_VALUE(ok, "a saved tensor has come back to the backward with another type, shape or device");
+}
+
 // The gradients of a function that can be differentiated once: an error where they are differentiated again.
 variable_list once(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -205,6 +210,7 @@ class NormsNode : public torch::autograd::Function<NormsNode> {
   static variable_list backward(AutogradContext* ctx, variable_list ups) {
     const variable_list s = ctx->get_saved_variables();
     Norms n{s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["eps"].toDouble()};
+    check_unpacked(n.x.is_cuda());
     const c10::DeviceGuard guard(n.x.device());
     const bool has_out = n.delta.defined();
     Tensor dout = has_out ? ups[0] : Tensor(), dnext = n.next.defined() ? ups[has_out ? 1 : 0] : Tensor();
@@ -214,6 +220,11 @@ class NormsNode : public torch::autograd::Function<NormsNode> {
     if (has_out) n.delta = rows_of(n.delta, &unused);
     for (Tensor* w : {&n.post, &n.gate, &n.scale, &n.next})
       if (w->defined()) *w = w->contiguous();
+    const auto fits = [&](const Tensor& g) {
+      return !g.defined() || (plain(g) && g.sizes() == n.x.sizes() && g.scalar_type() == n.x.scalar_type() &&
+                              g.device() == n.x.device());
+    };
+    check_unpacked(plain_case(n) && fits(dout) && fits(dnext));
     if (dout.defined()) dout = rows_of(dout, &out_stride);
     if (dnext.defined()) dnext = rows_of(dnext, &next_stride);
 
@@ -332,16 +343,22 @@ class XentNode : public torch::autograd::Function<XentNode> {
     const variable_list s = ctx->get_saved_variables();
     Xent e{s[0], s[1], s[2], s[3], ctx->saved_data["mix"].toDouble(), ctx->saved_data["smoothing"].toDouble(),
            ctx->saved_data["ignore"].toInt(), static_cast<int32_t>(ctx->saved_data["reduction"].toInt())};
+    check_unpacked(e.logits.is_cuda());
     const c10::DeviceGuard guard(e.logits.device());
     int64_t unused = 0;  // hooks on saved tensors may hand out copies that lie otherwise
     e.logits = rows_of(e.logits, &unused);
     for (Tensor* t : {&e.target, &e.target_b, &e.mix})
       if (t->defined()) *t = t->contiguous();
     const Tensor aux = s[4].contiguous(), up = ups[0].to(at::kFloat).contiguous();
+    const bool reduced = e.reduction != OW_REDUCE_NONE;
+    const int64_t rows = e.target.numel();
+    check_unpacked(plain_case(e) && plain(aux) && aux.scalar_type() == at::kFloat && aux.device() == e.logits.device() &&
+                   aux.numel() == 2 * rows + 1 + (reduced ? rows : 0) && plain(up) && up.device() == e.logits.device() &&
+                   up.numel() == (reduced ? 1 : rows));
     Tensor grad = like(e.logits);
     const OwCrossEntropy d = descriptor(e);
     const float* stats = static_cast<const float*>(ptr(aux));
-    check(ow_cross_entropy_bwd(&d, stats, e.reduction != OW_REDUCE_NONE ? stats + 2 * d.rows : nullptr,
+    check(ow_cross_entropy_bwd(&d, stats, reduced ? stats + 2 * d.rows : nullptr,
                                static_cast<const float*>(ptr(up)), out_ptr(grad), stream_of(e.logits)),
           "ow_cross_entropy_bwd");
     return once({std::move(grad), Tensor()});

@@ -23,28 +23,36 @@ def _check(logits, target, target_b, mix, label_smoothing, ignore_index, reducti
         raise ValueError(f"reduction must be 'none', 'sum' or 'mean', got {reduction!r}")
     if not isinstance(ignore_index, int):
         raise ValueError(f"ignore_index must be an integer, got {ignore_index!r}")
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError(f"label_smoothing must be in [0, 1], got {label_smoothing}")
+    if (target_b is None) != (mix is None):
+        raise ValueError("target_b and mix, the weight of target, come together")
+    if isinstance(mix, Tensor):
+        if mix.requires_grad:
+            raise ValueError("mix carries no gradient; detach it")
+    elif mix is not None and not 0.0 <= mix <= 1.0:
+        raise ValueError(f"mix must be in [0, 1], got {mix}")
+    _ready(logits, target, target_b, mix if isinstance(mix, Tensor) else None)
+
+
+def _ready(logits, target, target_b, mix) -> None:
+    """Raise for tensors that the kernels do not take, and where they cannot run."""
     if logits.dtype not in SUPPORTED_DTYPES:
         raise ValueError(f"unsupported dtype {logits.dtype}; expected float16, bfloat16 or float32")
     if logits.dim() < 1 or not 1 <= logits.shape[-1] < 1 << 30:
         raise ValueError(f"logits must be [..., classes] with 1 to 2^30 - 1 classes, got {tuple(logits.shape)}")
     if math.prod(logits.shape[:-1]) >= 1 << 31:
         raise ValueError(f"{math.prod(logits.shape[:-1])} rows; fewer than 2^31 are supported")
-    if not 0.0 <= label_smoothing <= 1.0:
-        raise ValueError(f"label_smoothing must be in [0, 1], got {label_smoothing}")
     for name, t in (("target", target), ("target_b", target_b)):
         if t is not None and (t.dtype != torch.int64 or t.shape != logits.shape[:-1] or t.device != logits.device):
             raise ValueError(f"{name} must be int64 {tuple(logits.shape[:-1])} on {logits.device}, got {t.dtype} "
                              f"{tuple(t.shape)} on {t.device}")
-    if (target_b is None) != (mix is None):
-        raise ValueError("target_b and mix, the weight of target, come together")
-    if isinstance(mix, Tensor):
-        if mix.shape != target.shape or not mix.is_floating_point() or mix.device != logits.device:
-            raise ValueError(f"mix must be a number or floating point {tuple(target.shape)} on {logits.device}, got "
-                             f"{mix.dtype} {tuple(mix.shape)} on {mix.device}")
-        if mix.requires_grad:
-            raise ValueError("mix carries no gradient; detach it")
-    elif mix is not None and not 0.0 <= mix <= 1.0:
-        raise ValueError(f"mix must be in [0, 1], got {mix}")
+    if mix is not None and (mix.shape != target.shape or not mix.is_floating_point() or mix.device != logits.device):
+        raise ValueError(f"mix must be a number or floating point {tuple(target.shape)} on {logits.device}, got "
+                         f"{mix.dtype} {tuple(mix.shape)} on {mix.device}")
+    reason = gpu_reason(logits)
+    if reason is not None:
+        raise RuntimeError(f"hip cross-entropy not supported: {reason}")
 
 
 def _descriptor(logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction):
@@ -61,6 +69,7 @@ def _run_forward(logits, target, target_b, mix, mix_value, label_smoothing, igno
                  reduction) -> tuple[Tensor, Tensor]:
     """(the loss, or the losses of the rows; what the backward needs beside the inputs: the statistics of the
     rows, a row's weight in the loss and, with a reduction, the losses)."""
+    _ready(logits, target, target_b, mix)  # the operator may be called by its name
     device, reduced = logits.device, reduction != 0
     desc, _keep = _descriptor(logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction)
     rows, lib = desc.rows, _native.lib()
@@ -78,11 +87,18 @@ def _run_forward(logits, target, target_b, mix, mix_value, label_smoothing, igno
 
 def _run_backward(up, aux, logits, target, target_b, mix, *options) -> Tensor:
     """The logits' gradient; ``up``: the upstream gradient of the loss (a value) or the losses."""
+    _ready(logits, target, target_b, mix)  # hooks on saved tensors may hand out others
+    rows, reduced = target.numel(), options[-1] != 0
+    if (up.device != logits.device or up.numel() != (1 if reduced else rows) or aux.device != logits.device
+            or aux.dtype != torch.float32 or aux.numel() != 2 * rows + 1 + (rows if reduced else 0)):
+        raise ValueError(f"the backward of {rows} rows got a gradient of {tuple(up.shape)} on {up.device} and statistics "
+                         f"of {aux.dtype} {tuple(aux.shape)} on {aux.device}")
     grad = torch.empty_like(logits, memory_format=torch.contiguous_format)
     if not grad.numel():
         return grad
     desc, _keep = _descriptor(logits, target, target_b, mix, *options)
-    up, at = up.to(torch.float32).contiguous(), aux.data_ptr()
+    up, aux = up.to(torch.float32).contiguous(), aux.contiguous()
+    at = aux.data_ptr()
     _on(logits.device, _native.lib().ow_cross_entropy_bwd, ctypes.byref(desc), at,
         at + 8 * desc.rows if desc.reduction else None, up.data_ptr(), grad.data_ptr())
     return grad
@@ -157,8 +173,5 @@ def cross_entropy_hip(logits: Tensor, target: Tensor, *, target_b: Tensor | None
             return loss
     # Everything else is checked, and goes through the operator.
     _check(logits, target, target_b, mix, label_smoothing, ignore_index, reduction)
-    reason = gpu_reason(logits)
-    if reason is not None:
-        raise RuntimeError(f"hip cross-entropy not supported: {reason}")
     return cross_entropy_fwd(logits, target, target_b, None if number else mix, 1.0 if mix is None or not number else float(mix),
                              float(label_smoothing), ignore_index, code)[0]

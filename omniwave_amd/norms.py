@@ -72,6 +72,14 @@ def _check(x, delta, post_weight, gate, scale, next_weight, eps) -> None:
             raise ValueError("scale carries no gradient (a gate of [B, C] does); detach it")
 
 
+def _ready(x, delta, post_weight, gate, scale, next_weight, eps) -> None:
+    """Raise for what the kernels do not take, and where they cannot run."""
+    _check(x, delta, post_weight, gate, scale, next_weight, eps)
+    reason = gpu_reason(x)
+    if reason is not None:
+        raise RuntimeError(f"hip norms not supported: {reason}")
+
+
 def _rows(t: Tensor) -> tuple[Tensor, int]:
     """``t`` or a contiguous copy, with the distance between its rows (the last dimension) in values:
     rows lie at one distance, one value after the other."""
@@ -128,6 +136,7 @@ def _empty(t: Tensor) -> Tensor:
 
 
 def _run_forward(x, delta, post_weight, gate, scale, next_weight, eps) -> tuple[Tensor | None, Tensor | None]:
+    _ready(x, delta, post_weight, gate, scale, next_weight, eps)  # the operator may be called by its name
     out = _empty(x) if delta is not None else None
     nxt = _empty(x) if next_weight is not None else None
     if x.numel():
@@ -140,6 +149,11 @@ def _run_forward(x, delta, post_weight, gate, scale, next_weight, eps) -> tuple[
 def _run_backward(dout, dnext, x, delta, post_weight, gate, scale, next_weight, eps, want) -> list[Tensor | None]:
     """Gradients of x, delta, post_weight, gate and next_weight where ``want`` asks for them and they
     exist; ``dout`` / ``dnext`` None: that output has no upstream gradient."""
+    _ready(x, delta, post_weight, gate, scale, next_weight, eps)  # hooks on saved tensors may hand out others
+    for g in (dout, dnext):
+        if g is not None and (g.shape != x.shape or g.dtype != x.dtype or g.device != x.device):
+            raise ValueError(f"the upstream gradient of {x.dtype} {tuple(x.shape)} on {x.device} is {g.dtype} "
+                             f"{tuple(g.shape)} on {g.device}")
     grads = [_empty(t) if w and t is not None else None for t, w in zip((x, delta, post_weight, gate, next_weight), want)]
     if x.numel() == 0 or (dout is None and dnext is None):
         return [None if g is None else g.zero_() for g in grads]
@@ -222,10 +236,7 @@ def _norms(x, delta, post_weight, gate, scale, next_weight, eps) -> tuple[Tensor
             return both
     # Everything else is checked, and goes through the operator.
     eps = float(eps)
-    _check(x, delta, post_weight, gate, scale, next_weight, eps)
-    reason = gpu_reason(x)
-    if reason is not None:
-        raise RuntimeError(f"hip norms not supported: {reason}")
+    _ready(x, delta, post_weight, gate, scale, next_weight, eps)
     out, nxt = block_norms_fwd(x, delta, post_weight, gate, scale, next_weight, eps)
     return (None if delta is None else out), (None if next_weight is None else nxt)
 
