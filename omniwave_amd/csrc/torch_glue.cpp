@@ -214,6 +214,8 @@ class NormsNode : public torch::autograd::Function<NormsNode> {
     const c10::DeviceGuard guard(n.x.device());
     const bool has_out = n.delta.defined();
     Tensor dout = has_out ? ups[0] : Tensor(), dnext = n.next.defined() ? ups[has_out ? 1 : 0] : Tensor();
+    for (Tensor* g : {&dout, &dnext})  // a gradient may stand for its negative (the imaginary part of a conjugate)
+      if (g->defined()) *g = g->resolve_neg();
     // Hooks on saved tensors may hand out copies that lie otherwise.
     int64_t unused = 0, out_stride = 0, next_stride = 0;
     n.x = rows_of(n.x, &unused);
@@ -349,7 +351,7 @@ class XentNode : public torch::autograd::Function<XentNode> {
     e.logits = rows_of(e.logits, &unused);
     for (Tensor* t : {&e.target, &e.target_b, &e.mix})
       if (t->defined()) *t = t->contiguous();
-    const Tensor aux = s[4].contiguous(), up = ups[0].to(at::kFloat).contiguous();
+    const Tensor aux = s[4].contiguous(), up = ups[0].resolve_neg().to(at::kFloat).contiguous();
     const bool reduced = e.reduction != OW_REDUCE_NONE;
     const int64_t rows = e.target.numel();
     check_unpacked(plain_case(e) && plain(aux) && aux.scalar_type() == at::kFloat && aux.device() == e.logits.device() &&

@@ -95,3 +95,26 @@ def test_copies_that_lie_otherwise_are_taken(make) -> None:
         loss = call()
         got = torch.autograd.grad(loss, leaves)
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("make", [norms, rms, xent])
+def test_upstream_gradients_that_stand_for_their_negatives(make) -> None:
+    announce(f"negated upstream gradients {make.__name__}")
+    leaves, call = make(torch.float32)
+    torch.manual_seed(1)
+    loss = call()
+    want = torch.autograd.grad(loss, leaves, torch.full((), 2.0, device=DEV), retain_graph=True)
+    up = torch._neg_view(torch.full((), -2.0, device=DEV))  # as the imaginary part of a conjugate is one
+    assert up.is_neg() and up.item() == 2.0
+    got = torch.autograd.grad(loss, leaves, up)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_upstream_gradients_of_outputs_that_stand_for_their_negatives() -> None:
+    announce("negated upstream gradients of the norms' outputs")
+    x, delta = (torch.randn(2, 30, 96, device=DEV, requires_grad=True) for _ in range(2))
+    w, up = torch.rand(96, device=DEV), torch.randn(2, 30, 96, device=DEV)
+    out = block_norms_hip(x, delta, next_weight=w)
+    want = torch.autograd.grad(out, (x, delta), (up, up), retain_graph=True)
+    got = torch.autograd.grad(out, (x, delta), (torch._neg_view(-up), torch._neg_view(-up)))
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
