@@ -691,6 +691,74 @@ int ow_cross_entropy_fwd(const OwCrossEntropy* ce, float* stats, float* losses, 
 int ow_cross_entropy_bwd(const OwCrossEntropy* ce, const float* stats, const float* weight, const float* upstream,
                          void* grad, void* stream);
 
+/*
+ * Layer norm of `rows` rows of `channels` values (no counterpart in the reference, whose blocks have RMS norms):
+ *
+ *   y = (x - mean_c x) / sqrt(mean_c (x - mean_c x)^2 + eps) * weight + bias     (each NULL: left out)
+ *
+ * x: `dtype`, value stride 1, row stride in values (any alignment); y, dx contiguous in `dtype`; weight and bias
+ * [C], each of a dtype of its own.  Sums and intermediates are fp32 and each output is rounded once.  At most
+ * 8,192 channels and 2^31 - 1 rows.
+ *
+ * The backward takes dy (row stride in values) and writes those of dx, dweight and dbias (in their inputs' dtypes)
+ * that are not NULL, sums over rows in a fixed order over ow_layer_norm_bwd_workspace bytes of workspace (4-byte
+ * aligned; 0 for few rows; not needed, and NULL, without dweight and dbias).  rows, channels >= 1 there.
+ */
+typedef struct OwLayerNorm {
+  int64_t rows;
+  int64_t x_stride;
+  const void* x;
+  const void* weight;
+  const void* bias;
+  int32_t channels;
+  int32_t dtype;
+  int32_t weight_dtype;
+  int32_t bias_dtype;
+  float eps;
+} OwLayerNorm;
+
+int ow_layer_norm_fwd(const OwLayerNorm* norm, void* y, void* stream);
+size_t ow_layer_norm_bwd_workspace(const OwLayerNorm* norm);
+int ow_layer_norm_bwd(const OwLayerNorm* norm, const void* dy, int64_t dy_stride, void* dx, void* dweight, void* dbias,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Distillation of rows of logits from a teacher's top logits (no counterpart in the reference): entries (class i_j,
+ * logit t_j), `top` a row, against all classes, both as softmax at a temperature T:
+ *
+ *   loss_r = T^2 sum_j q_j (ln q_j - ln softmax(x / T)_{i_j}),   q = softmax(t / T) over the row's entries
+ *
+ * An entry of class ignore_index or of logit -inf is none; rows without entries have loss 0 and do not count in
+ * the mean (NaN where no row counts).  A class may have several entries.  Classes outside [0, classes) and NaN
+ * logits make the row's loss and gradient NaN.  logits: `dtype`, value stride 1, row_stride values between rows (any
+ * alignment); teacher (`teacher_dtype`) and indices: [rows][top], contiguous.
+ *
+ * Forward: stats [rows][4] (what the backward needs), losses [rows], a workspace (8-byte aligned) of
+ * ow_distillation_workspace bytes, and with a reduction loss [1], the result, and weight [1], a row's weight in it
+ * (both NULL without).  Backward: the forward's stats and weight, upstream [1] or, without a reduction, [rows];
+ * grad [rows][classes] of the logits' dtype.
+ */
+typedef struct OwDistillation {
+  int64_t rows;
+  int64_t classes;
+  int64_t row_stride;
+  int64_t ignore_index;
+  const void* logits;
+  const void* teacher;
+  const int64_t* indices;
+  int32_t top;
+  int32_t dtype;
+  int32_t teacher_dtype;
+  int32_t reduction;
+  float temperature;
+} OwDistillation;
+
+size_t ow_distillation_workspace(const OwDistillation* d);
+int ow_distillation_fwd(const OwDistillation* d, float* stats, float* losses, float* loss, float* weight, void* workspace,
+                        size_t workspace_bytes, void* stream);
+int ow_distillation_bwd(const OwDistillation* d, const float* stats, const float* weight, const float* upstream, void* grad,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,9 +8,10 @@ __version__ = "0.1.0"
 
 from omniwave_amd.bigemm import bigemm, register_backend
 from omniwave_amd.block import enable_fp8
+from omniwave_amd.distillation import distillation_hip
 from omniwave_amd.hip import bigemm_block_hip, bigemm_delta_hip, hip_is_supported
 from omniwave_amd.loss import cross_entropy_hip
-from omniwave_amd.norms import block_norms_hip, rms_norm_hip
+from omniwave_amd.norms import block_norms_hip, layer_norm_hip, rms_norm_hip
 from omniwave_amd.optim import AdamW
 from omniwave_amd.registry import create_model, create_model_from_config
 from omniwave_amd.routing import RoutePlan, build_route_plan, build_stage_schedule
@@ -27,8 +28,10 @@ __all__ = [
     "create_model",
     "create_model_from_config",
     "cross_entropy_hip",
+    "distillation_hip",
     "enable_fp8",
     "hip_is_supported",
+    "layer_norm_hip",
     "register_backend",
     "rms_norm_hip",
 ]

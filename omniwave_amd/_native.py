@@ -53,6 +53,13 @@ class OwBlockNorms(ctypes.Structure):
     ]
 
 
+class OwLayerNorm(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("x_stride", ctypes.c_int64)]
+    _fields_ += [(name, ctypes.c_void_p) for name in ("x", "weight", "bias")]
+    _fields_ += [(name, ctypes.c_int32) for name in ("channels", "dtype", "weight_dtype", "bias_dtype")]
+    _fields_ += [("eps", ctypes.c_float)]
+
+
 class OwAdamwTensor(ctypes.Structure):
     _fields_ = [(name, ctypes.c_void_p) for name in ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale",
                                                      "exp_avg_sq_scale", "master", "step")]
@@ -69,6 +76,13 @@ class OwCrossEntropy(ctypes.Structure):
     _fields_ += [(name, ctypes.c_void_p) for name in ("logits", "target", "target_b", "mix")]
     _fields_ += [("mix_value", ctypes.c_float), ("smoothing", ctypes.c_float), ("dtype", ctypes.c_int32),
                  ("reduction", ctypes.c_int32)]
+
+
+class OwDistillation(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int64) for name in ("rows", "classes", "row_stride", "ignore_index")]
+    _fields_ += [(name, ctypes.c_void_p) for name in ("logits", "teacher", "indices")]
+    _fields_ += [(name, ctypes.c_int32) for name in ("top", "dtype", "teacher_dtype", "reduction")]
+    _fields_ += [("temperature", ctypes.c_float)]
 
 
 OW_REDUCE = {"none": 0, "sum": 1, "mean": 2}
@@ -282,6 +296,13 @@ _SIGNATURES = {
         [ctypes.POINTER(OwBlockNorms), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64]
         + [ctypes.c_void_p] * 6 + [ctypes.c_size_t, ctypes.c_void_p],
     ),
+    "ow_layer_norm_fwd": (ctypes.c_int, [ctypes.POINTER(OwLayerNorm)] + [ctypes.c_void_p] * 2),
+    "ow_layer_norm_bwd_workspace": (ctypes.c_size_t, [ctypes.POINTER(OwLayerNorm)]),
+    "ow_layer_norm_bwd": (
+        ctypes.c_int,
+        [ctypes.POINTER(OwLayerNorm), ctypes.c_void_p, ctypes.c_int64] + [ctypes.c_void_p] * 4
+        + [ctypes.c_size_t, ctypes.c_void_p],
+    ),
     "ow_grad_norm_partials": (ctypes.c_int64, [ctypes.c_void_p, ctypes.c_int32]),
     "ow_grad_norm": (
         ctypes.c_int,
@@ -297,6 +318,11 @@ _SIGNATURES = {
         ctypes.c_int, [ctypes.POINTER(OwCrossEntropy)] + [ctypes.c_void_p] * 5 + [ctypes.c_size_t, ctypes.c_void_p],
     ),
     "ow_cross_entropy_bwd": (ctypes.c_int, [ctypes.POINTER(OwCrossEntropy)] + [ctypes.c_void_p] * 5),
+    "ow_distillation_workspace": (ctypes.c_size_t, [ctypes.POINTER(OwDistillation)]),
+    "ow_distillation_fwd": (
+        ctypes.c_int, [ctypes.POINTER(OwDistillation)] + [ctypes.c_void_p] * 5 + [ctypes.c_size_t, ctypes.c_void_p],
+    ),
+    "ow_distillation_bwd": (ctypes.c_int, [ctypes.POINTER(OwDistillation)] + [ctypes.c_void_p] * 5),
     "ow_bwd_params": (
         ctypes.c_int,
         [ctypes.c_void_p] * 3 + [ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]

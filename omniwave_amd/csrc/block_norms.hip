@@ -64,73 +64,6 @@ constexpr int kWantPost = 1, kWantNext = 2, kWantGate = 4;
 constexpr int fwd_waves(int t) { return t == 1024 ? 4 : 6; }
 constexpr int bwd_waves(int vec, int t) { return t == 1024 ? 4 : vec == 8 ? 3 : 4; }
 
-template <int T>
-constexpr int kThreads = T > 256 ? T : 256;
-
-// Which channels a thread holds.
-template <class R, int T, int K, bool RAGGED>
-struct Place {
-  static constexpr int V = R::kVec;
-  int col[K];  // first channel; -1: none
-  int dup[K];  // values at its start that another lane counts
-  int n;       // values of a vector (less than V only for rows shorter than a vector)
-  __device__ __forceinline__ Place(int t, int c) {
-    n = RAGGED && c < V ? c : V;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int want = V * (t + T * k);
-      col[k] = want < c ? want : -1;
-      dup[k] = 0;
-      if (RAGGED && want < c && want + V > c) {
-        col[k] = c < V ? 0 : c - V;
-        dup[k] = want - col[k];
-      }
-    }
-  }
-  // Whether a value counts in sums over the row.
-  __device__ __forceinline__ bool counts(int k, int j) const { return col[k] >= 0 && j >= dup[k] && j < n; }
-  __device__ __forceinline__ typename R::Raw load(const typename R::Elem* row, int k, bool valid) const {
-    if (!valid || col[k] < 0) return R::zero();
-    if (RAGGED && n < V) {
-      typename R::Raw w = R::zero();
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (j < n) R::set(w, j, row[j]);
-      return w;
-    }
-    return R::raw(row + col[k]);
-  }
-  __device__ __forceinline__ void store(typename R::Elem* row, int k, bool valid, const float (&v)[V]) const {
-    if (!valid || col[k] < 0) return;
-    if (RAGGED && n < V) {
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (j < n) row[j] = R::from_f32(v[j]);
-    } else {
-      R::store(row + col[k], v);
-    }
-  }
-  // A vector of channels of a weight, `absent` where there is no weight.
-  __device__ __forceinline__ void weight(const void* p, int32_t dtype, int64_t base, int k, float absent,
-                                         float (&v)[V]) const {
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = absent;
-    if (p == nullptr || col[k] < 0) return;
-    if (RAGGED && n < V) {
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (j < n) v[j] = load_any(p, dtype, base + j);
-    } else {
-      load_any_vec<V>(p, dtype, base + col[k], v);
-    }
-  }
-};
-
-// A value as it enters its row's sums, 0 where another lane counts it (whole vectors need no mask).  Chosen, not
-// multiplied by 0 or 1: 0 times an infinity would make the whole row NaN.
-template <bool RAGGED>
-__device__ __forceinline__ float counted(float a, bool counts) { return !RAGGED || counts ? a : 0.f; }
-
 template <class Ty, int T, int K, bool RAGGED>
 __global__ void __launch_bounds__(kThreads<T>, fwd_waves(T)) block_norms_fwd_kernel(NormsArgs a) {
   typedef Row<Ty> R;

@@ -104,20 +104,20 @@ struct MaxUintOp {
   static __device__ __forceinline__ uint32_t apply(uint32_t a, uint32_t b) { return a > b ? a : b; }
 };
 
-// Op over aligned groups of T lanes (8, 16, 32 or 64); every lane gets the result.  Mirrors within a row of
+// Op over aligned groups of T lanes (a power of two up to 64); every lane gets the result.  Mirrors within a row of
 // 16 lanes, then gfx950's row and half swaps: of two copies of v, permlane16_swap leaves the even
 // rows in one and the odd rows in the other (permlane32_swap: the halves).
 template <class Op, int T, class V>
 __device__ __forceinline__ V lanes_reduce(V v) {
-  static_assert((T == 8 || T == 16 || T == 32 || T == 64) && sizeof(V) == 4, "lanes of a row");
+  static_assert(T >= 1 && T <= 64 && (T & (T - 1)) == 0 && sizeof(V) == 4, "lanes of a row");
   auto bits = [](V x) { return __builtin_bit_cast(uint32_t, x); };
   auto value = [](uint32_t x) { return __builtin_bit_cast(V, x); };
   auto dpp = [&](V x, auto ctrl) {
     return value(__builtin_amdgcn_update_dpp(0u, bits(x), decltype(ctrl)::value, 0xf, 0xf, false));
   };
-  v = Op::apply(v, dpp(v, std::integral_constant<int, 0xb1>{}));   // quad_perm 1,0,3,2
-  v = Op::apply(v, dpp(v, std::integral_constant<int, 0x4e>{}));   // quad_perm 2,3,0,1
-  v = Op::apply(v, dpp(v, std::integral_constant<int, 0x141>{}));  // row_half_mirror
+  if constexpr (T >= 2) v = Op::apply(v, dpp(v, std::integral_constant<int, 0xb1>{}));   // quad_perm 1,0,3,2
+  if constexpr (T >= 4) v = Op::apply(v, dpp(v, std::integral_constant<int, 0x4e>{}));   // quad_perm 2,3,0,1
+  if constexpr (T >= 8) v = Op::apply(v, dpp(v, std::integral_constant<int, 0x141>{}));  // row_half_mirror
   if constexpr (T >= 16) v = Op::apply(v, dpp(v, std::integral_constant<int, 0x140>{}));  // row_mirror
   if constexpr (T >= 32) {
     const auto s = __builtin_amdgcn_permlane16_swap(bits(v), bits(v), false, false);
@@ -160,5 +160,75 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float* red, int& turn) {
     }
   }
 }
+
+// ---------------------------------------------------------------------------------------
+// Rows that stay in registers: T threads a row, K vectors each
+
+template <int T>
+constexpr int kThreads = T > 256 ? T : 256;
+
+// Which channels a thread holds.
+template <class R, int T, int K, bool RAGGED>
+struct Place {
+  static constexpr int V = R::kVec;
+  int col[K];  // first channel; -1: none
+  int dup[K];  // values at its start that another lane counts
+  int n;       // values of a vector (less than V only for rows shorter than a vector)
+  __device__ __forceinline__ Place(int t, int c) {
+    n = RAGGED && c < V ? c : V;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int want = V * (t + T * k);
+      col[k] = want < c ? want : -1;
+      dup[k] = 0;
+      if (RAGGED && want < c && want + V > c) {
+        col[k] = c < V ? 0 : c - V;
+        dup[k] = want - col[k];
+      }
+    }
+  }
+  // Whether a value counts in sums over the row.
+  __device__ __forceinline__ bool counts(int k, int j) const { return col[k] >= 0 && j >= dup[k] && j < n; }
+  __device__ __forceinline__ typename R::Raw load(const typename R::Elem* row, int k, bool valid) const {
+    if (!valid || col[k] < 0) return R::zero();
+    if (RAGGED && n < V) {
+      typename R::Raw w = R::zero();
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (j < n) R::set(w, j, row[j]);
+      return w;
+    }
+    return R::raw(row + col[k]);
+  }
+  __device__ __forceinline__ void store(typename R::Elem* row, int k, bool valid, const float (&v)[V]) const {
+    if (!valid || col[k] < 0) return;
+    if (RAGGED && n < V) {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (j < n) row[j] = R::from_f32(v[j]);
+    } else {
+      R::store(row + col[k], v);
+    }
+  }
+  // A vector of channels of a weight, `absent` where there is no weight.
+  __device__ __forceinline__ void weight(const void* p, int32_t dtype, int64_t base, int k, float absent,
+                                         float (&v)[V]) const {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = absent;
+    if (p == nullptr || col[k] < 0) return;
+    if (RAGGED && n < V) {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (j < n) v[j] = load_any(p, dtype, base + j);
+    } else {
+      load_any_vec<V>(p, dtype, base + col[k], v);
+    }
+  }
+};
+
+// A value as it enters its row's sums, 0 where another lane counts it (whole vectors need no mask).  Chosen, not
+// multiplied by 0 or 1: 0 times an infinity would make the whole row NaN.
+template <bool RAGGED>
+__device__ __forceinline__ float counted(float a, bool counts) { return !RAGGED || counts ? a : 0.f; }
 
 }  // namespace ow

@@ -262,6 +262,94 @@ class NormsNode : public torch::autograd::Function<NormsNode> {
 };
 
 // ---------------------------------------------------------------------------------------
+// Layer norm
+
+struct LayerNorm {
+  Tensor x, weight, bias;
+  double eps = 0.0;
+};
+
+OwLayerNorm descriptor(const LayerNorm& n) {
+  OwLayerNorm d{};
+  d.channels = static_cast<int32_t>(n.x.size(-1));
+  d.rows = n.x.numel() / d.channels;
+  d.x_stride = row_stride(n.x);
+  d.x = ptr(n.x);
+  d.weight = ptr(n.weight);
+  d.bias = ptr(n.bias);
+  d.dtype = dtype_code(n.x);
+  d.weight_dtype = n.weight.defined() ? dtype_code(n.weight) : 0;
+  d.bias_dtype = n.bias.defined() ? dtype_code(n.bias) : 0;
+  d.eps = static_cast<float>(n.eps);
+  return d;
+}
+
+bool plain_case(const LayerNorm& n) {
+  const Tensor& x = n.x;
+  if (!x.defined() || !plain(x) || x.dim() < 1 || x.numel() == 0 || !device_ok(x)) return false;
+  const int64_t c = x.size(-1);
+  if (c > kMaxChannels || x.numel() / c >= (int64_t(1) << 31) || row_stride(x) < 0) return false;
+  return n.eps >= 0.0 && std::isfinite(n.eps) && weight_ok(n.weight, x, false) && weight_ok(n.bias, x, false);
+}
+
+Tensor run_layer_norm(const LayerNorm& n) {
+  const c10::DeviceGuard guard(n.x.device());
+  Tensor y = like(n.x);
+  const OwLayerNorm d = descriptor(n);
+  check(ow_layer_norm_fwd(&d, out_ptr(y), stream_of(n.x)), "ow_layer_norm_fwd");
+  return y;
+}
+
+class LayerNormNode : public torch::autograd::Function<LayerNormNode> {
+ public:
+  typedef std::optional<Tensor> Given;
+
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Given& weight, const Given& bias, double eps) {
+    const LayerNorm n{x, weight.value_or(Tensor()), bias.value_or(Tensor()), eps};
+    ctx->save_for_backward({n.x, n.weight, n.bias});
+    ctx->saved_data["eps"] = eps;
+    ctx->set_materialize_grads(false);
+    return run_layer_norm(n);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list ups) {
+    if (!ups[0].defined()) return variable_list(4);
+    const variable_list s = ctx->get_saved_variables();
+    LayerNorm n{s[0], s[1], s[2], ctx->saved_data["eps"].toDouble()};
+    check_unpacked(n.x.is_cuda());
+    const c10::DeviceGuard guard(n.x.device());
+    int64_t unused = 0, dy_stride = 0;
+    n.x = rows_of(n.x, &unused);
+    for (Tensor* w : {&n.weight, &n.bias})
+      if (w->defined()) *w = w->contiguous();
+    Tensor dy = ups[0].resolve_neg();
+    check_unpacked(plain_case(n) && plain(dy) && dy.sizes() == n.x.sizes() && dy.scalar_type() == n.x.scalar_type() &&
+                   dy.device() == n.x.device());
+    dy = rows_of(dy, &dy_stride);
+    // needs_input_grad counts the tensors that were given.
+    const Tensor* inputs[3] = {&n.x, &n.weight, &n.bias};
+    Tensor grads[3];
+    size_t edge = 0;
+    bool any = false;
+    for (int i = 0; i < 3; ++i)
+      if (inputs[i]->defined() && ctx->needs_input_grad(edge++)) grads[i] = like(*inputs[i]), any = true;
+    if (any) {
+      const OwLayerNorm d = descriptor(n);
+      size_t bytes = 0;
+      Tensor workspace;
+      if (grads[1].defined() || grads[2].defined()) {
+        bytes = ow_layer_norm_bwd_workspace(&d);
+        if (bytes) workspace = at::empty({static_cast<int64_t>(bytes)}, n.x.options().dtype(at::kByte));
+      }
+      check(ow_layer_norm_bwd(&d, ptr(dy), dy_stride, out_ptr(grads[0]), out_ptr(grads[1]), out_ptr(grads[2]),
+                              out_ptr(workspace), bytes, stream_of(n.x)),
+            "ow_layer_norm_bwd");
+    }
+    return once({grads[0], grads[1], grads[2], Tensor()});
+  }
+};
+
+// ---------------------------------------------------------------------------------------
 // Cross-entropy
 
 struct Xent {
@@ -368,6 +456,110 @@ class XentNode : public torch::autograd::Function<XentNode> {
 };
 
 // ---------------------------------------------------------------------------------------
+// Distillation
+
+struct Distill {
+  Tensor logits, teacher, indices;
+  double temperature = 1.0;
+  int64_t ignore_index = -100;
+  int32_t reduction = OW_REDUCE_MEAN;
+};
+
+OwDistillation descriptor(const Distill& e) {
+  OwDistillation d{};
+  d.classes = e.logits.size(-1);
+  d.rows = e.logits.numel() / d.classes;
+  d.row_stride = row_stride(e.logits);
+  d.ignore_index = e.ignore_index;
+  d.logits = ptr(e.logits);
+  d.teacher = ptr(e.teacher);
+  d.indices = static_cast<const int64_t*>(ptr(e.indices));
+  d.top = static_cast<int32_t>(e.teacher.size(-1));
+  d.dtype = dtype_code(e.logits);
+  d.teacher_dtype = dtype_code(e.teacher);
+  d.reduction = e.reduction;
+  d.temperature = static_cast<float>(e.temperature);
+  return d;
+}
+
+constexpr int64_t kMaxEntries = 1 << 16;  // of the distillation kernels
+
+bool plain_case(const Distill& e) {
+  const Tensor& x = e.logits;
+  if (!x.defined() || !e.teacher.defined() || !e.indices.defined()) return false;
+  if (!plain(x) || x.dim() < 1 || x.numel() == 0 || !device_ok(x)) return false;
+  const int64_t c = x.size(-1);
+  if (c >= (int64_t(1) << 30) || x.numel() / c >= (int64_t(1) << 31) || row_stride(x) < 0) return false;
+  const Tensor &t = e.teacher, &i = e.indices;
+  if (!plain(t) || t.device() != x.device() || t.dim() != x.dim() || t.size(-1) > kMaxEntries || !t.is_contiguous() ||
+      t.requires_grad() || t.sizes().slice(0, t.dim() - 1) != x.sizes().slice(0, x.dim() - 1))
+    return false;
+  if (!i.is_cuda() || i.layout() != at::kStrided || i.scalar_type() != at::kLong || i.device() != x.device() ||
+      i.sizes() != t.sizes() || !i.is_contiguous())
+    return false;
+  return e.temperature >= 1e-15 && e.temperature <= 1e15;
+}
+
+// The loss (or the rows' losses), and what the backward needs: the rows' statistics, a row's weight in the
+// loss and, with a reduction, the losses.
+std::pair<Tensor, Tensor> run_distill(const Distill& e) {
+  const c10::DeviceGuard guard(e.logits.device());
+  const OwDistillation d = descriptor(e);
+  const bool reduced = e.reduction != OW_REDUCE_NONE;
+  const auto f32 = e.logits.options().dtype(at::kFloat);
+  Tensor aux = at::empty({4 * d.rows + 1 + (reduced ? d.rows : 0)}, f32);
+  Tensor loss = reduced ? at::empty({}, f32) : at::empty(e.logits.sizes().slice(0, e.logits.dim() - 1), f32);
+  const size_t bytes = ow_distillation_workspace(&d);
+  Tensor workspace = bytes ? at::empty({static_cast<int64_t>(bytes)}, f32.dtype(at::kByte)) : Tensor();
+  float* stats = static_cast<float*>(out_ptr(aux));
+  float* weight = stats + 4 * d.rows;
+  float* out = static_cast<float*>(out_ptr(loss));
+  check(ow_distillation_fwd(&d, stats, reduced ? weight + 1 : out, reduced ? out : nullptr, reduced ? weight : nullptr,
+                            out_ptr(workspace), bytes, stream_of(e.logits)),
+        "ow_distillation_fwd");
+  return {std::move(loss), std::move(aux)};
+}
+
+class DistillNode : public torch::autograd::Function<DistillNode> {
+ public:
+  static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Distill& e) {
+    auto [loss, aux] = run_distill(e);
+    ctx->save_for_backward({logits, e.teacher, e.indices, aux});
+    ctx->saved_data["temperature"] = e.temperature;
+    ctx->saved_data["ignore"] = e.ignore_index;
+    ctx->saved_data["reduction"] = static_cast<int64_t>(e.reduction);
+    ctx->set_materialize_grads(false);
+    return loss;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list ups) {
+    if (!ups[0].defined()) return {Tensor(), Tensor()};
+    const variable_list s = ctx->get_saved_variables();
+    Distill e{s[0], s[1], s[2], ctx->saved_data["temperature"].toDouble(), ctx->saved_data["ignore"].toInt(),
+              static_cast<int32_t>(ctx->saved_data["reduction"].toInt())};
+    check_unpacked(e.logits.is_cuda());
+    const c10::DeviceGuard guard(e.logits.device());
+    int64_t unused = 0;  // hooks on saved tensors may hand out copies that lie otherwise
+    e.logits = rows_of(e.logits, &unused);
+    e.teacher = e.teacher.detach().contiguous();
+    e.indices = e.indices.contiguous();
+    const Tensor aux = s[3].contiguous(), up = ups[0].resolve_neg().to(at::kFloat).contiguous();
+    const bool reduced = e.reduction != OW_REDUCE_NONE;
+    check_unpacked(plain_case(e));
+    const OwDistillation d = descriptor(e);
+    check_unpacked(plain(aux) && aux.scalar_type() == at::kFloat && aux.device() == e.logits.device() &&
+                   aux.numel() == 4 * d.rows + 1 + (reduced ? d.rows : 0) && plain(up) &&
+                   up.device() == e.logits.device() && up.numel() == (reduced ? 1 : d.rows));
+    Tensor grad = like(e.logits);
+    const float* stats = static_cast<const float*>(ptr(aux));
+    check(ow_distillation_bwd(&d, stats, reduced ? stats + 4 * d.rows : nullptr, static_cast<const float*>(ptr(up)),
+                              out_ptr(grad), stream_of(e.logits)),
+          "ow_distillation_bwd");
+    return once({std::move(grad), Tensor()});
+  }
+};
+
+// ---------------------------------------------------------------------------------------
 // The module
 
 // A tensor argument, undefined for None; false: it is neither.
@@ -432,6 +624,35 @@ PyObject* py_norms(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// layer_norm(x, weight, bias, eps) -> y or None
+PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  if (n_args != 4) {
+    PyErr_SetString(PyExc_TypeError, "layer_norm takes 4 arguments");
+    return nullptr;
+  }
+  LayerNorm n;
+  Tensor* tensors[3] = {&n.x, &n.weight, &n.bias};
+  bool grad = false;
+  for (int i = 0; i < 3; ++i) {
+    if (!as_tensor(args[i], tensors[i])) Py_RETURN_NONE;
+    grad |= tensors[i]->defined() && tensors[i]->requires_grad();
+  }
+  if (!as_double(args[3], &n.eps) || !plain_case(n)) Py_RETURN_NONE;
+  Tensor y;
+  {
+    pybind11::gil_scoped_release no_gil;
+    if (grad && at::GradMode::is_enabled()) {
+      y = LayerNormNode::apply(n.x, NormsNode::given(n.weight), NormsNode::given(n.bias), n.eps);
+    } else {
+      at::AutoDispatchBelowADInplaceOrView below;
+      y = run_layer_norm(n);
+    }
+  }
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
 // cross_entropy(logits, target, target_b, mix, mix_value, label_smoothing, ignore_index, reduction) -> loss or None
 PyObject* py_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
@@ -457,6 +678,35 @@ PyObject* py_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n_args) 
     } else {
       at::AutoDispatchBelowADInplaceOrView below;
       loss = run_xent(e).first;
+    }
+  }
+  return THPVariable_Wrap(loss);
+  END_HANDLE_TH_ERRORS
+}
+
+// distillation(logits, teacher_logits, teacher_indices, temperature, ignore_index, reduction) -> loss or None
+PyObject* py_distillation(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  if (n_args != 6) {
+    PyErr_SetString(PyExc_TypeError, "distillation takes 6 arguments");
+    return nullptr;
+  }
+  Distill e;
+  Tensor* tensors[3] = {&e.logits, &e.teacher, &e.indices};
+  for (int i = 0; i < 3; ++i)
+    if (!as_tensor(args[i], tensors[i])) Py_RETURN_NONE;
+  int64_t reduction = 0;
+  if (!as_double(args[3], &e.temperature) || !as_int(args[4], &e.ignore_index) || !as_int(args[5], &reduction)) Py_RETURN_NONE;
+  e.reduction = static_cast<int32_t>(reduction);
+  if (!plain_case(e)) Py_RETURN_NONE;
+  Tensor loss;
+  {
+    pybind11::gil_scoped_release no_gil;
+    if (e.logits.requires_grad() && at::GradMode::is_enabled()) {
+      loss = DistillNode::apply(e.logits, e);
+    } else {
+      at::AutoDispatchBelowADInplaceOrView below;
+      loss = run_distill(e).first;
     }
   }
   return THPVariable_Wrap(loss);
@@ -588,7 +838,9 @@ PyMethodDef kMethods[] = {
     {"state_layouts", py_state_layouts, METH_O, nullptr},
     {"gradients", py_gradients, METH_O, nullptr},
     {"norms", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_norms)), METH_FASTCALL, nullptr},
+    {"layer_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_layer_norm)), METH_FASTCALL, nullptr},
     {"cross_entropy", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_cross_entropy)), METH_FASTCALL, nullptr},
+    {"distillation", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_distillation)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -4,14 +4,15 @@
   ``out = x + scale * gate * norm(delta)`` and ``norm(out)``, each read and written once.
 * ``rms_norm_hip`` — the norm before a block alone (``bigemm`` takes pre-normalised activations,
   omniweave/ops/bigemm.py:24-36).
+* ``layer_norm_hip`` — layer norm of rows, with weight and bias (no counterpart in the reference).
 
-Both are differentiable.  The reference has the norm before the block, the LayerScale gate, the drop-path
+All are differentiable.  The reference has the norm before the block, the LayerScale gate, the drop-path
 scale and the residual as eager steps (omniweave/models/block.py:83-108) and no norm after the block;
 ``OmniWeaveBlock(post_norm=True)`` is the block that has one.  All sums are fp32 and each output is rounded
 once from fp32.
 
 A plain call is native, its autograd node included (``torch_glue.cpp``); the operator
-``omniwave_amd::block_norms_fwd`` takes the others (compilation, tracing, transforms, tensors to copy first).
+``omniwave_amd::block_norms_fwd`` or ``layer_norm_fwd`` takes the others (compilation, tracing, transforms, tensors to copy first).
 """
 
 from __future__ import annotations
@@ -268,3 +269,124 @@ def rms_norm_hip(x: Tensor, weight: Tensor, eps: float = 1e-6) -> Tensor:
     if weight is None:
         raise ValueError("rms_norm_hip needs a weight")
     return _norms(x, None, None, None, None, weight, eps)[1]
+
+
+# ---------------------------------------------------------------------------------------
+# Layer norm
+
+
+def _layer_norm_ready(x, weight, bias, eps) -> None:
+    """Raise for what the kernels do not take, before anything touches the GPU, and where they cannot run."""
+    if x.dtype not in SUPPORTED_DTYPES:
+        raise ValueError(f"unsupported dtype {x.dtype}; expected float16, bfloat16 or float32")
+    if x.dim() < 1:
+        raise ValueError("x must be [..., C], got a scalar")
+    c = x.shape[-1]
+    if c > MAX_CHANNELS:
+        raise ValueError(f"{c} channels; at most {MAX_CHANNELS} are supported")
+    if x.numel() and x.numel() // c >= 1 << 31:
+        raise ValueError(f"{x.numel() // c} rows; fewer than 2^31 are supported")
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError(f"eps must be finite and not negative, got {eps}")
+    for name, w in (("weight", weight), ("bias", bias)):
+        if w is not None and (w.shape != (c,) or w.dtype not in SUPPORTED_DTYPES or w.device != x.device):
+            raise ValueError(f"{name} must be float16, bfloat16 or float32 [{c}] on {x.device}, got {w.dtype} "
+                             f"{tuple(w.shape)} on {w.device}")
+    reason = gpu_reason(x)
+    if reason is not None:
+        raise RuntimeError(f"hip layer norm not supported: {reason}")
+
+
+def _layer_norm_descriptor(x, weight, bias, eps):
+    """The C descriptor and the tensors it points into."""
+    x, stride = _rows(x)
+    keep = [x, *[None if w is None else w.contiguous() for w in (weight, bias)]]
+    code = [0 if t is None else _DTYPE_CODE[t.dtype] for t in keep]
+    return _native.OwLayerNorm(x.numel() // x.shape[-1], stride, *[None if t is None else t.data_ptr() for t in keep],
+                               x.shape[-1], *code, eps), keep
+
+
+def _run_layer_norm_forward(x, weight, bias, eps) -> Tensor:
+    _layer_norm_ready(x, weight, bias, eps)  # the operator may be called by its name
+    y = _empty(x)
+    if x.numel():
+        desc, _keep = _layer_norm_descriptor(x, weight, bias, eps)
+        _on(x.device, _native.lib().ow_layer_norm_fwd, ctypes.byref(desc), y.data_ptr())
+    return y
+
+
+def _run_layer_norm_backward(dy, x, weight, bias, eps, want) -> list[Tensor | None]:
+    """Gradients of x, weight and bias where ``want`` asks for them and they exist."""
+    _layer_norm_ready(x, weight, bias, eps)  # hooks on saved tensors may hand out others
+    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
+        raise ValueError(f"the upstream gradient of {x.dtype} {tuple(x.shape)} on {x.device} is {dy.dtype} "
+                         f"{tuple(dy.shape)} on {dy.device}")
+    grads = [_empty(t) if w and t is not None else None for t, w in zip((x, weight, bias), want)]
+    if x.numel() == 0:
+        return [None if g is None else g.zero_() for g in grads]
+    ptr = [None if g is None else g.data_ptr() for g in grads]
+    desc, _keep = _layer_norm_descriptor(x, weight, bias, eps)
+    dy, dy_stride = _rows(dy)
+    lib, ws_bytes, workspace = _native.lib(), 0, None
+    if any(ptr[1:]):
+        with torch.cuda.device(x.device):  # the size goes by the device's compute units
+            ws_bytes = lib.ow_layer_norm_bwd_workspace(ctypes.byref(desc))
+        workspace = torch.empty(ws_bytes // 4, dtype=torch.float32, device=x.device) if ws_bytes else None
+    if any(ptr):
+        _on(x.device, lib.ow_layer_norm_bwd, ctypes.byref(desc), dy.data_ptr(), dy_stride, *ptr,
+            None if workspace is None else workspace.data_ptr(), ws_bytes)
+    return grads
+
+
+@torch.library.custom_op("omniwave_amd::layer_norm_fwd", mutates_args=())
+def layer_norm_fwd(x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float) -> Tensor:
+    """``layer_norm_hip``'s result."""
+    return _run_layer_norm_forward(x, weight, bias, eps)
+
+
+@layer_norm_fwd.register_fake
+def _layer_norm_fwd_fake(x, weight, bias, eps):
+    return x.new_empty(x.shape)
+
+
+@torch.library.custom_op("omniwave_amd::layer_norm_bwd", mutates_args=())
+def layer_norm_bwd(dy: Tensor, x: Tensor, weight: Tensor | None, bias: Tensor | None, eps: float,
+                   want: list[bool]) -> tuple[Tensor, Tensor, Tensor]:
+    """Gradients of x, weight and bias; empty where ``want`` is false."""
+    grads = _run_layer_norm_backward(dy, x, weight, bias, eps, want)
+    return tuple(x.new_empty(0) if g is None else g for g in grads)
+
+
+@layer_norm_bwd.register_fake
+def _layer_norm_bwd_fake(dy, x, weight, bias, eps, want):
+    return tuple(x.new_empty(0) if t is None or not w else t.new_empty(t.shape) for t, w in zip((x, weight, bias), want))
+
+
+def _layer_norm_setup_context(ctx, inputs, output):
+    *tensors, eps = inputs
+    ctx.save_for_backward(*tensors)
+    ctx.eps = float(eps)
+
+
+def _layer_norm_backward(ctx, dy):
+    want = [n and t is not None for n, t in zip(ctx.needs_input_grad, ctx.saved_tensors)]
+    grads = layer_norm_bwd(dy, *ctx.saved_tensors, ctx.eps, want)
+    return *[g if w else None for g, w in zip(grads, want)], None
+
+
+layer_norm_fwd.register_autograd(_layer_norm_backward, setup_context=_layer_norm_setup_context)
+
+
+def layer_norm_hip(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = None, eps: float = 1e-6) -> Tensor:
+    """``(x - mean) / sqrt(variance + eps) * weight + bias`` over the last dimension (``[..., C]``, C up to 8,192,
+    float16, bfloat16 or float32, rows at any one distance), rounded once from fp32.  ``weight`` and ``bias`` ``[C]``, each
+    may be left out and may have another dtype than ``x``.  Differentiable once in x, weight and bias."""
+    glue = _native.glue()
+    if glue is not None and _plain(x, weight, bias):
+        y = glue.layer_norm(x, weight, bias, eps)
+        if y is not None:
+            return y
+    # Everything else is checked, and goes through the operator.
+    eps = float(eps)
+    _layer_norm_ready(x, weight, bias, eps)
+    return layer_norm_fwd(x, weight, bias, eps)
