@@ -759,6 +759,34 @@ int ow_distillation_fwd(const OwDistillation* d, float* stats, float* losses, fl
 int ow_distillation_bwd(const OwDistillation* d, const float* stats, const float* weight, const float* upstream, void* grad,
                         void* stream);
 
+/*
+ * The gated feed-forward products of `rows` tokens (no counterpart in the reference, whose gated products stay inside a
+ * channel group): h = silu(x gate_weight^T) * (x up_weight^T), silu(g) = g / (1 + e^-g).
+ *
+ * x: rows of `channels` values of `dtype` (value stride 1, row stride in values, any alignment a value may have);
+ * weights [hidden][channels], contiguous, and h [rows][hidden], contiguous, all of `dtype`.  Products and gates are fp32;
+ * h is rounded once.  channels, hidden <= 2^20, rows < 2^31; channels >= 1 where anything is computed.
+ *
+ * The backward takes dh (row stride in values) and writes those of dx [rows][channels], dgate_weight and dup_weight that
+ * are not NULL, over ow_gated_linear_bwd_workspace bytes of workspace (16-byte aligned).  The gradients of the two
+ * projections are rounded to `dtype` in between; sums have a fixed order.  rows, channels, hidden >= 1 there.
+ */
+typedef struct OwGatedLinear {
+  int64_t rows;
+  int64_t x_stride;
+  const void* x;
+  const void* gate_weight;
+  const void* up_weight;
+  int32_t channels;
+  int32_t hidden;
+  int32_t dtype;
+} OwGatedLinear;
+
+int ow_gated_linear_fwd(const OwGatedLinear* d, void* h, void* stream);
+size_t ow_gated_linear_bwd_workspace(const OwGatedLinear* d);
+int ow_gated_linear_bwd(const OwGatedLinear* d, const void* dh, int64_t dh_stride, void* dx, void* dgate_weight,
+                        void* dup_weight, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,6 +9,7 @@ __version__ = "0.1.0"
 from omniwave_amd.bigemm import bigemm, register_backend
 from omniwave_amd.block import enable_fp8
 from omniwave_amd.distillation import distillation_hip
+from omniwave_amd.gated import gated_linear_hip
 from omniwave_amd.hip import bigemm_block_hip, bigemm_delta_hip, hip_is_supported
 from omniwave_amd.loss import cross_entropy_hip
 from omniwave_amd.norms import block_norms_hip, layer_norm_hip, rms_norm_hip
@@ -30,6 +31,7 @@ __all__ = [
     "cross_entropy_hip",
     "distillation_hip",
     "enable_fp8",
+    "gated_linear_hip",
     "hip_is_supported",
     "layer_norm_hip",
     "register_backend",

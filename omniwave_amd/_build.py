@@ -23,7 +23,7 @@ CSRC = PKG_DIR / "csrc"
 INCLUDE = REPO_DIR / "include"
 LIB_PATH = PKG_DIR / "libomniwave_amd.so"
 SOURCES = ["route.cpp", "bigemm_fwd.hip", "bigemm_fwd_resident.hip", "bigemm_fwd_wave16.hip", "bigemm_fwd_persist.hip", "bigemm_fwd_split.hip", "bigemm_fwd_f32.hip", "bigemm_fwd_x3.hip", "bigemm_bwd.hip", "bigemm_bwd_f32.hip", "bigemm_bwd_x3.hip", "bwd_block.hip", "stem.hip", "fwd_noalloc.hip",
-           "block_norms.hip", "layer_norm.hip", "adamw.hip", "cross_entropy.hip", "distillation.hip"]
+           "block_norms.hip", "layer_norm.hip", "adamw.hip", "cross_entropy.hip", "distillation.hip", "gated_linear.hip", "gated_linear_bwd.hip"]
 GLUE_PATH = PKG_DIR / "_glue.so"
 GLUE_SOURCE = "torch_glue.cpp"
 ARCH = "gfx950"

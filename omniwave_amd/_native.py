@@ -85,6 +85,12 @@ class OwDistillation(ctypes.Structure):
     _fields_ += [("temperature", ctypes.c_float)]
 
 
+class OwGatedLinear(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("x_stride", ctypes.c_int64)]
+    _fields_ += [(name, ctypes.c_void_p) for name in ("x", "gate_weight", "up_weight")]
+    _fields_ += [(name, ctypes.c_int32) for name in ("channels", "hidden", "dtype")]
+
+
 OW_REDUCE = {"none": 0, "sum": 1, "mean": 2}
 OW_ADAMW_CHUNK, OW_ADAMW_BLOCK = 4096, 256
 
@@ -323,6 +329,13 @@ _SIGNATURES = {
         ctypes.c_int, [ctypes.POINTER(OwDistillation)] + [ctypes.c_void_p] * 5 + [ctypes.c_size_t, ctypes.c_void_p],
     ),
     "ow_distillation_bwd": (ctypes.c_int, [ctypes.POINTER(OwDistillation)] + [ctypes.c_void_p] * 5),
+    "ow_gated_linear_fwd": (ctypes.c_int, [ctypes.POINTER(OwGatedLinear)] + [ctypes.c_void_p] * 2),
+    "ow_gated_linear_bwd_workspace": (ctypes.c_size_t, [ctypes.POINTER(OwGatedLinear)]),
+    "ow_gated_linear_bwd": (
+        ctypes.c_int,
+        [ctypes.POINTER(OwGatedLinear), ctypes.c_void_p, ctypes.c_int64] + [ctypes.c_void_p] * 4
+        + [ctypes.c_size_t, ctypes.c_void_p],
+    ),
     "ow_bwd_params": (
         ctypes.c_int,
         [ctypes.c_void_p] * 3 + [ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]

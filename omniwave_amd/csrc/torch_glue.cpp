@@ -560,6 +560,94 @@ class DistillNode : public torch::autograd::Function<DistillNode> {
 };
 
 // ---------------------------------------------------------------------------------------
+// Gated feed-forward product
+
+struct Gated {
+  Tensor x, gate, up;
+};
+
+constexpr int64_t kMaxWidth = 1 << 20;  // channels, hidden
+
+OwGatedLinear descriptor(const Gated& g) {
+  OwGatedLinear d{};
+  d.channels = static_cast<int32_t>(g.x.size(-1));
+  d.rows = g.x.numel() / d.channels;
+  d.x_stride = row_stride(g.x);
+  d.x = ptr(g.x);
+  d.gate_weight = ptr(g.gate);
+  d.up_weight = ptr(g.up);
+  d.hidden = static_cast<int32_t>(g.gate.size(0));
+  d.dtype = dtype_code(g.x);
+  return d;
+}
+
+bool plain_case(const Gated& g) {
+  const Tensor& x = g.x;
+  if (!x.defined() || !g.gate.defined() || !g.up.defined()) return false;
+  if (!plain(x) || x.dim() < 1 || x.numel() == 0 || !device_ok(x) || row_stride(x) < 0) return false;
+  const int64_t c = x.size(-1);
+  if (c > kMaxWidth || x.numel() / c >= (int64_t(1) << 31)) return false;
+  for (const Tensor* w : {&g.gate, &g.up})
+    if (!plain(*w) || w->scalar_type() != x.scalar_type() || w->device() != x.device() || w->dim() != 2 || w->size(1) != c ||
+        w->size(0) != g.gate.size(0) || w->size(0) < 1 || w->size(0) > kMaxWidth || !w->is_contiguous())
+      return false;
+  return true;
+}
+
+std::vector<int64_t> hidden_shape(const Gated& g) {
+  std::vector<int64_t> shape = g.x.sizes().vec();
+  shape.back() = g.gate.size(0);
+  return shape;
+}
+
+Tensor run_gated(const Gated& g) {
+  const c10::DeviceGuard guard(g.x.device());
+  Tensor h = at::empty(hidden_shape(g), g.x.options());
+  const OwGatedLinear d = descriptor(g);
+  check(ow_gated_linear_fwd(&d, out_ptr(h), stream_of(g.x)), "ow_gated_linear_fwd");
+  return h;
+}
+
+class GatedNode : public torch::autograd::Function<GatedNode> {
+ public:
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& gate, const Tensor& up) {
+    ctx->save_for_backward({x, gate, up});
+    ctx->set_materialize_grads(false);
+    return run_gated(Gated{x, gate, up});
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list ups) {
+    if (!ups[0].defined()) return variable_list(3);
+    const variable_list s = ctx->get_saved_variables();
+    Gated g{s[0], s[1], s[2]};
+    check_unpacked(g.x.is_cuda());
+    const c10::DeviceGuard guard(g.x.device());
+    int64_t unused = 0, dh_stride = 0;  // hooks on saved tensors may hand out copies that lie otherwise
+    g.x = rows_of(g.x, &unused);
+    g.gate = g.gate.contiguous();
+    g.up = g.up.contiguous();
+    Tensor dh = ups[0].resolve_neg();
+    check_unpacked(plain_case(g) && plain(dh) && dh.sizes() == at::IntArrayRef(hidden_shape(g)) &&
+                   dh.scalar_type() == g.x.scalar_type() && dh.device() == g.x.device());
+    dh = rows_of(dh, &dh_stride);
+    const Tensor* inputs[3] = {&g.x, &g.gate, &g.up};
+    Tensor grads[3];
+    bool any = false;
+    for (size_t i = 0; i < 3; ++i)
+      if (ctx->needs_input_grad(i)) grads[i] = like(*inputs[i]), any = true;
+    if (any) {
+      const OwGatedLinear d = descriptor(g);
+      const size_t bytes = ow_gated_linear_bwd_workspace(&d);
+      const Tensor workspace = at::empty({static_cast<int64_t>(bytes)}, g.x.options().dtype(at::kByte));
+      check(ow_gated_linear_bwd(&d, ptr(dh), dh_stride, out_ptr(grads[0]), out_ptr(grads[1]), out_ptr(grads[2]),
+                                out_ptr(workspace), bytes, stream_of(g.x)),
+            "ow_gated_linear_bwd");
+    }
+    return once({grads[0], grads[1], grads[2]});
+  }
+};
+
+// ---------------------------------------------------------------------------------------
 // The module
 
 // A tensor argument, undefined for None; false: it is neither.
@@ -713,6 +801,35 @@ PyObject* py_distillation(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// gated_linear(x, gate_weight, up_weight) -> h or None
+PyObject* py_gated_linear(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  if (n_args != 3) {
+    PyErr_SetString(PyExc_TypeError, "gated_linear takes 3 arguments");
+    return nullptr;
+  }
+  Gated g;
+  Tensor* tensors[3] = {&g.x, &g.gate, &g.up};
+  bool grad = false;
+  for (int i = 0; i < 3; ++i) {
+    if (!as_tensor(args[i], tensors[i])) Py_RETURN_NONE;
+    grad |= tensors[i]->defined() && tensors[i]->requires_grad();
+  }
+  if (!plain_case(g)) Py_RETURN_NONE;
+  Tensor h;
+  {
+    pybind11::gil_scoped_release no_gil;
+    if (grad && at::GradMode::is_enabled()) {
+      h = GatedNode::apply(g.x, g.gate, g.up);
+    } else {
+      at::AutoDispatchBelowADInplaceOrView below;
+      h = run_gated(g);
+    }
+  }
+  return THPVariable_Wrap(h);
+  END_HANDLE_TH_ERRORS
+}
+
 // Numbers (addresses of tensors and what lies there) as bytes, 8 each, to be compared as a whole.
 class Numbers {
  public:
@@ -841,6 +958,7 @@ PyMethodDef kMethods[] = {
     {"layer_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_layer_norm)), METH_FASTCALL, nullptr},
     {"cross_entropy", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_cross_entropy)), METH_FASTCALL, nullptr},
     {"distillation", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_distillation)), METH_FASTCALL, nullptr},
+    {"gated_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_gated_linear)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 
