@@ -7,13 +7,14 @@
 //   dx = r (h - mean_c h - n mean_c(n h))    dweight = sum_rows g n    dbias = sum_rows g
 //
 // Both directions read every tensor once and are bound by memory; the backward forms mu and r again from x,
-// which it reads anyway, so the forward stores no statistics.  The variance is that of the differences from the mean,
-// which the row's registers still hold: a mean far above the deviations costs no digits.  All sums and intermediates are
-// fp32 and each stored value is rounded once.
+// which it reads anyway, so the forward stores no statistics.  Differences are taken from the rounded mean, and their own
+// mean is taken off again with the variance: a mean far above the deviations costs no digits (a row of one large
+// value times the rounded 1 / C would seem to vary).  All sums and intermediates are fp32 and each stored value is
+// rounded once.
 //
 // Rows lie in registers, T threads a row, as in block_norms.hip (Place, ow_rows.h); a row shorter than 8 vectors
-// takes as few threads as hold it.  Each round of sums over a row is two sums at once: backward, the mean of x with
-// that of h, then the variance with the sum of h (x - mu).
+// takes as few threads as hold it.  A row takes two rounds of sums: the mean of x (backward: with that of h), then the
+// differences, their squares (and their products with h).
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -44,6 +45,12 @@ constexpr int kWantWeight = 1, kWantBias = 2;
 // many workgroups as run at once.
 constexpr int fwd_waves(int t) { return t == 1024 ? 4 : 8; }
 constexpr int bwd_waves(int t) { return 4; }
+
+// The inverse root of the variance of values whose mean is `off` and whose mean square is `square`.
+__device__ __forceinline__ float inverse_root(float square, float off, float eps) {
+  const float variance = square - off * off;
+  return rsqrtf((variance < 0.f ? 0.f : variance) + eps);  // a NaN stays one
+}
 
 template <class Ty, int T, int K, bool RAGGED>
 __global__ void __launch_bounds__(kThreads<T>, fwd_waves(T)) layer_norm_fwd_kernel(LayerNormArgs a) {
@@ -84,21 +91,23 @@ __global__ void __launch_bounds__(kThreads<T>, fwd_waves(T)) layer_norm_fwd_kern
       for (int j = 0; j < V; ++j) sum[0] += counted<RAGGED>(x[k][j], mask[k][j]);
     row_sums<T>(sum, red, turn);
     const float mean = sum[0] * a.inv_c;
-    float ss[1] = {0.f};
+    float s2[2] = {0.f, 0.f};  // x - mean, its square
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         x[k][j] -= mean;
         const float w = at.col[k] < 0 ? 0.f : counted<RAGGED>(x[k][j], mask[k][j]);
-        ss[0] += w * w;
+        s2[0] += w;
+        s2[1] += w * w;
       }
-    row_sums<T>(ss, red, turn);
-    const float r = rsqrtf(ss[0] * a.inv_c + a.n.eps);
+    row_sums<T>(s2, red, turn);
+    const float off = s2[0] * a.inv_c;
+    const float r = inverse_root(s2[1] * a.inv_c, off, a.n.eps);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[k][j] = x[k][j] * r * weight[k][j] + bias[k][j];
+      for (int j = 0; j < V; ++j) x[k][j] = (x[k][j] - off) * r * weight[k][j] + bias[k][j];
       at.store(static_cast<Elem*>(a.y) + row * c, k, row < a.n.rows, x[k]);
     }
   }
@@ -163,23 +172,26 @@ __global__ void __launch_bounds__(kThreads<T>, bwd_waves(T)) layer_norm_bwd_kern
       }
     row_sums<T>(s1, red, turn);
     const float mean = s1[0] * a.inv_c, mean_h = s1[1] * a.inv_c;
-    float s2[2] = {0.f, 0.f};  // (x - mu)^2, h (x - mu)
+    float s2[3] = {0.f, 0.f, 0.f};  // x - mean, its square, its product with h
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         x[k][j] -= mean;
         const float w = at.col[k] < 0 ? 0.f : counted<RAGGED>(x[k][j], mask[k][j]);
-        s2[0] += w * w;
-        s2[1] += w * counted<RAGGED>(g[k][j] * weight[k][j], mask[k][j]);
+        s2[0] += w;
+        s2[1] += w * w;
+        s2[2] += w * counted<RAGGED>(g[k][j] * weight[k][j], mask[k][j]);
       }
     row_sums<T>(s2, red, turn);
-    const float r = valid ? rsqrtf(s2[0] * a.inv_c + a.n.eps) : 0.f;  // no row adds nothing, also where eps is 0
-    const float back = r * r * (s2[1] * a.inv_c);
+    const float off = s2[0] * a.inv_c;
+    const float r = valid ? inverse_root(s2[1] * a.inv_c, off, a.n.eps) : 0.f;  // no row adds nothing, also where eps is 0
+    const float back = r * r * (s2[2] * a.inv_c - off * mean_h);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
+        x[k][j] -= off;
         s_weight[k][j] += g[k][j] * (x[k][j] * r);
         s_bias[k][j] += g[k][j];
         x[k][j] = r * (g[k][j] * weight[k][j] - mean_h - x[k][j] * back);

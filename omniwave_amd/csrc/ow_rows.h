@@ -134,7 +134,7 @@ __device__ __forceinline__ V lanes_reduce(V v) {
 // [2][kRowSums * waves of the workgroup]; `turn` picks the half, so that one barrier a call suffices:
 // a half is written again only after the barrier of the call between).  Every thread of the workgroup
 // calls it.
-constexpr int kRowSums = 2;
+constexpr int kRowSums = 3;
 template <int T, int N>
 __device__ __forceinline__ void row_sums(float (&v)[N], float* red, int& turn) {
 #pragma unroll
