@@ -16,6 +16,7 @@ import torch.nn.functional as F
 from torch import Tensor
 
 from omniwave_amd.block import RMS_EPS, OmniWeaveBlock
+from omniwave_amd.feed_forward import GatedFeedForward
 from omniwave_amd.hip import stem_hip, stem_is_supported
 from omniwave_amd.norms import rms_norm_hip
 from omniwave_amd.routing import build_stage_schedule
@@ -35,7 +36,7 @@ class _Stage(nn.Module):
     """Optional anchor Linear, then blocks on the stage schedule (backbone.py:30-80)."""
 
     def __init__(self, height, width, dim, depth, channel_tile, expansion, layer_scale_init, spatial_tile,
-                 use_anchor, backend, drop_path_rates, post_norm=False) -> None:
+                 use_anchor, backend, drop_path_rates, post_norm=False, feed_forward=0.0) -> None:
         super().__init__()
         self.anchor: nn.Linear | None = nn.Linear(dim, dim, bias=False) if use_anchor else None
         self.blocks = nn.ModuleList()
@@ -45,15 +46,24 @@ class _Stage(nn.Module):
                 radix_level=radix_level, expansion=expansion, layer_scale_init=layer_scale_init,
                 spatial_tile=spatial_tile, backend=backend, drop_path_rate=rate, post_norm=post_norm,
             ))
+        # Behind the blocks, where asked for.
+        self.feed_forward: GatedFeedForward | None = (
+            GatedFeedForward(dim, max(1, round(dim * feed_forward)), layer_scale_init, backend) if feed_forward else None)
 
     def forward(self, x: Tensor) -> Tensor:
         if self.anchor is not None:
             x = self.anchor(x)
+        return self._end(self._forward_plain(x))
+
+    def _forward_plain(self, x: Tensor) -> Tensor:
         if self._takes_normed(x):
             return self._forward_normed(x)
         for block in self.blocks:
             x = block(x)
         return x
+
+    def _end(self, x: Tensor) -> Tensor:
+        return x if self.feed_forward is None else self.feed_forward(x)
 
     def _takes_normed(self, x: Tensor) -> bool:
         # A block may have been wrapped, and is then called like any module.
@@ -72,6 +82,8 @@ class _Stage(nn.Module):
         """``space_to_depth`` of the blocks' output (the anchor is the caller's); the last block
         writes that layout itself when it can, and each block hands the next its RMSNorm
         statistics when it can (``OmniWeaveBlock.forward_chain``)."""
+        if self.feed_forward is not None:
+            return space_to_depth_nhwc(self.forward_blocks(x), factor)
         if self._takes_normed(x):
             return space_to_depth_nhwc(self._forward_normed(x), factor)
         x, stats = self._chain(self.blocks[:-1], x)
@@ -82,10 +94,11 @@ class _Stage(nn.Module):
         return y if y is not None else space_to_depth_nhwc(self.blocks[-1](x), factor)
 
     def forward_blocks(self, x: Tensor) -> Tensor:
-        """The blocks (the anchor is the caller's), chained as in ``forward_blocks_s2d``."""
+        """The blocks and what follows them in the stage (the anchor is the caller's), chained as in
+        ``forward_blocks_s2d``."""
         if self._takes_normed(x):
-            return self._forward_normed(x)
-        return self._chain(self.blocks, x)[0]
+            return self._end(self._forward_normed(x))
+        return self._end(self._chain(self.blocks, x)[0])
 
     @staticmethod
     def _chain(blocks, x: Tensor) -> tuple[Tensor, Tensor | None]:
@@ -101,7 +114,8 @@ class _Stage(nn.Module):
 
 class OmniWeaveBackbone(nn.Module):
     """Input ``[B, 3, H, W]`` (NCHW) -> logits ``[B, num_classes]``.  ``post_norm``: every block also
-    normalises what it adds (``OmniWeaveBlock``)."""
+    normalises what it adds (``OmniWeaveBlock``).  ``feed_forward`` above 0: every stage ends with a
+    ``GatedFeedForward`` over that many times its width."""
 
     def __init__(
         self,
@@ -117,6 +131,7 @@ class OmniWeaveBackbone(nn.Module):
         input_size: int = 224,
         drop_path_rate: float = 0.0,
         post_norm: bool = False,
+        feed_forward: float = 0.0,
     ) -> None:
         super().__init__()
         widths = widths or [128, 256, 512, 1024]
@@ -128,6 +143,8 @@ class OmniWeaveBackbone(nn.Module):
             raise ValueError("widths, depths, and channel_tiles must each have length 4")
         if not 0.0 <= drop_path_rate < 1.0:
             raise ValueError("drop_path_rate must be in [0, 1)")
+        if not 0.0 <= feed_forward <= 64.0:
+            raise ValueError(f"feed_forward must be in [0, 64], got {feed_forward}")
         self.stem_proj = nn.Linear(3 * 4 * 4, widths[0], bias=False)
         res0 = input_size // 4
         resolutions = [res0 // (2 ** i) for i in range(4)]
@@ -143,7 +160,7 @@ class OmniWeaveBackbone(nn.Module):
                 height=resolutions[i], width=resolutions[i], dim=widths[i], depth=depths[i],
                 channel_tile=channel_tiles[i], expansion=expansion, layer_scale_init=layer_scale_init,
                 spatial_tile=spatial_tile, use_anchor=(i + 1) in anchor_stages, backend=backend,
-                drop_path_rates=rates[offset:offset + depths[i]], post_norm=post_norm,
+                drop_path_rates=rates[offset:offset + depths[i]], post_norm=post_norm, feed_forward=feed_forward,
             ))
             offset += depths[i]
         self.head = nn.Linear(widths[-1], num_classes)

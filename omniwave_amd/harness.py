@@ -250,13 +250,19 @@ def run_model_benchmark(config: dict[str, Any], device: torch.device) -> list[di
 class TrainingStep:
     """One training step of a model as the framework runs it: ``step(images, labels)`` returns the loss.
 
-    ``labels_b`` / ``mix``: the second labels and the weight of the first ones of mixed images."""
+    ``labels_b`` / ``mix``: the second labels and the weight of the first ones of mixed images.  ``teacher``: a teacher's top
+    logits and their classes for each image (``distillation_hip``), whose loss at ``temperature`` enters with the weight
+    ``distill_weight`` beside the labels' loss of the rest."""
 
     def __init__(self, model: nn.Module, *, lr: float = 1e-3, weight_decay: float = 0.05, state_bits: int = 32,
-                 master_weights: bool = True, max_grad_norm: float | None = 1.0, label_smoothing: float = 0.1) -> None:
+                 master_weights: bool = True, max_grad_norm: float | None = 1.0, label_smoothing: float = 0.1,
+                 distill_weight: float = 0.5, temperature: float = 1.0) -> None:
         from omniwave_amd.optim import AdamW
 
+        if not 0.0 <= distill_weight <= 1.0:
+            raise ValueError(f"distill_weight must be in [0, 1], got {distill_weight}")
         self.model, self.label_smoothing = model, label_smoothing
+        self.distill_weight, self.temperature = distill_weight, temperature
         matrices = [p for p in model.parameters() if p.requires_grad and p.dim() >= 2]
         vectors = [p for p in model.parameters() if p.requires_grad and p.dim() < 2]
         groups = [{"params": matrices, "weight_decay": weight_decay}, {"params": vectors, "weight_decay": 0.0}]
@@ -264,12 +270,17 @@ class TrainingStep:
                                master_weights=master_weights, max_grad_norm=max_grad_norm)
 
     def step(self, images: torch.Tensor, labels: torch.Tensor, labels_b: torch.Tensor | None = None,
-             mix: torch.Tensor | float | None = None) -> torch.Tensor:
+             mix: torch.Tensor | float | None = None,
+             teacher: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
+        from omniwave_amd.distillation import distillation_hip
         from omniwave_amd.loss import cross_entropy_hip
 
         self.optimizer.zero_grad(set_to_none=True)
-        loss = cross_entropy_hip(self.model(images), labels, target_b=labels_b, mix=mix,
-                                 label_smoothing=self.label_smoothing)
+        logits = self.model(images)
+        loss = cross_entropy_hip(logits, labels, target_b=labels_b, mix=mix, label_smoothing=self.label_smoothing)
+        if teacher is not None:
+            taught = distillation_hip(logits, *teacher, temperature=self.temperature)
+            loss = loss * (1.0 - self.distill_weight) + taught * self.distill_weight
         loss.backward()
         self.optimizer.step()
         return loss.detach()
@@ -277,7 +288,8 @@ class TrainingStep:
 
 def run_training_benchmark(config: dict[str, Any], device: torch.device) -> list[dict[str, Any]]:
     """Rows of training steps: ``models`` x ``resolutions`` x ``train_dtypes`` x ``train_batch_sizes``, with
-    ``training`` (``TrainingStep``'s options) and ``model_options`` (the model's)."""
+    ``training`` (``TrainingStep``'s options), ``model_options`` (the model's) and ``train_teacher_top`` (entries of a
+    teacher's list for each image; 0: no teacher)."""
     from omniwave_amd.registry import create_model
 
     rows: list[dict[str, Any]] = []
@@ -294,8 +306,11 @@ def run_training_benchmark(config: dict[str, Any], device: torch.device) -> list
                         training = TrainingStep(model, **config.get("training", {}))
                         images = torch.randn(batch, 3, resolution, resolution, device=device).to(dtype)
                         labels = torch.randint(0, model.head.out_features, (batch,), device=device)
+                        teacher, top = None, int(config.get("train_teacher_top", 0))
+                        if top:
+                            teacher = torch.randn(batch, model.head.out_features, device=device).topk(top, 1)
                         losses = []
-                        res = benchmark_fn(lambda: losses.append(training.step(images, labels)),
+                        res = benchmark_fn(lambda: losses.append(training.step(images, labels, teacher=teacher)),
                                            warmup=config.get("warmup", 100), iterations=config.get("iterations", 1000))
                         if not torch.isfinite(losses[-1]):
                             raise RuntimeError("the training step's loss is not finite")
