@@ -141,9 +141,9 @@ GatedArgs gated_args(const OwGatedLinear& d) {
   return a;
 }
 
-// Whether x, or both weights, lie in whole pieces of 16 bytes; offsets inside a copy of 8 rows have 31 bits.
+// Whether x, or both weights, lie in whole pieces of 16 bytes; offsets inside a tile of 256 rows have 31 bits.
 bool gated_x_direct(const GatedArgs& a, int64_t size) {
-  return reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_ld % 16 == 0 && a.x_ld >= 0 && a.x_ld < (int64_t(1) << 27) &&
+  return reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_ld % 16 == 0 && a.x_ld >= 0 && a.x_ld < (int64_t(1) << 22) &&
          a.channels * size % 16 == 0;
 }
 bool gated_w_direct(const GatedArgs& a, int64_t size) {

@@ -61,12 +61,12 @@ typedef Tile<2, 2, 1, 2> TileS;  // 64 x 128
 // Element types: K values of a 128-byte row, values of a 16-byte piece, one step's product.
 template <class Ty>
 struct Elem {  // BF16, F16
-  static constexpr int kSize = 2, kPiece = 8, kTile = 64;
+  static constexpr int kSize = 2, kPiece = 8, kTile = 64, kProducts = 1;
   static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) { return Ty::mma32(a, b, c); }
 };
 template <>
 struct Elem<F32> {
-  static constexpr int kSize = 4, kPiece = 4, kTile = 32;
+  static constexpr int kSize = 4, kPiece = 4, kTile = 32, kProducts = 4;
   static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -90,51 +90,64 @@ __device__ __forceinline__ u32x4 load_piece(const char* p, int64_t n) {
   return w;
 }
 
-__device__ __forceinline__ const char* uniform_bytes(const char* p) {
-  return reinterpret_cast<const char*>(uniform_ptr(reinterpret_cast<const uint16_t*>(p)));
+// A lane's pieces of an operand on their way to LDS.  DIRECT: `off` is each one's offset from the tile's base, kOffOut where
+// its index is outside the matrix; else offsets of any size, and what has been loaded.
+template <int COPIES, bool DIRECT>
+struct Pieces {
+  uint32_t off[COPIES];
+};
+template <int COPIES>
+struct Pieces<COPIES, false> {
+  int64_t off[COPIES];
+  int left[COPIES];  // values that are in the matrix
+  u32x4 held[COPIES];
+};
+__device__ __forceinline__ void put_piece(uint32_t lds, int lane, u32x4 v) {
+  *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(static_cast<uintptr_t>(lds + 16 * lane)) = v;
 }
 
-// One 16-byte piece of a lane on its way to LDS.
-template <int SIZE, bool DIRECT>
-struct Piece {
-  u32x4 held;
-  // base: uniform; voff: the lane's offset; n: its values that are in the matrix.
-  __device__ __forceinline__ void fetch(const char* base, int64_t voff, int64_t n, uint32_t lds) {
-    if constexpr (DIRECT) {
-      tile_copy(buffer_rsrc(uniform_bytes(base), 0x7fffffffu), n > 0 ? static_cast<uint32_t>(voff) : kOffOut, lds);
-    } else {
-      held = load_piece<SIZE>(base + voff, n);
-    }
-  }
-  __device__ __forceinline__ void put(uint32_t lds, int lane) const {
-    if constexpr (!DIRECT)
-      *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(static_cast<uintptr_t>(lds + 16 * lane)) = held;
-  }
-};
-
-// A tile of N output indexes, 128 bytes of k each: 1 KB (8 rows) an instruction.
-template <int N, int WAVES, int SIZE, bool DIRECT>
+// A tile of N output indexes, 128 bytes of k each: 1 KB (8 rows) an instruction.  PAIR: 32 of one matrix and 32 of the
+// other in turn.
+template <int N, int WAVES, int SIZE, bool DIRECT, bool PAIR>
 struct AlongK {
-  static constexpr int kCopies = N / 8 / WAVES;
-  Piece<SIZE, DIRECT> piece[kCopies];
-  static_assert(kCopies * 8 * WAVES == N, "whole copies");
-  // row(q, &rows): the first of rows q .. q + 7 at k = 0, and how many of them there are.
-  template <class Rows>
-  __device__ __forceinline__ void fetch(Rows row, int64_t ld, int64_t k0, int64_t k_end, uint32_t lds, int wave, int lane) {
-    constexpr int V = 16 / SIZE;
-    const int r = lane >> 3, p = (lane & 7) ^ r;
-    const int64_t n = k_end - (k0 + p * V);
+  static constexpr int kCopies = N / 8 / WAVES, kReads = 1, V = 16 / SIZE;
+  static_assert(kCopies * 8 * WAVES == N && (!PAIR || 32 % (8 * WAVES) == 0 || 8 * WAVES == 64), "whole copies of one matrix");
+  Pieces<kCopies, DIRECT> at;
+  int piece;  // of a row
+  static __device__ __forceinline__ int part(int i, int wave) { return PAIR ? ((8 * (i * WAVES + wave)) >> 5) & 1 : 0; }
+  // extent: indexes from the tile's first one on.
+  __device__ __forceinline__ void init(int64_t extent, int64_t ld, int wave, int lane) {
+    piece = (lane & 7) ^ (lane >> 3);
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) {
-      const int q = 8 * (i * WAVES + wave);
-      int64_t there;
-      const char* base = row(q, &there) + k0 * SIZE;
-      piece[i].fetch(base, r * ld + p * 16, r < there ? n : 0, lds + q * 128);
+      const int q = 8 * (i * WAVES + wave), index = (PAIR ? (q >> 6) * 32 + (q & 31) : q) + (lane >> 3);
+      if constexpr (DIRECT) {
+        at.off[i] = index < extent ? static_cast<uint32_t>(index * ld) + piece * 16 : kOffOut;
+      } else {
+        at.off[i] = index * ld + piece * 16;
+        at.left[i] = index < extent;
+      }
+    }
+  }
+  // base: the tile's first index of each matrix at the tile's k; k_left: values of k that are there, up to a tile's.
+  __device__ __forceinline__ void fetch(const char* base, const char* other, int k_left, uint32_t lds, int wave) {
+    if constexpr (DIRECT) {
+      const auto r0 = buffer_rsrc(base, 0x7fffffffu), r1 = buffer_rsrc(PAIR ? other : base, 0x7fffffffu);
+      const bool there = piece * V < k_left;
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i)
+        tile_copy(part(i, wave) ? r1 : r0, there ? at.off[i] : kOffOut, lds + 8 * (i * WAVES + wave) * 128);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i)
+        at.held[i] = load_piece<SIZE>((part(i, wave) ? other : base) + at.off[i], at.left[i] ? k_left - piece * V : 0);
     }
   }
   __device__ __forceinline__ void put(uint32_t lds, int wave, int lane) const {
+    if constexpr (!DIRECT) {
 #pragma unroll
-    for (int i = 0; i < kCopies; ++i) piece[i].put(lds + 8 * (i * WAVES + wave) * 128, lane);
+      for (int i = 0; i < kCopies; ++i) put_piece(lds + 8 * (i * WAVES + wave) * 128, lane, at.held[i]);
+    }
   }
   template <class Ty>
   static __device__ __forceinline__ u32x4 read(uint32_t lds, int first, int step, int lane) {
@@ -149,28 +162,45 @@ template <int N, int WAVES, int SIZE, bool DIRECT>
 struct AcrossK {
   static constexpr int kRow = N * SIZE, kPieces = kRow / 16;   // of a k
   static constexpr int kRowsOfCopy = 64 / kPieces > 0 ? 64 / kPieces : 1;
-  static constexpr int kCopies = N / 8 / WAVES;
+  static constexpr int kCopies = N / 8 / WAVES, kReads = SIZE, V = 16 / SIZE;
   static_assert(kRow <= 1024 && kCopies * 8 * WAVES == N, "whole copies");
-  Piece<SIZE, DIRECT> piece[kCopies];
+  Pieces<kCopies, DIRECT> at;
+  int in;  // the lane's k of a copy
   static constexpr int kPairs = kPieces / 2 < 8 ? kPieces / 2 : 8;
   static __device__ __forceinline__ int slot(int p, int k) {
     if constexpr (SIZE == 2) return p ^ ((k & (kPairs - 1)) << 1);
     else return p ^ ((k & 4) << 1);
   }
-  // at: the first output index at k = 0; n_out: output indexes from there on.
-  __device__ __forceinline__ void fetch(const char* at, int64_t ld, int64_t n_out, int64_t k0, int64_t k_end, uint32_t lds, int wave,
-                                        int lane) {
-    constexpr int V = 16 / SIZE;
+  // n_out: output indexes from the tile's first one on.
+  __device__ __forceinline__ void init(int64_t n_out, int64_t ld, int wave, int lane) {
+    in = lane / kPieces;
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) {
-      const int copy = i * WAVES + wave, first = copy * kRowsOfCopy;
-      const int in = lane / kPieces, k = first + in, p = slot(lane % kPieces, k);
-      piece[i].fetch(at + (k0 + first) * ld, in * ld + p * 16, k0 + k < k_end ? n_out - p * V : 0, lds + copy * 1024);
+      const int k = (i * WAVES + wave) * kRowsOfCopy + in, p = slot(lane % kPieces, k);
+      if constexpr (DIRECT) {
+        at.off[i] = p * V < n_out ? static_cast<uint32_t>(k * ld) + p * 16 : kOffOut;
+      } else {
+        at.off[i] = k * ld + p * 16;
+        at.left[i] = n_out - p * V < V ? static_cast<int>(n_out - p * V) : V;
+      }
+    }
+  }
+  // base: the first output index at the tile's k; k_left: values of k that are there, up to a tile's.
+  __device__ __forceinline__ void fetch(const char* base, int k_left, uint32_t lds, int wave) {
+    const auto r = buffer_rsrc(base, 0x7fffffffu);
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const int copy = i * WAVES + wave;
+      const bool there = in < k_left - copy * kRowsOfCopy;
+      if constexpr (DIRECT) tile_copy(r, there ? at.off[i] : kOffOut, lds + copy * 1024);
+      else at.held[i] = load_piece<SIZE>(base + at.off[i], there ? at.left[i] : 0);
     }
   }
   __device__ __forceinline__ void put(uint32_t lds, int wave, int lane) const {
+    if constexpr (!DIRECT) {
 #pragma unroll
-    for (int i = 0; i < kCopies; ++i) piece[i].put(lds + (i * WAVES + wave) * 1024, lane);
+      for (int i = 0; i < kCopies; ++i) put_piece(lds + (i * WAVES + wave) * 1024, lane, at.held[i]);
+    }
   }
   template <class Ty>
   static __device__ __forceinline__ u32x4 read(uint32_t lds, int first, int step, int lane) {
@@ -277,8 +307,8 @@ __global__ void __launch_bounds__(T::kThreads, 2) gated_tile_kernel(GatedArgs a)
   constexpr int S = Elem<Ty>::kSize, KT = Elem<Ty>::kTile, W = T::kWaves;
   constexpr bool kPair = MODE == kGatedForward || MODE == kGatedGates;  // columns: 32 of the gate, 32 of the other
   constexpr int kCols = kPair ? T::BC / 2 : T::BC;                      // output columns of a tile
-  typedef typename std::conditional<MODE == kGatedDw, AcrossK<T::BR, W, S, DIRECT>, AlongK<T::BR, W, S, DIRECT>>::type OpR;
-  typedef typename std::conditional<kPair, AlongK<T::BC, W, S, DIRECT>, AcrossK<T::BC, W, S, DIRECT>>::type OpC;
+  typedef typename std::conditional<MODE == kGatedDw, AcrossK<T::BR, W, S, DIRECT>, AlongK<T::BR, W, S, DIRECT, false>>::type OpR;
+  typedef typename std::conditional<kPair, AlongK<T::BC, W, S, DIRECT, true>, AcrossK<T::BC, W, S, DIRECT>>::type OpC;
   __shared__ __attribute__((aligned(1024))) char lds[2][T::kBytesR + T::kBytesC];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l32 = lane & 31, hh = lane >> 5;
@@ -297,31 +327,41 @@ __global__ void __launch_bounds__(T::kThreads, 2) gated_tile_kernel(GatedArgs a)
   const int64_t r0 = (MODE == kGatedDw ? tile_r - which * half_r : tile_r) * T::BR;
   const int64_t c0 = static_cast<int64_t>(tile_c) * kCols;
 
+  const int64_t kt_begin = split * a.k_split;
+  const int64_t kt_end = kt_begin + a.k_split < a.k_tiles ? kt_begin + a.k_split : a.k_tiles;
+
   OpR op_r;
   OpC op_c;
+  const int64_t ld_w = static_cast<int64_t>(a.channels) * S, ld_gu = static_cast<int64_t>(a.ld_gu) * S;
+  if constexpr (kPair) {
+    op_r.init(a.rows - r0, a.x_ld, wave, lane);
+    op_c.init(a.hidden - c0, ld_w, wave, lane);
+  } else if constexpr (MODE == kGatedDx) {
+    op_r.init(a.rows - r0, ld_gu, wave, lane);
+    op_c.init(a.channels - c0, ld_w, wave, lane);
+  } else {
+    op_r.init(a.ld_gu - r0, ld_gu, wave, lane);
+    op_c.init(a.channels - c0, a.x_ld, wave, lane);
+  }
+  // Tiles behind the last one read as zeros (nobody uses them: the loop needs no branch).
   auto fetch = [&](int64_t kt, int stage) {
     const uint32_t at_r = lds_addr(lds[stage]), at_c = at_r + T::kBytesR;
+    const auto left = [&](int64_t k) { return kt >= kt_end ? 0 : k < KT ? static_cast<int>(k) : KT; };
     if constexpr (kPair) {
-      const int64_t k0 = kt * KT;
-      op_r.fetch([&](int q, int64_t* there) { *there = a.rows - (r0 + q); return a.x + (r0 + q) * a.x_ld; }, a.x_ld, k0, a.channels,
-                 at_r, wave, lane);
-      const int64_t ld = static_cast<int64_t>(a.channels) * S;
-      op_c.fetch([&](int q, int64_t* there) {
-        const int64_t n = c0 + (q >> 6) * 32 + (q & 31);
-        *there = a.hidden - n;
-        return a.w[(q >> 5) & 1] + n * ld;
-      }, ld, k0, a.channels, at_c, wave, lane);
+      const int k_left = left(a.channels - kt * KT);
+      op_r.fetch(a.x + r0 * a.x_ld + kt * 128, nullptr, k_left, at_r, wave);
+      op_c.fetch(a.w[0] + c0 * ld_w + kt * 128, a.w[1] + c0 * ld_w + kt * 128, k_left, at_c, wave);
     } else if constexpr (MODE == kGatedDx) {
       const int64_t each = a.k_tiles / 2;
       const int w = kt >= each;
-      const int64_t k0 = (kt - w * each) * KT, ld = static_cast<int64_t>(a.ld_gu) * S, ld_w = static_cast<int64_t>(a.channels) * S;
-      op_r.fetch([&](int q, int64_t* there) { *there = a.rows - (r0 + q); return a.dgu[w] + (r0 + q) * ld; }, ld, k0, a.ld_gu, at_r,
-                 wave, lane);
-      op_c.fetch(a.w[w] + c0 * S, ld_w, a.channels - c0, k0, a.hidden, at_c, wave, lane);
+      const int64_t k0 = (kt - w * each) * KT;
+      op_r.fetch(a.dgu[w] + r0 * ld_gu + k0 * S, nullptr, left(a.ld_gu - k0), at_r, wave);
+      op_c.fetch(a.w[w] + k0 * ld_w + c0 * S, left(a.hidden - k0), at_c, wave);
     } else {
       const int64_t k0 = kt * KT;
-      op_r.fetch(a.dgu[which] + r0 * S, static_cast<int64_t>(a.ld_gu) * S, a.ld_gu - r0, k0, a.rows, at_r, wave, lane);
-      op_c.fetch(a.x + c0 * S, a.x_ld, a.channels - c0, k0, a.rows, at_c, wave, lane);
+      const int k_left = left(a.rows - k0);
+      op_r.fetch(a.dgu[which] + k0 * ld_gu + r0 * S, k_left, at_r, wave);
+      op_c.fetch(a.x + k0 * a.x_ld + c0 * S, k_left, at_c, wave);
     }
   };
   auto put = [&](int stage) {
@@ -337,34 +377,66 @@ __global__ void __launch_bounds__(T::kThreads, 2) gated_tile_kernel(GatedArgs a)
     for (int j = 0; j < T::RI; ++j) acc[i][j] = f32x16{};
   const int wr = wave / T::WC * (T::RI * 32), wc = wave % T::WC * (T::CI * 32);
 
-  const int64_t kt_begin = split * a.k_split;
-  const int64_t kt_end = kt_begin + a.k_split < a.k_tiles ? kt_begin + a.k_split : a.k_tiles;
-  fetch(kt_begin, 0);
-  if constexpr (!DIRECT) put(0);
-  for (int64_t kt = kt_begin; kt < kt_end; ++kt) {
-    const int stage = static_cast<int>((kt - kt_begin) & 1);
-    // This wave's copies are there; behind the barrier all waves' are, and nobody reads the other stage any more.
-    wait_vmcnt<0>();
-    __syncthreads();
-    const bool more = kt + 1 < kt_end;
-    if (more) fetch(kt + 1, stage ^ 1);
+  u32x4 fr[2][T::RI], fc[2][T::CI];
+  auto read = [&](int stage, int s, int buf) {
     const uint32_t at_r = lds_addr(lds[stage]), at_c = at_r + T::kBytesR;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      u32x4 fr[T::RI], fc[T::CI];
+    for (int i = 0; i < T::CI; ++i) fc[buf][i] = OpC::template read<Ty>(at_c, wc + 32 * i, s, lane);
 #pragma unroll
-      for (int i = 0; i < T::CI; ++i) fc[i] = OpC::template read<Ty>(at_c, wc + 32 * i, s, lane);
+    for (int j = 0; j < T::RI; ++j) fr[buf][j] = OpR::template read<Ty>(at_r, wr + 32 * j, s, lane);
+  };
+  auto multiply = [&](int buf) {
 #pragma unroll
-      for (int j = 0; j < T::RI; ++j) fr[j] = OpR::template read<Ty>(at_r, wr + 32 * j, s, lane);
+    for (int j = 0; j < T::RI; ++j)
 #pragma unroll
-      for (int i = 0; i < T::CI; ++i)
+      for (int i = 0; i < T::CI; ++i) acc[i][j] = Elem<Ty>::mma(fc[buf][i], fr[buf][j], acc[i][j]);
+  };
+  constexpr int kCopies = OpR::kCopies + OpC::kCopies;
+  // A step's reads go between its products, one after each; left alone, the compiler puts them right before their use.
+  constexpr int kReads = T::CI * OpC::kReads + T::RI * OpR::kReads, kProducts = T::CI * T::RI * Elem<Ty>::kProducts;
+  auto interleave = [&]() {
+    constexpr int kEach = kProducts / kReads > 0 ? kProducts / kReads : 1;
 #pragma unroll
-        for (int j = 0; j < T::RI; ++j) acc[i][j] = Elem<Ty>::mma(fc[i], fr[j], acc[i][j]);
+    for (int i = 0; i < kReads; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // a read of LDS
+      __builtin_amdgcn_sched_group_barrier(0x8, kEach, 0);  // products
     }
-    if constexpr (!DIRECT) {
-      if (more) put(stage ^ 1);
-    }
+    if constexpr (kProducts > kReads * kEach) __builtin_amdgcn_sched_group_barrier(0x8, kProducts - kReads * kEach, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  // Operands of a step are read while the step before it is multiplied, those of a tile's first step during the
+  // last one of the tile before: at that point the next tile has arrived, all of this one is in registers, and
+  // the tile after the next takes its place.
+  fetch(kt_begin, 0);
+  if constexpr (DIRECT) {
+    fetch(kt_begin + 1, 1);
+    wait_vmcnt<kCopies>();
+  } else {
+    put(0);
+    fetch(kt_begin + 1, 1);
   }
+  __syncthreads();
+  read(0, 0, 0);
+  for (int64_t kt = kt_begin; kt < kt_end; ++kt) {
+    const int stage = static_cast<int>((kt - kt_begin) & 1);
+#pragma unroll
+    for (int s = 0; s < 3; ++s) {
+      read(stage, s + 1, (s + 1) & 1);
+      multiply(s & 1);
+      interleave();
+    }
+    if constexpr (DIRECT) wait_vmcnt<0>();
+    else put(stage ^ 1);
+    __syncthreads();
+    __builtin_amdgcn_sched_barrier(0);
+    read(stage ^ 1, 0, 0);
+    fetch(kt + 2, stage);
+    multiply(1);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  // No copy may still be on its way when the workgroup ends.
+  wait_vmcnt<0>();
   mfma_drain();
 
   if constexpr (kPair) {
