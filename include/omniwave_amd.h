@@ -767,7 +767,10 @@ int ow_distillation_bwd(const OwDistillation* d, const float* stats, const float
  * weights [hidden][channels], contiguous, and h [rows][hidden], contiguous, all of `dtype`.  Products and gates are fp32;
  * h is rounded once.  channels, hidden <= 2^20, rows < 2^31; channels >= 1 where anything is computed.
  *
- * The backward takes dh (row stride in values) and writes those of dx [rows][channels], dgate_weight and dup_weight that
+ * A forward with a backward to come may be given kept (4-byte aligned), where ow_gated_linear_kept is not 0: that many bytes, in
+ * which it leaves both products in fp32 for the backward, which else forms them again (kept NULL there, too).
+ *
+ * The backward takes kept, dh (row stride in values) and writes those of dx [rows][channels], dgate_weight and dup_weight that
  * are not NULL, over ow_gated_linear_bwd_workspace bytes of workspace (16-byte aligned).  The gradients of the two
  * projections are rounded to `dtype` in between; sums have a fixed order.  rows, channels, hidden >= 1 there.
  */
@@ -782,10 +785,11 @@ typedef struct OwGatedLinear {
   int32_t dtype;
 } OwGatedLinear;
 
-int ow_gated_linear_fwd(const OwGatedLinear* d, void* h, void* stream);
+size_t ow_gated_linear_kept(const OwGatedLinear* d);
+int ow_gated_linear_fwd(const OwGatedLinear* d, void* h, void* kept, void* stream);
 size_t ow_gated_linear_bwd_workspace(const OwGatedLinear* d);
-int ow_gated_linear_bwd(const OwGatedLinear* d, const void* dh, int64_t dh_stride, void* dx, void* dgate_weight,
-                        void* dup_weight, void* workspace, size_t workspace_bytes, void* stream);
+int ow_gated_linear_bwd(const OwGatedLinear* d, const void* kept, const void* dh, int64_t dh_stride, void* dx,
+                        void* dgate_weight, void* dup_weight, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -329,11 +329,12 @@ _SIGNATURES = {
         ctypes.c_int, [ctypes.POINTER(OwDistillation)] + [ctypes.c_void_p] * 5 + [ctypes.c_size_t, ctypes.c_void_p],
     ),
     "ow_distillation_bwd": (ctypes.c_int, [ctypes.POINTER(OwDistillation)] + [ctypes.c_void_p] * 5),
-    "ow_gated_linear_fwd": (ctypes.c_int, [ctypes.POINTER(OwGatedLinear)] + [ctypes.c_void_p] * 2),
+    "ow_gated_linear_kept": (ctypes.c_size_t, [ctypes.POINTER(OwGatedLinear)]),
+    "ow_gated_linear_fwd": (ctypes.c_int, [ctypes.POINTER(OwGatedLinear)] + [ctypes.c_void_p] * 3),
     "ow_gated_linear_bwd_workspace": (ctypes.c_size_t, [ctypes.POINTER(OwGatedLinear)]),
     "ow_gated_linear_bwd": (
         ctypes.c_int,
-        [ctypes.POINTER(OwGatedLinear), ctypes.c_void_p, ctypes.c_int64] + [ctypes.c_void_p] * 4
+        [ctypes.POINTER(OwGatedLinear), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64] + [ctypes.c_void_p] * 4
         + [ctypes.c_size_t, ctypes.c_void_p],
     ),
     "ow_bwd_params": (

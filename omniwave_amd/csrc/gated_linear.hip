@@ -156,11 +156,23 @@ void apply_plan(GatedArgs& a, const GatedPlan& p) {
   a.splits = p.splits;
   a.k_tiles = p.k_tiles;
   a.k_split = p.k_split;
+  // (Numbers past 2^31 are refused before a launch.)
+  a.by_tiles = Divisor::of(static_cast<uint32_t>(p.tiles_r * p.tiles_c));
+  a.by_group = Divisor::of(8 * static_cast<uint32_t>(p.tiles_c));
 }
 
 }  // namespace ow
 
-extern "C" int ow_gated_linear_fwd(const OwGatedLinear* d, void* h, void* stream) {
+extern "C" {
+
+// The products are kept where forming them again (4 K operations a value) would take longer than to write and read them (16 bytes).
+size_t ow_gated_linear_kept(const OwGatedLinear* d) {
+  if (d == nullptr || d->rows <= ow::kFewRows || d->channels <= 0 || d->hidden <= 0) return 0;
+  const int32_t from = d->dtype == OW_DTYPE_F32 ? 128 : 1536;
+  return d->channels >= from ? static_cast<size_t>(2) * d->rows * d->hidden * sizeof(float) : 0;
+}
+
+int ow_gated_linear_fwd(const OwGatedLinear* d, void* h, void* kept, void* stream) {
   if (int rc = ow::check_gated(d)) return rc;
   if (d->rows == 0 || d->hidden == 0) {
     ow::clear_error();
@@ -168,6 +180,8 @@ extern "C" int ow_gated_linear_fwd(const OwGatedLinear* d, void* h, void* stream
   }
   OW_CHECK_ARG(d->channels > 0, "products over no channels have no kernel");
   OW_CHECK_ARG(h != nullptr, "h is NULL");
+  OW_CHECK_ARG(kept == nullptr || (ow_gated_linear_kept(d) != 0 && reinterpret_cast<uintptr_t>(kept) % 4 == 0),
+               "the products of these sizes are not kept, or have no place for fp32 values");
   ow::GatedArgs a = ow::gated_args(*d);
   a.out[0] = h;
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -178,12 +192,17 @@ extern "C" int ow_gated_linear_fwd(const OwGatedLinear* d, void* h, void* stream
     if (int rc = ow::hip_status(hipGetLastError(), "gated_few_kernel launch")) return rc;
   } else {
     const int64_t size = d->dtype == OW_DTYPE_F32 ? 4 : 2;
-    const ow::GatedPlan p = ow::gated_plan(d->rows, 2 * static_cast<int64_t>(d->hidden), ow::ceil_div(d->channels * size, 128), 1, false);
+    const ow::GatedPlan p = ow::gated_plan(d->rows, 2 * static_cast<int64_t>(d->hidden), ow::ceil_div(d->channels * size, 128), 1, false, size == 4);
     OW_CHECK_SUPPORTED(p.tiles_r * p.tiles_c < (int64_t(1) << 31), "gated linear: too many tiles for a launch");
     ow::apply_plan(a, p);
-    ow::launch_gated_mode<ow::kGatedForward>(a, p.size, d->dtype, ow::gated_x_direct(a, size) && ow::gated_w_direct(a, size), s);
+    a.kept = static_cast<float*>(kept);
+    const bool direct = ow::gated_x_direct(a, size) && ow::gated_w_direct(a, size);
+    if (kept != nullptr) ow::launch_gated_mode<ow::kGatedKeep>(a, p.size, d->dtype, direct, s);
+    else ow::launch_gated_mode<ow::kGatedForward>(a, p.size, d->dtype, direct, s);
     if (int rc = ow::hip_status(hipGetLastError(), "gated_tile_kernel launch")) return rc;
   }
   ow::clear_error();
   return OW_OK;
 }
+
+}  // extern "C"

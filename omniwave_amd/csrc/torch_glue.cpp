@@ -600,20 +600,24 @@ std::vector<int64_t> hidden_shape(const Gated& g) {
   return shape;
 }
 
-Tensor run_gated(const Gated& g) {
+// The result, and with `keep` what the backward needs beside the inputs (both products, or nothing).
+std::pair<Tensor, Tensor> run_gated(const Gated& g, bool keep) {
   const c10::DeviceGuard guard(g.x.device());
-  Tensor h = at::empty(hidden_shape(g), g.x.options());
+  Tensor h = at::empty(hidden_shape(g), g.x.options()), kept;
   const OwGatedLinear d = descriptor(g);
-  check(ow_gated_linear_fwd(&d, out_ptr(h), stream_of(g.x)), "ow_gated_linear_fwd");
-  return h;
+  if (const size_t bytes = keep ? ow_gated_linear_kept(&d) : 0)
+    kept = at::empty({static_cast<int64_t>(bytes / sizeof(float))}, g.x.options().dtype(at::kFloat));
+  check(ow_gated_linear_fwd(&d, out_ptr(h), out_ptr(kept), stream_of(g.x)), "ow_gated_linear_fwd");
+  return {std::move(h), std::move(kept)};
 }
 
 class GatedNode : public torch::autograd::Function<GatedNode> {
  public:
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& gate, const Tensor& up) {
-    ctx->save_for_backward({x, gate, up});
+    auto [h, kept] = run_gated(Gated{x, gate, up}, true);
+    ctx->save_for_backward({x, gate, up, kept});
     ctx->set_materialize_grads(false);
-    return run_gated(Gated{x, gate, up});
+    return h;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list ups) {
@@ -630,16 +634,22 @@ class GatedNode : public torch::autograd::Function<GatedNode> {
     check_unpacked(plain_case(g) && plain(dh) && dh.sizes() == at::IntArrayRef(hidden_shape(g)) &&
                    dh.scalar_type() == g.x.scalar_type() && dh.device() == g.x.device());
     dh = rows_of(dh, &dh_stride);
+    const OwGatedLinear d = descriptor(g);
+    Tensor kept = s[3];
+    if (kept.defined()) {
+      kept = kept.contiguous();
+      check_unpacked(plain(kept) && kept.scalar_type() == at::kFloat && kept.device() == g.x.device() &&
+                     static_cast<size_t>(kept.numel()) * sizeof(float) == ow_gated_linear_kept(&d));
+    }
     const Tensor* inputs[3] = {&g.x, &g.gate, &g.up};
     Tensor grads[3];
     bool any = false;
     for (size_t i = 0; i < 3; ++i)
       if (ctx->needs_input_grad(i)) grads[i] = like(*inputs[i]), any = true;
     if (any) {
-      const OwGatedLinear d = descriptor(g);
       const size_t bytes = ow_gated_linear_bwd_workspace(&d);
       const Tensor workspace = at::empty({static_cast<int64_t>(bytes)}, g.x.options().dtype(at::kByte));
-      check(ow_gated_linear_bwd(&d, ptr(dh), dh_stride, out_ptr(grads[0]), out_ptr(grads[1]), out_ptr(grads[2]),
+      check(ow_gated_linear_bwd(&d, ptr(kept), ptr(dh), dh_stride, out_ptr(grads[0]), out_ptr(grads[1]), out_ptr(grads[2]),
                                 out_ptr(workspace), bytes, stream_of(g.x)),
             "ow_gated_linear_bwd");
     }
@@ -823,7 +833,7 @@ PyObject* py_gated_linear(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
       h = GatedNode::apply(g.x, g.gate, g.up);
     } else {
       at::AutoDispatchBelowADInplaceOrView below;
-      h = run_gated(g);
+      h = run_gated(g, false).first;
     }
   }
   return THPVariable_Wrap(h);

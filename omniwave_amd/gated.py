@@ -50,20 +50,34 @@ def _descriptor(x, gate_weight, up_weight):
                                  gate_weight.shape[0], _DTYPE_CODE[x.dtype]), keep
 
 
-def _run_forward(x, gate_weight, up_weight) -> Tensor:
+def _kept_values(x, gate_weight) -> int:
+    """Values of both products that a forward keeps for its backward, 0 where that forms them again."""
+    desc = _native.OwGatedLinear(rows=math.prod(x.shape[:-1]), channels=x.shape[-1], hidden=gate_weight.shape[0],
+                                 dtype=_DTYPE_CODE[x.dtype])
+    return _native.lib().ow_gated_linear_kept(ctypes.byref(desc)) // 4
+
+
+def _run_forward(x, gate_weight, up_weight, keep) -> tuple[Tensor, Tensor]:
+    """(the result, what the backward needs beside the inputs: both products in float32, or nothing)."""
     _ready(x, gate_weight, up_weight)  # the operator may be called by its name
     h = torch.empty((*x.shape[:-1], gate_weight.shape[0]), dtype=x.dtype, device=x.device)
+    kept = torch.empty(_kept_values(x, gate_weight) if keep else 0, dtype=torch.float32, device=x.device)
     if not x.shape[-1]:
-        return h.zero_()
+        return h.zero_(), kept
     if h.numel():
         desc, _keep = _descriptor(x, gate_weight, up_weight)
-        _on(x.device, _native.lib().ow_gated_linear_fwd, ctypes.byref(desc), h.data_ptr())
-    return h
+        _on(x.device, _native.lib().ow_gated_linear_fwd, ctypes.byref(desc), h.data_ptr(),
+            kept.data_ptr() if kept.numel() else None)
+    return h, kept
 
 
-def _run_backward(dh, x, gate_weight, up_weight, want) -> list[Tensor | None]:
+def _run_backward(dh, kept, x, gate_weight, up_weight, want) -> list[Tensor | None]:
     """Gradients of x, gate_weight and up_weight where ``want`` asks for them."""
     _ready(x, gate_weight, up_weight)  # hooks on saved tensors may hand out others
+    if kept.numel() and (kept.device != x.device or kept.dtype != torch.float32
+                         or kept.numel() != _kept_values(x, gate_weight)):
+        raise ValueError(f"the products kept of {tuple(x.shape)} and {tuple(gate_weight.shape)} on {x.device} are {kept.dtype} "
+                         f"{tuple(kept.shape)} on {kept.device}")
     shape = (*x.shape[:-1], gate_weight.shape[0])
     if dh.shape != shape or dh.dtype != x.dtype or dh.device != x.device:
         raise ValueError(f"the upstream gradient of {x.dtype} {shape} on {x.device} is {dh.dtype} {tuple(dh.shape)} on "
@@ -75,46 +89,53 @@ def _run_backward(dh, x, gate_weight, up_weight, want) -> list[Tensor | None]:
     if any(want):
         desc, _keep = _descriptor(x, gate_weight, up_weight)
         dh, dh_stride = _rows(dh)
+        kept = kept.contiguous()
         lib = _native.lib()
         with torch.cuda.device(x.device):  # the size goes by the device's compute units
             ws_bytes = lib.ow_gated_linear_bwd_workspace(ctypes.byref(desc))
         workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
-        _on(x.device, lib.ow_gated_linear_bwd, ctypes.byref(desc), dh.data_ptr(), dh_stride,
+        _on(x.device, lib.ow_gated_linear_bwd, ctypes.byref(desc), kept.data_ptr() if kept.numel() else None,
+            dh.data_ptr(), dh_stride,
             *[None if g is None else g.data_ptr() for g in grads], workspace.data_ptr(), ws_bytes)
     return grads
 
 
 @torch.library.custom_op("omniwave_amd::gated_linear_fwd", mutates_args=())
-def gated_linear_fwd(x: Tensor, gate_weight: Tensor, up_weight: Tensor) -> Tensor:
-    """``gated_linear_hip``'s result."""
-    return _run_forward(x, gate_weight, up_weight)
+def gated_linear_fwd(x: Tensor, gate_weight: Tensor, up_weight: Tensor, keep: bool) -> tuple[Tensor, Tensor]:
+    """(``gated_linear_hip``'s result; what the backward needs beside the inputs where ``keep`` says that there will be
+    one, which may be nothing)."""
+    return _run_forward(x, gate_weight, up_weight, keep)
 
 
 @gated_linear_fwd.register_fake
-def _gated_linear_fwd_fake(x, gate_weight, up_weight):
-    return x.new_empty((*x.shape[:-1], gate_weight.shape[0]))
+def _gated_linear_fwd_fake(x, gate_weight, up_weight, keep):
+    return (x.new_empty((*x.shape[:-1], gate_weight.shape[0])),
+            x.new_empty(_kept_values(x, gate_weight) if keep else 0, dtype=torch.float32))
 
 
 @torch.library.custom_op("omniwave_amd::gated_linear_bwd", mutates_args=())
-def gated_linear_bwd(dh: Tensor, x: Tensor, gate_weight: Tensor, up_weight: Tensor,
+def gated_linear_bwd(dh: Tensor, kept: Tensor, x: Tensor, gate_weight: Tensor, up_weight: Tensor,
                      want: list[bool]) -> tuple[Tensor, Tensor, Tensor]:
     """Gradients of x, gate_weight and up_weight; empty where ``want`` is false."""
-    grads = _run_backward(dh, x, gate_weight, up_weight, want)
+    grads = _run_backward(dh, kept, x, gate_weight, up_weight, want)
     return tuple(x.new_empty(0) if g is None else g for g in grads)
 
 
 @gated_linear_bwd.register_fake
-def _gated_linear_bwd_fake(dh, x, gate_weight, up_weight, want):
+def _gated_linear_bwd_fake(dh, kept, x, gate_weight, up_weight, want):
     return tuple(t.new_empty(t.shape) if w else x.new_empty(0) for t, w in zip((x, gate_weight, up_weight), want))
 
 
 def _setup_context(ctx, inputs, output):
-    ctx.save_for_backward(*inputs)
+    ctx.mark_non_differentiable(output[1])
+    ctx.save_for_backward(*inputs[:3], output[1])
 
 
-def _backward(ctx, dh):
-    want = list(ctx.needs_input_grad)
-    return tuple(g if w else None for g, w in zip(gated_linear_bwd(dh, *ctx.saved_tensors, want), want))
+def _backward(ctx, dh, _kept):
+    x, gate_weight, up_weight, kept = ctx.saved_tensors
+    want = list(ctx.needs_input_grad[:3])
+    grads = gated_linear_bwd(dh, kept, x, gate_weight, up_weight, want)
+    return *[g if w else None for g, w in zip(grads, want)], None
 
 
 gated_linear_fwd.register_autograd(_backward, setup_context=_setup_context)
@@ -123,8 +144,9 @@ gated_linear_fwd.register_autograd(_backward, setup_context=_setup_context)
 def gated_linear_hip(x: Tensor, gate_weight: Tensor, up_weight: Tensor) -> Tensor:
     """``silu(x @ gate_weight.T) * (x @ up_weight.T)``, the first half of a gated feed-forward block in one kernel: ``x``
     ``[..., C]`` (rows at any one distance) and weights ``[hidden, C]``, all of one type (float16, bfloat16 or float32),
-    to ``[..., hidden]``.  Products and gate are fp32 and the result is rounded once.  Differentiable once in all three; the
-    backward forms the products again instead of keeping them, and rounds their gradients to the type in between."""
+    to ``[..., hidden]``.  Products and gate are fp32 and the result is rounded once.  Differentiable once in all three.  The
+    backward rounds the gradients of both products to the type in between; where C is large (1,536 for 16-bit types, 128 for
+    float32) the forward of a call with a graph keeps both products for it, 8 bytes a value, else they are formed again."""
     glue = _native.glue()
     if glue is not None and _plain(x, gate_weight, up_weight):
         h = glue.gated_linear(x, gate_weight, up_weight)
@@ -132,4 +154,5 @@ def gated_linear_hip(x: Tensor, gate_weight: Tensor, up_weight: Tensor) -> Tenso
             return h
     # Everything else is checked, and goes through the operator.
     _ready(x, gate_weight, up_weight)
-    return gated_linear_fwd(x, gate_weight, up_weight)
+    keep = torch.is_grad_enabled() and any(t.requires_grad for t in (x, gate_weight, up_weight))
+    return gated_linear_fwd(x, gate_weight, up_weight, keep)[0]

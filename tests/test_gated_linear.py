@@ -9,7 +9,7 @@ import torch
 
 from omniwave_amd import _native, gated, gated_linear_hip
 
-X, W = torch.zeros(2, 3, 10), torch.zeros(6, 10)
+X, W, NONE = torch.zeros(2, 3, 10), torch.zeros(6, 10), torch.zeros(0)
 
 
 @pytest.mark.parametrize("kwargs,text", [
@@ -34,8 +34,8 @@ def test_refusals(kwargs, text) -> None:
 
 def test_the_cpu_has_no_kernel() -> None:
     ops = torch.ops.omniwave_amd
-    for call in (lambda: gated_linear_hip(X, W, W), lambda: ops.gated_linear_fwd(X, W, W),
-                 lambda: ops.gated_linear_bwd(torch.zeros(2, 3, 6), X, W, W, [True] * 3)):
+    for call in (lambda: gated_linear_hip(X, W, W), lambda: ops.gated_linear_fwd(X, W, W, True),
+                 lambda: ops.gated_linear_bwd(torch.zeros(2, 3, 6), NONE, X, W, W, [True] * 3)):
         with pytest.raises(RuntimeError, match="not supported"):
             call()
 
@@ -65,20 +65,38 @@ def launches(monkeypatch):
 def test_what_the_operators_get(launches, bad) -> None:
     t = {"x": X, "gate": W, "up": W, **bad}
     with pytest.raises(ValueError):
-        gated._run_forward(*t.values())
+        gated._run_forward(*t.values(), True)
     with pytest.raises(ValueError):
-        gated._run_backward(torch.zeros(2, 3, 6), *t.values(), [True] * 3)
+        gated._run_backward(torch.zeros(2, 3, 6), NONE, *t.values(), [True] * 3)
     assert not launches
 
 
 @pytest.mark.parametrize("up", [torch.zeros(2, 3, 5), torch.zeros(6, 6), torch.zeros(2, 3, 6).half(), torch.zeros(2, 3, 6, device="meta")])
 def test_upstream_gradients(launches, up) -> None:
     with pytest.raises(ValueError, match="upstream"):
-        gated._run_backward(up, X, W, W, [True] * 3)
+        gated._run_backward(up, NONE, X, W, W, [True] * 3)
     assert not launches
-    gated._run_backward(torch.zeros(2, 3, 6), X, W, W, [True] * 3)
-    gated._run_backward(torch.zeros(2, 3, 6), X, W, W, [False] * 3)  # nothing is asked for
-    gated._run_forward(X, W, W)
+    gated._run_backward(torch.zeros(2, 3, 6), NONE, X, W, W, [True] * 3)
+    gated._run_backward(torch.zeros(2, 3, 6), NONE, X, W, W, [False] * 3)  # nothing is asked for
+    gated._run_forward(X, W, W, False)
+    assert len(launches) == 2
+
+
+def test_kept_products(launches) -> None:
+    """Two values of fp32 for each of the result, for more than 64 tokens of many channels; the backward looks at them."""
+    for dtype, c, n in ((torch.bfloat16, 1535, 0), (torch.bfloat16, 1536, 2 * 70 * 6), (torch.float32, 127, 0), (torch.float32, 128, 2 * 70 * 6)):
+        x, w = torch.zeros(70, c, dtype=dtype), torch.zeros(6, c, dtype=dtype)
+        assert gated._run_forward(x, w, w, True)[1].numel() == n
+        assert gated._run_forward(x, w, w, False)[1].numel() == 0
+        assert gated._run_forward(x[:64], w, w, True)[1].numel() == 0
+    launches.clear()
+    up = torch.zeros(70, 6)
+    for kept in (torch.zeros(839), torch.zeros(840).half(), torch.zeros(840, device="meta")):
+        with pytest.raises(ValueError, match="kept"):
+            gated._run_backward(up, kept, x, w, w, [True] * 3)
+    assert not launches
+    for kept in (torch.zeros(840), NONE):
+        gated._run_backward(up, kept, x, w, w, [True] * 3)
     assert len(launches) == 2
 
 
@@ -94,27 +112,31 @@ def test_c_entry_points_check_their_arguments() -> None:
     def refused(rc, text, code=1):
         assert rc == code and text in lib.ow_last_error(), lib.ow_last_error()
 
-    refused(lib.ow_gated_linear_fwd(None, p, None), b"NULL")
-    refused(lib.ow_gated_linear_fwd(desc(dtype=3), p, None), b"dtype", 2)
-    refused(lib.ow_gated_linear_fwd(desc(hidden=-1), p, None), b"negative")
-    refused(lib.ow_gated_linear_fwd(desc(channels=(1 << 20) + 1), p, None), b"at most", 2)
-    refused(lib.ow_gated_linear_fwd(desc(rows=1 << 31), p, None), b"2^31", 2)
-    refused(lib.ow_gated_linear_fwd(desc(up_weight=None), p, None), b"NULL")
-    refused(lib.ow_gated_linear_fwd(desc(x=257), p, None), b"aligned")
-    refused(lib.ow_gated_linear_fwd(desc(), None, None), b"NULL")
-    refused(lib.ow_gated_linear_fwd(desc(channels=0), p, None), b"no channels")
-    assert lib.ow_gated_linear_fwd(desc(rows=0), None, None) == 0 and lib.ow_gated_linear_fwd(desc(hidden=0), None, None) == 0
+    refused(lib.ow_gated_linear_fwd(None, p, None, None), b"NULL")
+    refused(lib.ow_gated_linear_fwd(desc(dtype=3), p, None, None), b"dtype", 2)
+    refused(lib.ow_gated_linear_fwd(desc(hidden=-1), p, None, None), b"negative")
+    refused(lib.ow_gated_linear_fwd(desc(channels=(1 << 20) + 1), p, None, None), b"at most", 2)
+    refused(lib.ow_gated_linear_fwd(desc(rows=1 << 31), p, None, None), b"2^31", 2)
+    refused(lib.ow_gated_linear_fwd(desc(up_weight=None), p, None, None), b"NULL")
+    refused(lib.ow_gated_linear_fwd(desc(x=257), p, None, None), b"aligned")
+    refused(lib.ow_gated_linear_fwd(desc(), None, None, None), b"NULL")
+    refused(lib.ow_gated_linear_fwd(desc(channels=0), p, None, None), b"no channels")
+    assert lib.ow_gated_linear_fwd(desc(rows=0), None, None, None) == 0 and lib.ow_gated_linear_fwd(desc(hidden=0), None, None, None) == 0
     assert lib.ow_gated_linear_bwd_workspace(None) == 0 and lib.ow_gated_linear_bwd_workspace(desc(rows=0)) == 0
     need = lib.ow_gated_linear_bwd_workspace(desc())
     assert need >= 2 * 100 * 6 * 2
 
-    def bwd(d, dh=p, ws=p, n=need):
-        return lib.ow_gated_linear_bwd(d, dh, 6, p, p, p, ws, n, None)
+    def bwd(d, dh=p, ws=p, n=need, kept=None):
+        return lib.ow_gated_linear_bwd(d, kept, dh, 6, p, p, p, ws, n, None)
 
     for empty in (dict(rows=0), dict(channels=0), dict(hidden=0)):
         refused(bwd(desc(**empty)), b"empty")
     refused(bwd(desc(), dh=None), b"NULL")
     refused(bwd(desc(), dh=ctypes.c_void_p(257)), b"aligned")
+    refused(bwd(desc(), kept=ctypes.c_void_p(258)), b"aligned")
+    refused(lib.ow_gated_linear_fwd(desc(), p, p, None), b"kept")
+    refused(lib.ow_gated_linear_fwd(desc(channels=1536), p, ctypes.c_void_p(258), None), b"kept")
+    assert lib.ow_gated_linear_kept(None) == 0 and lib.ow_gated_linear_kept(desc(channels=1536)) == 2 * 100 * 6 * 4
     refused(bwd(desc(), ws=None), b"workspace")
     refused(bwd(desc(), n=need - 1), b"workspace")
     refused(bwd(desc(), ws=ctypes.c_void_p(264)), b"workspace")
