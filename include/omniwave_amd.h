@@ -765,7 +765,9 @@ int ow_distillation_bwd(const OwDistillation* d, const float* stats, const float
  *
  * x: rows of `channels` values of `dtype` (value stride 1, row stride in values, any alignment a value may have);
  * weights [hidden][channels], contiguous, and h [rows][hidden], contiguous, all of `dtype`.  Products and gates are fp32;
- * h is rounded once.  channels, hidden <= 2^20, rows < 2^31; channels >= 1 where anything is computed.
+ * h is rounded once.  channels, hidden <= 2^20, rows < 2^31; channels >= 1 where anything is computed.  A workspace (16-byte
+ * aligned) of ow_gated_linear_fwd_workspace bytes, 0 for few rows and many others.  fp32 operands are three bf16 parts each for
+ * more than 64 rows: an infinity makes its results NaN, and values below about 2^-110 have fewer than 24 bits.
  *
  * A forward with a backward to come may be given kept (4-byte aligned), where ow_gated_linear_kept is not 0: that many bytes, in
  * which it leaves both products in fp32 for the backward, which else forms them again (kept NULL there, too).
@@ -786,7 +788,8 @@ typedef struct OwGatedLinear {
 } OwGatedLinear;
 
 size_t ow_gated_linear_kept(const OwGatedLinear* d);
-int ow_gated_linear_fwd(const OwGatedLinear* d, void* h, void* kept, void* stream);
+size_t ow_gated_linear_fwd_workspace(const OwGatedLinear* d);
+int ow_gated_linear_fwd(const OwGatedLinear* d, void* h, void* kept, void* workspace, size_t workspace_bytes, void* stream);
 size_t ow_gated_linear_bwd_workspace(const OwGatedLinear* d);
 int ow_gated_linear_bwd(const OwGatedLinear* d, const void* kept, const void* dh, int64_t dh_stride, void* dx,
                         void* dgate_weight, void* dup_weight, void* workspace, size_t workspace_bytes, void* stream);

@@ -330,7 +330,10 @@ _SIGNATURES = {
     ),
     "ow_distillation_bwd": (ctypes.c_int, [ctypes.POINTER(OwDistillation)] + [ctypes.c_void_p] * 5),
     "ow_gated_linear_kept": (ctypes.c_size_t, [ctypes.POINTER(OwGatedLinear)]),
-    "ow_gated_linear_fwd": (ctypes.c_int, [ctypes.POINTER(OwGatedLinear)] + [ctypes.c_void_p] * 3),
+    "ow_gated_linear_fwd_workspace": (ctypes.c_size_t, [ctypes.POINTER(OwGatedLinear)]),
+    "ow_gated_linear_fwd": (
+        ctypes.c_int, [ctypes.POINTER(OwGatedLinear)] + [ctypes.c_void_p] * 3 + [ctypes.c_size_t, ctypes.c_void_p],
+    ),
     "ow_gated_linear_bwd_workspace": (ctypes.c_size_t, [ctypes.POINTER(OwGatedLinear)]),
     "ow_gated_linear_bwd": (
         ctypes.c_int,

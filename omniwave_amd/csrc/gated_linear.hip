@@ -3,9 +3,9 @@
 //
 //   G = x Wg^T    U = x Wu^T    h = silu(G) U,  silu(g) = g / (1 + e^-g)
 //
-// Tokens enough for tiles go through gated_tile_kernel (ow_gated.h): a tile's columns are 32 of the gate beside the same
-// 32 of the other projection, so that a lane has both values of an output.  G and U are never stored; they are fp32 until
-// h is rounded.
+// More than 64 tokens go through gated_tile_kernel (ow_gated.h): a tile's columns are 32 of the gate beside the same
+// 32 of the other projection, so that a lane has both values of an output.  G and U are fp32 until h is rounded; for a
+// backward to come they are stored as they are where that costs less than forming them again.
 //
 // Up to 64 tokens take gated_few_kernel, which is bound by reading the weights: a workgroup has 16 columns of both,
 // its 8 waves take k in turns of 64 bytes a column and go from memory to the matrix cores without LDS; their sums meet there.
@@ -20,6 +20,16 @@ namespace {
 
 constexpr int kFewRows = 64, kFewWaves = 8;
 
+// Values of 16 bytes, of the few tokens' kernel, which takes fp32 as it is.
+template <class Ty>
+struct Elem {
+  static constexpr int kSize = 2, kPiece = 8;
+};
+template <>
+struct Elem<F32> {
+  static constexpr int kSize = 4, kPiece = 4;
+};
+
 template <class Ty>
 __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) { return Ty::mma16k32(a, b, c); }
 template <>
@@ -31,22 +41,22 @@ __device__ __forceinline__ f32x4 mma16<F32>(u32x4 a, u32x4 b, f32x4 c) {
 
 // TG: groups of 16 tokens.
 template <class Ty, int TG>
-__global__ void __launch_bounds__(kFewWaves * 64, 2) gated_few_kernel(GatedArgs a) {
+__global__ void __launch_bounds__(kFewWaves * 64, 2) gated_few_kernel(OwGatedLinear d, void* h_out) {
   constexpr int S = Elem<Ty>::kSize, V = Elem<Ty>::kPiece, KS = 4 * V;  // k of a step
   __shared__ f32x4 part[kFewWaves][2 * TG][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, h = lane >> 4;
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
   // Columns and tokens behind the last one are the last one; nobody stores them.
-  const int64_t n = n0 + l16 < a.hidden ? n0 + l16 : a.hidden - 1, ld = static_cast<int64_t>(a.channels) * S;
-  const char* w[2] = {a.w[0] + n * ld + h * 16, a.w[1] + n * ld + h * 16};
+  const int64_t n = n0 + l16 < d.hidden ? n0 + l16 : d.hidden - 1, at_w = n * d.channels * S + h * 16;
+  const char* w[2] = {static_cast<const char*>(d.gate_weight) + at_w, static_cast<const char*>(d.up_weight) + at_w};
   const char* x[TG];
 #pragma unroll
-  for (int g = 0; g < TG; ++g) x[g] = a.x + (16 * g + l16 < a.rows ? 16 * g + l16 : a.rows - 1) * a.x_ld + h * 16;
+  for (int g = 0; g < TG; ++g) x[g] = static_cast<const char*>(d.x) + (16 * g + l16 < d.rows ? 16 * g + l16 : d.rows - 1) * d.x_stride * S + h * 16;
   f32x4 acc[2][TG];
 #pragma unroll
   for (int g = 0; g < TG; ++g) acc[0][g] = acc[1][g] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int whole = a.channels / KS;
+  const int whole = d.channels / KS;
   // Four steps' loads are in flight together.
   constexpr int U = 4;
   for (int s = wave; s < whole; s += U * kFewWaves) {
@@ -73,8 +83,8 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) gated_few_kernel(GatedArgs 
         acc[1][g] = mma16<Ty>(wu[u], v[u][g], acc[1][g]);
       }
   }
-  if (whole * KS < a.channels && wave == whole % kFewWaves) {
-    const int64_t at = static_cast<int64_t>(whole) * 64, left = a.channels - whole * KS - h * V;
+  if (whole * KS < d.channels && wave == whole % kFewWaves) {
+    const int64_t at = static_cast<int64_t>(whole) * 64, left = d.channels - whole * KS - h * V;
     const u32x4 wg = load_piece<S>(w[0] + at, left), wu = load_piece<S>(w[1] + at, left);
 #pragma unroll
     for (int g = 0; g < TG; ++g) {
@@ -94,17 +104,17 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) gated_few_kernel(GatedArgs 
 #pragma unroll
     for (int k = 0; k < kFewWaves; ++k) G += part[k][g][at][e], U += part[k][TG + g][at][e];
     const int64_t row = 16 * g + (at & 15), col = n0 + 4 * (at >> 4) + e;
-    if (row >= a.rows || col >= a.hidden) continue;
-    static_cast<typename Row<Ty>::Elem*>(a.out[0])[row * a.hidden + col] = Row<Ty>::from_f32(G * U * sigmoid(G));
+    if (row >= d.rows || col >= d.hidden) continue;
+    static_cast<typename Row<Ty>::Elem*>(h_out)[row * d.hidden + col] = Row<Ty>::from_f32(G * U * sigmoid(G));
   }
 }
 
 template <class Ty>
-void launch_few(const GatedArgs& a, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>(ceil_div(a.hidden, 16))), block(kFewWaves * 64);
-  if (a.rows <= 16) hipLaunchKernelGGL((gated_few_kernel<Ty, 1>), grid, block, 0, s, a);
-  else if (a.rows <= 32) hipLaunchKernelGGL((gated_few_kernel<Ty, 2>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((gated_few_kernel<Ty, 4>), grid, block, 0, s, a);
+void launch_few(const OwGatedLinear& d, void* h, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>(ceil_div(d.hidden, 16))), block(kFewWaves * 64);
+  if (d.rows <= 16) hipLaunchKernelGGL((gated_few_kernel<Ty, 1>), grid, block, 0, s, d, h);
+  else if (d.rows <= 32) hipLaunchKernelGGL((gated_few_kernel<Ty, 2>), grid, block, 0, s, d, h);
+  else hipLaunchKernelGGL((gated_few_kernel<Ty, 4>), grid, block, 0, s, d, h);
 }
 
 }  // namespace
@@ -127,52 +137,111 @@ int check_gated(const OwGatedLinear* d) {
   return OW_OK;
 }
 
-GatedArgs gated_args(const OwGatedLinear& d) {
-  GatedArgs a{};
-  const int64_t size = d.dtype == OW_DTYPE_F32 ? 4 : 2, piece = 16 / size;
-  a.x = static_cast<const char*>(d.x);
-  a.w[0] = static_cast<const char*>(d.gate_weight);
-  a.w[1] = static_cast<const char*>(d.up_weight);
-  a.x_ld = d.x_stride * size;
-  a.rows = d.rows;
-  a.channels = d.channels;
-  a.hidden = d.hidden;
-  a.ld_gu = static_cast<int32_t>(ceil_div(d.hidden, piece) * piece);
-  return a;
+namespace {
+
+// Rows of values, of any alignment, to planes of rows of whole pieces with zeros behind them: a copy of 16-bit values, or fp32
+// ones in three bf16 parts.  A thread has a piece of 8 values.
+template <bool WIDE>
+__global__ void __launch_bounds__(256) gated_pack_kernel(const char* src, int64_t src_ld, int64_t rows, int32_t values, char* dst, int64_t ld,
+                                                         int64_t plane) {
+  const uint32_t pieces = static_cast<uint32_t>(ld / 16);
+  const int64_t all = rows * pieces, step = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += step) {
+    const int64_t row = i / pieces;
+    const int c = static_cast<int>(i - row * pieces) * 8, n = values - c;
+    char* out = dst + row * ld + c * 2;
+    if constexpr (WIDE) {
+      const char* in = src + row * src_ld + static_cast<int64_t>(c) * 4;
+      const u32x4 lo = load_piece<4>(in, n), hi = load_piece<4>(in + 16, n - 4);
+      const X3 parts = x3_split8<true>([&](int j) { return __uint_as_float(j < 4 ? lo[j] : hi[j - 4]); });
+#pragma unroll
+      for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4*>(out + p * plane) = parts.p[p];
+    } else {
+      *reinterpret_cast<u32x4*>(out) = load_piece<2>(src + row * src_ld + static_cast<int64_t>(c) * 2, n);
+    }
+  }
 }
 
-// Whether x, or both weights, lie in whole pieces of 16 bytes; offsets inside a tile of 256 rows have 31 bits.
-bool gated_x_direct(const GatedArgs& a, int64_t size) {
-  return reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_ld % 16 == 0 && a.x_ld >= 0 && a.x_ld < (int64_t(1) << 22) &&
-         a.channels * size % 16 == 0;
-}
-bool gated_w_direct(const GatedArgs& a, int64_t size) {
-  return (reinterpret_cast<uintptr_t>(a.w[0]) | reinterpret_cast<uintptr_t>(a.w[1])) % 16 == 0 && a.channels * size % 16 == 0;
-}
-
-void apply_plan(GatedArgs& a, const GatedPlan& p) {
-  a.tiles_r = p.tiles_r;
-  a.tiles_c = p.tiles_c;
-  a.splits = p.splits;
-  a.k_tiles = p.k_tiles;
-  a.k_split = p.k_split;
-  // (Numbers past 2^31 are refused before a launch.)
-  a.by_tiles = Divisor::of(static_cast<uint32_t>(p.tiles_r * p.tiles_c));
-  a.by_group = Divisor::of(8 * static_cast<uint32_t>(p.tiles_c));
+int pack(const void* src, int64_t src_ld, int64_t rows, int32_t values, bool wide, const GatedPlanes& to, hipStream_t s) {
+  const int64_t groups = ceil_div(rows * (to.ld / 16), 256), most = 16 * static_cast<int64_t>(device_cus());
+  const dim3 grid(static_cast<unsigned>(groups < most ? groups : most));
+  char* dst = const_cast<char*>(to.at);
+  const char* from = static_cast<const char*>(src);
+  if (wide) hipLaunchKernelGGL((gated_pack_kernel<true>), grid, dim3(256), 0, s, from, src_ld, rows, values, dst, to.ld, to.plane);
+  else hipLaunchKernelGGL((gated_pack_kernel<false>), grid, dim3(256), 0, s, from, src_ld, rows, values, dst, to.ld, to.plane);
+  return hip_status(hipGetLastError(), "gated_pack_kernel launch");
 }
 
+size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+int64_t row_bytes(int32_t values) { return ceil_div(values, 8) * 16; }
+
+// Whether x, or both weights, can be read as they lie: 16-bit values in whole pieces, offsets inside a tile of 256 rows of 31 bits.
+bool x_direct(const OwGatedLinear& d) {
+  return d.dtype != OW_DTYPE_F32 && reinterpret_cast<uintptr_t>(d.x) % 16 == 0 && d.x_stride % 8 == 0 && d.x_stride >= 0 &&
+         d.x_stride < (int64_t(1) << 21) && d.channels % 8 == 0;
+}
+bool w_direct(const OwGatedLinear& d) {
+  return d.dtype != OW_DTYPE_F32 && d.channels % 8 == 0 &&
+         (reinterpret_cast<uintptr_t>(d.gate_weight) | reinterpret_cast<uintptr_t>(d.up_weight)) % 16 == 0;
+}
+
+}  // namespace
+
+size_t gated_operand_bytes(const OwGatedLinear& d) {
+  const size_t planes = d.dtype == OW_DTYPE_F32 ? 3 : 1, row = static_cast<size_t>(row_bytes(d.channels));
+  return (x_direct(d) ? 0 : aligned(planes * d.rows * row)) + (w_direct(d) ? 0 : 2 * aligned(planes * d.hidden * row));
+}
+
+int gated_operands(const OwGatedLinear& d, char* workspace, GatedArgs* a, hipStream_t s) {
+  const bool wide = d.dtype == OW_DTYPE_F32;
+  const int64_t size = wide ? 4 : 2, ld = row_bytes(d.channels);
+  a->rows = d.rows;
+  a->channels = d.channels;
+  a->hidden = d.hidden;
+  a->x = GatedPlanes{static_cast<const char*>(d.x), d.x_stride * 2, 0};
+  const void* weights[2] = {d.gate_weight, d.up_weight};
+  for (int i = 0; i < 2; ++i) a->w[i] = GatedPlanes{static_cast<const char*>(weights[i]), d.channels * 2, 0};
+  if (!x_direct(d)) {
+    a->x = GatedPlanes{workspace, ld, d.rows * ld};
+    workspace += aligned((wide ? 3 : 1) * d.rows * ld);
+    if (int rc = pack(d.x, d.x_stride * size, d.rows, d.channels, wide, a->x, s)) return rc;
+  }
+  if (!w_direct(d)) {
+    for (int i = 0; i < 2; ++i) {
+      a->w[i] = GatedPlanes{workspace, ld, d.hidden * ld};
+      workspace += aligned((wide ? 3 : 1) * d.hidden * ld);
+      if (int rc = pack(weights[i], d.channels * size, d.hidden, d.channels, wide, a->w[i], s)) return rc;
+    }
+  }
+  return OW_OK;
+}
+
+namespace {
+
+GatedPlan plan_forward(const OwGatedLinear& d) {
+  return gated_plan(d.rows, 2 * static_cast<int64_t>(d.hidden), gated_k_tiles(d.channels, d.dtype), 1, true, true);
+}
+
+}  // namespace
 }  // namespace ow
 
 extern "C" {
 
-// The products are kept where forming them again (4 K operations a value) would take longer than to write and read them (16 bytes).
+// The products are kept where forming them again (4 K operations a value, six times as many for fp32) would take longer than
+// to write and read them (16 bytes).
 size_t ow_gated_linear_kept(const OwGatedLinear* d) {
   if (d == nullptr || d->rows <= ow::kFewRows || d->channels <= 0 || d->hidden <= 0) return 0;
   const int32_t from = d->dtype == OW_DTYPE_F32 ? 128 : 1536;
   return d->channels >= from ? static_cast<size_t>(2) * d->rows * d->hidden * sizeof(float) : 0;
 }
 
-int ow_gated_linear_fwd(const OwGatedLinear* d, void* h, void* kept, void* stream) {
+size_t ow_gated_linear_fwd_workspace(const OwGatedLinear* d) {
+  if (d == nullptr || d->rows <= ow::kFewRows || d->channels <= 0 || d->hidden <= 0) return 0;
+  return ow::gated_operand_bytes(*d) + ow::gated_partial_bytes(ow::plan_forward(*d));
+}
+
+int ow_gated_linear_fwd(const OwGatedLinear* d, void* h, void* kept, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = ow::check_gated(d)) return rc;
   if (d->rows == 0 || d->hidden == 0) {
     ow::clear_error();
@@ -182,24 +251,29 @@ int ow_gated_linear_fwd(const OwGatedLinear* d, void* h, void* kept, void* strea
   OW_CHECK_ARG(h != nullptr, "h is NULL");
   OW_CHECK_ARG(kept == nullptr || (ow_gated_linear_kept(d) != 0 && reinterpret_cast<uintptr_t>(kept) % 4 == 0),
                "the products of these sizes are not kept, or have no place for fp32 values");
-  ow::GatedArgs a = ow::gated_args(*d);
-  a.out[0] = h;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (d->rows <= ow::kFewRows) {
-    if (d->dtype == OW_DTYPE_BF16) ow::launch_few<ow::BF16>(a, s);
-    else if (d->dtype == OW_DTYPE_F16) ow::launch_few<ow::F16>(a, s);
-    else ow::launch_few<ow::F32>(a, s);
+    if (d->dtype == OW_DTYPE_BF16) ow::launch_few<ow::BF16>(*d, h, s);
+    else if (d->dtype == OW_DTYPE_F16) ow::launch_few<ow::F16>(*d, h, s);
+    else ow::launch_few<ow::F32>(*d, h, s);
     if (int rc = ow::hip_status(hipGetLastError(), "gated_few_kernel launch")) return rc;
   } else {
-    const int64_t size = d->dtype == OW_DTYPE_F32 ? 4 : 2;
-    const ow::GatedPlan p = ow::gated_plan(d->rows, 2 * static_cast<int64_t>(d->hidden), ow::ceil_div(d->channels * size, 128), 1, false, size == 4);
-    OW_CHECK_SUPPORTED(p.tiles_r * p.tiles_c < (int64_t(1) << 31), "gated linear: too many tiles for a launch");
-    ow::apply_plan(a, p);
+    const ow::GatedPlan p = ow::plan_forward(*d);
+    OW_CHECK_SUPPORTED(p.units < (int64_t(1) << 31), "gated linear: too many tiles for a launch");
+    const size_t need = ow_gated_linear_fwd_workspace(d), operands = ow::gated_operand_bytes(*d);
+    OW_CHECK_ARG(need == 0 || (workspace != nullptr && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
+                 "workspace of %zu bytes; %zu are needed, 16-byte aligned", workspace_bytes, need);
+    ow::GatedArgs a{};
+    char* ws = static_cast<char*>(workspace);
+    if (int rc = ow::gated_operands(*d, ws, &a, s)) return rc;
+    a.out[0] = h;
     a.kept = static_cast<float*>(kept);
-    const bool direct = ow::gated_x_direct(a, size) && ow::gated_w_direct(a, size);
-    if (kept != nullptr) ow::launch_gated_mode<ow::kGatedKeep>(a, p.size, d->dtype, direct, s);
-    else ow::launch_gated_mode<ow::kGatedForward>(a, p.size, d->dtype, direct, s);
-    if (int rc = ow::hip_status(hipGetLastError(), "gated_tile_kernel launch")) return rc;
+    float* partial = reinterpret_cast<float*>(ws + operands);
+    if (kept != nullptr) {
+      if (int rc = ow::launch_gated_mode<ow::kGatedKeep>(a, p, d->dtype, d->channels, partial, s)) return rc;
+    } else {
+      if (int rc = ow::launch_gated_mode<ow::kGatedForward>(a, p, d->dtype, d->channels, partial, s)) return rc;
+    }
   }
   ow::clear_error();
   return OW_OK;

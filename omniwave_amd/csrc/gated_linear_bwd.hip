@@ -5,9 +5,6 @@
 // Three products on the tiles of ow_gated.h: G and U are formed again from x and become dG and dU in the same kernel, or
 // gated_gates_kernel reads what the forward kept of them (ow_gated_linear_kept); dx is one product over both halves; the weights' gradients are
 // products over the tokens.  dG and dU are rounded to x's type, the operands of the other two.
-//
-// Where an output has fewer tiles than the chip has compute units, k is cut into parts, whose fp32 sums
-// gated_sum_kernel adds in their order.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -17,116 +14,85 @@
 namespace ow {
 
 int check_gated(const OwGatedLinear* d);
-GatedArgs gated_args(const OwGatedLinear& d);
-bool gated_x_direct(const GatedArgs& a, int64_t size);
-bool gated_w_direct(const GatedArgs& a, int64_t size);
-void apply_plan(GatedArgs& a, const GatedPlan& p);
+size_t gated_operand_bytes(const OwGatedLinear& d);
+int gated_operands(const OwGatedLinear& d, char* workspace, GatedArgs* a, hipStream_t s);
 
 namespace {
 
-struct GatedSumArgs {
-  const float* partial;  // [splits][sets][n]
-  void* out[2];
-  int64_t n;
-  int32_t splits, sets, dtype;
-};
-
-__global__ void __launch_bounds__(256) gated_sum_kernel(GatedSumArgs a) {
-  const int set = blockIdx.y;
-  if (a.out[set] == nullptr) return;
-  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
-  if (i >= a.n) return;
-  const float* p = a.partial + set * a.n + i;
-  const int64_t step = a.sets * a.n;
-  if (i + 4 <= a.n) {
-    f32x4 sum = *reinterpret_cast<const f32x4_any*>(p);
-#pragma unroll 4
-    for (int s = 1; s < a.splits; ++s) sum += *reinterpret_cast<const f32x4_any*>(p + s * step);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) store_any(a.out[set], a.dtype, i + j, sum[j]);
-  } else {
-    for (int j = 0; i + j < a.n; ++j) {
-      float sum = p[j];
-      for (int s = 1; s < a.splits; ++s) sum += p[s * step + j];
-      store_any(a.out[set], a.dtype, i + j, sum);
-    }
-  }
-}
-
-int sum_parts(const GatedArgs& a, int64_t n, int sets, int dtype, hipStream_t s) {
-  GatedSumArgs m{};
-  m.partial = a.partial;
-  m.out[0] = a.out[0], m.out[1] = a.out[1];
-  m.n = n;
-  m.splits = a.splits;
-  m.sets = sets;
-  m.dtype = dtype;
-  hipLaunchKernelGGL(gated_sum_kernel, dim3(static_cast<unsigned>(ceil_div(n, 1024)), sets), dim3(256), 0, s, m);
-  return hip_status(hipGetLastError(), "gated_sum_kernel launch");
-}
-
-// dG and dU from kept products, a piece of 16 bytes of a row a thread; pieces behind `hidden` are zeros.
-template <class Ty>
+// dG and dU from kept products, a piece of 8 values of a row a thread; values behind `hidden` are zeros.
+template <class Ty, class Out>
 __global__ void __launch_bounds__(256) gated_gates_kernel(GatedArgs a) {
-  constexpr int S = Elem<Ty>::kSize, V = Elem<Ty>::kPiece;
-  typedef Row<Ty> R;
-  const uint32_t pieces = static_cast<uint32_t>(a.ld_gu / V);
+  constexpr bool kWide = std::is_same<Out, F32>::value;
+  constexpr int S = kWide ? 4 : 2, V = 16 / S;
+  typedef Row<Out> R;
+  const uint32_t pieces = static_cast<uint32_t>(a.gu[0].ld / 16);
   const int64_t all = a.rows * pieces, step = static_cast<int64_t>(gridDim.x) * 256;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += step) {
     const int64_t row = i / pieces;
-    const int c = static_cast<int>(i - row * pieces) * V, n = a.hidden - c;
-    const float *g = a.kept + row * a.hidden + c, *u = g + a.rows * a.hidden;
-    float dh[V], dg[V], du[V];
-    R::widen(__builtin_bit_cast(typename R::Raw, load_piece<S>(a.dh + row * a.dh_ld + c * S, n)), dh);
-    u32x4 gw[V / 4], uw[V / 4];
+    const int c = static_cast<int>(i - row * pieces) * 8, n = a.hidden - c;
+    const char* g = reinterpret_cast<const char*>(a.kept + row * a.hidden + c);
+    const char* u = g + a.rows * a.hidden * 4;
+    float dh[8], d[2][8];
 #pragma unroll
-    for (int k = 0; k < V / 4; ++k) {
-      gw[k] = load_piece<4>(reinterpret_cast<const char*>(g + 4 * k), n - 4 * k);
-      uw[k] = load_piece<4>(reinterpret_cast<const char*>(u + 4 * k), n - 4 * k);
+    for (int k = 0; k < 8 / V; ++k) {
+      float v[V];
+      R::widen(__builtin_bit_cast(typename R::Raw, load_piece<S>(a.dh + row * a.dh_ld + (c + k * V) * S, n - k * V)), v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) dh[k * V + j] = v[j];
+    }
+    u32x4 gw[2], uw[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      gw[k] = load_piece<4>(g + 16 * k, n - 4 * k);
+      uw[k] = load_piece<4>(u + 16 * k, n - 4 * k);
     }
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float gj = __uint_as_float(gw[j / 4][j % 4]), uj = __uint_as_float(uw[j / 4][j % 4]), s = sigmoid(gj);
-      du[j] = dh[j] * (gj * s);
-      dg[j] = dh[j] * uj * (s * (1.f + gj * (1.f - s)));
+    for (int j = 0; j < 8; ++j) gates(dh[j], __uint_as_float(gw[j / 4][j % 4]), __uint_as_float(uw[j / 4][j % 4]), d[0][j], d[1][j]);
+    const int64_t at = row * a.gu[0].ld + c * 2;
+#pragma unroll
+    for (int o = 0; o < 2; ++o) {
+      char* out = static_cast<char*>(a.out[o]) + at;
+      if constexpr (kWide) {
+        const X3 parts = x3_split8([&](int j) { return d[o][j]; });
+#pragma unroll
+        for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4*>(out + p * a.gu[0].plane) = parts.p[p];
+      } else {
+        R::store(reinterpret_cast<typename R::Elem*>(out), d[o]);
+      }
     }
-    const int64_t at = row * a.ld_gu + c;
-    R::store(static_cast<typename R::Elem*>(a.out[0]) + at, dg);
-    R::store(static_cast<typename R::Elem*>(a.out[1]) + at, du);
   }
 }
 
 int gates_of_kept(const GatedArgs& a, int dtype, hipStream_t s) {
-  const int64_t all = a.rows * (a.ld_gu / (dtype == OW_DTYPE_F32 ? 4 : 8)), most = 16 * static_cast<int64_t>(device_cus());
-  const int64_t groups = ceil_div(all, 256);
+  const int64_t groups = ceil_div(a.rows * (a.gu[0].ld / 16), 256), most = 16 * static_cast<int64_t>(device_cus());
   const dim3 grid(static_cast<unsigned>(groups < most ? groups : most));
-  if (dtype == OW_DTYPE_BF16) hipLaunchKernelGGL((gated_gates_kernel<BF16>), grid, dim3(256), 0, s, a);
-  else if (dtype == OW_DTYPE_F16) hipLaunchKernelGGL((gated_gates_kernel<F16>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((gated_gates_kernel<F32>), grid, dim3(256), 0, s, a);
+  if (dtype == OW_DTYPE_BF16) hipLaunchKernelGGL((gated_gates_kernel<BF16, BF16>), grid, dim3(256), 0, s, a);
+  else if (dtype == OW_DTYPE_F16) hipLaunchKernelGGL((gated_gates_kernel<F16, F16>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((gated_gates_kernel<BF16, F32>), grid, dim3(256), 0, s, a);
   return hip_status(hipGetLastError(), "gated_gates_kernel launch");
 }
 
-GatedPlan plan_gates(const OwGatedLinear& d, int64_t size) {
-  return gated_plan(d.rows, 2 * static_cast<int64_t>(d.hidden), ceil_div(d.channels * size, 128), 1, false, size == 4);
+GatedPlan plan_gates(const OwGatedLinear& d) {
+  return gated_plan(d.rows, 2 * static_cast<int64_t>(d.hidden), gated_k_tiles(d.channels, d.dtype), 1, true, false);
 }
-GatedPlan plan_dx(const OwGatedLinear& d, int64_t size) {
-  return gated_plan(d.rows, d.channels, 2 * ceil_div(d.hidden * size, 128), 1, true, size == 4);
-}
-GatedPlan plan_dw(const OwGatedLinear& d, int64_t size) {
-  return gated_plan(d.hidden, d.channels, ceil_div(d.rows * size, 128), 2, true, size == 4);
-}
+GatedPlan plan_dx(const OwGatedLinear& d) { return gated_plan(d.rows, d.channels, 2 * gated_k_tiles(d.hidden, d.dtype), 1, false, true); }
+GatedPlan plan_dw(const OwGatedLinear& d) { return gated_plan(d.hidden, d.channels, gated_k_tiles(d.rows, d.dtype), 2, false, true); }
 
-// Bytes of dG and dU (each), and of the parts of dx or the weights' gradients.
+// Bytes of x and the weights where they are copied, of a plane of dG and dU, and of the parts of dx or the weights' gradients.
 struct Space {
-  size_t gu, parts;
+  size_t operands, ld, plane, parts;
+  int planes;
+  size_t all() const { return operands + 2 * planes * plane + parts; }
 };
 Space space_of(const OwGatedLinear& d) {
-  const int64_t size = d.dtype == OW_DTYPE_F32 ? 4 : 2;
-  const GatedPlan x = plan_dx(d, size), w = plan_dw(d, size);
-  const size_t px = x.splits > 1 ? static_cast<size_t>(x.splits) * d.rows * d.channels * 4 : 0;
-  const size_t pw = w.splits > 1 ? static_cast<size_t>(w.splits) * 2 * d.hidden * d.channels * 4 : 0;
-  const GatedArgs a = gated_args(d);
-  return Space{(static_cast<size_t>(d.rows) * a.ld_gu * size + 255) / 256 * 256, px > pw ? px : pw};
+  const size_t x = gated_partial_bytes(plan_dx(d)), w = gated_partial_bytes(plan_dw(d));
+  Space s;
+  s.operands = gated_operand_bytes(d);
+  s.ld = static_cast<size_t>(ceil_div(d.hidden, 8)) * 16;
+  s.plane = (static_cast<size_t>(d.rows) * s.ld + 255) / 256 * 256;
+  s.parts = x > w ? x : w;
+  s.planes = d.dtype == OW_DTYPE_F32 ? 3 : 1;
+  return s;
 }
 
 }  // namespace
@@ -136,60 +102,50 @@ extern "C" {
 
 size_t ow_gated_linear_bwd_workspace(const OwGatedLinear* d) {
   if (d == nullptr || d->rows <= 0 || d->channels <= 0 || d->hidden <= 0) return 0;
-  const ow::Space s = ow::space_of(*d);
-  return 2 * s.gu + s.parts;
+  return ow::space_of(*d).all();
 }
 
-int ow_gated_linear_bwd(const OwGatedLinear* d, const void* kept, const void* dh, int64_t dh_stride, void* dx, void* dgate_weight,
-                        void* dup_weight, void* workspace, size_t workspace_bytes, void* stream) {
+int ow_gated_linear_bwd(const OwGatedLinear* d, const void* kept, const void* dh, int64_t dh_stride, void* dx,
+                        void* dgate_weight, void* dup_weight, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = ow::check_gated(d)) return rc;
   OW_CHECK_ARG(d->rows > 0 && d->channels > 0 && d->hidden > 0, "the backward of empty products has no kernel");
   const int64_t size = d->dtype == OW_DTYPE_F32 ? 4 : 2;
   OW_CHECK_ARG(dh != nullptr && reinterpret_cast<uintptr_t>(dh) % size == 0, "dh is NULL or not aligned to its values");
   OW_CHECK_ARG(reinterpret_cast<uintptr_t>(kept) % 4 == 0, "the kept products are not aligned to fp32 values");
-  const size_t need = ow_gated_linear_bwd_workspace(d);
+  const ow::Space space = ow::space_of(*d);
+  const size_t need = space.all();
   OW_CHECK_ARG(workspace != nullptr && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
                "workspace of %zu bytes; %zu are needed, 16-byte aligned", workspace_bytes, need);
-  const ow::GatedPlan gates = ow::plan_gates(*d, size), to_x = ow::plan_dx(*d, size), to_w = ow::plan_dw(*d, size);
+  const ow::GatedPlan gates = ow::plan_gates(*d), to_x = ow::plan_dx(*d), to_w = ow::plan_dw(*d);
   for (const ow::GatedPlan& p : {gates, to_x, to_w})
-    OW_CHECK_SUPPORTED(p.tiles_r * p.tiles_c * p.splits < (int64_t(1) << 31), "gated linear: too many tiles for a launch");
-  const ow::Space space = ow::space_of(*d);
-  char* ws = static_cast<char*>(workspace);
+    OW_CHECK_SUPPORTED(p.units < (int64_t(1) << 31), "gated linear: too many tiles for a launch");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  ow::GatedArgs a = ow::gated_args(*d);
-  const bool x_direct = ow::gated_x_direct(a, size), w_direct = ow::gated_w_direct(a, size);
+  ow::GatedArgs a{};
+  char* ws = static_cast<char*>(workspace);
+  if (int rc = ow::gated_operands(*d, ws, &a, s)) return rc;
+  ws += space.operands;
+  for (int i = 0; i < 2; ++i) {
+    a.gu[i] = ow::GatedPlanes{ws, static_cast<int64_t>(space.ld), static_cast<int64_t>(space.plane)};
+    a.out[i] = ws;
+    ws += space.planes * space.plane;
+  }
+  float* partial = reinterpret_cast<float*>(ws);
   a.dh = static_cast<const char*>(dh);
   a.dh_ld = dh_stride * size;
-  a.dgu[0] = ws;
-  a.dgu[1] = ws + space.gu;
-  a.partial = reinterpret_cast<float*>(ws + 2 * space.gu);
-  a.out[0] = ws;
-  a.out[1] = ws + space.gu;
   if (kept != nullptr) {
     a.kept = static_cast<float*>(const_cast<void*>(kept));
     if (int rc = ow::gates_of_kept(a, d->dtype, s)) return rc;
   } else {
-    ow::apply_plan(a, gates);
-    ow::launch_gated_mode<ow::kGatedGates>(a, gates.size, d->dtype, x_direct && w_direct, s);
-    if (int rc = ow::hip_status(hipGetLastError(), "gated_tile_kernel launch")) return rc;
+    if (int rc = ow::launch_gated_mode<ow::kGatedGates>(a, gates, d->dtype, d->channels, partial, s)) return rc;
   }
   if (dx != nullptr) {
     a.out[0] = dx;
-    a.out[1] = nullptr;
-    ow::apply_plan(a, to_x);
-    ow::launch_gated_mode<ow::kGatedDx>(a, to_x.size, d->dtype, w_direct, s);
-    if (int rc = ow::hip_status(hipGetLastError(), "gated_tile_kernel launch")) return rc;
-    if (a.splits > 1)
-      if (int rc = ow::sum_parts(a, d->rows * d->channels, 1, d->dtype, s)) return rc;
+    if (int rc = ow::launch_gated_mode<ow::kGatedDx>(a, to_x, d->dtype, d->hidden, partial, s)) return rc;
   }
   if (dgate_weight != nullptr || dup_weight != nullptr) {
     a.out[0] = dgate_weight;
     a.out[1] = dup_weight;
-    ow::apply_plan(a, to_w);
-    ow::launch_gated_mode<ow::kGatedDw>(a, to_w.size, d->dtype, x_direct, s);
-    if (int rc = ow::hip_status(hipGetLastError(), "gated_tile_kernel launch")) return rc;
-    if (a.splits > 1)
-      if (int rc = ow::sum_parts(a, static_cast<int64_t>(d->hidden) * d->channels, 2, d->dtype, s)) return rc;
+    if (int rc = ow::launch_gated_mode<ow::kGatedDw>(a, to_w, d->dtype, d->rows, partial, s)) return rc;
   }
   ow::clear_error();
   return OW_OK;

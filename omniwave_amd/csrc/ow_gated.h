@@ -1,25 +1,30 @@
 // Tiles of the gated feed-forward products (gated_linear.hip, gated_linear_bwd.hip): one matrix product kernel in which
 // an output tile O[r][c] = sum_k R[r][k] C[c][k] is formed by MFMA from tiles of both operands in LDS.
 //
-// An operand lies in memory with its contraction index contiguous (kAlongK: x and the weights forward, the gates'
-// gradients in dx) or with its output index contiguous (kAcrossK: the weights in dx, every operand of the weights'
-// gradients).  The tile in LDS keeps that order, in pieces of 16 bytes:
+// Operands are of 16 bits.  fp32 ones are three bf16 planes each (ow_x3.h), and a product of two is the six products of
+// planes whose weight is above 2^-24, one after the other along k: to the kernel, k is six times as long.  (fp32 MFMAs have a
+// sixteenth of the bf16 ones' rate; 25,088 tokens, 256 to 512: forward 141 us by them.)
 //
-//   kAlongK    rows of 128 bytes (64 values of 16 bits, 32 of fp32); piece p of row r at slot p ^ (r & 7), so that eight
-//              rows' pieces of one column fall in eight bank windows; a lane reads its 16 bytes of k at once
-//   kAcrossK   a row for each k; 16-bit values are read transposed (ds_read_b64_tr_b16: 4 k of 16 output indexes by
-//              16 lanes), 32-byte pairs of row k at pair ^ (k & 7), fp32 values one by one, rows with k & 4 moved by 128 bytes
+// An operand lies in memory with its contraction index contiguous (AlongK: x and the weights forward, the gates'
+// gradients in dx) or with its output index contiguous (AcrossK: the weights in dx, every operand of the weights'
+// gradients), in rows of whole 16-byte pieces: what does not lie so is copied first (gated_pack_kernel).  The tile in LDS
+// keeps that order:
 //
-// A step takes 16 bytes of k from each half of the wave: one 32x32x16 MFMA for 16-bit types, four 32x32x2 for fp32.  Its A operand is
-// C, its B operand R: a lane then has 16 values of one row r, in runs of 4 along c, which go through LDS to be stored
-// in whole rows of the wave's tile (Turn).
+//   AlongK     rows of 128 bytes (64 values), of which a lane reads 16 bytes of k at once; piece p of row r at slot
+//              p ^ (r / 2 & 7), so that 16 rows' pieces of one column fill the 256 bytes of all banks
+//   AcrossK    a row for each k, read transposed (ds_read_b64_tr_b16: 4 k of 16 output indexes by 16 lanes); piece p of row k
+//              at p ^ 4 (k & 3), so that 4 rows' 64 bytes fill them
 //
-// Tiles come by direct copies into LDS (16 bytes a lane; what lies outside the matrix reads as zeros), one tile ahead
-// of the products: 128 KB for both stages of 256 x 256, one workgroup of 8 waves a compute unit.  Operands that do not lie in whole 16-byte
-// pieces come through registers instead, value by value at the ends of rows.
+// A step is one 32x32x16 MFMA for each product of a wave.  Its A operand is C, its B operand R: a lane then has 16 values of
+// one row r, in runs of 4 along c, which go through LDS to be stored in whole rows of the wave's tile (Turn).
+//
+// Tiles come by direct copies into LDS (16 bytes a lane; what lies outside the matrix reads as zeros), a tile ahead of
+// the products, and a step's operands are read during the step before it.  6,272 tokens of 4,096 to 8,192 bf16: 738 us
+// forward (1,140 TFLOP/s; the library's product of that size 719 us), the weights' gradients 745.
 #pragma once
 
 #include "ow_rows.h"
+#include "ow_x3.h"
 
 namespace ow {
 
@@ -32,6 +37,7 @@ enum GatedMode {
   kGatedDx,       // dG Wg + dU Wu
   kGatedDw,       // dG^T x, dU^T x
 };
+constexpr bool gated_pair(int mode) { return mode == kGatedForward || mode == kGatedKeep || mode == kGatedGates; }
 
 // Division of numbers below 2^31 by one that the host knows: n / d = n mul >> shift.
 struct Divisor {
@@ -44,21 +50,34 @@ struct Divisor {
   __device__ __forceinline__ uint32_t divide(uint32_t n) const { return static_cast<uint32_t>(static_cast<uint64_t>(n) * mul >> shift); }
 };
 
-struct GatedArgs {
-  const char* x;
-  const char* w[2];   // gate, up
-  const char* dh;
-  const char* dgu[2]; // dG, dU: [rows][ld_gu]
-  int64_t x_ld, dh_ld;  // bytes
-  void* out[2];       // h; dG, dU; dx; dgate, dup
-  float* partial;     // [splits][outputs], fp32; used where splits > 1
-  float* kept;        // [2][rows][hidden]: G and U, for kGatedKeep
-  int64_t rows;
-  int32_t channels, hidden, ld_gu;  // ld_gu: hidden, up to whole 16-byte pieces
+// An operand's planes, rows of `ld` bytes, whole pieces.
+struct GatedPlanes {
+  const char* at;
+  int64_t ld, plane;
+};
+
+// How a product is cut: a unit is a tile with its whole k (the first `whole` of them), or one of `parts` parts of the k of one of
+// the other tiles.
+struct GatedPlan {
+  int size;  // 0: TileL, 1: TileM, 2: TileS
   int64_t tiles_r;
-  int32_t tiles_c, splits;
-  int64_t k_tiles, k_split;  // tiles of k in all, and of a split
-  Divisor by_tiles, by_group;  // tiles_r tiles_c, 8 tiles_c
+  int32_t tiles_c, parts;
+  int64_t whole, units;
+  int64_t k_tiles, k_part;  // tiles of k (64 values) in all, and of a part
+};
+
+struct GatedArgs {
+  GatedPlanes x, w[2], gu[2];  // w: gate, up; gu: dG, dU
+  const char* dh;
+  int64_t dh_ld;       // bytes
+  void* out[2];        // h; dG, dU; dx; dgate, dup
+  float* kept;         // [2][rows][hidden]: G and U
+  float* partial;      // [units - whole][tile rows][tile columns]
+  int64_t rows;
+  int32_t channels, hidden;
+  int32_t k_each;      // tiles of k of one product of planes
+  GatedPlan p;
+  Divisor by_group, by_split, by_each;  // 8 tiles_c; tiles that are cut; k_each
 };
 
 // Geometry of a tile: WR x WC waves, each RI x CI products of 32 x 32.
@@ -72,23 +91,6 @@ struct Tile {
 typedef Tile<2, 4, 4, 2> TileL;  // 256 x 256
 typedef Tile<2, 2, 2, 2> TileM;  // 128 x 128
 typedef Tile<2, 2, 1, 2> TileS;  // 64 x 128
-
-// Element types: K values of a 128-byte row, values of a 16-byte piece, one step's product.
-template <class Ty>
-struct Elem {  // BF16, F16
-  static constexpr int kSize = 2, kPiece = 8, kTile = 64, kProducts = 1;
-  static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) { return Ty::mma32(a, b, c); }
-};
-template <>
-struct Elem<F32> {
-  static constexpr int kSize = 4, kPiece = 4, kTile = 32, kProducts = 4;
-  static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
-    return c;
-  }
-};
 
 // Up to n values of `size` bytes at p as 16 bytes, zeros behind them; p may have any alignment that a value may have.
 template <int SIZE>
@@ -105,137 +107,76 @@ __device__ __forceinline__ u32x4 load_piece(const char* p, int64_t n) {
   return w;
 }
 
-// A lane's pieces of an operand on their way to LDS.  DIRECT: `off` is each one's offset from the tile's base, kOffOut where
-// its index is outside the matrix; else offsets of any size, and what has been loaded.
-template <int COPIES, bool DIRECT>
-struct Pieces {
-  uint32_t off[COPIES];
-};
-template <int COPIES>
-struct Pieces<COPIES, false> {
-  int64_t off[COPIES];
-  int left[COPIES];  // values that are in the matrix
-  u32x4 held[COPIES];
-};
-__device__ __forceinline__ void put_piece(uint32_t lds, int lane, u32x4 v) {
-  *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(static_cast<uintptr_t>(lds + 16 * lane)) = v;
-}
-
-// A tile of N output indexes, 128 bytes of k each: 1 KB (8 rows) an instruction.  PAIR: 32 of one matrix and 32 of the
-// other in turn.
-template <int N, int WAVES, int SIZE, bool DIRECT, bool PAIR>
+// A tile of N output indexes, 64 values of k each: 1 KB (8 rows) an instruction.  PAIR: 32 of one matrix and 32 of the
+// other in turn.  `off`: a lane's offsets from the tile's first byte, kOffOut where the index is outside the matrix.
+template <int N, int WAVES, bool PAIR>
 struct AlongK {
-  static constexpr int kCopies = N / 8 / WAVES, kReads = 1, V = 16 / SIZE;
+  static constexpr int kCopies = N / 8 / WAVES, kReads = 1;
   static_assert(kCopies * 8 * WAVES == N && (!PAIR || 32 % (8 * WAVES) == 0 || 8 * WAVES == 64), "whole copies of one matrix");
-  Pieces<kCopies, DIRECT> at;
+  uint32_t off[kCopies];
   int piece;  // of a row
+  static __device__ __forceinline__ int slot_of(int row) { return row >> 1 & 7; }
   static __device__ __forceinline__ int part(int i, int wave) { return PAIR ? ((8 * (i * WAVES + wave)) >> 5) & 1 : 0; }
   // extent: indexes from the tile's first one on.
   __device__ __forceinline__ void init(int64_t extent, int64_t ld, int wave, int lane) {
-    piece = (lane & 7) ^ (lane >> 3);
+    static_assert(WAVES % 2 == 0, "copies of a wave begin at the same row of 16");
+    piece = (lane & 7) ^ slot_of(8 * wave + (lane >> 3));
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) {
       const int q = 8 * (i * WAVES + wave), index = (PAIR ? (q >> 6) * 32 + (q & 31) : q) + (lane >> 3);
-      if constexpr (DIRECT) {
-        at.off[i] = index < extent ? static_cast<uint32_t>(index) * static_cast<uint32_t>(ld) + piece * 16 : kOffOut;
-      } else {
-        at.off[i] = index * ld + piece * 16;
-        at.left[i] = index < extent;
-      }
+      off[i] = index < extent ? static_cast<uint32_t>(index) * static_cast<uint32_t>(ld) + piece * 16 : kOffOut;
     }
   }
-  // base: the tile's first index of each matrix at the tile's k; k_left: values of k that are there, up to a tile's.
-  __device__ __forceinline__ void fetch(const char* base, const char* other, int k_left, uint32_t lds, int wave) {
-    if constexpr (DIRECT) {
-      const auto r0 = buffer_rsrc(base, 0x7fffffffu), r1 = buffer_rsrc(PAIR ? other : base, 0x7fffffffu);
-      const bool there = piece * V < k_left;
+  // base, other: the tile's first index of each matrix at the tile's k; k_left: values of k that are there, up to a tile's.
+  __device__ __forceinline__ void fetch(const char* base, const char* other, int k_left, uint32_t lds, int wave) const {
+    const auto r0 = buffer_rsrc(base, 0x7fffffffu), r1 = buffer_rsrc(PAIR ? other : base, 0x7fffffffu);
+    const bool there = piece * 8 < k_left;
 #pragma unroll
-      for (int i = 0; i < kCopies; ++i)
-        tile_copy(part(i, wave) ? r1 : r0, there ? at.off[i] : kOffOut, lds + 8 * (i * WAVES + wave) * 128);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kCopies; ++i)
-        at.held[i] = load_piece<SIZE>((part(i, wave) ? other : base) + at.off[i], at.left[i] ? k_left - piece * V : 0);
-    }
+    for (int i = 0; i < kCopies; ++i)
+      tile_copy(part(i, wave) ? r1 : r0, there ? off[i] : kOffOut, lds + 8 * (i * WAVES + wave) * 128);
   }
-  __device__ __forceinline__ void put(uint32_t lds, int wave, int lane) const {
-    if constexpr (!DIRECT) {
-#pragma unroll
-      for (int i = 0; i < kCopies; ++i) put_piece(lds + 8 * (i * WAVES + wave) * 128, lane, at.held[i]);
-    }
-  }
-  template <class Ty>
   static __device__ __forceinline__ u32x4 read(uint32_t lds, int first, int step, int lane) {
     const int l32 = lane & 31, hh = lane >> 5;
-    const uint32_t at = lds + (first + l32) * 128 + (((2 * step + hh) ^ (l32 & 7)) << 4);
+    const uint32_t at = lds + (first + l32) * 128 + (((2 * step + hh) ^ slot_of(l32)) << 4);
     return *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(static_cast<uintptr_t>(at));
   }
 };
 
-// A tile of 128 / SIZE values of k, N output indexes each.
-template <int N, int WAVES, int SIZE, bool DIRECT>
+// A tile of 64 values of k, N output indexes each.
+template <int N, int WAVES>
 struct AcrossK {
-  static constexpr int kRow = N * SIZE, kPieces = kRow / 16;   // of a k
-  static constexpr int kRowsOfCopy = 64 / kPieces > 0 ? 64 / kPieces : 1;
-  static constexpr int kCopies = N / 8 / WAVES, kReads = SIZE, V = 16 / SIZE;
+  static constexpr int kRow = N * 2, kPieces = kRow / 16;   // of a k
+  static constexpr int kRowsOfCopy = 64 / kPieces;
+  static constexpr int kCopies = N / 8 / WAVES, kReads = 2;
   static_assert(kRow <= 1024 && kCopies * 8 * WAVES == N, "whole copies");
-  Pieces<kCopies, DIRECT> at;
+  uint32_t off[kCopies];
   int in;  // the lane's k of a copy
-  static constexpr int kPairs = kPieces / 2 < 8 ? kPieces / 2 : 8;
-  static __device__ __forceinline__ int slot(int p, int k) {
-    if constexpr (SIZE == 2) return p ^ ((k & (kPairs - 1)) << 1);
-    else return p ^ ((k & 4) << 1);
-  }
+  static __device__ __forceinline__ int slot(int p, int k) { return p ^ (kRow >= 256 ? (k & 3) << 2 : (k & 2) << 1); }
   // n_out: output indexes from the tile's first one on.
   __device__ __forceinline__ void init(int64_t n_out, int64_t ld, int wave, int lane) {
     in = lane / kPieces;
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) {
       const int k = (i * WAVES + wave) * kRowsOfCopy + in, p = slot(lane % kPieces, k);
-      if constexpr (DIRECT) {
-        at.off[i] = p * V < n_out ? static_cast<uint32_t>(k) * static_cast<uint32_t>(ld) + p * 16 : kOffOut;
-      } else {
-        at.off[i] = k * ld + p * 16;
-        at.left[i] = n_out - p * V < V ? static_cast<int>(n_out - p * V) : V;
-      }
+      off[i] = p * 8 < n_out ? static_cast<uint32_t>(k) * static_cast<uint32_t>(ld) + p * 16 : kOffOut;
     }
   }
   // base: the first output index at the tile's k; k_left: values of k that are there, up to a tile's.
-  __device__ __forceinline__ void fetch(const char* base, int k_left, uint32_t lds, int wave) {
+  __device__ __forceinline__ void fetch(const char* base, int k_left, uint32_t lds, int wave) const {
     const auto r = buffer_rsrc(base, 0x7fffffffu);
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) {
       const int copy = i * WAVES + wave;
-      const bool there = in < k_left - copy * kRowsOfCopy;
-      if constexpr (DIRECT) tile_copy(r, there ? at.off[i] : kOffOut, lds + copy * 1024);
-      else at.held[i] = load_piece<SIZE>(base + at.off[i], there ? at.left[i] : 0);
+      tile_copy(r, in < k_left - copy * kRowsOfCopy ? off[i] : kOffOut, lds + copy * 1024);
     }
   }
-  __device__ __forceinline__ void put(uint32_t lds, int wave, int lane) const {
-    if constexpr (!DIRECT) {
-#pragma unroll
-      for (int i = 0; i < kCopies; ++i) put_piece(lds + (i * WAVES + wave) * 1024, lane, at.held[i]);
-    }
-  }
-  template <class Ty>
   static __device__ __forceinline__ u32x4 read(uint32_t lds, int first, int step, int lane) {
-    const int l32 = lane & 31, hh = lane >> 5, l16 = lane & 15;
-    if constexpr (SIZE == 2) {
-      const int c = first + 16 * ((lane >> 4) & 1) + 4 * (l16 & 3);
-      const int k = 16 * step + 8 * hh + (l16 >> 2);
-      const auto at = [&](int kk) { return lds + kk * kRow + (slot(c >> 3, kk) << 4) + ((c & 4) << 1); };
-      const u32x2 a = lds_read_tr16(at(k)), b = lds_read_tr16(at(k + 4));
-      return u32x4{a[0], a[1], b[0], b[1]};
-    } else {
-      u32x4 v;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int k = 8 * step + 4 * hh + j, c = first + l32;
-        const uint32_t at = lds + k * kRow + (slot(c >> 2, k) << 4) + ((c & 3) << 2);
-        v[j] = *reinterpret_cast<__attribute__((address_space(3))) uint32_t*>(static_cast<uintptr_t>(at));
-      }
-      return v;
-    }
+    const int hh = lane >> 5, l16 = lane & 15;
+    const int c = first + 16 * ((lane >> 4) & 1) + 4 * (l16 & 3);
+    const int k = 16 * step + 8 * hh + (l16 >> 2);
+    const auto at = [&](int kk) { return lds + kk * kRow + (slot(c >> 3, kk) << 4) + ((c & 4) << 1); };
+    const u32x2 a = lds_read_tr16(at(k)), b = lds_read_tr16(at(k + 4));
+    return u32x4{a[0], a[1], b[0], b[1]};
   }
 };
 
@@ -328,65 +269,98 @@ struct Turn {
 // silu(g) u = g u / (1 + e^-g)
 __device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(kNegLog2e * g)); }
 
-// Workgroups of an XCD take neighbouring tiles (round-robin dispatch), in groups of 8 rows of tiles.
+// dG and dU of a value.
+__device__ __forceinline__ void gates(float dh, float g, float u, float& dg, float& du) {
+  const float s = sigmoid(g);
+  du = dh * (g * s);
+  dg = dh * u * (s * (1.f + g * (1.f - s)));
+}
+
+// Workgroups of an XCD take neighbouring tiles (round-robin dispatch).
 __device__ __forceinline__ uint32_t xcd_tile(uint32_t id, uint32_t n) {
   const uint32_t xcd = id & 7, at = id >> 3, per = n >> 3, rem = n & 7;
   return (xcd < rem ? xcd * (per + 1) : rem * (per + 1) + (xcd - rem) * per) + at;
 }
 
-template <class Ty, int MODE, class T, bool DIRECT>
+// Where a tile lies: groups of 8 rows of tiles, column by column.
+struct TilePlace {
+  int64_t r0;
+  int64_t c0;
+  int which;  // the weights' gradients: the first half of the rows of tiles is the gate's
+};
+template <int MODE, class T>
+__device__ __forceinline__ TilePlace tile_place(const GatedArgs& a, uint32_t tile) {
+  constexpr uint32_t kGroup = 8;
+  const uint32_t group = a.by_group.divide(tile), in = tile - group * kGroup * a.p.tiles_c;
+  const uint32_t high = static_cast<uint32_t>(a.p.tiles_r) - group * kGroup;
+  const uint32_t tile_c = high >= kGroup ? in / kGroup : in / high;
+  const uint32_t tile_r = group * kGroup + (high >= kGroup ? in % kGroup : in - tile_c * high);
+  const uint32_t half_r = static_cast<uint32_t>(a.p.tiles_r) / 2;
+  TilePlace t;
+  t.which = MODE == kGatedDw && tile_r >= half_r ? 1 : 0;
+  t.r0 = static_cast<int64_t>(t.which ? tile_r - half_r : tile_r) * T::BR;
+  t.c0 = static_cast<int64_t>(tile_c) * (gated_pair(MODE) ? T::BC / 2 : T::BC);
+  return t;
+}
+
+// Ty: the operands' type; Out: x's and the outputs' (F32: three planes of bf16 operands).
+template <class Ty, class Out, int MODE, class T>
 __global__ void __launch_bounds__(T::kThreads, 2) gated_tile_kernel(GatedArgs a) {
-  constexpr int S = Elem<Ty>::kSize, KT = Elem<Ty>::kTile, W = T::kWaves;
-  constexpr bool kPair = MODE == kGatedForward || MODE == kGatedKeep || MODE == kGatedGates;  // columns: 32 of the gate, 32 of the other
-  constexpr int kCols = kPair ? T::BC / 2 : T::BC;                      // output columns of a tile
-  typedef typename std::conditional<MODE == kGatedDw, AcrossK<T::BR, W, S, DIRECT>, AlongK<T::BR, W, S, DIRECT, false>>::type OpR;
-  typedef typename std::conditional<kPair, AlongK<T::BC, W, S, DIRECT, true>, AcrossK<T::BC, W, S, DIRECT>>::type OpC;
+  constexpr bool kWide = std::is_same<Out, F32>::value, kPair = gated_pair(MODE);
+  constexpr int W = T::kWaves, S = kWide ? 4 : 2;  // S: bytes of an output
+  constexpr int kProducts = kWide ? 6 : 1;         // of planes
+  typedef typename std::conditional<MODE == kGatedDw, AcrossK<T::BR, W>, AlongK<T::BR, W, false>>::type OpR;
+  typedef typename std::conditional<kPair, AlongK<T::BC, W, true>, AcrossK<T::BC, W>>::type OpC;
   __shared__ __attribute__((aligned(1024))) char lds[2][T::kBytesR + T::kBytesC];
   __shared__ __attribute__((aligned(1024))) char turns[W][4096];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int l32 = lane & 31, hh = lane >> 5;
 
-  // A workgroup takes units (a tile, or a part of its k) in turn, and their tiles of k as one sequence: a unit's first
-  // operands are on their way while the one before it is stored.
+  // A workgroup takes units in turn, and their tiles of k as one sequence: a unit's first operands are on their way while the
+  // one before it is stored.
   struct Unit {
-    int64_t r0, c0, kt, kt_end;
-    int which, split;
+    TilePlace at;
+    uint32_t kt, kt_end, product, k_in;  // tiles of k; the product of planes of the next one, and its place there
+    int part;                            // of the tile; -1: whole
   };
-  const uint32_t tiles = static_cast<uint32_t>(a.tiles_r) * a.tiles_c, units = tiles * a.splits;
+  const uint32_t units = static_cast<uint32_t>(a.p.units), whole = static_cast<uint32_t>(a.p.whole);
   auto unit_at = [&](uint32_t index) {
-    const uint32_t id = xcd_tile(index, units), split = a.by_tiles.divide(id), tile = id - split * tiles;
-    constexpr uint32_t kGroup = 8;
-    const uint32_t group = a.by_group.divide(tile), in = tile - group * kGroup * a.tiles_c;
-    const uint32_t high = static_cast<uint32_t>(a.tiles_r) - group * kGroup;
-    const uint32_t tile_c = high >= kGroup ? in / kGroup : in / high;
-    const uint32_t tile_r = group * kGroup + (high >= kGroup ? in % kGroup : in - tile_c * high);
-    // The weights' gradients: the first half of the rows of tiles is the gate's.
-    const uint32_t half_r = static_cast<uint32_t>(a.tiles_r) / 2;
     Unit u;
-    u.split = static_cast<int>(split);
-    u.which = MODE == kGatedDw && tile_r >= half_r ? 1 : 0;
-    u.r0 = static_cast<int64_t>(MODE == kGatedDw && u.which ? tile_r - half_r : tile_r) * T::BR;
-    u.c0 = static_cast<int64_t>(tile_c) * kCols;
-    u.kt = static_cast<int64_t>(split) * a.k_split;
-    u.kt_end = u.kt + a.k_split < a.k_tiles ? u.kt + a.k_split : a.k_tiles;
+    uint32_t tile;
+    u.kt = 0;
+    u.kt_end = static_cast<uint32_t>(a.p.k_tiles);
+    if (index < whole) {
+      tile = xcd_tile(index, whole);
+      u.part = -1;
+      u.product = u.k_in = 0;
+    } else {
+      // Parts with the same k lie side by side: they share rows of an operand.
+      const uint32_t id = xcd_tile(index - whole, units - whole), part = a.by_split.divide(id);
+      tile = whole + id - part * (static_cast<uint32_t>(a.p.tiles_r) * a.p.tiles_c - whole);
+      u.part = static_cast<int>(part);
+      u.kt = part * static_cast<uint32_t>(a.p.k_part);
+      const uint32_t end = u.kt + static_cast<uint32_t>(a.p.k_part);
+      u.kt_end = end < u.kt_end ? end : u.kt_end;
+      u.product = a.by_each.divide(u.kt);
+      u.k_in = u.kt - u.product * a.k_each;
+    }
+    u.at = tile_place<MODE, T>(a, tile);
     return u;
   };
 
   OpR op_r;
   OpC op_c;
-  const int64_t ld_w = static_cast<int64_t>(a.channels) * S, ld_gu = static_cast<int64_t>(a.ld_gu) * S;
   uint32_t next = blockIdx.x;  // the unit that is fetched
   Unit f = unit_at(next);
   auto init = [&]() {
     if constexpr (kPair) {
-      op_r.init(a.rows - f.r0, a.x_ld, wave, lane);
-      op_c.init(a.hidden - f.c0, ld_w, wave, lane);
+      op_r.init(a.rows - f.at.r0, a.x.ld, wave, lane);
+      op_c.init(a.hidden - f.at.c0, a.w[0].ld, wave, lane);
     } else if constexpr (MODE == kGatedDx) {
-      op_r.init(a.rows - f.r0, ld_gu, wave, lane);
-      op_c.init(a.channels - f.c0, ld_w, wave, lane);
+      op_r.init(a.rows - f.at.r0, a.gu[0].ld, wave, lane);
+      op_c.init(a.channels - f.at.c0, a.w[0].ld, wave, lane);
     } else {
-      op_r.init(a.ld_gu - f.r0, ld_gu, wave, lane);
-      op_c.init(a.channels - f.c0, a.x_ld, wave, lane);
+      op_r.init(a.hidden - f.at.r0, a.gu[0].ld, wave, lane);
+      op_c.init(a.channels - f.at.c0, a.x.ld, wave, lane);
     }
   };
   // To the next unit, where this one's tiles have all been asked for; behind the last unit tiles read as zeros that
@@ -400,30 +374,29 @@ __global__ void __launch_bounds__(T::kThreads, 2) gated_tile_kernel(GatedArgs a)
   };
   auto fetch = [&](int stage) {
     const uint32_t at_r = lds_addr(lds[stage]), at_c = at_r + T::kBytesR;
-    const auto left = [&](int64_t k) { return f.kt >= f.kt_end ? 0 : k < KT ? static_cast<int>(k) : KT; };
-    const int64_t kt = f.kt;
+    const auto left = [&](int64_t k) { return f.kt >= f.kt_end ? 0 : k < 64 ? static_cast<int>(k) : 64; };
+    // Products of planes, the smallest first: (2, 0), (1, 1), (0, 2), (1, 0), (0, 1), (0, 0).  In dx all of dG's come before dU's.
+    const uint32_t which = MODE == kGatedDx && f.product >= kProducts ? 1 : 0, pair = f.product - which * kProducts;
+    const int plane_r = kWide ? (0x001012 >> (4 * pair)) & 3 : 0, plane_c = kWide ? (0x010210 >> (4 * pair)) & 3 : 0;
+    const int64_t k0 = static_cast<int64_t>(f.k_in) * 64;
     if constexpr (kPair) {
-      const int k_left = left(a.channels - kt * KT);
-      op_r.fetch(a.x + f.r0 * a.x_ld + kt * 128, nullptr, k_left, at_r, wave);
-      op_c.fetch(a.w[0] + f.c0 * ld_w + kt * 128, a.w[1] + f.c0 * ld_w + kt * 128, k_left, at_c, wave);
+      const int k_left = left(a.channels - k0);
+      op_r.fetch(a.x.at + plane_r * a.x.plane + f.at.r0 * a.x.ld + k0 * 2, nullptr, k_left, at_r, wave);
+      const int64_t at = plane_c * a.w[0].plane + f.at.c0 * a.w[0].ld + k0 * 2;
+      op_c.fetch(a.w[0].at + at, a.w[1].at + at, k_left, at_c, wave);
     } else if constexpr (MODE == kGatedDx) {
-      const int64_t each = a.k_tiles / 2;
-      const int w = kt >= each;
-      const int64_t k0 = (kt - w * each) * KT;
-      op_r.fetch(a.dgu[w] + f.r0 * ld_gu + k0 * S, nullptr, left(a.ld_gu - k0), at_r, wave);
-      op_c.fetch(a.w[w] + k0 * ld_w + f.c0 * S, left(a.hidden - k0), at_c, wave);
+      const int k_left = left(a.hidden - k0);
+      op_r.fetch(a.gu[which].at + plane_r * a.gu[0].plane + f.at.r0 * a.gu[0].ld + k0 * 2, nullptr, k_left, at_r, wave);
+      op_c.fetch(a.w[which].at + plane_c * a.w[0].plane + k0 * a.w[0].ld + f.at.c0 * 2, k_left, at_c, wave);
     } else {
-      const int64_t k0 = kt * KT;
       const int k_left = left(a.rows - k0);
-      op_r.fetch(a.dgu[f.which] + k0 * ld_gu + f.r0 * S, k_left, at_r, wave);
-      op_c.fetch(a.x + k0 * a.x_ld + f.c0 * S, k_left, at_c, wave);
+      op_r.fetch(a.gu[f.at.which].at + plane_r * a.gu[0].plane + k0 * a.gu[0].ld + f.at.r0 * 2, k_left, at_r, wave);
+      op_c.fetch(a.x.at + plane_c * a.x.plane + k0 * a.x.ld + f.at.c0 * 2, k_left, at_c, wave);
     }
-    f.kt += f.kt < f.kt_end;
-  };
-  auto put = [&](int stage) {
-    const uint32_t at_r = lds_addr(lds[stage]), at_c = at_r + T::kBytesR;
-    op_r.put(at_r, wave, lane);
-    op_c.put(at_c, wave, lane);
+    if (f.kt < f.kt_end) {
+      ++f.kt;
+      if (++f.k_in == static_cast<uint32_t>(a.k_each)) f.k_in = 0, ++f.product;
+    }
   };
 
   f32x16 acc[T::CI][T::RI];
@@ -434,32 +407,30 @@ __global__ void __launch_bounds__(T::kThreads, 2) gated_tile_kernel(GatedArgs a)
       for (int j = 0; j < T::RI; ++j) acc[i][j] = f32x16{};
   };
   const int wr = wave / T::WC * (T::RI * 32), wc = wave % T::WC * (T::CI * 32);
-
   u32x4 fr[2][T::RI], fc[2][T::CI];
   auto read = [&](int stage, int s, int buf) {
     const uint32_t at_r = lds_addr(lds[stage]), at_c = at_r + T::kBytesR;
 #pragma unroll
-    for (int i = 0; i < T::CI; ++i) fc[buf][i] = OpC::template read<Ty>(at_c, wc + 32 * i, s, lane);
+    for (int i = 0; i < T::CI; ++i) fc[buf][i] = OpC::read(at_c, wc + 32 * i, s, lane);
 #pragma unroll
-    for (int j = 0; j < T::RI; ++j) fr[buf][j] = OpR::template read<Ty>(at_r, wr + 32 * j, s, lane);
+    for (int j = 0; j < T::RI; ++j) fr[buf][j] = OpR::read(at_r, wr + 32 * j, s, lane);
   };
   auto multiply = [&](int buf) {
 #pragma unroll
     for (int j = 0; j < T::RI; ++j)
 #pragma unroll
-      for (int i = 0; i < T::CI; ++i) acc[i][j] = Elem<Ty>::mma(fc[buf][i], fr[buf][j], acc[i][j]);
+      for (int i = 0; i < T::CI; ++i) acc[i][j] = Ty::mma32(fc[buf][i], fr[buf][j], acc[i][j]);
   };
   constexpr int kCopies = OpR::kCopies + OpC::kCopies;
   // A step's reads go between its products, one after each; left alone, the compiler puts them right before their use.
-  constexpr int kReads = T::CI * OpC::kReads + T::RI * OpR::kReads, kProducts = T::CI * T::RI * Elem<Ty>::kProducts;
+  constexpr int kReads = T::CI * OpC::kReads + T::RI * OpR::kReads, kMfma = T::CI * T::RI;
   auto interleave = [&]() {
-    constexpr int kEach = kProducts / kReads > 0 ? kProducts / kReads : 1;
 #pragma unroll
     for (int i = 0; i < kReads; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // a read of LDS
-      __builtin_amdgcn_sched_group_barrier(0x8, kEach, 0);  // products
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);    // a product
     }
-    if constexpr (kProducts > kReads * kEach) __builtin_amdgcn_sched_group_barrier(0x8, kProducts - kReads * kEach, 0);
+    if constexpr (kMfma > kReads) __builtin_amdgcn_sched_group_barrier(0x8, kMfma - kReads, 0);
     __builtin_amdgcn_sched_barrier(0);
   };
 
@@ -470,13 +441,8 @@ __global__ void __launch_bounds__(T::kThreads, 2) gated_tile_kernel(GatedArgs a)
   init();
   fetch(0);
   turn();
-  if constexpr (DIRECT) {
-    fetch(1);
-    wait_vmcnt<kCopies>();
-  } else {
-    put(0);
-    fetch(1);
-  }
+  fetch(1);
+  wait_vmcnt<kCopies>();
   __syncthreads();
   read(0, 0, 0);
   clear();
@@ -489,8 +455,7 @@ __global__ void __launch_bounds__(T::kThreads, 2) gated_tile_kernel(GatedArgs a)
       multiply(s & 1);
       interleave();
     }
-    if constexpr (DIRECT) wait_vmcnt<0>();
-    else put(stage ^ 1);
+    wait_vmcnt<0>();
     __syncthreads();
     __builtin_amdgcn_sched_barrier(0);
     read(stage ^ 1, 0, 0);
@@ -500,34 +465,53 @@ __global__ void __launch_bounds__(T::kThreads, 2) gated_tile_kernel(GatedArgs a)
     stage ^= 1;
     if (++u.kt < u.kt_end) continue;
     mfma_drain();
+
     const uint32_t own = lds_addr(turns[wave]);
-    if constexpr (kPair) {
+    auto values = [&](int i, int j, float (&v)[16]) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] = acc[i][j][e];
+    };
+    if (u.part >= 0) {
+      // Fewer tiles are cut than there are units, so this is the part's place among all units that are no whole tile.
+      constexpr int64_t kLd = T::BC * 4;
+      const uint32_t id = xcd_tile(index - whole, units - whole);
+      char* out = reinterpret_cast<char*>(a.partial) + static_cast<int64_t>(id) * T::BR * kLd + wr * kLd + wc * 4;
+#pragma unroll
+      for (int j = 0; j < T::RI; ++j)
+#pragma unroll
+        for (int i = 0; i < T::CI; ++i) {
+          float v[16];
+          values(i, j, v);
+          Turn<128>::put<F32>(own, 0, v, lane);
+          Turn<128>::store<4>(own, out + 32 * j * kLd + 32 * i * 4, kLd, 32, 32, lane);
+        }
+    } else if constexpr (kPair) {
       typedef Turn<32 * S> Tn;
-      const int64_t c = u.c0 + (wc >> 1), r = u.r0 + wr;
+      const int64_t c = u.at.c0 + (wc >> 1), r = u.at.r0 + wr;
       if constexpr (MODE != kGatedGates) {
 #pragma unroll
         for (int j = 0; j < T::RI; ++j) {
+          const int64_t row = r + 32 * j, ld = static_cast<int64_t>(a.hidden) * S;
           if constexpr (MODE == kGatedKeep) {
-            const int64_t ld = static_cast<int64_t>(a.hidden) * 4, row = r + 32 * j;
+            const int64_t ld_kept = static_cast<int64_t>(a.hidden) * 4;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               float v[16];
-#pragma unroll
-              for (int e = 0; e < 16; ++e) v[e] = acc[i][j][e];
+              values(i, j, v);
               Turn<128>::put<F32>(own, 0, v, lane);
-              Turn<128>::store<4>(own, reinterpret_cast<char*>(a.kept) + (i * a.rows + row) * ld + c * 4, ld, a.rows - row, a.hidden - c, lane);
+              Turn<128>::store<4>(own, reinterpret_cast<char*>(a.kept) + (i * a.rows + row) * ld_kept + c * 4, ld_kept, a.rows - row,
+                                  a.hidden - c, lane);
             }
           }
           float h[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) h[i] = acc[0][j][i] * acc[1][j][i] * sigmoid(acc[0][j][i]);
-          Tn::template put<Ty>(own, 0, h, lane);
-          const int64_t ld = static_cast<int64_t>(a.hidden) * S, row = r + 32 * j;
+          Tn::template put<Out>(own, 0, h, lane);
           Tn::template store<S>(own, static_cast<char*>(a.out[0]) + row * ld + c * S, ld, a.rows - row, a.hidden - c, lane);
         }
       } else {
         // Columns up to a whole piece are written: there both products are 0.  The gradients of G and U are
-        // rounded to the operands' type here, as the products that take them need it (fp32 stays fp32).
+        // rounded to the operands' type here, as the products that take them need it (fp32: to its three planes).
         u32x4 w[T::RI][Tn::kCopies];
 #pragma unroll
         for (int j = 0; j < T::RI; ++j) {
@@ -536,61 +520,54 @@ __global__ void __launch_bounds__(T::kThreads, 2) gated_tile_kernel(GatedArgs a)
         }
 #pragma unroll
         for (int j = 0; j < T::RI; ++j) {
-          const int64_t row = r + 32 * j, at = row * ld_gu + c * S;
-          float dh[16], dg[16], du[16];
+          const int64_t row = r + 32 * j, at = row * a.gu[0].ld + c * 2;
+          float dh[16], d[2][16];
           Tn::keep(own, w[j], lane);
-          Tn::template get<Ty>(own, dh, lane);
+          Tn::template get<Out>(own, dh, lane);
           wave_lds_sync();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float g = acc[0][j][i], up = acc[1][j][i], s = sigmoid(g);
-            du[i] = dh[i] * (g * s);
-            dg[i] = dh[i] * up * (s * (1.f + g * (1.f - s)));
+          for (int i = 0; i < 16; ++i) gates(dh[i], acc[0][j][i], acc[1][j][i], d[0][i], d[1][i]);
+#pragma unroll
+          for (int o = 0; o < 2; ++o) {
+#pragma unroll
+            for (int plane = 0; plane < (kWide ? 3 : 1); ++plane) {
+              Turn<64>::put<Ty>(own, 0, d[o], lane);
+              Turn<64>::store<2>(own, static_cast<char*>(a.out[o]) + plane * a.gu[0].plane + at, a.gu[0].ld, a.rows - row,
+                                 a.gu[0].ld / 2 - c, lane);
+              if constexpr (kWide) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) d[o][i] -= BF16::to_f32(BF16::from_f32(d[o][i]));
+              }
+            }
           }
-          Tn::template put<Ty>(own, 0, dg, lane);
-          Tn::template store<S>(own, static_cast<char*>(a.out[0]) + at, ld_gu, a.rows - row, a.ld_gu - c, lane);
-          Tn::template put<Ty>(own, 0, du, lane);
-          Tn::template store<S>(own, static_cast<char*>(a.out[1]) + at, ld_gu, a.rows - row, a.ld_gu - c, lane);
         }
       }
-    } else {
-      const int64_t n_r = MODE == kGatedDw ? a.hidden : a.rows;
+    } else if (a.out[u.at.which] != nullptr) {  // NULL: one weight's gradient is not asked for
+      const int64_t n_r = MODE == kGatedDw ? a.hidden : a.rows, ld = static_cast<int64_t>(a.channels) * S;
+      char* out = static_cast<char*>(a.out[u.at.which]);
 #pragma unroll
       for (int j = 0; j < T::RI; ++j) {
-        const int64_t row = u.r0 + wr + 32 * j, c = u.c0 + wc;
-        if (a.splits > 1 || S == 4) {  // fp32: 32 columns at a time
-          if (a.splits == 1 && a.out[u.which] == nullptr) continue;  // one weight's gradient is not asked for
-          const int64_t ld = static_cast<int64_t>(a.channels) * 4;
-          char* out = a.splits > 1 ? reinterpret_cast<char*>(a.partial) +
-                                         (static_cast<int64_t>(u.split) * (MODE == kGatedDw ? 2 : 1) + u.which) * n_r * ld
-                                   : static_cast<char*>(a.out[u.which]);
+        const int64_t row = u.at.r0 + wr + 32 * j, c = u.at.c0 + wc;
+        static_assert(T::CI == 2, "64 columns of a wave");
 #pragma unroll
-          for (int i = 0; i < T::CI; ++i) {
-            float v[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = acc[i][j][e];
+        for (int i = 0; i < T::CI; ++i) {
+          float v[16];
+          values(i, j, v);
+          if constexpr (kWide) {  // 32 columns at a time
             Turn<128>::put<F32>(own, 0, v, lane);
             Turn<128>::store<4>(own, out + row * ld + (c + 32 * i) * 4, ld, n_r - row, a.channels - c - 32 * i, lane);
-          }
-        } else if constexpr (S == 2) {
-          if (a.out[u.which] == nullptr) continue;
-          static_assert(T::CI == 2, "64 columns of a wave");
-#pragma unroll
-          for (int i = 0; i < T::CI; ++i) {
-            float v[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = acc[i][j][e];
+          } else {
             Turn<128>::put<Ty>(own, 4 * i, v, lane);
           }
-          Turn<128>::store<2>(own, static_cast<char*>(a.out[u.which]) + row * ld_w + c * 2, ld_w, n_r - row, a.channels - c, lane);
         }
+        if constexpr (!kWide) Turn<128>::store<2>(own, out + row * ld + c * 2, ld, n_r - row, a.channels - c, lane);
       }
     }
     index += gridDim.x;
     if (!T::kTurns || index >= units) break;
     if (index == next) {
       u = f;
-      u.kt = static_cast<int64_t>(u.split) * a.k_split;
+      u.kt = u.part < 0 ? 0 : u.part * static_cast<uint32_t>(a.p.k_part);
     } else {
       u = unit_at(index);
     }
@@ -601,30 +578,44 @@ __global__ void __launch_bounds__(T::kThreads, 2) gated_tile_kernel(GatedArgs a)
   wait_vmcnt<0>();
 }
 
-// Tiles of a launch.
-struct GatedPlan {
-  int size;  // 0: TileL, 1: TileM, 2: TileS
-  int64_t tiles_r;
-  int32_t tiles_c, splits;
-  int64_t k_tiles, k_split;
-};
-
-template <class Ty, int MODE, bool DIRECT>
-void launch_gated(const GatedArgs& a, int size, hipStream_t s) {
-  // As many workgroups as run at once (by the LDS of their two stages, two of TileM and three of TileS on a compute
-  // unit), which take units in turn; TileL takes one each.
-  const int64_t units = a.tiles_r * a.tiles_c * a.splits, most = static_cast<int64_t>(device_cus()) * 2;
-  const dim3 grid(static_cast<unsigned>(size == 0 || units < most ? units : most));
-  if (size == 0) hipLaunchKernelGGL((gated_tile_kernel<Ty, MODE, TileL, DIRECT>), grid, dim3(TileL::kThreads), 0, s, a);
-  else if (size == 1) hipLaunchKernelGGL((gated_tile_kernel<Ty, MODE, TileM, DIRECT>), grid, dim3(TileM::kThreads), 0, s, a);
-  else hipLaunchKernelGGL((gated_tile_kernel<Ty, MODE, TileS, DIRECT>), grid, dim3(TileS::kThreads), 0, s, a);
-}
-
-template <int MODE>
-void launch_gated_mode(const GatedArgs& a, int size, int dtype, bool direct, hipStream_t s) {
-  if (dtype == OW_DTYPE_BF16) return direct ? launch_gated<BF16, MODE, true>(a, size, s) : launch_gated<BF16, MODE, false>(a, size, s);
-  if (dtype == OW_DTYPE_F16) return direct ? launch_gated<F16, MODE, true>(a, size, s) : launch_gated<F16, MODE, false>(a, size, s);
-  return direct ? launch_gated<F32, MODE, true>(a, size, s) : launch_gated<F32, MODE, false>(a, size, s);
+// The outputs of tiles whose k was cut: parts are added in their order.  A thread has 4 columns of a row, of the gate and of the other
+// projection where there are both.
+template <class Out, int MODE, class T>
+__global__ void __launch_bounds__(256) gated_join_kernel(GatedArgs a) {
+  constexpr bool kPair = gated_pair(MODE);
+  constexpr int kRuns = (kPair ? T::BC / 2 : T::BC) / 4;
+  typedef Row<Out> R;
+  const uint32_t cut = static_cast<uint32_t>(a.p.tiles_r) * a.p.tiles_c - static_cast<uint32_t>(a.p.whole);
+  const uint32_t per_tile = T::BR * kRuns / 256, t = blockIdx.x / per_tile, in = blockIdx.x % per_tile * 256 + threadIdx.x;
+  const int row_in = in / kRuns, run = in % kRuns;
+  const TilePlace at = tile_place<MODE, T>(a, static_cast<uint32_t>(a.p.whole) + t);
+  const int64_t row = at.r0 + row_in, c = at.c0 + run * 4;
+  const int64_t n_r = MODE == kGatedDw ? a.hidden : a.rows, n_c = kPair ? a.hidden : a.channels;
+  void* const out = a.out[MODE == kGatedDw ? at.which : 0];
+  if (row >= n_r || c >= n_c || out == nullptr) return;
+  const int q = kPair ? run / 8 * 64 + run % 8 * 4 : run * 4;  // columns of the tile
+  const float* p = a.partial + (static_cast<int64_t>(t) * T::BR + row_in) * T::BC + q;
+  const int64_t step = static_cast<int64_t>(cut) * T::BR * T::BC;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f}, other = sum;
+#pragma unroll 4
+  for (int s = 0; s < a.p.parts; ++s) {
+    sum += *reinterpret_cast<const f32x4*>(p + s * step);
+    if constexpr (kPair) other += *reinterpret_cast<const f32x4*>(p + s * step + 32);
+  }
+  typename R::Elem* o = static_cast<typename R::Elem*>(out) + row * n_c + c;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (c + j >= n_c) break;
+    if constexpr (kPair) {
+      if constexpr (MODE == kGatedKeep) {
+        a.kept[row * n_c + c + j] = sum[j];
+        a.kept[(a.rows + row) * n_c + c + j] = other[j];
+      }
+      o[j] = R::from_f32(sum[j] * other[j] * sigmoid(sum[j]));
+    } else {
+      o[j] = R::from_f32(sum[j]);
+    }
+  }
 }
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -632,33 +623,94 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Rows and columns of a tile's operands (gate and up columns together).
 inline int gated_tile_rows(int size) { return size == 0 ? TileL::BR : size == 1 ? TileM::BR : TileS::BR; }
 inline int gated_tile_cols(int size) { return size == 0 ? TileL::BC : size == 1 ? TileM::BC : TileS::BC; }
+// Units that run at once (the LDS of two stages and Turn: one workgroup a compute unit of TileL, two of the others).
+inline int64_t gated_at_once(int size) { return static_cast<int64_t>(device_cus()) * (size == 0 ? 1 : 2); }
 
-// How an output of `rows` x `cols` (cols: gate and up together; `row_sets` of them) is cut.  TileL where k is long and every
-// compute unit gets one (16-bit types, 6,272 tokens, 4,096 to 8,192: forward 738 us, 860 with TileM; 25,088 tokens, 512 to 1,024:
-// 72 and 66; fp32, 5,728 tokens, 1,024 to 2,048: 527 and 438); else TileM, and TileS where that leaves compute units without
-// work, or where k may be cut (can_split) TileM with k in parts (6,272 tokens, 1,024 to 2,048, the weights' gradients: 63 us and 9 for
-// the sum of the parts; TileL 68 and 23).
-inline GatedPlan gated_plan(int64_t rows, int64_t cols, int64_t k_tiles, int row_sets, bool can_split, bool wide) {
-  const int64_t cus = device_cus();
-  GatedPlan p;
-  const auto tiles_of = [&](int size) {
-    return ceil_div(rows, gated_tile_rows(size)) * row_sets * ceil_div(cols, gated_tile_cols(size));
-  };
-  p.size = !wide && k_tiles >= 16 && tiles_of(0) >= cus ? 0 : can_split || tiles_of(1) >= cus ? 1 : 2;
-  p.tiles_r = ceil_div(rows, gated_tile_rows(p.size)) * row_sets;
-  p.tiles_c = static_cast<int32_t>(ceil_div(cols, gated_tile_cols(p.size)));
-  p.k_tiles = k_tiles;
-  int64_t splits = 1;
-  const int64_t tiles = p.tiles_r * p.tiles_c;
-  if (can_split && tiles < 2 * cus) {
-    splits = 2 * cus / tiles;
-    const int64_t most = ceil_div(k_tiles, 8);  // 8 tiles of k at least
-    splits = splits < most ? splits : most;
-    splits = splits < 1 ? 1 : splits;
+// How an output of `rows` x `cols` (cols: gate and up together; `row_sets` of them) is cut: the tile, and the parts of k of those tiles
+// that fill no whole round of what runs at once, by their time.  A unit takes kStep us for a tile of k, more where an
+// operand is read across k, and kBesides us for its beginning and its outputs (measured: 6,272 tokens, 4,096 to 8,192: 738, 860 and 995 us
+// forward for TileL, M and S; 25,088 tokens, 512 to 1,024: 72, 66 and 72; the weights' gradients of 6,272 tokens, 1,024 to 2,048: 68, 63
+// and 86 and, for L and M, 23 and 9 to join parts).  Parts are written and read at 0.4 us a MB, and joined by a launch
+// of 6 us.
+inline GatedPlan gated_plan(int64_t rows, int64_t cols, int64_t k_tiles, int row_sets, bool pair, bool may_cut) {
+  constexpr double kSteps[2][3] = {{1.88, 1.3, 0.87}, {1.6, 0.98, 0.58}}, kBesides[3] = {7.0, 3.1, 2.0};
+  const double(&kStep)[3] = kSteps[pair];
+  GatedPlan best{};
+  double least = 0.0;
+  for (int size = 0; size < 3; ++size) {
+    GatedPlan p{};
+    p.size = size;
+    p.tiles_r = ceil_div(rows, gated_tile_rows(size)) * row_sets;
+    p.tiles_c = static_cast<int32_t>(ceil_div(cols, gated_tile_cols(size)));
+    p.k_tiles = k_tiles;
+    const int64_t tiles = p.tiles_r * p.tiles_c, slots = gated_at_once(size);
+    const int64_t whole = tiles / slots * slots, rest = tiles - whole;
+    const double unit = k_tiles * kStep[size] + kBesides[size];
+    const double tile_mb = gated_tile_rows(size) * gated_tile_cols(size) * 4e-6;
+    const auto consider = [&](int64_t parts) {
+      if (parts < 1 || (parts > 1 && (!may_cut || rest == 0 || ceil_div(k_tiles, parts) < 4 || rest * parts > (1 << 24)))) return;
+      const int64_t k_part = ceil_div(k_tiles, parts);
+      parts = ceil_div(k_tiles, k_part);
+      double time = static_cast<double>(whole / slots) * unit;
+      if (rest > 0) time += static_cast<double>(ceil_div(rest * parts, slots)) * (k_part * kStep[size] + kBesides[size]);
+      if (parts > 1) time += 6.0 + 0.4 * static_cast<double>(rest * parts) * tile_mb;
+      if (best.k_tiles != 0 && time >= least) return;
+      least = time;
+      best = p;
+      best.parts = static_cast<int32_t>(parts);
+      best.k_part = k_part;
+      best.whole = parts > 1 ? whole : tiles;
+      best.units = parts > 1 ? whole + rest * parts : tiles;
+    };
+    for (int64_t parts = 1; parts <= 8; ++parts) consider(parts);
+    for (int64_t rounds = 1; rounds <= 4 && rest > 0; ++rounds) consider(rounds * slots / rest);
   }
-  p.k_split = ceil_div(k_tiles, splits);
-  p.splits = static_cast<int32_t>(ceil_div(k_tiles, p.k_split));
-  return p;
+  return best;
 }
+
+inline size_t gated_partial_bytes(const GatedPlan& p) {
+  return static_cast<size_t>(p.units - p.whole) * gated_tile_rows(p.size) * gated_tile_cols(p.size) * (p.parts > 1 ? 4 : 0);
+}
+
+template <class Ty, class Out, int MODE, class T>
+int launch_gated_tile(const GatedArgs& a, hipStream_t s) {
+  const int64_t most = T::kTurns ? gated_at_once(a.p.size) : a.p.units;
+  const unsigned grid = static_cast<unsigned>(a.p.units < most ? a.p.units : most);
+  hipLaunchKernelGGL((gated_tile_kernel<Ty, Out, MODE, T>), dim3(grid), dim3(T::kThreads), 0, s, a);
+  if (int rc = hip_status(hipGetLastError(), "gated_tile_kernel launch")) return rc;
+  if constexpr (MODE != kGatedGates) {
+    if (a.p.parts > 1) {
+      constexpr int64_t kPerTile = T::BR * (gated_pair(MODE) ? T::BC / 2 : T::BC) / 4 / 256;
+      const int64_t cut = a.p.tiles_r * a.p.tiles_c - a.p.whole;
+      hipLaunchKernelGGL((gated_join_kernel<Out, MODE, T>), dim3(static_cast<unsigned>(cut * kPerTile)), dim3(256), 0, s, a);
+      return hip_status(hipGetLastError(), "gated_join_kernel launch");
+    }
+  }
+  return OW_OK;
+}
+
+template <class Ty, class Out, int MODE>
+int launch_gated(const GatedArgs& a, hipStream_t s) {
+  if (a.p.size == 0) return launch_gated_tile<Ty, Out, MODE, TileL>(a, s);
+  if (a.p.size == 1) return launch_gated_tile<Ty, Out, MODE, TileM>(a, s);
+  return launch_gated_tile<Ty, Out, MODE, TileS>(a, s);
+}
+
+template <int MODE>
+int launch_gated_mode(GatedArgs& a, const GatedPlan& p, int dtype, int64_t k, float* partial, hipStream_t s) {
+  a.p = p;
+  a.partial = partial;
+  a.k_each = static_cast<int32_t>(ceil_div(k, 64));
+  const int64_t cut = p.tiles_r * p.tiles_c - p.whole;
+  a.by_group = Divisor::of(8 * static_cast<uint32_t>(p.tiles_c));
+  a.by_split = Divisor::of(cut > 0 ? static_cast<uint32_t>(cut) : 1u);
+  a.by_each = Divisor::of(static_cast<uint32_t>(a.k_each));
+  if (dtype == OW_DTYPE_BF16) return launch_gated<BF16, BF16, MODE>(a, s);
+  if (dtype == OW_DTYPE_F16) return launch_gated<F16, F16, MODE>(a, s);
+  return launch_gated<BF16, F32, MODE>(a, s);
+}
+
+// Tiles of k of a product over `k` values.
+inline int64_t gated_k_tiles(int64_t k, int dtype) { return ceil_div(k, 64) * (dtype == OW_DTYPE_F32 ? 6 : 1); }
 
 }  // namespace ow

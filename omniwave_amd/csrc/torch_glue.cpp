@@ -605,9 +605,11 @@ std::pair<Tensor, Tensor> run_gated(const Gated& g, bool keep) {
   const c10::DeviceGuard guard(g.x.device());
   Tensor h = at::empty(hidden_shape(g), g.x.options()), kept;
   const OwGatedLinear d = descriptor(g);
-  if (const size_t bytes = keep ? ow_gated_linear_kept(&d) : 0)
-    kept = at::empty({static_cast<int64_t>(bytes / sizeof(float))}, g.x.options().dtype(at::kFloat));
-  check(ow_gated_linear_fwd(&d, out_ptr(h), out_ptr(kept), stream_of(g.x)), "ow_gated_linear_fwd");
+  if (const size_t size = keep ? ow_gated_linear_kept(&d) : 0)
+    kept = at::empty({static_cast<int64_t>(size / sizeof(float))}, g.x.options().dtype(at::kFloat));
+  const size_t bytes = ow_gated_linear_fwd_workspace(&d);
+  const Tensor workspace = bytes ? at::empty({static_cast<int64_t>(bytes)}, g.x.options().dtype(at::kByte)) : Tensor();
+  check(ow_gated_linear_fwd(&d, out_ptr(h), out_ptr(kept), out_ptr(workspace), bytes, stream_of(g.x)), "ow_gated_linear_fwd");
   return {std::move(h), std::move(kept)};
 }
 

@@ -66,8 +66,12 @@ def _run_forward(x, gate_weight, up_weight, keep) -> tuple[Tensor, Tensor]:
         return h.zero_(), kept
     if h.numel():
         desc, _keep = _descriptor(x, gate_weight, up_weight)
-        _on(x.device, _native.lib().ow_gated_linear_fwd, ctypes.byref(desc), h.data_ptr(),
-            kept.data_ptr() if kept.numel() else None)
+        lib = _native.lib()
+        with torch.cuda.device(x.device):  # the size goes by the device's compute units
+            ws_bytes = lib.ow_gated_linear_fwd_workspace(ctypes.byref(desc))
+        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
+        _on(x.device, lib.ow_gated_linear_fwd, ctypes.byref(desc), h.data_ptr(), kept.data_ptr() if kept.numel() else None,
+            None if workspace is None else workspace.data_ptr(), ws_bytes)
     return h, kept
 
 
@@ -146,7 +150,10 @@ def gated_linear_hip(x: Tensor, gate_weight: Tensor, up_weight: Tensor) -> Tenso
     ``[..., C]`` (rows at any one distance) and weights ``[hidden, C]``, all of one type (float16, bfloat16 or float32),
     to ``[..., hidden]``.  Products and gate are fp32 and the result is rounded once.  Differentiable once in all three.  The
     backward rounds the gradients of both products to the type in between; where C is large (1,536 for 16-bit types, 128 for
-    float32) the forward of a call with a graph keeps both products for it, 8 bytes a value, else they are formed again."""
+    float32) the forward of a call with a graph keeps both products for it, 8 bytes a value, else they are formed again.
+
+    float32 of more than 64 rows runs on the bf16 matrix cores in three-part operands: an infinity makes its results NaN,
+    and values below about 2^-110 are held to fewer than 24 bits."""
     glue = _native.glue()
     if glue is not None and _plain(x, gate_weight, up_weight):
         h = glue.gated_linear(x, gate_weight, up_weight)

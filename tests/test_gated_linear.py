@@ -112,16 +112,16 @@ def test_c_entry_points_check_their_arguments() -> None:
     def refused(rc, text, code=1):
         assert rc == code and text in lib.ow_last_error(), lib.ow_last_error()
 
-    refused(lib.ow_gated_linear_fwd(None, p, None, None), b"NULL")
-    refused(lib.ow_gated_linear_fwd(desc(dtype=3), p, None, None), b"dtype", 2)
-    refused(lib.ow_gated_linear_fwd(desc(hidden=-1), p, None, None), b"negative")
-    refused(lib.ow_gated_linear_fwd(desc(channels=(1 << 20) + 1), p, None, None), b"at most", 2)
-    refused(lib.ow_gated_linear_fwd(desc(rows=1 << 31), p, None, None), b"2^31", 2)
-    refused(lib.ow_gated_linear_fwd(desc(up_weight=None), p, None, None), b"NULL")
-    refused(lib.ow_gated_linear_fwd(desc(x=257), p, None, None), b"aligned")
-    refused(lib.ow_gated_linear_fwd(desc(), None, None, None), b"NULL")
-    refused(lib.ow_gated_linear_fwd(desc(channels=0), p, None, None), b"no channels")
-    assert lib.ow_gated_linear_fwd(desc(rows=0), None, None, None) == 0 and lib.ow_gated_linear_fwd(desc(hidden=0), None, None, None) == 0
+    refused(lib.ow_gated_linear_fwd(None, p, None, None, 0, None), b"NULL")
+    refused(lib.ow_gated_linear_fwd(desc(dtype=3), p, None, None, 0, None), b"dtype", 2)
+    refused(lib.ow_gated_linear_fwd(desc(hidden=-1), p, None, None, 0, None), b"negative")
+    refused(lib.ow_gated_linear_fwd(desc(channels=(1 << 20) + 1), p, None, None, 0, None), b"at most", 2)
+    refused(lib.ow_gated_linear_fwd(desc(rows=1 << 31), p, None, None, 0, None), b"2^31", 2)
+    refused(lib.ow_gated_linear_fwd(desc(up_weight=None), p, None, None, 0, None), b"NULL")
+    refused(lib.ow_gated_linear_fwd(desc(x=257), p, None, None, 0, None), b"aligned")
+    refused(lib.ow_gated_linear_fwd(desc(), None, None, None, 0, None), b"NULL")
+    refused(lib.ow_gated_linear_fwd(desc(channels=0), p, None, None, 0, None), b"no channels")
+    assert lib.ow_gated_linear_fwd(desc(rows=0), None, None, None, 0, None) == 0 and lib.ow_gated_linear_fwd(desc(hidden=0), None, None, None, 0, None) == 0
     assert lib.ow_gated_linear_bwd_workspace(None) == 0 and lib.ow_gated_linear_bwd_workspace(desc(rows=0)) == 0
     need = lib.ow_gated_linear_bwd_workspace(desc())
     assert need >= 2 * 100 * 6 * 2
@@ -134,8 +134,8 @@ def test_c_entry_points_check_their_arguments() -> None:
     refused(bwd(desc(), dh=None), b"NULL")
     refused(bwd(desc(), dh=ctypes.c_void_p(257)), b"aligned")
     refused(bwd(desc(), kept=ctypes.c_void_p(258)), b"aligned")
-    refused(lib.ow_gated_linear_fwd(desc(), p, p, None), b"kept")
-    refused(lib.ow_gated_linear_fwd(desc(channels=1536), p, ctypes.c_void_p(258), None), b"kept")
+    refused(lib.ow_gated_linear_fwd(desc(), p, p, None, 0, None), b"kept")
+    refused(lib.ow_gated_linear_fwd(desc(channels=1536), p, ctypes.c_void_p(258), None, 0, None), b"kept")
     assert lib.ow_gated_linear_kept(None) == 0 and lib.ow_gated_linear_kept(desc(channels=1536)) == 2 * 100 * 6 * 4
     refused(bwd(desc(), ws=None), b"workspace")
     refused(bwd(desc(), n=need - 1), b"workspace")
