@@ -127,17 +127,17 @@ struct AlongK {
       off[i] = index < extent ? static_cast<uint32_t>(index) * static_cast<uint32_t>(ld) + piece * 16 : kOffOut;
     }
   }
-  // base, other: the tile's first index of each matrix at the tile's k; k_left: values of k that are there, up to a tile's.
-  __device__ __forceinline__ void fetch(const char* base, const char* other, int k_left, uint32_t lds, int wave) const {
-    const auto r0 = buffer_rsrc(base, 0x7fffffffu), r1 = buffer_rsrc(PAIR ? other : base, 0x7fffffffu);
-    const bool there = piece * 8 < k_left;
-#pragma unroll
-    for (int i = 0; i < kCopies; ++i)
-      tile_copy(part(i, wave) ? r1 : r0, there ? off[i] : kOffOut, lds + 8 * (i * WAVES + wave) * 128);
+  // Copy i.  r0, r1: from the tile's first index of each matrix at the tile's k; k_left: values of k that are there, up to a tile's.
+  __device__ __forceinline__ void copy(int i, __amdgpu_buffer_rsrc_t r0, __amdgpu_buffer_rsrc_t r1, int k_left, uint32_t lds, int wave) const {
+    tile_copy(part(i, wave) ? r1 : r0, piece * 8 < k_left ? off[i] : kOffOut, lds + 8 * (i * WAVES + wave) * 128);
   }
-  static __device__ __forceinline__ u32x4 read(uint32_t lds, int first, int step, int lane) {
+  // A lane's address for the wave's first index, of step 0; a step's pieces are a XOR away, further indexes an offset.
+  static __device__ __forceinline__ uint32_t lane_at(uint32_t lds, int first, int lane) {
     const int l32 = lane & 31, hh = lane >> 5;
-    const uint32_t at = lds + (first + l32) * 128 + (((2 * step + hh) ^ slot_of(l32)) << 4);
+    return lds + (first + l32) * 128 + ((hh ^ slot_of(l32)) << 4);
+  }
+  static __device__ __forceinline__ u32x4 read(uint32_t lane_at, uint32_t stage, int i, int step) {
+    const uint32_t at = (lane_at ^ (step << 5)) + stage + i * 4096;
     return *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(static_cast<uintptr_t>(at));
   }
 };
@@ -161,21 +161,21 @@ struct AcrossK {
       off[i] = p * 8 < n_out ? static_cast<uint32_t>(k) * static_cast<uint32_t>(ld) + p * 16 : kOffOut;
     }
   }
-  // base: the first output index at the tile's k; k_left: values of k that are there, up to a tile's.
-  __device__ __forceinline__ void fetch(const char* base, int k_left, uint32_t lds, int wave) const {
-    const auto r = buffer_rsrc(base, 0x7fffffffu);
-#pragma unroll
-    for (int i = 0; i < kCopies; ++i) {
-      const int copy = i * WAVES + wave;
-      tile_copy(r, in < k_left - copy * kRowsOfCopy ? off[i] : kOffOut, lds + copy * 1024);
-    }
+  // Copy i.  r: from the first output index at the tile's k; k_left: values of k that are there, up to a tile's.
+  __device__ __forceinline__ void copy(int i, __amdgpu_buffer_rsrc_t r, __amdgpu_buffer_rsrc_t, int k_left, uint32_t lds, int wave) const {
+    const int copy = i * WAVES + wave;
+    tile_copy(r, in < k_left - copy * kRowsOfCopy ? off[i] : kOffOut, lds + copy * 1024);
   }
-  static __device__ __forceinline__ u32x4 read(uint32_t lds, int first, int step, int lane) {
-    const int hh = lane >> 5, l16 = lane & 15;
+  // A lane's address for the wave's first index, of step 0; the next 32 indexes are a XOR away (the wave's first is a
+  // multiple of what it has of them), steps an offset.
+  static __device__ __forceinline__ uint32_t lane_at(uint32_t lds, int first, int lane) {
+    const int l16 = lane & 15, k = 8 * (lane >> 5) + (l16 >> 2);
     const int c = first + 16 * ((lane >> 4) & 1) + 4 * (l16 & 3);
-    const int k = 16 * step + 8 * hh + (l16 >> 2);
-    const auto at = [&](int kk) { return lds + kk * kRow + (slot(c >> 3, kk) << 4) + ((c & 4) << 1); };
-    const u32x2 a = lds_read_tr16(at(k)), b = lds_read_tr16(at(k + 4));
+    return lds + k * kRow + (slot(c >> 3, k) << 4) + ((c & 4) << 1);
+  }
+  static __device__ __forceinline__ u32x4 read(uint32_t lane_at, uint32_t stage, int i, int step) {
+    const uint32_t at = (lane_at ^ (i << 6)) + stage + step * 16 * kRow;
+    const u32x2 a = lds_read_tr16(at), b = lds_read_tr16(at + 4 * kRow);
     return u32x4{a[0], a[1], b[0], b[1]};
   }
 };
@@ -238,13 +238,11 @@ struct Turn {
       if (row < rows) {
         if (c + V <= cols) {
           *reinterpret_cast<u32x4_any*>(out) = w;
-        } else {
-#pragma unroll
-          for (int j = 0; j < V; ++j)
-            if (c + j < cols) {
-              if constexpr (SIZE == 2) reinterpret_cast<uint16_t*>(out)[j] = j & 1 ? hi16(w[j >> 1]) : lo16(w[j >> 1]);
-              else reinterpret_cast<uint32_t*>(out)[j] = w[j];
-            }
+        } else {  // the last piece of ragged rows, from LDS value by value
+          typedef typename std::conditional<SIZE == 2, uint16_t, uint32_t>::type Value;
+          const auto* from = reinterpret_cast<__attribute__((address_space(3))) Value*>(static_cast<uintptr_t>(at(lds, row, piece)));
+#pragma unroll 1
+          for (int j = 0; c + j < cols; ++j) reinterpret_cast<Value*>(out)[j] = from[j];
         }
       }
       out += kRows * ld;
@@ -372,31 +370,50 @@ __global__ void __launch_bounds__(T::kThreads, 2) gated_tile_kernel(GatedArgs a)
     f = unit_at(next);
     init();
   };
-  auto fetch = [&](int stage) {
-    const uint32_t at_r = lds_addr(lds[stage]), at_c = at_r + T::kBytesR;
-    const auto left = [&](int64_t k) { return f.kt >= f.kt_end ? 0 : k < 64 ? static_cast<int>(k) : 64; };
+  // Where the next tile of k is, and to the one after it.
+  struct Source {
+    __amdgpu_buffer_rsrc_t r, c, other;
+    int k_left;
+  };
+  auto source = [&]() {
     // Products of planes, the smallest first: (2, 0), (1, 1), (0, 2), (1, 0), (0, 1), (0, 0).  In dx all of dG's come before dU's.
     const uint32_t which = MODE == kGatedDx && f.product >= kProducts ? 1 : 0, pair = f.product - which * kProducts;
     const int plane_r = kWide ? (0x001012 >> (4 * pair)) & 3 : 0, plane_c = kWide ? (0x010210 >> (4 * pair)) & 3 : 0;
     const int64_t k0 = static_cast<int64_t>(f.k_in) * 64;
+    const char *r, *c, *other;
+    int64_t left;
     if constexpr (kPair) {
-      const int k_left = left(a.channels - k0);
-      op_r.fetch(a.x.at + plane_r * a.x.plane + f.at.r0 * a.x.ld + k0 * 2, nullptr, k_left, at_r, wave);
+      left = a.channels - k0;
+      r = a.x.at + plane_r * a.x.plane + f.at.r0 * a.x.ld + k0 * 2;
       const int64_t at = plane_c * a.w[0].plane + f.at.c0 * a.w[0].ld + k0 * 2;
-      op_c.fetch(a.w[0].at + at, a.w[1].at + at, k_left, at_c, wave);
+      c = a.w[0].at + at, other = a.w[1].at + at;
     } else if constexpr (MODE == kGatedDx) {
-      const int k_left = left(a.hidden - k0);
-      op_r.fetch(a.gu[which].at + plane_r * a.gu[0].plane + f.at.r0 * a.gu[0].ld + k0 * 2, nullptr, k_left, at_r, wave);
-      op_c.fetch(a.w[which].at + plane_c * a.w[0].plane + k0 * a.w[0].ld + f.at.c0 * 2, k_left, at_c, wave);
+      left = a.hidden - k0;
+      r = a.gu[which].at + plane_r * a.gu[0].plane + f.at.r0 * a.gu[0].ld + k0 * 2;
+      c = other = a.w[which].at + plane_c * a.w[0].plane + k0 * a.w[0].ld + f.at.c0 * 2;
     } else {
-      const int k_left = left(a.rows - k0);
-      op_r.fetch(a.gu[f.at.which].at + plane_r * a.gu[0].plane + k0 * a.gu[0].ld + f.at.r0 * 2, k_left, at_r, wave);
-      op_c.fetch(a.x.at + plane_c * a.x.plane + k0 * a.x.ld + f.at.c0 * 2, k_left, at_c, wave);
+      left = a.rows - k0;
+      r = a.gu[f.at.which].at + plane_r * a.gu[0].plane + k0 * a.gu[0].ld + f.at.r0 * 2;
+      c = other = a.x.at + plane_c * a.x.plane + k0 * a.x.ld + f.at.c0 * 2;
     }
+    Source s{buffer_rsrc(r, 0x7fffffffu), buffer_rsrc(c, 0x7fffffffu), buffer_rsrc(other, 0x7fffffffu),
+             f.kt >= f.kt_end ? 0 : left < 64 ? static_cast<int>(left) : 64};
     if (f.kt < f.kt_end) {
       ++f.kt;
       if (++f.k_in == static_cast<uint32_t>(a.k_each)) f.k_in = 0, ++f.product;
     }
+    return s;
+  };
+  constexpr int kCopies = OpR::kCopies + OpC::kCopies;
+  auto copy = [&](const Source& s, int stage, int i) {
+    const uint32_t at_r = lds_addr(lds[stage]), at_c = at_r + T::kBytesR;
+    if (i < OpR::kCopies) op_r.copy(i, s.r, s.r, s.k_left, at_r, wave);
+    else op_c.copy(i - OpR::kCopies, s.c, s.other, s.k_left, at_c, wave);
+  };
+  auto fetch = [&](int stage) {
+    const Source s = source();
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) copy(s, stage, i);
   };
 
   f32x16 acc[T::CI][T::RI];
@@ -408,12 +425,13 @@ __global__ void __launch_bounds__(T::kThreads, 2) gated_tile_kernel(GatedArgs a)
   };
   const int wr = wave / T::WC * (T::RI * 32), wc = wave % T::WC * (T::CI * 32);
   u32x4 fr[2][T::RI], fc[2][T::CI];
+  const uint32_t lane_r = OpR::lane_at(lds_addr(lds[0]), wr, lane), lane_c = OpC::lane_at(lds_addr(lds[0]) + T::kBytesR, wc, lane);
   auto read = [&](int stage, int s, int buf) {
-    const uint32_t at_r = lds_addr(lds[stage]), at_c = at_r + T::kBytesR;
+    const uint32_t from = stage * (T::kBytesR + T::kBytesC);
 #pragma unroll
-    for (int i = 0; i < T::CI; ++i) fc[buf][i] = OpC::read(at_c, wc + 32 * i, s, lane);
+    for (int i = 0; i < T::CI; ++i) fc[buf][i] = OpC::read(lane_c, from, i, s);
 #pragma unroll
-    for (int j = 0; j < T::RI; ++j) fr[buf][j] = OpR::read(at_r, wr + 32 * j, s, lane);
+    for (int j = 0; j < T::RI; ++j) fr[buf][j] = OpR::read(lane_r, from, j, s);
   };
   auto multiply = [&](int buf) {
 #pragma unroll
@@ -421,7 +439,6 @@ __global__ void __launch_bounds__(T::kThreads, 2) gated_tile_kernel(GatedArgs a)
 #pragma unroll
       for (int i = 0; i < T::CI; ++i) acc[i][j] = Ty::mma32(fc[buf][i], fr[buf][j], acc[i][j]);
   };
-  constexpr int kCopies = OpR::kCopies + OpC::kCopies;
   // A step's reads go between its products, one after each; left alone, the compiler puts them right before their use.
   constexpr int kReads = T::CI * OpC::kReads + T::RI * OpR::kReads, kMfma = T::CI * T::RI;
   auto interleave = [&]() {
@@ -449,6 +466,7 @@ __global__ void __launch_bounds__(T::kThreads, 2) gated_tile_kernel(GatedArgs a)
   int stage = 0;
   for (uint32_t index = blockIdx.x;;) {
     turn();
+    const Source tile = source();
 #pragma unroll
     for (int s = 0; s < 3; ++s) {
       read(stage, s + 1, (s + 1) & 1);
@@ -458,15 +476,25 @@ __global__ void __launch_bounds__(T::kThreads, 2) gated_tile_kernel(GatedArgs a)
     wait_vmcnt<0>();
     __syncthreads();
     __builtin_amdgcn_sched_barrier(0);
+    // The copies go between this step's products.
     read(stage ^ 1, 0, 0);
-    fetch(stage);
-    multiply(1);
-    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int m = 0; m < kMfma; ++m) {
+      const int i = m % T::CI, j = m / T::CI;
+      acc[i][j] = Ty::mma32(fc[1][i], fr[1][j], acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int n = kCopies * m / kMfma; n < kCopies * (m + 1) / kMfma; ++n) copy(tile, stage, n);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     stage ^= 1;
     if (++u.kt < u.kt_end) continue;
     mfma_drain();
 
     const uint32_t own = lds_addr(turns[wave]);
+    // What the stores compute of the lane stays behind the loop: hoisted, it takes registers that the loop needs.
+    int out_lane = lane;
+    asm volatile("" : "+v"(out_lane));
     auto values = [&](int i, int j, float (&v)[16]) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) v[e] = acc[i][j][e];
@@ -482,8 +510,8 @@ __global__ void __launch_bounds__(T::kThreads, 2) gated_tile_kernel(GatedArgs a)
         for (int i = 0; i < T::CI; ++i) {
           float v[16];
           values(i, j, v);
-          Turn<128>::put<F32>(own, 0, v, lane);
-          Turn<128>::store<4>(own, out + 32 * j * kLd + 32 * i * 4, kLd, 32, 32, lane);
+          Turn<128>::put<F32>(own, 0, v, out_lane);
+          Turn<128>::store<4>(own, out + 32 * j * kLd + 32 * i * 4, kLd, 32, 32, out_lane);
         }
     } else if constexpr (kPair) {
       typedef Turn<32 * S> Tn;
@@ -498,32 +526,35 @@ __global__ void __launch_bounds__(T::kThreads, 2) gated_tile_kernel(GatedArgs a)
             for (int i = 0; i < 2; ++i) {
               float v[16];
               values(i, j, v);
-              Turn<128>::put<F32>(own, 0, v, lane);
+              Turn<128>::put<F32>(own, 0, v, out_lane);
               Turn<128>::store<4>(own, reinterpret_cast<char*>(a.kept) + (i * a.rows + row) * ld_kept + c * 4, ld_kept, a.rows - row,
-                                  a.hidden - c, lane);
+                                  a.hidden - c, out_lane);
             }
           }
           float h[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) h[i] = acc[0][j][i] * acc[1][j][i] * sigmoid(acc[0][j][i]);
-          Tn::template put<Out>(own, 0, h, lane);
-          Tn::template store<S>(own, static_cast<char*>(a.out[0]) + row * ld + c * S, ld, a.rows - row, a.hidden - c, lane);
+          Tn::template put<Out>(own, 0, h, out_lane);
+          Tn::template store<S>(own, static_cast<char*>(a.out[0]) + row * ld + c * S, ld, a.rows - row, a.hidden - c, out_lane);
         }
       } else {
         // Columns up to a whole piece are written: there both products are 0.  The gradients of G and U are
         // rounded to the operands' type here, as the products that take them need it (fp32: to its three planes).
-        u32x4 w[T::RI][Tn::kCopies];
-#pragma unroll
-        for (int j = 0; j < T::RI; ++j) {
+        constexpr int kAhead = T::RI <= 2 ? T::RI : 1;  // rows of products whose upstream gradients are read at once
+        u32x4 w[kAhead][Tn::kCopies];
+        auto upstream = [&](int j) {
           const int64_t row = r + 32 * j;
-          Tn::template load<S>(w[j], a.dh + row * a.dh_ld + c * S, a.dh_ld, a.rows - row, a.hidden - c, lane);
-        }
+          Tn::template load<S>(w[j % kAhead], a.dh + row * a.dh_ld + c * S, a.dh_ld, a.rows - row, a.hidden - c, out_lane);
+        };
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) upstream(j);
 #pragma unroll
         for (int j = 0; j < T::RI; ++j) {
           const int64_t row = r + 32 * j, at = row * a.gu[0].ld + c * 2;
           float dh[16], d[2][16];
-          Tn::keep(own, w[j], lane);
-          Tn::template get<Out>(own, dh, lane);
+          if (j >= kAhead) upstream(j);
+          Tn::keep(own, w[j % kAhead], out_lane);
+          Tn::template get<Out>(own, dh, out_lane);
           wave_lds_sync();
 #pragma unroll
           for (int i = 0; i < 16; ++i) gates(dh[i], acc[0][j][i], acc[1][j][i], d[0][i], d[1][i]);
@@ -531,9 +562,9 @@ __global__ void __launch_bounds__(T::kThreads, 2) gated_tile_kernel(GatedArgs a)
           for (int o = 0; o < 2; ++o) {
 #pragma unroll
             for (int plane = 0; plane < (kWide ? 3 : 1); ++plane) {
-              Turn<64>::put<Ty>(own, 0, d[o], lane);
+              Turn<64>::put<Ty>(own, 0, d[o], out_lane);
               Turn<64>::store<2>(own, static_cast<char*>(a.out[o]) + plane * a.gu[0].plane + at, a.gu[0].ld, a.rows - row,
-                                 a.gu[0].ld / 2 - c, lane);
+                                 a.gu[0].ld / 2 - c, out_lane);
               if constexpr (kWide) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) d[o][i] -= BF16::to_f32(BF16::from_f32(d[o][i]));
@@ -554,13 +585,13 @@ __global__ void __launch_bounds__(T::kThreads, 2) gated_tile_kernel(GatedArgs a)
           float v[16];
           values(i, j, v);
           if constexpr (kWide) {  // 32 columns at a time
-            Turn<128>::put<F32>(own, 0, v, lane);
-            Turn<128>::store<4>(own, out + row * ld + (c + 32 * i) * 4, ld, n_r - row, a.channels - c - 32 * i, lane);
+            Turn<128>::put<F32>(own, 0, v, out_lane);
+            Turn<128>::store<4>(own, out + row * ld + (c + 32 * i) * 4, ld, n_r - row, a.channels - c - 32 * i, out_lane);
           } else {
-            Turn<128>::put<Ty>(own, 4 * i, v, lane);
+            Turn<128>::put<Ty>(own, 4 * i, v, out_lane);
           }
         }
-        if constexpr (!kWide) Turn<128>::store<2>(own, out + row * ld + c * 2, ld, n_r - row, a.channels - c, lane);
+        if constexpr (!kWide) Turn<128>::store<2>(own, out + row * ld + c * 2, ld, n_r - row, a.channels - c, out_lane);
       }
     }
     index += gridDim.x;
