@@ -140,16 +140,26 @@ int check_gated(const OwGatedLinear* d) {
 namespace {
 
 // Rows of values, of any alignment, to planes of rows of whole pieces with zeros behind them: a copy of 16-bit values, or fp32
-// ones in three bf16 parts.  A thread has a piece of 8 values.
+// ones in three bf16 parts.  A thread has a piece of 8 values; x and the weights go in one launch (blockIdx.y).
+struct PackArgs {
+  const char* src[3];
+  int64_t src_ld[3], rows[3], plane[3];
+  char* dst[3];
+  int64_t ld;
+  int32_t values;
+};
+
 template <bool WIDE>
-__global__ void __launch_bounds__(256) gated_pack_kernel(const char* src, int64_t src_ld, int64_t rows, int32_t values, char* dst, int64_t ld,
-                                                         int64_t plane) {
-  const uint32_t pieces = static_cast<uint32_t>(ld / 16);
-  const int64_t all = rows * pieces, step = static_cast<int64_t>(gridDim.x) * 256;
+__global__ void __launch_bounds__(256) gated_pack_kernel(PackArgs a) {
+  const int o = blockIdx.y;
+  const char* const src = a.src[o];
+  const int64_t src_ld = a.src_ld[o], plane = a.plane[o];
+  const uint32_t pieces = static_cast<uint32_t>(a.ld / 16);
+  const int64_t all = a.rows[o] * pieces, step = static_cast<int64_t>(gridDim.x) * 256;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += step) {
     const int64_t row = i / pieces;
-    const int c = static_cast<int>(i - row * pieces) * 8, n = values - c;
-    char* out = dst + row * ld + c * 2;
+    const int c = static_cast<int>(i - row * pieces) * 8, n = a.values - c;
+    char* out = a.dst[o] + row * a.ld + c * 2;
     if constexpr (WIDE) {
       const char* in = src + row * src_ld + static_cast<int64_t>(c) * 4;
       const u32x4 lo = load_piece<4>(in, n), hi = load_piece<4>(in + 16, n - 4);
@@ -160,16 +170,6 @@ __global__ void __launch_bounds__(256) gated_pack_kernel(const char* src, int64_
       *reinterpret_cast<u32x4*>(out) = load_piece<2>(src + row * src_ld + static_cast<int64_t>(c) * 2, n);
     }
   }
-}
-
-int pack(const void* src, int64_t src_ld, int64_t rows, int32_t values, bool wide, const GatedPlanes& to, hipStream_t s) {
-  const int64_t groups = ceil_div(rows * (to.ld / 16), 256), most = 16 * static_cast<int64_t>(device_cus());
-  const dim3 grid(static_cast<unsigned>(groups < most ? groups : most));
-  char* dst = const_cast<char*>(to.at);
-  const char* from = static_cast<const char*>(src);
-  if (wide) hipLaunchKernelGGL((gated_pack_kernel<true>), grid, dim3(256), 0, s, from, src_ld, rows, values, dst, to.ld, to.plane);
-  else hipLaunchKernelGGL((gated_pack_kernel<false>), grid, dim3(256), 0, s, from, src_ld, rows, values, dst, to.ld, to.plane);
-  return hip_status(hipGetLastError(), "gated_pack_kernel launch");
 }
 
 size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -202,19 +202,32 @@ int gated_operands(const OwGatedLinear& d, char* workspace, GatedArgs* a, hipStr
   a->x = GatedPlanes{static_cast<const char*>(d.x), d.x_stride * 2, 0};
   const void* weights[2] = {d.gate_weight, d.up_weight};
   for (int i = 0; i < 2; ++i) a->w[i] = GatedPlanes{static_cast<const char*>(weights[i]), d.channels * 2, 0};
-  if (!x_direct(d)) {
-    a->x = GatedPlanes{workspace, ld, d.rows * ld};
-    workspace += aligned((wide ? 3 : 1) * d.rows * ld);
-    if (int rc = pack(d.x, d.x_stride * size, d.rows, d.channels, wide, a->x, s)) return rc;
-  }
+  PackArgs pack{};
+  int n = 0;
+  const auto copy = [&](GatedPlanes* to, const void* src, int64_t src_ld, int64_t rows) {
+    *to = GatedPlanes{workspace, ld, rows * ld};
+    pack.src[n] = static_cast<const char*>(src);
+    pack.src_ld[n] = src_ld;
+    pack.rows[n] = rows;
+    pack.plane[n] = rows * ld;
+    pack.dst[n++] = workspace;
+    workspace += aligned((wide ? 3 : 1) * rows * ld);
+  };
+  if (!x_direct(d)) copy(&a->x, d.x, d.x_stride * size, d.rows);
   if (!w_direct(d)) {
-    for (int i = 0; i < 2; ++i) {
-      a->w[i] = GatedPlanes{workspace, ld, d.hidden * ld};
-      workspace += aligned((wide ? 3 : 1) * d.hidden * ld);
-      if (int rc = pack(weights[i], d.channels * size, d.hidden, d.channels, wide, a->w[i], s)) return rc;
-    }
+    for (int i = 0; i < 2; ++i) copy(&a->w[i], weights[i], d.channels * size, d.hidden);
   }
-  return OW_OK;
+  if (n == 0) return OW_OK;
+  pack.ld = ld;
+  pack.values = d.channels;
+  int64_t rows = 0;
+  for (int i = 0; i < n; ++i) rows = pack.rows[i] > rows ? pack.rows[i] : rows;
+  const int64_t groups = ceil_div(rows * (ld / 16), 256);
+  const int64_t most = 16 * static_cast<int64_t>(device_cus());
+  const dim3 grid(static_cast<unsigned>(groups < most ? groups : most), n);
+  if (wide) hipLaunchKernelGGL((gated_pack_kernel<true>), grid, dim3(256), 0, s, pack);
+  else hipLaunchKernelGGL((gated_pack_kernel<false>), grid, dim3(256), 0, s, pack);
+  return hip_status(hipGetLastError(), "gated_pack_kernel launch");
 }
 
 namespace {

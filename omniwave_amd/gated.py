@@ -18,6 +18,7 @@ from omniwave_amd.hip import _DTYPE_CODE, SUPPORTED_DTYPES, _plain
 from omniwave_amd.norms import _on, _rows, gpu_reason
 
 MAX_WIDTH = 1 << 20  # channels, hidden
+FEW_ROWS = 64  # for which there is a kernel of its own
 
 
 def _ready(x, gate_weight, up_weight) -> None:
@@ -51,10 +52,10 @@ def _descriptor(x, gate_weight, up_weight):
 
 
 def _kept_values(x, gate_weight) -> int:
-    """Values of both products that a forward keeps for its backward, 0 where that forms them again."""
-    desc = _native.OwGatedLinear(rows=math.prod(x.shape[:-1]), channels=x.shape[-1], hidden=gate_weight.shape[0],
-                                 dtype=_DTYPE_CODE[x.dtype])
-    return _native.lib().ow_gated_linear_kept(ctypes.byref(desc)) // 4
+    """Values of both products that a forward keeps for its backward, 0 where that forms them again (the library's
+    ``ow_gated_linear_kept``, for sizes that are not yet known, too)."""
+    rows, channels, hidden = math.prod(x.shape[:-1]), x.shape[-1], gate_weight.shape[0]
+    return 2 * rows * hidden if rows > FEW_ROWS and channels >= (128 if x.dtype == torch.float32 else 1536) else 0
 
 
 def _run_forward(x, gate_weight, up_weight, keep) -> tuple[Tensor, Tensor]:

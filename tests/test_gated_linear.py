@@ -89,6 +89,9 @@ def test_kept_products(launches) -> None:
         assert gated._run_forward(x, w, w, True)[1].numel() == n
         assert gated._run_forward(x, w, w, False)[1].numel() == 0
         assert gated._run_forward(x[:64], w, w, True)[1].numel() == 0
+        for rows in (64, 65, 70):
+            d = _native.OwGatedLinear(rows=rows, channels=c, hidden=6, dtype=1 if dtype == torch.bfloat16 else 0)
+            assert _native.lib().ow_gated_linear_kept(ctypes.byref(d)) == 4 * gated._kept_values(x[:rows], w)
     launches.clear()
     up = torch.zeros(70, 6)
     for kept in (torch.zeros(839), torch.zeros(840).half(), torch.zeros(840, device="meta")):
@@ -134,6 +137,13 @@ def test_c_entry_points_check_their_arguments() -> None:
     refused(bwd(desc(), dh=None), b"NULL")
     refused(bwd(desc(), dh=ctypes.c_void_p(257)), b"aligned")
     refused(bwd(desc(), kept=ctypes.c_void_p(258)), b"aligned")
+    # rows of 10 values fill no whole pieces: x and the weights are copied
+    space = lib.ow_gated_linear_fwd_workspace(desc())
+    assert space >= (100 + 2 * 6) * 32 and lib.ow_gated_linear_fwd_workspace(None) == 0
+    assert lib.ow_gated_linear_fwd_workspace(desc(rows=64)) == 0 and lib.ow_gated_linear_fwd_workspace(desc(channels=8, x_stride=8)) == 0
+    refused(lib.ow_gated_linear_fwd(desc(), p, None, None, 0, None), b"workspace")
+    refused(lib.ow_gated_linear_fwd(desc(), p, None, p, space - 1, None), b"workspace")
+    refused(lib.ow_gated_linear_fwd(desc(), p, None, ctypes.c_void_p(264), space, None), b"workspace")
     refused(lib.ow_gated_linear_fwd(desc(), p, p, None, 0, None), b"kept")
     refused(lib.ow_gated_linear_fwd(desc(channels=1536), p, ctypes.c_void_p(258), None, 0, None), b"kept")
     assert lib.ow_gated_linear_kept(None) == 0 and lib.ow_gated_linear_kept(desc(channels=1536)) == 2 * 100 * 6 * 4

@@ -128,6 +128,10 @@ def test_hidden(rows, hidden, dtype) -> None:
     (100, 2816, 2896),  # 256 x 256 tiles in the weights' gradients
     (99, 2815, 2895),
     (9000, 128, 256),   # sums of many parts
+    (33000, 256, 1100), # whole tiles and parts of others
+    (70, 1408, 130),    # parts of both projections
+    (300, 1600, 70),    # both products kept
+    (300, 1537, 33),
     (4097, 1024, 64),
     (70, 4096, 130),
 ])
@@ -255,6 +259,37 @@ def test_leaves_that_need_no_gradient() -> None:
             t = [q.detach().clone() for q in (x, wg, wu)]
             t[n].requires_grad_(True)
             assert torch.equal(torch.autograd.grad(gated_linear_hip(*t), t[n], dh)[0], full[n])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows,c,hidden", [(100, 1600, 72), (257, 1537, 31), (1100, 1536, 640)])
+def test_products_kept_and_formed_again(rows, c, hidden, dtype) -> None:
+    """The backward's two ways to both products: the same sums, in other orders at most."""
+    announce(f"gated kept products rows={rows} c={c} hidden={hidden} {dtype}")
+    from omniwave_amd.gated import gated_linear_bwd, gated_linear_fwd
+
+    x, wg, wu, dh = make(rows, c, hidden, TYPES[dtype])
+    h, kept = gated_linear_fwd(x, wg, wu, True)
+    plain, none = gated_linear_fwd(x, wg, wu, False)
+    assert kept.numel() == 2 * rows * hidden and not none.numel() and torch.equal(h, plain)
+    ref = formula(x, wg, wu, dh)
+    for n, w in enumerate((wg, wu)):
+        slack = (c + 64) * U * (x.double().abs() @ w.double().abs().T)
+        assert ((kept.view(2, rows, hidden)[n].double() - x.double() @ w.double().T).abs() <= slack).all()
+    for saved in (kept, none):
+        for name, g in zip(("dx", "dgate", "dup"), gated_linear_bwd(dh, saved, x, wg, wu, [True] * 3)):
+            close(g, *ref[name], name)
+
+
+def test_sizes_that_are_not_known_while_compiling() -> None:
+    announce("gated compiled with dynamic sizes")
+    torch._dynamo.reset()
+    fn = torch.compile(lambda *t: gated_linear_hip(*t), backend="aot_eager", dynamic=True)
+    for rows in (80, 90, 30):
+        x, wg, wu, dh = make(rows, 128, 24, torch.float32)
+        leaves = [t.requires_grad_(True) for t in (x, wg, wu)]
+        got = torch.autograd.grad(fn(*leaves), leaves, dh)
+        assert all(torch.equal(a, b) for a, b in zip(got, torch.autograd.grad(gated_linear_hip(*leaves), leaves, dh)))
 
 
 @pytest.mark.parametrize("rows,c,hidden", [(1, 256, 512), (49, 1024, 2048), (700, 128, 96), (3000, 200, 256)])
