@@ -767,7 +767,7 @@ int ow_distillation_bwd(const OwDistillation* d, const float* stats, const float
  * weights [hidden][channels], contiguous, and h [rows][hidden], contiguous, all of `dtype`.  Products and gates are fp32;
  * h is rounded once.  channels, hidden <= 2^20, rows < 2^31; channels >= 1 where anything is computed.  A workspace (16-byte
  * aligned) of ow_gated_linear_fwd_workspace bytes, 0 for few rows and many others.  fp32 operands are three bf16 parts each for
- * more than 64 rows: an infinity makes its results NaN, and values below about 2^-110 have fewer than 24 bits.
+ * many rows and in the backward: an infinity makes its results NaN, and values below about 2^-110 have fewer than 24 bits.
  *
  * A forward with a backward to come may be given kept (4-byte aligned), where ow_gated_linear_kept is not 0: that many bytes, in
  * which it leaves both products in fp32 for the backward, which else forms them again (kept NULL there, too).

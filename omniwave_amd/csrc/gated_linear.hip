@@ -3,11 +3,11 @@
 //
 //   G = x Wg^T    U = x Wu^T    h = silu(G) U,  silu(g) = g / (1 + e^-g)
 //
-// More than 64 tokens go through gated_tile_kernel (ow_gated.h): a tile's columns are 32 of the gate beside the same
+// Many tokens go through gated_tile_kernel (ow_gated.h): a tile's columns are 32 of the gate beside the same
 // 32 of the other projection, so that a lane has both values of an output.  G and U are fp32 until h is rounded; for a
 // backward to come they are stored as they are where that costs less than forming them again.
 //
-// Up to 64 tokens take gated_few_kernel, which is bound by reading the weights: a workgroup has 16 columns of both,
+// Few tokens take gated_few_kernel, which is bound by reading the weights: a workgroup has 16 columns of both and up to 64 tokens,
 // its 8 waves take k in turns of 64 bytes a column and go from memory to the matrix cores without LDS; their sums meet there.
 #include <hip/hip_runtime.h>
 
@@ -46,13 +46,16 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) gated_few_kernel(OwGatedLin
   __shared__ f32x4 part[kFewWaves][2 * TG][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, h = lane >> 4;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16, first = static_cast<int64_t>(blockIdx.y) * 16 * TG;  // token
   // Columns and tokens behind the last one are the last one; nobody stores them.
   const int64_t n = n0 + l16 < d.hidden ? n0 + l16 : d.hidden - 1, at_w = n * d.channels * S + h * 16;
   const char* w[2] = {static_cast<const char*>(d.gate_weight) + at_w, static_cast<const char*>(d.up_weight) + at_w};
   const char* x[TG];
 #pragma unroll
-  for (int g = 0; g < TG; ++g) x[g] = static_cast<const char*>(d.x) + (16 * g + l16 < d.rows ? 16 * g + l16 : d.rows - 1) * d.x_stride * S + h * 16;
+  for (int g = 0; g < TG; ++g) {
+    const int64_t token = first + 16 * g + l16 < d.rows ? first + 16 * g + l16 : d.rows - 1;
+    x[g] = static_cast<const char*>(d.x) + token * d.x_stride * S + h * 16;
+  }
   f32x4 acc[2][TG];
 #pragma unroll
   for (int g = 0; g < TG; ++g) acc[0][g] = acc[1][g] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -103,7 +106,7 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) gated_few_kernel(OwGatedLin
     float G = 0.f, U = 0.f;
 #pragma unroll
     for (int k = 0; k < kFewWaves; ++k) G += part[k][g][at][e], U += part[k][TG + g][at][e];
-    const int64_t row = 16 * g + (at & 15), col = n0 + 4 * (at >> 4) + e;
+    const int64_t row = first + 16 * g + (at & 15), col = n0 + 4 * (at >> 4) + e;
     if (row >= d.rows || col >= d.hidden) continue;
     static_cast<typename Row<Ty>::Elem*>(h_out)[row * d.hidden + col] = Row<Ty>::from_f32(G * U * sigmoid(G));
   }
@@ -111,7 +114,7 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) gated_few_kernel(OwGatedLin
 
 template <class Ty>
 void launch_few(const OwGatedLinear& d, void* h, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>(ceil_div(d.hidden, 16))), block(kFewWaves * 64);
+  const dim3 grid(static_cast<unsigned>(ceil_div(d.hidden, 16)), static_cast<unsigned>(ceil_div(d.rows, kFewRows))), block(kFewWaves * 64);
   if (d.rows <= 16) hipLaunchKernelGGL((gated_few_kernel<Ty, 1>), grid, block, 0, s, d, h);
   else if (d.rows <= 32) hipLaunchKernelGGL((gated_few_kernel<Ty, 2>), grid, block, 0, s, d, h);
   else hipLaunchKernelGGL((gated_few_kernel<Ty, 4>), grid, block, 0, s, d, h);
@@ -232,6 +235,14 @@ int gated_operands(const OwGatedLinear& d, char* workspace, GatedArgs* a, hipStr
 
 namespace {
 
+// Whether gated_few_kernel takes the tokens (no workspace, nothing kept): 64 at most, or more where its workgroups, of 64 tokens and
+// 16 columns, are one round of a GPU's 256 (bf16, 128 tokens of 1,024 to 2,048: 8.6 us, 9.8 in tiles; 192: 15.0 and 9.9), and fp32
+// up to 128, which it takes without splitting the operands (2,048 to 4,096: 74 us, 78 in tiles; 192: 107 and 96).
+bool few(const OwGatedLinear& d) {
+  if (d.rows <= kFewRows || (d.dtype == OW_DTYPE_F32 && d.rows <= 2 * kFewRows)) return true;
+  return d.channels <= (d.dtype == OW_DTYPE_F32 ? 2048 : 1024) && ceil_div(d.hidden, 16) * ceil_div(d.rows, kFewRows) <= 256;
+}
+
 GatedPlan plan_forward(const OwGatedLinear& d) {
   return gated_plan(d.rows, 2 * static_cast<int64_t>(d.hidden), gated_k_tiles(d.channels, d.dtype), 1, true, true);
 }
@@ -244,13 +255,13 @@ extern "C" {
 // The products are kept where forming them again (4 K operations a value, six times as many for fp32) would take longer than
 // to write and read them (16 bytes).
 size_t ow_gated_linear_kept(const OwGatedLinear* d) {
-  if (d == nullptr || d->rows <= ow::kFewRows || d->channels <= 0 || d->hidden <= 0) return 0;
+  if (d == nullptr || ow::few(*d) || d->channels <= 0 || d->hidden <= 0) return 0;
   const int32_t from = d->dtype == OW_DTYPE_F32 ? 128 : 1536;
   return d->channels >= from ? static_cast<size_t>(2) * d->rows * d->hidden * sizeof(float) : 0;
 }
 
 size_t ow_gated_linear_fwd_workspace(const OwGatedLinear* d) {
-  if (d == nullptr || d->rows <= ow::kFewRows || d->channels <= 0 || d->hidden <= 0) return 0;
+  if (d == nullptr || ow::few(*d) || d->channels <= 0 || d->hidden <= 0) return 0;
   return ow::gated_operand_bytes(*d) + ow::gated_partial_bytes(ow::plan_forward(*d));
 }
 
@@ -265,7 +276,7 @@ int ow_gated_linear_fwd(const OwGatedLinear* d, void* h, void* kept, void* works
   OW_CHECK_ARG(kept == nullptr || (ow_gated_linear_kept(d) != 0 && reinterpret_cast<uintptr_t>(kept) % 4 == 0),
                "the products of these sizes are not kept, or have no place for fp32 values");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (d->rows <= ow::kFewRows) {
+  if (ow::few(*d)) {
     if (d->dtype == OW_DTYPE_BF16) ow::launch_few<ow::BF16>(*d, h, s);
     else if (d->dtype == OW_DTYPE_F16) ow::launch_few<ow::F16>(*d, h, s);
     else ow::launch_few<ow::F32>(*d, h, s);

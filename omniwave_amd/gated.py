@@ -18,7 +18,7 @@ from omniwave_amd.hip import _DTYPE_CODE, SUPPORTED_DTYPES, _plain
 from omniwave_amd.norms import _on, _rows, gpu_reason
 
 MAX_WIDTH = 1 << 20  # channels, hidden
-FEW_ROWS = 64  # for which there is a kernel of its own
+FEW_ROWS = 64  # the kernel for few tokens takes them at once
 
 
 def _ready(x, gate_weight, up_weight) -> None:
@@ -54,8 +54,10 @@ def _descriptor(x, gate_weight, up_weight):
 def _kept_values(x, gate_weight) -> int:
     """Values of both products that a forward keeps for its backward, 0 where that forms them again (the library's
     ``ow_gated_linear_kept``, for sizes that are not yet known, too)."""
-    rows, channels, hidden = math.prod(x.shape[:-1]), x.shape[-1], gate_weight.shape[0]
-    return 2 * rows * hidden if rows > FEW_ROWS and channels >= (128 if x.dtype == torch.float32 else 1536) else 0
+    rows, channels, hidden, wide = math.prod(x.shape[:-1]), x.shape[-1], gate_weight.shape[0], x.dtype == torch.float32
+    few = rows <= (2 * FEW_ROWS if wide else FEW_ROWS) or (
+        channels <= (2048 if wide else 1024) and (hidden + 15) // 16 * ((rows + FEW_ROWS - 1) // FEW_ROWS) <= 256)
+    return 0 if few or channels < (128 if wide else 1536) else 2 * rows * hidden
 
 
 def _run_forward(x, gate_weight, up_weight, keep) -> tuple[Tensor, Tensor]:
@@ -153,8 +155,8 @@ def gated_linear_hip(x: Tensor, gate_weight: Tensor, up_weight: Tensor) -> Tenso
     backward rounds the gradients of both products to the type in between; where C is large (1,536 for 16-bit types, 128 for
     float32) the forward of a call with a graph keeps both products for it, 8 bytes a value, else they are formed again.
 
-    float32 of more than 64 rows runs on the bf16 matrix cores in three-part operands: an infinity makes its results NaN,
-    and values below about 2^-110 are held to fewer than 24 bits."""
+    float32 of many rows (more than 128, and more than fit one round of the kernel for few) runs on the bf16 matrix cores in
+    three-part operands: an infinity makes its results NaN, and values below about 2^-110 are held to fewer than 24 bits."""
     glue = _native.glue()
     if glue is not None and _plain(x, gate_weight, up_weight):
         h = glue.gated_linear(x, gate_weight, up_weight)

@@ -83,22 +83,24 @@ def test_upstream_gradients(launches, up) -> None:
 
 
 def test_kept_products(launches) -> None:
-    """Two values of fp32 for each of the result, for more than 64 tokens of many channels; the backward looks at them."""
-    for dtype, c, n in ((torch.bfloat16, 1535, 0), (torch.bfloat16, 1536, 2 * 70 * 6), (torch.float32, 127, 0), (torch.float32, 128, 2 * 70 * 6)):
-        x, w = torch.zeros(70, c, dtype=dtype), torch.zeros(6, c, dtype=dtype)
-        assert gated._run_forward(x, w, w, True)[1].numel() == n
-        assert gated._run_forward(x, w, w, False)[1].numel() == 0
-        assert gated._run_forward(x[:64], w, w, True)[1].numel() == 0
-        for rows in (64, 65, 70):
-            d = _native.OwGatedLinear(rows=rows, channels=c, hidden=6, dtype=1 if dtype == torch.bfloat16 else 0)
-            assert _native.lib().ow_gated_linear_kept(ctypes.byref(d)) == 4 * gated._kept_values(x[:rows], w)
+    """Two values of fp32 for each of the result, for many tokens of many channels; the backward looks at them."""
+    sizes = [(rows, c, h) for rows in (1, 64, 65, 128, 129, 192, 300, 5000) for c in (127, 128, 1024, 1025, 1535, 1536, 2048, 2049)
+             for h in (6, 16, 1000, 4096)]
+    for dtype, code in ((torch.bfloat16, 1), (torch.float16, 2), (torch.float32, 0)):
+        for rows, c, h in sizes:
+            d = _native.OwGatedLinear(rows=rows, channels=c, hidden=h, dtype=code)
+            n = gated._kept_values(torch.zeros(rows, c, dtype=dtype, device="meta"), torch.zeros(h, c, dtype=dtype, device="meta"))
+            assert _native.lib().ow_gated_linear_kept(ctypes.byref(d)) == 4 * n and n in (0, 2 * rows * h)
+            assert n == 0 or (rows > 64 and c >= (128 if code == 0 else 1536))
+    x, w = torch.zeros(200, 2049), torch.zeros(6, 2049)
+    assert gated._run_forward(x, w, w, True)[1].numel() == 2400 and not gated._run_forward(x, w, w, False)[1].numel()
     launches.clear()
-    up = torch.zeros(70, 6)
-    for kept in (torch.zeros(839), torch.zeros(840).half(), torch.zeros(840, device="meta")):
+    up = torch.zeros(200, 6)
+    for kept in (torch.zeros(2399), torch.zeros(2400).half(), torch.zeros(2400, device="meta")):
         with pytest.raises(ValueError, match="kept"):
             gated._run_backward(up, kept, x, w, w, [True] * 3)
     assert not launches
-    for kept in (torch.zeros(840), NONE):
+    for kept in (torch.zeros(2400), NONE):
         gated._run_backward(up, kept, x, w, w, [True] * 3)
     assert len(launches) == 2
 
@@ -138,12 +140,14 @@ def test_c_entry_points_check_their_arguments() -> None:
     refused(bwd(desc(), dh=ctypes.c_void_p(257)), b"aligned")
     refused(bwd(desc(), kept=ctypes.c_void_p(258)), b"aligned")
     # rows of 10 values fill no whole pieces: x and the weights are copied
-    space = lib.ow_gated_linear_fwd_workspace(desc())
-    assert space >= (100 + 2 * 6) * 32 and lib.ow_gated_linear_fwd_workspace(None) == 0
-    assert lib.ow_gated_linear_fwd_workspace(desc(rows=64)) == 0 and lib.ow_gated_linear_fwd_workspace(desc(channels=8, x_stride=8)) == 0
-    refused(lib.ow_gated_linear_fwd(desc(), p, None, None, 0, None), b"workspace")
-    refused(lib.ow_gated_linear_fwd(desc(), p, None, p, space - 1, None), b"workspace")
-    refused(lib.ow_gated_linear_fwd(desc(), p, None, ctypes.c_void_p(264), space, None), b"workspace")
+    many = desc(rows=20000)
+    space = lib.ow_gated_linear_fwd_workspace(many)
+    assert space >= (20000 + 2 * 6) * 32 and lib.ow_gated_linear_fwd_workspace(None) == 0
+    assert lib.ow_gated_linear_fwd_workspace(desc(rows=64)) == 0
+    assert lib.ow_gated_linear_fwd_workspace(desc(rows=20000, channels=8, x_stride=8)) == 0
+    refused(lib.ow_gated_linear_fwd(many, p, None, None, 0, None), b"workspace")
+    refused(lib.ow_gated_linear_fwd(many, p, None, p, space - 1, None), b"workspace")
+    refused(lib.ow_gated_linear_fwd(many, p, None, ctypes.c_void_p(264), space, None), b"workspace")
     refused(lib.ow_gated_linear_fwd(desc(), p, p, None, 0, None), b"kept")
     refused(lib.ow_gated_linear_fwd(desc(channels=1536), p, ctypes.c_void_p(258), None, 0, None), b"kept")
     assert lib.ow_gated_linear_kept(None) == 0 and lib.ow_gated_linear_kept(desc(channels=1536)) == 2 * 100 * 6 * 4

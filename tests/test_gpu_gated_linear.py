@@ -103,7 +103,7 @@ def test_rows(rows, c, hidden, dtype) -> None:
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("c", [1, 2, 7, 8, 15, 16, 31, 32, 40, 63, 64, 65, 72, 96, 127, 128, 129, 136, 257])
-@pytest.mark.parametrize("rows", [9, 300])
+@pytest.mark.parametrize("rows", [9, 6000])
 def test_channels(rows, c, dtype) -> None:
     announce(f"gated rows={rows} c={c} {dtype}")
     check(*make(rows, c, 40, TYPES[dtype], seed=c))
@@ -111,7 +111,7 @@ def test_channels(rows, c, dtype) -> None:
 
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 @pytest.mark.parametrize("hidden", [1, 3, 4, 8, 9, 31, 32, 33, 63, 64, 65, 127, 128, 129, 300])
-@pytest.mark.parametrize("rows", [5, 140])
+@pytest.mark.parametrize("rows", [5, 140, 6000])
 def test_hidden(rows, hidden, dtype) -> None:
     announce(f"gated rows={rows} hidden={hidden} {dtype}")
     check(*make(rows, 48, hidden, TYPES[dtype], seed=hidden))
@@ -129,9 +129,12 @@ def test_hidden(rows, hidden, dtype) -> None:
     (99, 2815, 2895),
     (9000, 128, 256),   # sums of many parts
     (33000, 256, 1100), # whole tiles and parts of others
-    (70, 1408, 130),    # parts of both projections
-    (300, 1600, 70),    # both products kept
-    (300, 1537, 33),
+    (300, 1408, 130),   # parts of both projections
+    (300, 2064, 70),    # both products kept
+    (300, 2049, 33),
+    (1200, 1024, 200),  # 256 workgroups of the kernel for few tokens, and more
+    (1300, 1024, 200),
+    (129, 1030, 2100),
     (4097, 1024, 64),
     (70, 4096, 130),
 ])
@@ -262,7 +265,7 @@ def test_leaves_that_need_no_gradient() -> None:
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
-@pytest.mark.parametrize("rows,c,hidden", [(100, 1600, 72), (257, 1537, 31), (1100, 1536, 640)])
+@pytest.mark.parametrize("rows,c,hidden", [(200, 2056, 72), (257, 2049, 31), (1100, 2064, 640)])
 def test_products_kept_and_formed_again(rows, c, hidden, dtype) -> None:
     """The backward's two ways to both products: the same sums, in other orders at most."""
     announce(f"gated kept products rows={rows} c={c} hidden={hidden} {dtype}")
