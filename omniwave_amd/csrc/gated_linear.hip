@@ -7,8 +7,10 @@
 // 32 of the other projection, so that a lane has both values of an output.  G and U are fp32 until h is rounded; for a
 // backward to come they are stored as they are where that costs less than forming them again.
 //
-// Few tokens take gated_few_kernel, which is bound by reading the weights: a workgroup has 16 columns of both and up to 64 tokens,
-// its 8 waves take k in turns of 64 bytes a column and go from memory to the matrix cores without LDS; their sums meet there.
+// Few tokens take gated_few_kernel, which is bound by reading the weights: a workgroup has 16 columns of both and up to 64
+// tokens, its 8 waves take k in turns of 64 bytes a column and go from memory to the matrix cores without LDS; their sums meet there.
+// One token of 1,024 to 2,048 f16: 4.8 us, 49 tokens bf16 8.2 (8.4 MB of weights, a copy's time 1.7: the rest is a launch,
+// the latency of the first reads and the meeting of the waves).
 #include <hip/hip_runtime.h>
 
 #include <cstdint>

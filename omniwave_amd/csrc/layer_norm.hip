@@ -15,6 +15,10 @@
 // Rows lie in registers, T threads a row, as in block_norms.hip (Place, ow_rows.h); a row shorter than 8 vectors
 // takes as few threads as hold it.  A row takes two rounds of sums: the mean of x (backward: with that of h), then the
 // differences, their squares (and their products with h).
+//
+// Measured: 401,408 rows of 128 bf16 forward 33 us (206 MB, what a copy moves in 42: part of it is still in the last
+// cache); 25,088 of 512 bf16 forward 11.9, backward 19.5 and 3.9 for the column sums; 102,400 of 95 fp32, whose vectors lie
+// at any 4 bytes, 14.2 and 24.0 + 4.1; one row 2.4, a launch and one read's latency.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>

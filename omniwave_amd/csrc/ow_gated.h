@@ -3,7 +3,7 @@
 //
 // Operands are of 16 bits.  fp32 ones are three bf16 planes each (ow_x3.h), and a product of two is the six products of
 // planes whose weight is above 2^-24, one after the other along k: to the kernel, k is six times as long.  (fp32 MFMAs have a
-// sixteenth of the bf16 ones' rate; 25,088 tokens, 256 to 512: forward 141 us by them.)
+// sixteenth of the bf16 ones' rate; 25,088 tokens, 256 to 512: forward 141 us by them, 104 and 16 for the copies by planes.)
 //
 // An operand lies in memory with its contraction index contiguous (AlongK: x and the weights forward, the gates'
 // gradients in dx) or with its output index contiguous (AcrossK: the weights in dx, every operand of the weights'
@@ -20,7 +20,8 @@
 //
 // Tiles come by direct copies into LDS (16 bytes a lane; what lies outside the matrix reads as zeros), a tile ahead of
 // the products, and a step's operands are read during the step before it.  6,272 tokens of 4,096 to 8,192 bf16: 738 us
-// forward (1,140 TFLOP/s; the library's product of that size 719 us), the weights' gradients 745.
+// forward (1,140 TFLOP/s; the library's product of that size 719 us), the weights' gradients 719.  Small k is bound by what
+// surrounds a unit's two to four steps: 401,408 tokens of 128 to 256 bf16 take 123 us forward, where its bytes would take 63.
 #pragma once
 
 #include "ow_rows.h"
