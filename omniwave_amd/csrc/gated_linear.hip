@@ -43,7 +43,7 @@ __device__ __forceinline__ f32x4 mma16<F32>(u32x4 a, u32x4 b, f32x4 c) {
 
 // TG: groups of 16 tokens.
 template <class Ty, int TG>
-__global__ void __launch_bounds__(kFewWaves * 64, 2) gated_few_kernel(OwGatedLinear d, void* h_out) {
+__global__ void __launch_bounds__(kFewWaves * 64, 2) gated_few_kernel(OwGatedLinear d, void* h_out, float* kept) {
   constexpr int S = Elem<Ty>::kSize, V = Elem<Ty>::kPiece, KS = 4 * V;  // k of a step
   __shared__ f32x4 part[kFewWaves][2 * TG][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -110,16 +110,17 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) gated_few_kernel(OwGatedLin
     for (int k = 0; k < kFewWaves; ++k) G += part[k][g][at][e], U += part[k][TG + g][at][e];
     const int64_t row = first + 16 * g + (at & 15), col = n0 + 4 * (at >> 4) + e;
     if (row >= d.rows || col >= d.hidden) continue;
+    if (kept != nullptr) kept[row * d.hidden + col] = G, kept[(d.rows + row) * d.hidden + col] = U;
     static_cast<typename Row<Ty>::Elem*>(h_out)[row * d.hidden + col] = Row<Ty>::from_f32(G * U * sigmoid(G));
   }
 }
 
 template <class Ty>
-void launch_few(const OwGatedLinear& d, void* h, hipStream_t s) {
+void launch_few(const OwGatedLinear& d, void* h, float* kept, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(ceil_div(d.hidden, 16)), static_cast<unsigned>(ceil_div(d.rows, kFewRows))), block(kFewWaves * 64);
-  if (d.rows <= 16) hipLaunchKernelGGL((gated_few_kernel<Ty, 1>), grid, block, 0, s, d, h);
-  else if (d.rows <= 32) hipLaunchKernelGGL((gated_few_kernel<Ty, 2>), grid, block, 0, s, d, h);
-  else hipLaunchKernelGGL((gated_few_kernel<Ty, 4>), grid, block, 0, s, d, h);
+  if (d.rows <= 16) hipLaunchKernelGGL((gated_few_kernel<Ty, 1>), grid, block, 0, s, d, h, kept);
+  else if (d.rows <= 32) hipLaunchKernelGGL((gated_few_kernel<Ty, 2>), grid, block, 0, s, d, h, kept);
+  else hipLaunchKernelGGL((gated_few_kernel<Ty, 4>), grid, block, 0, s, d, h, kept);
 }
 
 }  // namespace
@@ -237,7 +238,7 @@ int gated_operands(const OwGatedLinear& d, char* workspace, GatedArgs* a, hipStr
 
 namespace {
 
-// Whether gated_few_kernel takes the tokens (no workspace, nothing kept): 64 at most, or more where its workgroups, of 64 tokens and
+// Whether gated_few_kernel takes the tokens (no workspace): 64 at most, or more where its workgroups, of 64 tokens and
 // 16 columns, are one round of a GPU's 256 (bf16, 128 tokens of 1,024 to 2,048: 8.6 us, 9.8 in tiles; 192: 15.0 and 9.9), and fp32
 // up to 128, which it takes without splitting the operands (2,048 to 4,096: 74 us, 78 in tiles; 192: 107 and 96).
 bool few(const OwGatedLinear& d) {
@@ -255,9 +256,10 @@ GatedPlan plan_forward(const OwGatedLinear& d) {
 extern "C" {
 
 // The products are kept where forming them again (4 K operations a value, six times as many for fp32) would take longer than
-// to write and read them (16 bytes).
+// to write and read them (16 bytes).  With few tokens, too: forward and backward of 49 tokens of 2,048 to 4,096 fp32 233 us
+// with the products formed again, 130 with them kept; below those widths a call's host hides it.
 size_t ow_gated_linear_kept(const OwGatedLinear* d) {
-  if (d == nullptr || ow::few(*d) || d->channels <= 0 || d->hidden <= 0) return 0;
+  if (d == nullptr || d->rows <= 0 || d->channels <= 0 || d->hidden <= 0) return 0;
   const int32_t from = d->dtype == OW_DTYPE_F32 ? 128 : 1536;
   return d->channels >= from ? static_cast<size_t>(2) * d->rows * d->hidden * sizeof(float) : 0;
 }
@@ -279,9 +281,9 @@ int ow_gated_linear_fwd(const OwGatedLinear* d, void* h, void* kept, void* works
                "the products of these sizes are not kept, or have no place for fp32 values");
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (ow::few(*d)) {
-    if (d->dtype == OW_DTYPE_BF16) ow::launch_few<ow::BF16>(*d, h, s);
-    else if (d->dtype == OW_DTYPE_F16) ow::launch_few<ow::F16>(*d, h, s);
-    else ow::launch_few<ow::F32>(*d, h, s);
+    if (d->dtype == OW_DTYPE_BF16) ow::launch_few<ow::BF16>(*d, h, static_cast<float*>(kept), s);
+    else if (d->dtype == OW_DTYPE_F16) ow::launch_few<ow::F16>(*d, h, static_cast<float*>(kept), s);
+    else ow::launch_few<ow::F32>(*d, h, static_cast<float*>(kept), s);
     if (int rc = ow::hip_status(hipGetLastError(), "gated_few_kernel launch")) return rc;
   } else {
     const ow::GatedPlan p = ow::plan_forward(*d);

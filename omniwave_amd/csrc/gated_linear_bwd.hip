@@ -116,7 +116,8 @@ int ow_gated_linear_bwd(const OwGatedLinear* d, const void* kept, const void* dh
   OW_CHECK_ARG(d->rows > 0 && d->channels > 0 && d->hidden > 0, "the backward of empty products has no kernel");
   const int64_t size = d->dtype == OW_DTYPE_F32 ? 4 : 2;
   OW_CHECK_ARG(dh != nullptr && reinterpret_cast<uintptr_t>(dh) % size == 0, "dh is NULL or not aligned to its values");
-  OW_CHECK_ARG(reinterpret_cast<uintptr_t>(kept) % 4 == 0, "the kept products are not aligned to fp32 values");
+  OW_CHECK_ARG(kept == nullptr || (ow_gated_linear_kept(d) != 0 && reinterpret_cast<uintptr_t>(kept) % 4 == 0),
+               "the products of these sizes are not kept, or are not aligned to fp32 values");
   const ow::Space space = ow::space_of(*d);
   const size_t need = space.all();
   OW_CHECK_ARG(workspace != nullptr && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,

@@ -18,7 +18,6 @@ from omniwave_amd.hip import _DTYPE_CODE, SUPPORTED_DTYPES, _plain
 from omniwave_amd.norms import _on, _rows, gpu_reason
 
 MAX_WIDTH = 1 << 20  # channels, hidden
-FEW_ROWS = 64  # the kernel for few tokens takes them at once
 
 
 def _ready(x, gate_weight, up_weight) -> None:
@@ -54,10 +53,7 @@ def _descriptor(x, gate_weight, up_weight):
 def _kept_values(x, gate_weight) -> int:
     """Values of both products that a forward keeps for its backward, 0 where that forms them again (the library's
     ``ow_gated_linear_kept``, for sizes that are not yet known, too)."""
-    rows, channels, hidden, wide = math.prod(x.shape[:-1]), x.shape[-1], gate_weight.shape[0], x.dtype == torch.float32
-    few = rows <= (2 * FEW_ROWS if wide else FEW_ROWS) or (
-        channels <= (2048 if wide else 1024) and (hidden + 15) // 16 * ((rows + FEW_ROWS - 1) // FEW_ROWS) <= 256)
-    return 0 if few or channels < (128 if wide else 1536) else 2 * rows * hidden
+    return 2 * math.prod(x.shape[:-1]) * gate_weight.shape[0] if x.shape[-1] >= (128 if x.dtype == torch.float32 else 1536) else 0
 
 
 def _run_forward(x, gate_weight, up_weight, keep) -> tuple[Tensor, Tensor]:

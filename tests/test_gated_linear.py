@@ -83,15 +83,15 @@ def test_upstream_gradients(launches, up) -> None:
 
 
 def test_kept_products(launches) -> None:
-    """Two values of fp32 for each of the result, for many tokens of many channels; the backward looks at them."""
-    sizes = [(rows, c, h) for rows in (1, 64, 65, 128, 129, 192, 300, 5000) for c in (127, 128, 1024, 1025, 1535, 1536, 2048, 2049)
+    """Two values of fp32 for each of the result, for many channels; the backward looks at them."""
+    sizes = [(rows, c, h) for rows in (0, 1, 64, 65, 128, 129, 192, 300, 5000) for c in (0, 127, 128, 1024, 1025, 1535, 1536, 2048, 2049)
              for h in (6, 16, 1000, 4096)]
     for dtype, code in ((torch.bfloat16, 1), (torch.float16, 2), (torch.float32, 0)):
         for rows, c, h in sizes:
             d = _native.OwGatedLinear(rows=rows, channels=c, hidden=h, dtype=code)
             n = gated._kept_values(torch.zeros(rows, c, dtype=dtype, device="meta"), torch.zeros(h, c, dtype=dtype, device="meta"))
             assert _native.lib().ow_gated_linear_kept(ctypes.byref(d)) == 4 * n and n in (0, 2 * rows * h)
-            assert n == 0 or (rows > 64 and c >= (128 if code == 0 else 1536))
+            assert n == (2 * rows * h if c >= (128 if code == 0 else 1536) else 0)
     x, w = torch.zeros(200, 2049), torch.zeros(6, 2049)
     assert gated._run_forward(x, w, w, True)[1].numel() == 2400 and not gated._run_forward(x, w, w, False)[1].numel()
     launches.clear()
@@ -148,7 +148,8 @@ def test_c_entry_points_check_their_arguments() -> None:
     refused(lib.ow_gated_linear_fwd(many, p, None, None, 0, None), b"workspace")
     refused(lib.ow_gated_linear_fwd(many, p, None, p, space - 1, None), b"workspace")
     refused(lib.ow_gated_linear_fwd(many, p, None, ctypes.c_void_p(264), space, None), b"workspace")
-    refused(lib.ow_gated_linear_fwd(desc(), p, p, None, 0, None), b"kept")
+    refused(lib.ow_gated_linear_fwd(many, p, p, p, space, None), b"kept")
+    refused(bwd(many, kept=p), b"kept")
     refused(lib.ow_gated_linear_fwd(desc(channels=1536), p, ctypes.c_void_p(258), None, 0, None), b"kept")
     assert lib.ow_gated_linear_kept(None) == 0 and lib.ow_gated_linear_kept(desc(channels=1536)) == 2 * 100 * 6 * 4
     refused(bwd(desc(), ws=None), b"workspace")

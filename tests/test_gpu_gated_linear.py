@@ -265,7 +265,8 @@ def test_leaves_that_need_no_gradient() -> None:
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
-@pytest.mark.parametrize("rows,c,hidden", [(200, 2056, 72), (257, 2049, 31), (1100, 2064, 640)])
+@pytest.mark.parametrize("rows,c,hidden", [(200, 2056, 72), (257, 2049, 31), (1100, 2064, 640), (1, 1536, 1), (5, 1540, 300), (64, 1600, 40),
+                                            (130, 1537, 90)])
 def test_products_kept_and_formed_again(rows, c, hidden, dtype) -> None:
     """The backward's two ways to both products: the same sums, in other orders at most."""
     announce(f"gated kept products rows={rows} c={c} hidden={hidden} {dtype}")
