@@ -233,8 +233,8 @@ __global__ void __launch_bounds__(256) distill_bwd_kernel(DistillBwdArgs a) {
   constexpr int V = R::kVec, UNITS = 256 / T;
   // Bits of a unit's classes: of a part, or of a whole row.
   constexpr int WORDS = (T == 256 ? 2 * kPart : T == 64 ? kLong : T * V * kBwdVectors) / 32;
-  __shared__ uint32_t seen_of[UNITS][WORDS];
-  uint32_t* seen = seen_of[threadIdx.x / T];
+  __shared__ uint32_t seen_of[UNITS][WORDS], again_of[UNITS][WORDS];
+  uint32_t *seen = seen_of[threadIdx.x / T], *again = again_of[threadIdx.x / T];
   const int t = threadIdx.x % T;
   const int64_t k = a.d.classes, units = a.d.rows * a.n_parts;
   const float row_weight = a.weight != nullptr ? *a.weight : 1.f;
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(256) distill_bwd_kernel(DistillBwdArgs a) {
     if (inv_zt != inv_zt) w = inv_zt;
     const float p = w * s[1];
     const int words = static_cast<int>((end - begin + 31) / 32);
-    for (int i = t; i < words; i += T) seen[i] = 0u;
+    for (int i = t; i < words; i += T) seen[i] = again[i] = 0u;
     for (int64_t i = begin + t * V; i < end; i += T * V) {
       float v[V];
       const int n = end - i < V ? static_cast<int>(end - i) : V;
@@ -293,25 +293,41 @@ __global__ void __launch_bounds__(256) distill_bwd_kernel(DistillBwdArgs a) {
       const Entry e(a.d, row, j);
       if (!e.given || e.at < begin || e.at >= end) continue;
       const int bit = static_cast<int>(e.at - begin);
-      if (atomicOr(&seen[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1u) twice = true;
-      else write(e.at, q_of(e));
+      if (atomicOr(&seen[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1u) {
+        atomicOr(&again[bit >> 5], 1u << (bit & 31));
+        twice = true;
+      } else {
+        write(e.at, q_of(e));
+      }
     }
     if (T <= 64) unit_sync<T>();
-    // Rare: a class has several entries.
+    // Rare: a class has several entries.  Only these look for the others, and only the first of them through all (64 rows
+    // of 8,192 entries, forward and gradient: no class twice 120 us, one of them 450, every one eight times 4,900).
     if (T > 64 ? __syncthreads_or(twice) : __any(twice)) {
       for (int j = t; j < top; j += T) {
         const Entry e(a.d, row, j);
         if (!e.given || e.at < begin || e.at >= end) continue;
+        const int bit = static_cast<int>(e.at - begin);
+        if (!(again[bit >> 5] >> (bit & 31) & 1u)) continue;
         float q = 0.f;
-        bool first = true, alone = true;
-        for (int o = 0; o < top; ++o) {
-          const Entry f(a.d, row, o);
-          if (!f.given || f.at != e.at) continue;
-          if (o < j) first = false;
-          if (o != j) alone = false;
-          q += q_of(f);
+        bool first = true;
+        constexpr int U = 16;  // classes that are read together
+        for (int o = 0; o < top && first; o += U) {
+          int64_t at[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) at[u] = a.d.indices[row * a.d.top + (o + u < top ? o + u : top - 1)];
+          uint32_t same = 0u;
+#pragma unroll
+          for (int u = 0; u < U; ++u) same |= (at[u] == e.at && o + u < top ? 1u : 0u) << u;
+          for (; same != 0u && first; same &= same - 1u) {
+            const int of = o + __builtin_ctz(same);
+            const Entry f(a.d, row, of);
+            if (!f.given) continue;
+            first = of >= j;
+            q += q_of(f);
+          }
         }
-        if (first && !alone) write(e.at, q);
+        if (first) write(e.at, q);
       }
     }
     unit_sync<T>();  // before the bits are cleared again

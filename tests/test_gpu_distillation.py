@@ -138,6 +138,21 @@ def test_a_class_with_several_entries(rows, k, dtype) -> None:
         assert all(torch.equal(a, b) for a, b in zip(first, again))
 
 
+@pytest.mark.parametrize("rows,k,top", [(6, 50, 700), (5, 3000, 2999), (4, 40000, 8000), (2100, 200, 190)])
+def test_long_lists_with_repeated_classes(rows, k, top) -> None:
+    """One class twice, every class of the list eight times, and one class alone in the list."""
+    announce(f"distillation long lists with repeated classes rows={rows} k={k} top={top}")
+    x, v, _ = make(rows, max(k, top), top, torch.float32)
+    x = x[:, :k].contiguous()
+    gen = torch.Generator().manual_seed(1)
+    i = torch.stack([torch.randperm(max(k, top), generator=gen)[:top] % k for _ in range(rows)])
+    i[0, -1] = i[0, 0]
+    i[1] = i[1, : (top + 7) // 8].repeat(8)[:top]
+    i[2] = k // 2
+    for reduction in ("mean", "none"):
+        check(x, v, i.to(DEV), 1.5, reduction=reduction)
+
+
 def test_a_student_that_is_its_teacher_and_all_classes() -> None:
     """Every class is an entry and both have the same logits: loss and gradient are rounding alone."""
     announce("distillation of itself")
