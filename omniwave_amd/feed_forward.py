@@ -52,7 +52,8 @@ class GatedFeedForward(nn.Module):
     def forward(self, x: Tensor) -> Tensor:
         if self._hip(x):
             normed = layer_norm_hip(x, self.norm_weight, self.norm_bias, EPS)
-            delta = self.down(gated_linear_hip(normed, self.gate.weight, self.up.weight))
-            return block_norms_hip(x, delta, gate=self.gamma)[0]
+            # Under autocast the weights are of another type than x, and so is what the projection back returns.
+            hidden = gated_linear_hip(normed, self.gate.weight.to(x.dtype), self.up.weight.to(x.dtype))
+            return block_norms_hip(x, self.down(hidden).to(x.dtype), gate=self.gamma)[0]
         normed = F.layer_norm(x, (self.dim,), self.norm_weight.to(x.dtype), self.norm_bias.to(x.dtype), EPS)
         return x + self.gamma.to(x.dtype) * self.down(F.silu(self.gate(normed)) * self.up(normed))

@@ -77,6 +77,27 @@ def test_block(shape, hidden, dtype) -> None:
         assert rel(got, ref) <= TOL[dtype], name
 
 
+@pytest.mark.parametrize("x_dtype", [torch.bfloat16, torch.float32])
+def test_block_under_autocast(x_dtype) -> None:
+    """Weights of 32 bits: an x of 16 bits, as the layers before it return there, and one of 32."""
+    announce(f"feed-forward under autocast x {x_dtype}")
+    torch.manual_seed(0)
+    block = GatedFeedForward(128, 200, 0.5, "hip").to(DEV)
+    x, up = (torch.randn(3, 9, 9, 128, device=DEV).to(x_dtype) for _ in range(2))
+    x.requires_grad_(True)
+    with torch.autocast("cuda", torch.bfloat16):
+        y = block(x)
+    assert y.dtype == x_dtype
+    names, params = zip(*block.named_parameters())
+    grads = torch.autograd.grad(y, (x, *params), up)
+    p = {k: v.detach().double().requires_grad_(True) for k, v in zip(names, params)}
+    xd = x.detach().double().requires_grad_(True)
+    want = formula(p, xd, torch.bfloat16)
+    assert rel(y.detach(), want.detach()) <= TOL[torch.bfloat16]
+    for name, got, ref in zip(("x", *names), grads, torch.autograd.grad(want, (xd, *p.values()), up.double())):
+        assert got.dtype == (x_dtype if name == "x" else torch.float32) and rel(got, ref) <= TOL[torch.bfloat16], name
+
+
 def make(dtype):
     torch.manual_seed(0)
     model = create_model("omniweave_t", backend="hip", **MODEL).to(device=DEV, dtype=dtype)
