@@ -9,8 +9,8 @@
 //
 // Few tokens take gated_few_kernel, which is bound by reading the weights: a workgroup has 16 columns of both and up to 64
 // tokens, its 8 waves take k in turns of 64 bytes a column and go from memory to the matrix cores without LDS; their sums meet there.
-// One token of 1,024 to 2,048 f16: 4.8 us, 49 tokens bf16 8.2 (8.4 MB of weights, a copy's time 1.7: the rest is a launch,
-// the latency of the first reads and the meeting of the waves).
+// One token of 1,024 to 2,048 f16: 4.8 us, 49 tokens bf16 6.6 (8.4 MB of weights, a copy's time 1.7: the rest is a launch,
+// the latency of the first reads and the meeting of the waves); one token of 4,096 to 8,192 bf16 28.8, 4.7 TB/s.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -117,9 +117,15 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) gated_few_kernel(OwGatedLin
 
 template <class Ty>
 void launch_few(const OwGatedLinear& d, void* h, float* kept, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>(ceil_div(d.hidden, 16)), static_cast<unsigned>(ceil_div(d.rows, kFewRows))), block(kFewWaves * 64);
-  if (d.rows <= 16) hipLaunchKernelGGL((gated_few_kernel<Ty, 1>), grid, block, 0, s, d, h, kept);
-  else if (d.rows <= 32) hipLaunchKernelGGL((gated_few_kernel<Ty, 2>), grid, block, 0, s, d, h, kept);
+  // Fewer tokens a workgroup, where compute units would else be idle: each workgroup reads the weights' columns anew, but
+  // less of x (49 tokens bf16: 1,024 to 2,048 in 64s 7.9 us, in 32s 6.6, in 16s, which is two rounds, 8.4; 2,048 to 1,024 in 64s
+  // 12.6, in 16s 8.3; fp32 31 and 15).
+  const int64_t columns = ceil_div(d.hidden, 16);
+  int tokens = d.rows <= 16 ? 16 : d.rows <= 32 ? 32 : kFewRows;
+  while (tokens > 16 && columns * ceil_div(d.rows, tokens / 2) <= device_cus()) tokens /= 2;
+  const dim3 grid(static_cast<unsigned>(columns), static_cast<unsigned>(ceil_div(d.rows, tokens))), block(kFewWaves * 64);
+  if (tokens == 16) hipLaunchKernelGGL((gated_few_kernel<Ty, 1>), grid, block, 0, s, d, h, kept);
+  else if (tokens == 32) hipLaunchKernelGGL((gated_few_kernel<Ty, 2>), grid, block, 0, s, d, h, kept);
   else hipLaunchKernelGGL((gated_few_kernel<Ty, 4>), grid, block, 0, s, d, h, kept);
 }
 

@@ -135,6 +135,8 @@ def test_hidden(rows, hidden, dtype) -> None:
     (1200, 1024, 200),  # 256 workgroups of the kernel for few tokens, and more
     (1300, 1024, 200),
     (129, 1030, 2100),
+    (49, 264, 2050),    # few tokens: 32 a workgroup; then 16
+    (50, 264, 1000),
     (4097, 1024, 64),
     (70, 4096, 130),
 ])
