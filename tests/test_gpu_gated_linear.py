@@ -101,6 +101,14 @@ def test_rows(rows, c, hidden, dtype) -> None:
     check(*make(rows, c, hidden, TYPES[dtype], seed=rows + c))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows", [65, 127, 128, 129, 191, 192, 193, 255, 256, 257, 400])
+@pytest.mark.parametrize("c,hidden", [(40, 4104), (95, 4101)])
+def test_rows_of_tiles(rows, c, hidden, dtype) -> None:
+    announce(f"gated tiles rows={rows} c={c} hidden={hidden} {dtype}")
+    check(*make(rows, c, hidden, TYPES[dtype], seed=rows + c))
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("c", [1, 2, 7, 8, 15, 16, 31, 32, 40, 63, 64, 65, 72, 96, 127, 128, 129, 136, 257])
 @pytest.mark.parametrize("rows", [9, 6000])
@@ -146,7 +154,7 @@ def test_every_tile(rows, c, hidden, dtype) -> None:
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-@pytest.mark.parametrize("rows", [6, 300])
+@pytest.mark.parametrize("rows", [6, 300, 2900])
 def test_large_and_small_gates(rows, dtype) -> None:
     announce(f"gated large gates rows={rows} {dtype}")
     x, wg, wu, dh = make(rows, 64, 96, TYPES[dtype])
@@ -161,7 +169,7 @@ def test_large_and_small_gates(rows, dtype) -> None:
     check(x, wg, wu, dh, whole=False)
 
 
-@pytest.mark.parametrize("rows", [10, 300])
+@pytest.mark.parametrize("rows", [10, 300, 3400])
 @pytest.mark.parametrize("c", [64, 95])
 def test_a_row_that_is_no_number_stays_in_its_row(rows, c) -> None:
     announce(f"gated NaN and inf rows={rows} c={c}")
@@ -185,7 +193,7 @@ def test_a_row_that_is_no_number_stays_in_its_row(rows, c) -> None:
         assert h[:3, 4].isnan().all() and h[:, :4].isfinite().all() and h[:, 5:].isfinite().all()
 
 
-@pytest.mark.parametrize("rows", [11, 150])
+@pytest.mark.parametrize("rows", [11, 150, 5601])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_rows_of_wider_tensors_at_odd_addresses(rows, dtype) -> None:
     announce(f"gated strides rows={rows} {dtype}")
@@ -236,7 +244,7 @@ def test_nothing() -> None:
         assert all(g.shape == t.shape and not g.any() for g, t in zip(grads, (x, wg, wu)))
 
 
-@pytest.mark.parametrize("rows", [7, 90])
+@pytest.mark.parametrize("rows", [7, 90, 8300])
 def test_gradient_against_differences(rows) -> None:
     """Central differences of the formula in 64 bits: their own error is of order h^2 and 2^-52 / h."""
     announce(f"gated differences rows={rows}")
@@ -257,7 +265,7 @@ def test_gradient_against_differences(rows) -> None:
 
 def test_leaves_that_need_no_gradient() -> None:
     announce("gated partial gradients")
-    for rows, c in ((40, 64), (300, 95)):
+    for rows, c in ((40, 64), (300, 95), (5600, 95)):
         x, wg, wu, dh = make(rows, c, 48, torch.bfloat16)
         full = check(x, wg, wu, dh)[1:]
         for n in range(3):
@@ -291,7 +299,7 @@ def test_sizes_that_are_not_known_while_compiling() -> None:
     announce("gated compiled with dynamic sizes")
     torch._dynamo.reset()
     fn = torch.compile(lambda *t: gated_linear_hip(*t), backend="aot_eager", dynamic=True)
-    for rows in (80, 90, 30):
+    for rows in (80, 90, 30, 9000):
         x, wg, wu, dh = make(rows, 128, 24, torch.float32)
         leaves = [t.requires_grad_(True) for t in (x, wg, wu)]
         got = torch.autograd.grad(fn(*leaves), leaves, dh)

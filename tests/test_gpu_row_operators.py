@@ -39,6 +39,16 @@ def few(dtype=torch.float32, seed=0):
     return [leaves[0].detach()[0, :9].requires_grad_(True), *leaves[1:]], fn
 
 
+def kept(dtype=torch.float32, seed=0, rows=150):
+    gen = torch.Generator().manual_seed(seed)
+    leaves = [torch.randn(*s, generator=gen).to(dtype).to(DEV) for s in ((2, rows, 160), (40, 160), (40, 160))]
+    return [t.requires_grad_(True) for t in leaves], lambda *t: (gated_linear_hip(*t).float() * 0.5).sum()
+
+
+def tiles(dtype=torch.float32, seed=0):
+    return kept(dtype, seed, 3000)
+
+
 def distill(dtype=torch.bfloat16, seed=0):
     gen = torch.Generator().manual_seed(seed)
     x = torch.randn(33, 96, generator=gen).to(dtype).to(DEV).requires_grad_(True)
@@ -47,7 +57,7 @@ def distill(dtype=torch.bfloat16, seed=0):
     return [x], lambda x: distillation_hip(x, v, i, temperature=2.0)
 
 
-CASES = {"lnorm": lnorm, "gated": gated, "few": few, "distill": distill}
+CASES = {"lnorm": lnorm, "gated": gated, "few": few, "kept": kept, "tiles": tiles, "distill": distill}
 
 
 @pytest.fixture(params=sorted(CASES))
