@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kFewWaves * 64, 2) gated_few_kernel(OwGatedLin
     const int64_t row = first + 16 * g + (at & 15), col = n0 + 4 * (at >> 4) + e;
     if (row >= d.rows || col >= d.hidden) continue;
     if (kept != nullptr) kept[row * d.hidden + col] = G, kept[(d.rows + row) * d.hidden + col] = U;
-    static_cast<typename Row<Ty>::Elem*>(h_out)[row * d.hidden + col] = Row<Ty>::from_f32(G * U * sigmoid(G));
+    static_cast<typename Row<Ty>::Elem*>(h_out)[row * d.hidden + col] = Row<Ty>::from_f32(gated(G, U));
   }
 }
 

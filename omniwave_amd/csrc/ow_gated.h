@@ -265,14 +265,16 @@ struct Turn {
   }
 };
 
-// silu(g) u = g u / (1 + e^-g)
 __device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(kNegLog2e * g)); }
 
-// dG and dU of a value.
+// silu(g) u.  The sigmoid meets g before u does: g u may leave fp32's range where the gate is closed (-1e20 and 1e20: 0).
+__device__ __forceinline__ float gated(float g, float u) { return g * sigmoid(g) * u; }
+
+// dG and dU of a value; the gate's factors come first here, too.
 __device__ __forceinline__ void gates(float dh, float g, float u, float& dg, float& du) {
   const float s = sigmoid(g);
   du = dh * (g * s);
-  dg = dh * u * (s * (1.f + g * (1.f - s)));
+  dg = dh * (u * (s * (1.f + g * (1.f - s))));
 }
 
 // Workgroups of an XCD take neighbouring tiles (round-robin dispatch).
@@ -534,7 +536,7 @@ __global__ void __launch_bounds__(T::kThreads, 2) gated_tile_kernel(GatedArgs a)
           }
           float h[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) h[i] = acc[0][j][i] * acc[1][j][i] * sigmoid(acc[0][j][i]);
+          for (int i = 0; i < 16; ++i) h[i] = gated(acc[0][j][i], acc[1][j][i]);
           Tn::template put<Out>(own, 0, h, out_lane);
           Tn::template store<S>(own, static_cast<char*>(a.out[0]) + row * ld + c * S, ld, a.rows - row, a.hidden - c, out_lane);
         }
@@ -643,7 +645,7 @@ __global__ void __launch_bounds__(256) gated_join_kernel(GatedArgs a) {
         a.kept[row * n_c + c + j] = sum[j];
         a.kept[(a.rows + row) * n_c + c + j] = other[j];
       }
-      o[j] = R::from_f32(sum[j] * other[j] * sigmoid(sum[j]));
+      o[j] = R::from_f32(gated(sum[j], other[j]));
     } else {
       o[j] = R::from_f32(sum[j]);
     }
