@@ -12,11 +12,13 @@
 // counted).  A class outside the row, or a NaN among the entries, makes the row NaN, as a NaN logit does.
 //
 // Forward and backward read the logits once each, as the cross-entropy does (ow_softmax.h); a row's entries
-// are read by the lanes that have its m and z.  Differences are taken from the maxima before anything is summed, so
-// the loss of a student near its teacher keeps its digits.  The backward writes w T p for every class
-// first, and then the classes that have an entry once more: the same threads write both, with a barrier between them,
-// and a class is written by one entry only.  A bitmap of the part's classes in LDS finds classes that have
-// several; then the first of these adds all of them up in their order, so results do not depend on timing.
+// are read by the lanes that have its m and z.  Differences are taken from the maxima before anything is summed.  The loss
+// of a student near its teacher keeps its digits where the list has all classes (near_row); a shorter list's loss is at least
+// the student's share of the other classes, and is off by some 1e-7 T^2 (1,000 classes: 0.6 to 1.4e-7 in the mean square).
+//
+// The backward writes w T p for every class first, and then the classes that have an entry once more: the same threads write
+// both, with a barrier between them, and a class is written by one entry only.  A bitmap of the part's classes in LDS finds
+// classes that have several; then the first of these adds all of them up in their order, so results do not depend on timing.
 // Exponentials, sums and losses are fp32 (the sum of losses fp64); the gradient is rounded once.
 //
 // Bound by memory for long rows (4,096 of 21,841 bf16 with 64 entries: forward 40.6 us and 4.7 for the sum, 179 MB;
@@ -59,8 +61,62 @@ struct Entry {
   }
 };
 
-// A row's teacher and loss, from its m and z, by T lanes; all of them get the loss, and lane 0 writes.
+// e^d - 1 - d for |d| <= 1/2: the first eight terms, the next one is below 2^-28 of them.
+__device__ __forceinline__ float power_rest(float d) {
+  float s = 1.f / 40320.f + d * (1.f / 362880.f);
+  s = 1.f / 5040.f + d * s;
+  s = 1.f / 720.f + d * s;
+  s = 1.f / 120.f + d * s;
+  s = 1.f / 24.f + d * s;
+  s = 1.f / 6.f + d * s;
+  return d * d * (0.5f + d * s);
+}
+
+// The loss of a row, T^2 left out, whose entries are all classes, one each, by T lanes.  A student near its teacher has a
+// small one, the rest of sums that cancel.  With d_j = ln(p_j / q_j) and both distributions over the same classes,
+// sum_j (p_j - q_j) = 0, so
+//   sum_j q_j (-d_j) = sum_j q_j (e^{d_j} - 1 - d_j)
+// of which no term is negative, and an error of d that the entries have in common (ln of the sums) enters by its square:
+// 1,000 classes, T = 4, logits 0.01 apart, a loss of 5e-5: 11% off as sum_j q_j (-d_j), 6e-8 this way.  Such entries are known by
+// their number and their part of z, which is all of it within what rounding does to two sums; `loss` comes back for others.
+// The row's entries are read twice more (8,192 x 1,000 fp32, every row near: 85 us forward without, 204 with).
 template <int T>
+__device__ __forceinline__ float near_row(const DistillArgs& a, int64_t row, float m, float z, float mt, float zt, int lane, int top, float loss) {
+  const OwDistillation& d = a.d;
+  float given = 0.f, part = 0.f;
+  for (int j = lane; j < top; j += T) {
+    const Entry e(d, row, j);
+    if (!e.given || !e.known) continue;
+    given += 1.f;
+    part += __builtin_amdgcn_exp2f((load_any(d.logits, d.dtype, row * d.row_stride + e.at) - m) * a.scale);
+  }
+  given = lanes_reduce<AddOp, T>(given);
+  part = lanes_reduce<AddOp, T>(part);
+  const float k = static_cast<float>(d.classes);  // at most the entries of a row
+  const bool all = given == k && fabsf(part - z) <= (128.f + k / 16.f) * 0x1p-24f * z;
+  const float log_ratio = logf(part / zt), to_p = zt / part;
+  float sum = 0.f;
+  for (int j = all ? lane : top; j < top; j += T) {
+    const Entry e(d, row, j);
+    if (!e.given || !e.known) continue;  // more entries than classes: some are none
+    const float x = load_any(d.logits, d.dtype, row * d.row_stride + e.at);
+    const float q = __builtin_amdgcn_exp2f((e.t - mt) * a.scale);
+    const double apart = (static_cast<double>(x) - m) - (static_cast<double>(e.t) - mt);  // four fp32 numbers that cancel
+    const float diff = static_cast<float>(apart) / d.temperature - log_ratio;
+    if (q > 0.f && fabsf(diff) < 0.5f) {
+      sum += q * power_rest(diff);
+    } else {
+      sum += __builtin_amdgcn_exp2f((x - m) * a.scale) * to_p;
+      if (q > 0.f) sum -= q + q * diff;
+    }
+  }
+  sum = lanes_reduce<AddOp, T>(sum);
+  return all ? sum / zt : loss;
+}
+
+// A row's teacher and loss, from its m and z, by T lanes of whole waves; all of them get the loss, and lane 0 writes.  ALL: lists
+// may be as long as the classes (registers for near_row cost the others 5%, 200,000 rows of 100 bf16).
+template <int T, bool ALL>
 __device__ __forceinline__ float finish_row(const DistillArgs& a, int64_t row, float m, float z, int lane, bool valid, bool* counted) {
   const OwDistillation& d = a.d;
   const int top = valid ? d.top : 0;
@@ -86,10 +142,13 @@ __device__ __forceinline__ float finish_row(const DistillArgs& a, int64_t row, f
   if (bad != 0.f) zt = __builtin_nanf("");
   *counted = zt != 0.f;  // a NaN counts
   float loss = 0.f;
-  if (zt != 0.f) {
-    const float temp = d.temperature;
-    loss = temp * temp * (sum / zt / temp + (logf(z) - logf(zt)));
+  if (zt != 0.f) loss = sum / zt / d.temperature + logf(z / zt);
+  // From 1/32 on a loss this way has five digits.
+  if (ALL && d.top >= d.classes) {
+    const bool near = zt > 0.f && loss < 0.03125f;
+    if (__any(near)) loss = near_row<T>(a, row, m, z, mt, zt, lane, near ? top : 0, loss);
   }
+  loss *= d.temperature * d.temperature;
   if (lane == 0 && valid) {
     float* s = a.stats + 4 * row;
     s[0] = m, s[1] = 1.f / z, s[2] = mt, s[3] = zt != 0.f ? 1.f / zt : 0.f;
@@ -99,7 +158,7 @@ __device__ __forceinline__ float finish_row(const DistillArgs& a, int64_t row, f
 }
 
 // T threads a (row, part); one part a row for T <= 64.
-template <class Ty, int T>
+template <class Ty, int T, bool ALL>
 __global__ void __launch_bounds__(256) distill_fwd_kernel(DistillArgs a) {
   typedef Row<Ty> R;
   constexpr int UNITS = 256 / T;
@@ -138,7 +197,7 @@ __global__ void __launch_bounds__(256) distill_fwd_kernel(DistillArgs a) {
       }
     } else if (T <= 64 || t < 64) {  // whole waves
       bool counted = false;
-      const float loss = finish_row<(T > 64 ? 64 : T)>(a, row, s.m, s.z, t, valid, &counted);
+      const float loss = finish_row<(T > 64 ? 64 : T), ALL>(a, row, s.m, s.z, t, valid, &counted);
       if (t == 0 && valid) sum += loss, count += counted;
     }
   }
@@ -180,7 +239,7 @@ __global__ void __launch_bounds__(kSumThreads) distill_few_kernel(DistillArgs a)
     s.template scan<R, 64>(static_cast<const typename R::Elem*>(a.d.logits) + row * a.d.row_stride, 0, a.d.classes, lane);
     s.template join_row<64>();
     bool counted;
-    finish_row<64>(a, row, s.m, s.z, lane, true, &counted);
+    finish_row<64, true>(a, row, s.m, s.z, lane, true, &counted);
   }
   __syncthreads();
   sum_rows(a);
@@ -202,7 +261,7 @@ __global__ void __launch_bounds__(kSumThreads) distill_sum_kernel(DistillArgs a)
       }
       join_lanes<kSumLanes>(f, m, z, unused);
       bool counted;
-      finish_row<kSumLanes>(a, row, m, z, lane, valid, &counted);
+      finish_row<kSumLanes, true>(a, row, m, z, lane, valid, &counted);
     }
     __syncthreads();  // the losses of this workgroup's rows, which are all rows where they are summed
   }
@@ -336,14 +395,20 @@ __global__ void __launch_bounds__(256) distill_bwd_kernel(DistillBwdArgs a) {
 
 LogitRows shape(const OwDistillation& d) { return LogitRows{d.rows, d.classes, d.dtype}; }
 
+template <class Ty, bool ALL>
+void launch_fwd_rows(const DistillArgs& a, int t, unsigned groups, hipStream_t s) {
+  if (t == 8) hipLaunchKernelGGL((distill_fwd_kernel<Ty, 8, ALL>), dim3(groups), dim3(256), 0, s, a);
+  else if (t == 16) hipLaunchKernelGGL((distill_fwd_kernel<Ty, 16, ALL>), dim3(groups), dim3(256), 0, s, a);
+  else if (t == 32) hipLaunchKernelGGL((distill_fwd_kernel<Ty, 32, ALL>), dim3(groups), dim3(256), 0, s, a);
+  else if (t == 64) hipLaunchKernelGGL((distill_fwd_kernel<Ty, 64, ALL>), dim3(groups), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((distill_fwd_kernel<Ty, 256, ALL>), dim3(groups), dim3(256), 0, s, a);
+}
+
 template <class Ty>
 void launch_fwd(const DistillArgs& a, int t, unsigned groups, hipStream_t s) {
   if (few_rows(shape(a.d), a.loss != nullptr)) hipLaunchKernelGGL((distill_few_kernel<Ty>), dim3(1), dim3(kSumThreads), 0, s, a);
-  else if (t == 8) hipLaunchKernelGGL((distill_fwd_kernel<Ty, 8>), dim3(groups), dim3(256), 0, s, a);
-  else if (t == 16) hipLaunchKernelGGL((distill_fwd_kernel<Ty, 16>), dim3(groups), dim3(256), 0, s, a);
-  else if (t == 32) hipLaunchKernelGGL((distill_fwd_kernel<Ty, 32>), dim3(groups), dim3(256), 0, s, a);
-  else if (t == 64) hipLaunchKernelGGL((distill_fwd_kernel<Ty, 64>), dim3(groups), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((distill_fwd_kernel<Ty, 256>), dim3(groups), dim3(256), 0, s, a);
+  else if (a.d.top >= a.d.classes) launch_fwd_rows<Ty, true>(a, t, groups, s);
+  else launch_fwd_rows<Ty, false>(a, t, groups, s);
 }
 
 template <class Ty>

@@ -157,6 +157,9 @@ def distillation_hip(logits: Tensor, teacher_logits: Tensor, teacher_indices: Te
     entry count neither in the loss nor in the mean, and have no gradient; a mean of no rows is NaN.  A class may have
     several entries.  An index outside ``[0, classes)``, or a NaN logit, makes its row NaN.
     ``reduction``: ``"mean"``, ``"sum"`` or ``"none"``.  Differentiable once in the logits.
+
+    A row whose entries are all classes, one each, has a loss with the digits of fp32 however small it is; that of a shorter list,
+    which is at least the share of the classes left out, is off by a few 1e-7 of ``T^2`` besides.
     """
     glue, code = _native.glue(), _native.OW_REDUCE.get(reduction)
     if glue is not None and code is not None and _plain(logits, teacher_logits, teacher_indices):
