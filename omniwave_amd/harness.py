@@ -252,7 +252,8 @@ class TrainingStep:
 
     ``labels_b`` / ``mix``: the second labels and the weight of the first ones of mixed images.  ``teacher``: a teacher's top
     logits and their classes for each image (``distillation_hip``), whose loss at ``temperature`` enters with the weight
-    ``distill_weight`` beside the labels' loss of the rest."""
+    ``distill_weight`` beside the labels' loss of the rest; images without an entry have only the labels', and so has a batch
+    of them."""
 
     def __init__(self, model: nn.Module, *, lr: float = 1e-3, weight_decay: float = 0.05, state_bits: int = 32,
                  master_weights: bool = True, max_grad_norm: float | None = 1.0, label_smoothing: float = 0.1,
@@ -269,18 +270,32 @@ class TrainingStep:
         self.optimizer = AdamW([g for g in groups if g["params"]], lr=lr, state_bits=state_bits,
                                master_weights=master_weights, max_grad_norm=max_grad_norm)
 
-    def step(self, images: torch.Tensor, labels: torch.Tensor, labels_b: torch.Tensor | None = None,
+    def loss(self, logits: torch.Tensor, labels: torch.Tensor, labels_b: torch.Tensor | None = None,
              mix: torch.Tensor | float | None = None,
              teacher: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
+        """The step's loss of a model's logits.  A part without weight is left out."""
         from omniwave_amd.distillation import distillation_hip
         from omniwave_amd.loss import cross_entropy_hip
 
-        self.optimizer.zero_grad(set_to_none=True)
-        logits = self.model(images)
+        weight = 0.0 if teacher is None else self.distill_weight
+        taught = None
+        if weight > 0.0:
+            values, classes = teacher
+            taught = distillation_hip(logits, values, classes, temperature=self.temperature) * weight
+            # The mean of no rows is NaN; a batch without an entry has nothing to add.  (Over rows first: no reduction over
+            # several workgroups, which would record a memset into a captured step.)
+            some = ((classes != -100) & (values != -math.inf)).any(-1).any()
+            taught = torch.where(some, taught, 0.0)
+            if weight == 1.0:
+                return taught
         loss = cross_entropy_hip(logits, labels, target_b=labels_b, mix=mix, label_smoothing=self.label_smoothing)
-        if teacher is not None:
-            taught = distillation_hip(logits, *teacher, temperature=self.temperature)
-            loss = loss * (1.0 - self.distill_weight) + taught * self.distill_weight
+        return loss if taught is None else loss * (1.0 - weight) + taught
+
+    def step(self, images: torch.Tensor, labels: torch.Tensor, labels_b: torch.Tensor | None = None,
+             mix: torch.Tensor | float | None = None,
+             teacher: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
+        self.optimizer.zero_grad(set_to_none=True)
+        loss = self.loss(self.model(images), labels, labels_b, mix, teacher)
         loss.backward()
         self.optimizer.step()
         return loss.detach()
