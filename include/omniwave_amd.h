@@ -794,6 +794,22 @@ size_t ow_gated_linear_bwd_workspace(const OwGatedLinear* d);
 int ow_gated_linear_bwd(const OwGatedLinear* d, const void* kept, const void* dh, int64_t dh_stride, void* dx,
                         void* dgate_weight, void* dup_weight, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * How a product of these sizes runs on the current device (for measurements and tests): its tile (gate and up columns together;
+ * 0 x 0: the kernel for few tokens), how many tiles take their whole k, and how many are cut into how many parts of k.
+ * OW_GATED_GATES runs only where nothing was kept.  Sizes and alignments alone are looked at, never memory.
+ */
+enum { OW_GATED_FORWARD = 0, OW_GATED_GATES = 1, OW_GATED_DX = 2, OW_GATED_DW = 3 };
+typedef struct OwGatedPlan {
+  int64_t whole;
+  int64_t cut;
+  int32_t tile_rows;
+  int32_t tile_cols;
+  int32_t parts; /* of each tile that is cut */
+} OwGatedPlan;
+
+int ow_gated_linear_plan(const OwGatedLinear* d, int32_t product, OwGatedPlan* plan);
+
 #ifdef __cplusplus
 }
 #endif

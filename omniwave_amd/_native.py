@@ -91,6 +91,12 @@ class OwGatedLinear(ctypes.Structure):
     _fields_ += [(name, ctypes.c_int32) for name in ("channels", "hidden", "dtype")]
 
 
+class OwGatedPlan(ctypes.Structure):
+    _fields_ = [("whole", ctypes.c_int64), ("cut", ctypes.c_int64)]
+    _fields_ += [(name, ctypes.c_int32) for name in ("tile_rows", "tile_cols", "parts")]
+
+
+OW_GATED = {"forward": 0, "gates": 1, "dx": 2, "dw": 3}
 OW_REDUCE = {"none": 0, "sum": 1, "mean": 2}
 OW_ADAMW_CHUNK, OW_ADAMW_BLOCK = 4096, 256
 
@@ -334,6 +340,7 @@ _SIGNATURES = {
     "ow_gated_linear_fwd": (
         ctypes.c_int, [ctypes.POINTER(OwGatedLinear)] + [ctypes.c_void_p] * 3 + [ctypes.c_size_t, ctypes.c_void_p],
     ),
+    "ow_gated_linear_plan": (ctypes.c_int, [ctypes.POINTER(OwGatedLinear), ctypes.c_int32, ctypes.POINTER(OwGatedPlan)]),
     "ow_gated_linear_bwd_workspace": (ctypes.c_size_t, [ctypes.POINTER(OwGatedLinear)]),
     "ow_gated_linear_bwd": (
         ctypes.c_int,

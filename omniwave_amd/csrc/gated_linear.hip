@@ -242,21 +242,18 @@ int gated_operands(const OwGatedLinear& d, char* workspace, GatedArgs* a, hipStr
   return hip_status(hipGetLastError(), "gated_pack_kernel launch");
 }
 
-namespace {
-
 // Whether gated_few_kernel takes the tokens (no workspace): 64 at most, or more where its workgroups, of 64 tokens and
 // 16 columns, are one round of a GPU's 256 (bf16, 128 tokens of 1,024 to 2,048: 8.6 us, 9.8 in tiles; 192: 15.0 and 9.9), and fp32
 // up to 128, which it takes without splitting the operands (2,048 to 4,096: 74 us, 78 in tiles; 192: 107 and 96).
-bool few(const OwGatedLinear& d) {
+bool gated_few(const OwGatedLinear& d) {
   if (d.rows <= kFewRows || (d.dtype == OW_DTYPE_F32 && d.rows <= 2 * kFewRows)) return true;
   return d.channels <= (d.dtype == OW_DTYPE_F32 ? 2048 : 1024) && ceil_div(d.hidden, 16) * ceil_div(d.rows, kFewRows) <= 256;
 }
 
-GatedPlan plan_forward(const OwGatedLinear& d) {
+GatedPlan gated_plan_forward(const OwGatedLinear& d) {
   return gated_plan(d.rows, 2 * static_cast<int64_t>(d.hidden), gated_k_tiles(d.channels, d.dtype), 1, true, true);
 }
 
-}  // namespace
 }  // namespace ow
 
 extern "C" {
@@ -271,8 +268,8 @@ size_t ow_gated_linear_kept(const OwGatedLinear* d) {
 }
 
 size_t ow_gated_linear_fwd_workspace(const OwGatedLinear* d) {
-  if (d == nullptr || ow::few(*d) || d->channels <= 0 || d->hidden <= 0) return 0;
-  return ow::gated_operand_bytes(*d) + ow::gated_partial_bytes(ow::plan_forward(*d));
+  if (d == nullptr || ow::gated_few(*d) || d->channels <= 0 || d->hidden <= 0) return 0;
+  return ow::gated_operand_bytes(*d) + ow::gated_partial_bytes(ow::gated_plan_forward(*d));
 }
 
 int ow_gated_linear_fwd(const OwGatedLinear* d, void* h, void* kept, void* workspace, size_t workspace_bytes, void* stream) {
@@ -286,13 +283,13 @@ int ow_gated_linear_fwd(const OwGatedLinear* d, void* h, void* kept, void* works
   OW_CHECK_ARG(kept == nullptr || (ow_gated_linear_kept(d) != 0 && reinterpret_cast<uintptr_t>(kept) % 4 == 0),
                "the products of these sizes are not kept, or have no place for fp32 values");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (ow::few(*d)) {
+  if (ow::gated_few(*d)) {
     if (d->dtype == OW_DTYPE_BF16) ow::launch_few<ow::BF16>(*d, h, static_cast<float*>(kept), s);
     else if (d->dtype == OW_DTYPE_F16) ow::launch_few<ow::F16>(*d, h, static_cast<float*>(kept), s);
     else ow::launch_few<ow::F32>(*d, h, static_cast<float*>(kept), s);
     if (int rc = ow::hip_status(hipGetLastError(), "gated_few_kernel launch")) return rc;
   } else {
-    const ow::GatedPlan p = ow::plan_forward(*d);
+    const ow::GatedPlan p = ow::gated_plan_forward(*d);
     OW_CHECK_SUPPORTED(p.units < (int64_t(1) << 31), "gated linear: too many tiles for a launch");
     const size_t need = ow_gated_linear_fwd_workspace(d), operands = ow::gated_operand_bytes(*d);
     OW_CHECK_ARG(need == 0 || (workspace != nullptr && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),

@@ -21,6 +21,8 @@ namespace ow {
 int check_gated(const OwGatedLinear* d);
 size_t gated_operand_bytes(const OwGatedLinear& d);
 int gated_operands(const OwGatedLinear& d, char* workspace, GatedArgs* a, hipStream_t s);
+bool gated_few(const OwGatedLinear& d);
+GatedPlan gated_plan_forward(const OwGatedLinear& d);
 
 namespace {
 
@@ -108,6 +110,27 @@ extern "C" {
 size_t ow_gated_linear_bwd_workspace(const OwGatedLinear* d) {
   if (d == nullptr || d->rows <= 0 || d->channels <= 0 || d->hidden <= 0) return 0;
   return ow::space_of(*d).all();
+}
+
+int ow_gated_linear_plan(const OwGatedLinear* d, int32_t product, OwGatedPlan* plan) {
+  if (int rc = ow::check_gated(d)) return rc;
+  OW_CHECK_ARG(plan != nullptr, "plan is NULL");
+  OW_CHECK_ARG(product >= OW_GATED_FORWARD && product <= OW_GATED_DW, "unknown product %d", product);
+  OW_CHECK_ARG(d->rows > 0 && d->channels > 0 && d->hidden > 0, "empty products have no plan");
+  *plan = OwGatedPlan{};
+  if (product != OW_GATED_FORWARD || !ow::gated_few(*d)) {
+    const ow::GatedPlan p = product == OW_GATED_FORWARD ? ow::gated_plan_forward(*d)
+                            : product == OW_GATED_GATES ? ow::plan_gates(*d)
+                            : product == OW_GATED_DX    ? ow::plan_dx(*d)
+                                                        : ow::plan_dw(*d);
+    plan->tile_rows = ow::gated_tile_rows(p.size);
+    plan->tile_cols = ow::gated_tile_cols(p.size);
+    plan->parts = p.parts;
+    plan->whole = p.whole;
+    plan->cut = p.tiles_r * p.tiles_c - p.whole;
+  }
+  ow::clear_error();
+  return OW_OK;
 }
 
 int ow_gated_linear_bwd(const OwGatedLinear* d, const void* kept, const void* dh, int64_t dh_stride, void* dx,
