@@ -33,8 +33,6 @@
 namespace ow {
 namespace {
 
-constexpr float kLn2 = 0.6931471805599453f;
-
 struct DistillArgs {
   OwDistillation d;
   float scale;        // log2(e) / T
