@@ -115,7 +115,7 @@ class _Stage(nn.Module):
 class OmniWeaveBackbone(nn.Module):
     """Input ``[B, 3, H, W]`` (NCHW) -> logits ``[B, num_classes]``.  ``post_norm``: every block also
     normalises what it adds (``OmniWeaveBlock``).  ``feed_forward`` above 0: every stage ends with a
-    ``GatedFeedForward`` over that many times its width."""
+    ``GatedFeedForward`` over that many times its width, which ``drop_path_rate`` leaves alone."""
 
     def __init__(
         self,

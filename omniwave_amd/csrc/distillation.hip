@@ -21,9 +21,9 @@
 // classes that have several; then the first of these adds all of them up in their order, so results do not depend on timing.
 // Exponentials, sums and losses are fp32 (the sum of losses fp64); the gradient is rounded once.
 //
-// Bound by memory for long rows (4,096 of 21,841 bf16 with 64 entries: forward 40.6 us and 4.7 for the sum, 179 MB;
-// backward 68.4, 358 MB, a copy's time 73), by launches for few (8 of 1,000: 5.6 and 3.9; 1,024 of 1,000 fp32 with 100 entries
-// 5.2 + 2.8 and 5.7).
+// Bound by memory for long rows (4,096 of 21,841 bf16 with 64 entries: forward 40.2 us and 4.6 for the sum, 179 MB;
+// backward 69.7, 358 MB, a copy's time 73), by launches for few (8 of 1,000: 5.2 and 3.7; 1,024 of 1,000 fp32 with 100 entries
+// 5.2 + 3.0 and 5.7).
 #include <hip/hip_runtime.h>
 
 #include <cstdint>

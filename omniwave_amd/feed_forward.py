@@ -4,7 +4,7 @@ mixed, where a BiGEMM block mixes 16 tokens and the channels of one group.
     x + gamma * ((silu(n W_g^T) * (n W_u^T)) W_d^T),   n = LayerNorm(x)
 
 On the hip backend the norm is ``layer_norm_hip``, both projections with their gate are ``gated_linear_hip``, and LayerScale with
-the residual is ``block_norms_hip``; the projection back is a plain Linear.
+the residual is ``block_norms_hip``; the projection back is a plain Linear.  Drop-path is for the BiGEMM blocks: this one runs always.
 """
 
 from __future__ import annotations
@@ -52,7 +52,8 @@ class GatedFeedForward(nn.Module):
     def forward(self, x: Tensor) -> Tensor:
         if self._hip(x):
             normed = layer_norm_hip(x, self.norm_weight, self.norm_bias, EPS)
-            # Under autocast the weights are of another type than x, and so is what the projection back returns.
+            # Under autocast the weights are of another type than x, and so is what the projection back returns; the products
+            # are x's (in fp32 where x is).
             hidden = gated_linear_hip(normed, self.gate.weight.to(x.dtype), self.up.weight.to(x.dtype))
             return block_norms_hip(x, self.down(hidden).to(x.dtype), gate=self.gamma)[0]
         normed = F.layer_norm(x, (self.dim,), self.norm_weight.to(x.dtype), self.norm_bias.to(x.dtype), EPS)
