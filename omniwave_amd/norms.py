@@ -215,8 +215,9 @@ def _norms_setup_context(ctx, inputs, output):
 
 
 def _norms_backward(ctx, dout, dnext):
-    x, delta, post_weight, gate, scale, next_weight = ctx.saved_tensors
-    need = [n and t is not None for n, t in zip(ctx.needs_input_grad, ctx.saved_tensors)]
+    saved = ctx.saved_tensors  # asked for once: recomputation and hooks answer once
+    x, delta, post_weight, gate, scale, next_weight = saved
+    need = [n and t is not None for n, t in zip(ctx.needs_input_grad, saved)]
     want = [need[0], need[1], need[2], need[3], need[5]]
     dout, dnext = (dout if delta is not None else None), (dnext if next_weight is not None else None)
     if dout is None and dnext is None:
@@ -369,8 +370,9 @@ def _layer_norm_setup_context(ctx, inputs, output):
 
 
 def _layer_norm_backward(ctx, dy):
-    want = [n and t is not None for n, t in zip(ctx.needs_input_grad, ctx.saved_tensors)]
-    grads = layer_norm_bwd(dy, *ctx.saved_tensors, ctx.eps, want)
+    saved = ctx.saved_tensors  # once, as above
+    want = [n and t is not None for n, t in zip(ctx.needs_input_grad, saved)]
+    grads = layer_norm_bwd(dy, *saved, ctx.eps, want)
     return *[g if w else None for g, w in zip(grads, want)], None
 
 
